@@ -19,6 +19,9 @@ Entry points
 ``seed_states``     per-row xoroshiro128+ states, seeded like Sampler::reset
 ``Batch``           B generation streams with device-side RNG states and windows
 ``Tail``            the logits producer tail: final RMSNorm + LM head on the device
+``Q4Linear``        products with 4-bit weights and group scales (ops.py)
+``process_logits``  penalties, biases and masks on logits rows, before the pick (ops.py)
+``token_logprobs``  log-probabilities and ranks of tokens, after it (ops.py)
 """
 from __future__ import annotations
 
@@ -29,7 +32,8 @@ from pathlib import Path
 from typing import Optional, Sequence
 
 __all__ = ["Sampling", "Sampler", "VerboCudaError", "load_library", "sample", "sample_noalloc", "full_vocab_fallbacks", "shard_topk", "merge_sample",
-           "seed_states", "check", "version", "ROW_STATS_FIELDS", "Batch", "Server", "Tail", "Comm"]
+           "seed_states", "check", "version", "ROW_STATS_FIELDS", "Batch", "Server", "Tail", "Comm",
+           "Penalties", "process_logits", "token_logprobs", "Q4Linear"]
 __version__ = "0.1.0"
 
 _HERE = Path(__file__).resolve().parent
@@ -641,3 +645,6 @@ class Tail:
                                              _dptr(out, True), out.stride(0) if n else self.vocab,
                                              _stream(stream)))
         return out
+
+
+from .ops import Penalties, Q4Linear, process_logits, token_logprobs  # noqa: E402

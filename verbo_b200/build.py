@@ -19,9 +19,11 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB_DIR = PKG / "_lib"
 LIB = LIB_DIR / "libverbo_cuda.so"
-SOURCES = [CSRC / "kernels.cu", CSRC / "nucleus.cu", CSRC / "tail.cu", CSRC / "capi.cpp"]
+SOURCES = [CSRC / "kernels.cu", CSRC / "nucleus.cu", CSRC / "tail.cu", CSRC / "ops_logits.cu", CSRC / "ops_q4.cu",
+           CSRC / "capi.cpp", CSRC / "ops_capi.cpp"]
 HEADERS = [CSRC / "device.cuh", CSRC / "kernels.cuh", CSRC / "rowdev.cuh", CSRC / "tail.cuh",
-           ROOT / "include" / "verbo_cuda.h"]
+           CSRC / "ops.cuh", CSRC / "capi_guard.hpp", ROOT / "include" / "verbo_cuda.h",
+           ROOT / "include" / "verbo_ops.h"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

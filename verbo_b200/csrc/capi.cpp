@@ -21,32 +21,17 @@
 #include <utility>
 #include <vector>
 
+#include "capi_guard.hpp"
 #include "kernels.cuh"
 #include "tail.cuh"
 #include "verbo_cuda.h"
 
 namespace {
 
-thread_local std::string g_err;
-
-template <typename F>
-auto guard(F&& fn, decltype(fn()) fail) -> decltype(fn()) {
-  try {
-    g_err.clear();
-    return fn();
-  } catch (const std::exception& e) {
-    g_err = e.what();
-  } catch (...) {
-    g_err = "verbo_cuda: unknown error";
-  }
-  return fail;
-}
-
-[[noreturn]] void fail(const std::string& m) { throw std::runtime_error("verbo_cuda: " + m); }
-
-void cuda_ok(cudaError_t e, const char* what) {
-  if (e != cudaSuccess) fail(std::string(what) + ": " + cudaGetErrorString(e));
-}
+using vb::cuda_ok;
+using vb::fail;
+using vb::g_err;
+using vb::guard;
 
 int bitlen(unsigned long long x) {
   int b = 0;
