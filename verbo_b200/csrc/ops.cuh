@@ -16,7 +16,8 @@ struct ProcArgs {
   const void* logits;
   long long ld;
   int rows, vocab;
-  int slices;  // CTAs per row
+  int parts;      // CTAs per row
+  int part_cols;  // columns of a part
   float repeat, frequency, presence;
   int last;
   const float* row_pen;       // [rows][3] or null
@@ -46,7 +47,6 @@ struct LogprobArgs {
   int top;
   int* top_ids;
   float* top_logprobs;
-  int slice;  // columns per CTA of the row's cluster
 };
 cudaError_t launch_logprobs(LogprobArgs a, int dtype, cudaStream_t s);
 

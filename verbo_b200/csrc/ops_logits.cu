@@ -69,155 +69,222 @@ __device__ __forceinline__ int row_shift(const T* row) {
 }
 
 // =============================================================== process ==
-// out = mask(bias(penalties(logits))), include/verbo_ops.h.  One pass: each CTA
-// takes NT * V vectors of one row.  The loads of its logits go out first; while
-// they are in flight it counts the row's window into one shared counter per
-// column (integer atomics: exact in any order) and marks each biased column
-// with the place of its last entry (atomicMax), so no later step depends on the
-// order in which threads ran.  A CTA re-reads its row's whole window, from L2.
+// out = mask(bias(penalties(logits))), include/verbo_ops.h.  One pass over the
+// row; a CTA walks a part of it in slices of NT * 16 columns.  Per slice it
+// counts the window's ids into one shared counter per column (integer atomics:
+// exact in any order), with the top bit for a biased column, whose last entry
+// is found by atomicMax; so nothing depends on the order in which threads ran.
+// The thread that owns a column takes its counter back to 0.  The first ids of
+// the window stay in registers over the slices, and the next slice's logits
+// and mask words are on their way while a slice is counted and stored.
 // In place nothing of the row is loaded but columns that change.
-template <class T, int NT, int V, bool INPLACE>
-__global__ void __launch_bounds__(NT, 2048 / NT / 2) process_kernel(const ProcArgs a) {
-  constexpr int N = Vec<T>::N;
-  constexpr int S = NT * V * N;
-  extern __shared__ __align__(16) int smem_i[];  // counts [S], then bias places [S]: whichever the call has
+constexpr int kProcThreads = 256;
+constexpr int kProcCols = 16;                         // columns per thread and slice
+constexpr int kProcSlice = kProcThreads * kProcCols;  // 4096
+constexpr int kProcHist = 4, kProcBias = 1;           // ids per thread in registers
+
+template <class T, bool LISTS, bool INPLACE>
+__global__ void __launch_bounds__(kProcThreads, 4) process_kernel(const ProcArgs a) {
+  constexpr int N = Vec<T>::N, NT = kProcThreads, V = kProcCols / N, S = kProcSlice;
+  constexpr uint32_t kAll = (1u << N) - 1;
+  constexpr int kNone = -(1 << 30);  // an id that lies in no slice
+  extern __shared__ __align__(16) int smem_i[];  // counters [S], then (with biases) last entries [S]
   grid_wait();
-  const int row = blockIdx.x / a.slices;
-  const int u0 = (blockIdx.x - row * a.slices) * S;
+  const int row = blockIdx.x / a.parts;
+  const int part = blockIdx.x - row * a.parts;
   const int tid = threadIdx.x;
   const T* in = static_cast<const T*>(a.logits) + row * a.ld;
   float* out = a.out + row * a.ld_out;
+  const uint32_t* mask = a.mask ? a.mask + row * a.ld_mask : nullptr;
   const int shift = row_shift(in);
-  const int c0 = u0 - shift;  // column of the slice's first place
-  if (c0 >= a.vocab) return;
-
-  long long hb = 0, he = 0, bb = 0, be = 0;
-  if (a.hist) {
-    hb = a.hist_off[row];
-    he = a.hist_off[row + 1];
-    if (a.last > 0 && he - hb > a.last) hb = he - a.last;
-  }
-  if (a.bias) {
-    bb = a.bias_off[row];
-    be = a.bias_off[row + 1];
-  }
+  const int c0 = part * a.part_cols - shift;
+  const int c1 = min(a.vocab, c0 + a.part_cols);
+  if (c0 >= c1) return;
 
   Vec<T> x[V];
-  if (!INPLACE) {
+  uint32_t ml[V], mh[V];
+  auto load = [&](int cs) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int c = c0 + (i * NT + tid) * N;
-      if (c >= 0 && c + N <= a.vocab) x[i].raw = ld_stream16(in + c);
+      const int c = cs + (i * NT + tid) * N;
+      if (c >= 0 && c + N <= a.vocab) {
+        if (!INPLACE) x[i].raw = ld_stream16(in + c);
+        if (mask) {
+          const uint32_t* w = mask + (c >> 5);
+          ml[i] = __ldg(w);
+          mh[i] = (c & 31) + N > 32 ? __ldg(w + 1) : 0u;
+        }
+      }
     }
-  }
+  };
+  if (!LISTS) load(c0);
 
   int* cnt = smem_i;
-  int* at = smem_i + (a.hist ? S : 0);
-  const bool have_h = he > hb, have_b = be > bb;  // the same in every thread of the CTA
+  int* at = smem_i + S;
+  long long hb = 0, hn = 0, bb = 0, bn = 0;
+  int hid[kProcHist], bid[kProcBias];
   float rep = a.repeat, freq = a.frequency, pres = a.presence;
-  if (have_h || have_b) {
-    if (have_h && a.row_pen) {
+  if (LISTS) {
+    if (a.hist) {
+      hb = a.hist_off[row];
+      hn = max(0ll, a.hist_off[row + 1] - hb);
+    }
+    if (a.bias) {
+      bb = a.bias_off[row];
+      bn = max(0ll, a.bias_off[row + 1] - bb);
+    }
+    load(c0);
+    if (a.last > 0 && hn > a.last) {
+      hb += hn - a.last;
+      hn = a.last;
+    }
+    auto valid = [&](int id) { return id >= 0 && id < a.vocab ? id : kNone; };
+#pragma unroll
+    for (int i = 0; i < kProcHist; ++i) hid[i] = i * NT + tid < hn ? valid(a.hist[hb + i * NT + tid]) : kNone;
+#pragma unroll
+    for (int i = 0; i < kProcBias; ++i) bid[i] = i * NT + tid < bn ? valid(a.bias_ids[bb + i * NT + tid]) : kNone;
+    if (hn > 0 && a.row_pen) {
       rep = a.row_pen[3ll * row];
       freq = a.row_pen[3ll * row + 1];
       pres = a.row_pen[3ll * row + 2];
     }
+  }
+  const bool lists = LISTS && (hn > 0 || bn > 0);  // the same in every thread of the CTA
+  if (lists) {
 #pragma unroll
-    for (int i = 0; i < V * N / 4; ++i) {
-      if (have_h) reinterpret_cast<int4*>(cnt)[i * NT + tid] = make_int4(0, 0, 0, 0);
-      if (have_b) reinterpret_cast<int4*>(at)[i * NT + tid] = make_int4(0, 0, 0, 0);
-    }
-    __syncthreads();
-    for (long long i = hb + tid; i < he; i += NT) {
-      const int id = a.hist[i];
-      if (id < 0 || id >= a.vocab) continue;
-      const int p = id - c0;
-      if (p >= 0 && p < S) atomicAdd(&cnt[p], 1);
-    }
-    for (long long i = bb + tid; i < be; i += NT) {
-      const int id = a.bias_ids[i];
-      if (id < 0 || id >= a.vocab) continue;
-      const int p = id - c0;
-      if (p >= 0 && p < S) atomicMax(&at[p], static_cast<int>(i - bb) + 1);
+    for (int i = 0; i < S / 4 / NT; ++i) {
+      reinterpret_cast<int4*>(cnt)[i * NT + tid] = make_int4(0, 0, 0, 0);
+      if (a.bias) reinterpret_cast<int4*>(at)[i * NT + tid] = make_int4(0, 0, 0, 0);
     }
     __syncthreads();
   }
-  const float* bias = a.bias + bb - 1;
-  const uint32_t* mask = a.mask ? a.mask + row * a.ld_mask : nullptr;
+  // one column: the whole of the operator but the mask
+  auto apply = [&](float v, int k, int p) {
+    if (k & 0x7fffffff) {
+      v = penalize(v, rep);
+      v = __fsub_rn(v, __fmul_rn(freq, static_cast<float>(k & 0x7fffffff)));
+      v = __fsub_rn(v, pres);
+    }
+    if (k < 0) {
+      v = __fadd_rn(v, a.bias[bb + at[p] - 1]);
+      at[p] = 0;
+    }
+    return v;
+  };
 
+  for (int cs = c0; cs < c1; cs += S) {
+    if (lists) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int p = (i * NT + tid) * N;
-    const int c = c0 + p;
-    if (c >= a.vocab || c + N <= 0) continue;
-    const bool full = c >= 0 && c + N <= a.vocab;
-    uint32_t ok = (1u << N) - 1;  // bit j: column c + j is allowed
-    if (mask) {
-      if (full) {
-        const int w = c >> 5, sh = c & 31;
-        const uint32_t lo = __ldg(mask + w);
-        const uint32_t hi = sh + N > 32 ? __ldg(mask + w + 1) : 0u;
-        ok &= __funnelshift_r(lo, hi, sh);
-      } else {
-        for (int j = 0; j < N; ++j)
-          if (c + j >= 0 && c + j < a.vocab && !((__ldg(mask + ((c + j) >> 5)) >> ((c + j) & 31)) & 1u))
-            ok &= ~(1u << j);
+      for (int i = 0; i < kProcHist; ++i) {
+        const int p = hid[i] - cs;
+        if (p >= 0 && p < S) atomicAdd(&cnt[p], 1);
       }
-    }
-    int k[N], b[N];
-    int any = 0;
-#pragma unroll
-    for (int j = 0; j < N; j += 4) {
-      int4 t = make_int4(0, 0, 0, 0), s = t;
-      if (have_h) t = *reinterpret_cast<const int4*>(cnt + p + j);
-      if (have_b) s = *reinterpret_cast<const int4*>(at + p + j);
-      k[j] = t.x, k[j + 1] = t.y, k[j + 2] = t.z, k[j + 3] = t.w;
-      b[j] = s.x, b[j + 1] = s.y, b[j + 2] = s.z, b[j + 3] = s.w;
-      any |= t.x | t.y | t.z | t.w | s.x | s.y | s.z | s.w;
-    }
-    if (INPLACE) {
-      if (any == 0 && ok == (1u << N) - 1) continue;
-      if (full && ok == 0) {
-#pragma unroll
-        for (int j = 0; j < N; j += 4)
-          *reinterpret_cast<float4*>(out + c + j) = make_float4(kNegInf, kNegInf, kNegInf, kNegInf);
-        continue;
+      for (long long i = kProcHist * NT + tid; i < hn; i += NT) {
+        const int id = a.hist[hb + i];
+        const int p = id >= 0 && id < a.vocab ? id - cs : -1;
+        if (p >= 0 && p < S) atomicAdd(&cnt[p], 1);
       }
-    }
-    float v[N];
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const bool inside = full || (c + j >= 0 && c + j < a.vocab);
-      const bool touched = (k[j] | b[j]) != 0;
-      v[j] = 0.0f;
-      if (INPLACE) {
-        if (inside && touched && ((ok >> j) & 1u)) v[j] = out[c + j];
-      } else if (full) {
-        v[j] = x[i].get(j);
-      } else if (inside) {
-        v[j] = to_float(in[c + j]);
-      }
-      if (touched) {
-        if (k[j] > 0) {
-          v[j] = penalize(v[j], rep);
-          v[j] = __fsub_rn(v[j], __fmul_rn(freq, static_cast<float>(k[j])));
-          v[j] = __fsub_rn(v[j], pres);
+      for (int i = 0; i < kProcBias; ++i) {
+        const int p = bid[i] - cs;
+        if (p >= 0 && p < S) {
+          atomicOr(&cnt[p], INT_MIN);
+          atomicMax(&at[p], i * NT + tid + 1);
         }
-        if (b[j] > 0) v[j] = __fadd_rn(v[j], bias[b[j]]);
       }
-      if (!((ok >> j) & 1u)) v[j] = kNegInf;
-      if (INPLACE && inside && (touched || !((ok >> j) & 1u))) out[c + j] = v[j];
+      for (long long i = kProcBias * NT + tid; i < bn; i += NT) {
+        const int id = a.bias_ids[bb + i];
+        const int p = id >= 0 && id < a.vocab ? id - cs : -1;
+        if (p >= 0 && p < S) {
+          atomicOr(&cnt[p], INT_MIN);
+          atomicMax(&at[p], static_cast<int>(i) + 1);
+        }
+      }
+      __syncthreads();
     }
-    if (!INPLACE) {
-      if (full && (reinterpret_cast<uintptr_t>(out + c) & 15) == 0) {
+    Vec<T> y[V];
+    uint32_t ok[V];  // bit j: the vector's column j is allowed
 #pragma unroll
-        for (int j = 0; j < N; j += 4)
-          *reinterpret_cast<float4*>(out + c + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-      } else {
+    for (int i = 0; i < V; ++i) {
+      y[i] = x[i];
+      ok[i] = mask ? __funnelshift_r(ml[i], mh[i], (cs + (i * NT + tid) * N) & 31) & kAll : kAll;
+    }
+    if (cs + S < c1) load(cs + S);
 #pragma unroll
-        for (int j = 0; j < N; ++j)
-          if (full || (c + j >= 0 && c + j < a.vocab)) out[c + j] = v[j];
+    for (int i = 0; i < V; ++i) {
+      const int p = (i * NT + tid) * N;
+      const int c = cs + p;
+      if (c >= 0 && c + N <= a.vocab) {
+        int k[N];
+        int any = 0;
+        if (lists) {
+#pragma unroll
+          for (int j = 0; j < N; j += 4) {
+            const int4 t = *reinterpret_cast<const int4*>(cnt + p + j);
+            k[j] = t.x, k[j + 1] = t.y, k[j + 2] = t.z, k[j + 3] = t.w;
+            any |= t.x | t.y | t.z | t.w;
+          }
+          if (any) {
+#pragma unroll
+            for (int j = 0; j < N; j += 4) *reinterpret_cast<int4*>(cnt + p + j) = make_int4(0, 0, 0, 0);
+          }
+        }
+        if (INPLACE) {
+          if (any) {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+              if (k[j]) {
+                const float v = apply((ok[i] >> j) & 1u ? out[c + j] : 0.0f, k[j], p + j);
+                if ((ok[i] >> j) & 1u) out[c + j] = v;
+              }
+          }
+          if (ok[i] == 0) {
+#pragma unroll
+            for (int j = 0; j < N; j += 4)
+              *reinterpret_cast<float4*>(out + c + j) = make_float4(kNegInf, kNegInf, kNegInf, kNegInf);
+          } else if (ok[i] != kAll) {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+              if (!((ok[i] >> j) & 1u)) out[c + j] = kNegInf;
+          }
+        } else {
+          float v[N];
+#pragma unroll
+          for (int j = 0; j < N; ++j) v[j] = y[i].get(j);
+          if (any) {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+              if (k[j]) v[j] = apply(v[j], k[j], p + j);
+          }
+          if (ok[i] != kAll) {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+              if (!((ok[i] >> j) & 1u)) v[j] = kNegInf;
+          }
+          if ((reinterpret_cast<uintptr_t>(out + c) & 15) == 0) {
+#pragma unroll
+            for (int j = 0; j < N; j += 4)
+              *reinterpret_cast<float4*>(out + c + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j) out[c + j] = v[j];
+          }
+        }
+      } else if (c + N > 0 && c < a.vocab) {  // the row's ragged ends
+        for (int j = max(0, -c); j < min(N, a.vocab - c); ++j) {
+          const int k = lists ? cnt[p + j] : 0;
+          const bool allowed = !mask || ((__ldg(mask + ((c + j) >> 5)) >> ((c + j) & 31)) & 1u);
+          if (INPLACE && allowed && k == 0) continue;
+          float v = to_float(in[c + j]);
+          if (k) {
+            v = apply(v, k, p + j);
+            cnt[p + j] = 0;
+          }
+          out[c + j] = allowed ? v : kNegInf;
+        }
       }
     }
+    if (lists) __syncthreads();
   }
 }
 
@@ -240,28 +307,19 @@ cudaError_t launch_chained(K kernel, unsigned grid, int threads, size_t smem, in
   return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
-template <class T, int NT, int V, bool INPLACE>
-cudaError_t run_process(ProcArgs a, cudaStream_t s) {
-  constexpr int N = Vec<T>::N;
-  constexpr int S = NT * V * N;
-  a.slices = static_cast<int>((static_cast<long long>(a.vocab) + N - 1 + S - 1) / S);
-  const long long grid = static_cast<long long>(a.rows) * a.slices;
-  if (grid > INT_MAX) return cudaErrorInvalidConfiguration;
-  const size_t smem = (a.hist ? S * 4u : 0u) + (a.bias ? S * 4u : 0u);
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(process_kernel<T, NT, V, INPLACE>,
-                                               cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (e != cudaSuccess) return e;
-  }
-  return launch_chained(process_kernel<T, NT, V, INPLACE>, static_cast<unsigned>(grid), NT, smem, 1, s, a);
-}
-
-// Slices of 8192 columns, or of 2048 while those leave SMs idle.
+// Parts of as many slices as leave at least four waves of CTAs, 8 at most.
 template <class T, bool INPLACE>
-cudaError_t pick_process(const ProcArgs& a, cudaStream_t s) {
-  constexpr int V = 16 / Vec<T>::N;
-  if (static_cast<long long>(a.rows) * a.vocab <= 148ll * 8192) return run_process<T, 256, V / 2, INPLACE>(a, s);
-  return run_process<T, 512, V, INPLACE>(a, s);
+cudaError_t run_process(ProcArgs a, cudaStream_t s) {
+  const long long slices = (static_cast<long long>(a.vocab) + Vec<T>::N - 1 + kProcSlice - 1) / kProcSlice;
+  long long per = std::max(1ll, std::min(8ll, a.rows * slices / (148 * 4 * 4)));
+  a.part_cols = static_cast<int>(per) * kProcSlice;
+  a.parts = static_cast<int>((slices + per - 1) / per);
+  const long long grid = static_cast<long long>(a.rows) * a.parts;
+  if (grid > INT_MAX) return cudaErrorInvalidConfiguration;
+  const unsigned n = static_cast<unsigned>(grid);
+  if (!a.hist && !a.bias) return launch_chained(process_kernel<T, false, INPLACE>, n, kProcThreads, 0, 1, s, a);
+  const size_t smem = kProcSlice * 4u * (a.bias ? 2 : 1);
+  return launch_chained(process_kernel<T, true, INPLACE>, n, kProcThreads, smem, 1, s, a);
 }
 
 // ============================================================== logprobs ==
@@ -271,15 +329,20 @@ cudaError_t pick_process(const ProcArgs& a, cudaStream_t s) {
 // one fma each, 2^(c v + b) with b = -c m rounded; c v is exact inside the fma,
 // so the rounding of b is one factor for the whole batch, 2^(-c m - b), which is
 // multiplied back.
-// The first columns: a bound T with at least `top` columns of the CTA at or
-// above it comes from the maxima of the first batch (below); every column that
-// reaches T is put into a shared list, from which the `top` first are ranked by
-// counting.  A list that overflows is gathered anew with a sharper bound.
+// The rank counts the columns v >= t, t the chosen value for columns before the
+// chosen one and the next larger float for those after it.
+// The first columns cost the pass nothing: of the threads' maxima, which it has
+// anyway, a bound T is taken that `top` of them reach, so that `top` columns do;
+// T is close to the `top`-th column itself, since two of the first columns
+// seldom meet in one thread.  The few threads whose maximum reaches T have their
+// columns read again (L2), and what reaches T is listed and ranked by counting.
+// A list that overflows (ties) is gathered anew with a sharper bound.
 constexpr int kLpThreads = 512;
 constexpr int kLpWarps = kLpThreads / 32;
-constexpr int kLpBatch = 16;  // columns per thread and batch
+constexpr int kLpVecs = 4;    // vectors per thread and batch
 constexpr int kLpCap = 2048;  // listed columns per CTA
 constexpr int kLpMaxCluster = 8;
+constexpr float kLowest = -3.402823466e38f;
 
 struct LpPart {
   float m, s;  // maximum, sum of 2^(c (v - m))
@@ -302,7 +365,7 @@ __device__ __forceinline__ float lp_scaled(float s, float from, float m, float c
 struct LpAcc {
   float m = kNegInf, s = 0.0f;
   int ninf = 0;
-  // bm: the maximum of x[0, n)
+  // bm: the maximum of x[0, n), which may hold NaNs (they count as -inf)
   template <int n>
   __device__ __forceinline__ void add(const float (&x)[n], float bm, float c) {
     if (bm == -kNegInf) {  // +inf alone counts then
@@ -315,30 +378,51 @@ struct LpAcc {
       s = lp_scaled(s, m, bm, c);
       m = bm;
     }
+    if (m == kNegInf) return;
+    float t = 0.0f;
     if (fabsf(m) < 1e30f) {
       const float b = -m * c;
-      float t = 0.0f;
 #pragma unroll
       for (int j = 0; j < n; ++j) t += ex2(fmaf(x[j], c, b));
-      s += t * ex2(fmaf(-m, c, -b));
-    } else if (m != kNegInf) {  // c m may overflow (rows masked with the type's lowest value)
-#pragma unroll
-      for (int j = 0; j < n; ++j) s += ex2((x[j] - m) * c);
+      t *= ex2(fmaf(-m, c, -b));
     }
+    // c m may overflow (rows masked with the type's lowest value), or a NaN was met
+    if (!(fabsf(m) < 1e30f && t == t)) {
+      t = 0.0f;
+#pragma unroll
+      for (int j = 0; j < n; ++j) t += ex2((fmaxf(x[j], kNegInf) - m) * c);
+    }
+    s += t;
   }
 };
 
+template <class T>
+__device__ __forceinline__ uint4 all_neg_inf();
+template <>
+__device__ __forceinline__ uint4 all_neg_inf<float>() {
+  return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u);
+}
+template <>
+__device__ __forceinline__ uint4 all_neg_inf<__half>() {
+  return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u);
+}
+template <>
+__device__ __forceinline__ uint4 all_neg_inf<__nv_bfloat16>() {
+  return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
+}
+
 template <class T, bool TOP>
 __global__ void __launch_bounds__(kLpThreads, 2) logprob_kernel(const LogprobArgs a) {
-  constexpr int N = Vec<T>::N;
-  constexpr int NV = kLpBatch / N;  // vectors per thread and batch
+  constexpr int N = Vec<T>::N, NV = kLpVecs, NT = kLpThreads;
+  constexpr int SUB = 16 / N;  // vectors whose terms are summed together
   __shared__ LpPart parts[kLpWarps];
   __shared__ LpPart slots[kLpMaxCluster];  // the leader's: one per CTA
   __shared__ uint64_t slot_keys[TOP ? kLpMaxCluster * kLpMaxTop : 1];
   __shared__ uint64_t list[TOP ? kLpCap : 1];
   __shared__ uint64_t best[TOP ? kLpMaxTop : 1];
+  __shared__ unsigned short hits[TOP ? NT : 1];
   __shared__ uint32_t offer[kLpWarps];
-  __shared__ int count;
+  __shared__ int count, nhits;
   __shared__ uint64_t bound_key;
 
   cg::cluster_group cl = cg::this_cluster();
@@ -349,133 +433,89 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprob_kernel(const LogprobArg
   const int row = blockIdx.x / C;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const T* in = static_cast<const T*>(a.logits) + row * a.ld;
-  const int shift = row_shift(in);
   const float c = 1.4426950408889634f / a.temp;
   const int top = a.top;
-  // this CTA's columns [lo, hi), counted from the row's 16-byte boundary
-  const long long ulo = static_cast<long long>(rankc) * a.slice;
-  const int lo = static_cast<int>(max(0ll, ulo - shift));
-  const int hi = static_cast<int>(min(static_cast<long long>(a.vocab), ulo + a.slice - shift));
-  const int cu = static_cast<int>(min(ulo - shift, static_cast<long long>(a.vocab)));  // its first vector's column
-  const int nbatch = hi > lo ? (hi - cu + kLpThreads * kLpBatch - 1) / (kLpThreads * kLpBatch) : 0;
+  // the row's aligned vectors [0, nvec) from column `head` on; the columns before
+  // and after them go one to a thread of the first and of the last CTA
+  const int head = min(a.vocab, (N - row_shift(in)) % N);
+  const int nvec = (a.vocab - head) / N;
+  const int tail = head + nvec * N;
+  const int v0 = static_cast<int>(static_cast<long long>(nvec) * rankc / C);
+  const int v1 = static_cast<int>(static_cast<long long>(nvec) * (rankc + 1) / C);
+  const T* vin = in + head;
+  int edge = -1;
+  if (rankc == 0 && tid < head) edge = tid;
+  if (rankc == C - 1 && tid >= N && tid - N < a.vocab - tail) edge = tail + tid - N;
 
   int id = -1;
   if (a.ids) {
     id = a.ids[row];
     if (id < 0 || id >= a.vocab) id = -1;
   }
-  if (TOP && tid == 0) count = 0;
-
+  if (TOP && tid == 0) {
+    count = 0;
+    nhits = 0;
+  }
   Vec<T> x[NV], y[NV];
-  auto load = [&](int batch, Vec<T>(&v)[NV]) {
+  auto load = [&](int v, Vec<T>(&to)[NV]) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int col = cu + ((batch * NV + i) * kLpThreads + tid) * N;
-      if (col >= lo && col + N <= hi) {
-        v[i].raw = ld_stream16(in + col);
-      } else {
-        const bool any = col + N > lo && col < hi;
-        v[i].raw = make_uint4(0, 0, 0, 0);
-        if (any) {  // the row's ragged ends, element by element
-          uint32_t w[4] = {0, 0, 0, 0};
-          for (int j = 0; j < N; ++j)
-            if (col + j >= lo && col + j < hi) {
-              const T e = in[col + j];
-              if (sizeof(T) == 4)
-                w[j & 3] = *reinterpret_cast<const uint32_t*>(&e);
-              else
-                w[(j >> 1) & 3] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(&e)) << (16 * (j & 1));
-            }
-          v[i].raw = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-      }
+      if (v + i * NT < v1)
+        to[i].raw = ld_stream16(vin + static_cast<long long>(v + i * NT) * N);
+      else
+        to[i].raw = all_neg_inf<T>();
     }
   };
-  if (nbatch > 0) load(0, x);
-  const float chosen = id >= 0 ? fmaxf(to_float(in[id]), kNegInf) : 0.0f;  // a NaN counts as -inf
+  load(v0 + tid, x);
+  const float edge_value = edge >= 0 ? fmaxf(to_float(in[edge]), kNegInf) : kNegInf;
+  // thresholds of the rank; nothing reaches a NaN
+  const float nan = __uint_as_float(0x7fffffffu);
+  float chosen = kNegInf, t_before = nan, t_after = nan;
+  int before = 0;
+  if (id >= 0) {
+    chosen = fmaxf(to_float(in[id]), kNegInf) + 0.0f;  // a NaN counts as -inf, -0 as 0
+    t_before = chosen;
+    t_after = __uint_as_float(chosen >= 0.0f ? __float_as_uint(chosen) + 1u : __float_as_uint(chosen) - 1u);
+    if (chosen == kNegInf) {  // every column before it counts, NaN and -inf among them
+      t_before = nan;
+      before = rankc == 0 && tid == 0 ? id : 0;
+    }
+  }
 
   LpAcc acc;
-  int before = 0;
-  float thr = kNegInf;  // T: columns at or above it are listed
-  for (int bt = 0; bt < nbatch; ++bt) {
-    if (bt + 1 < nbatch) load(bt + 1, y);
-    float v[kLpBatch];
-    float bm = kNegInf;
+  for (int v = v0 + tid; v < v1; v += NV * NT) {
+    if (v + NV * NT < v1) load(v + NV * NT, y);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int col = cu + ((bt * NV + i) * kLpThreads + tid) * N;
-      const bool full = col >= lo && col + N <= hi;
+    for (int i0 = 0; i0 < NV; i0 += SUB) {
+      float e[SUB * N];
+      float bm = kNegInf;
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        float e = fmaxf(x[i].get(j), kNegInf);
-        if (!full && !(col + j >= lo && col + j < hi)) e = kNegInf;
-        v[i * N + j] = e;
-        bm = fmaxf(bm, e);
-      }
-      if (id >= 0) {
-        if (full && col > id) {
+      for (int i = i0; i < i0 + SUB; ++i) {
+        const int col = head + (v + i * NT) * N;
+        const float t = col + N <= id ? t_before : t_after;
 #pragma unroll
-          for (int j = 0; j < N; ++j) before += v[i * N + j] > chosen;
-        } else if (full && col + N <= id) {
-#pragma unroll
-          for (int j = 0; j < N; ++j) before += v[i * N + j] >= chosen;
-        } else {
-          for (int j = 0; j < N; ++j)
-            if (col + j >= lo && col + j < hi)
-              before += v[i * N + j] > chosen || (v[i * N + j] == chosen && col + j < id);
+        for (int j = 0; j < N; ++j) {
+          const float w = x[i].get(j);
+          e[(i - i0) * N + j] = w;
+          bm = fmaxf(bm, w);
+          before += w >= t;
         }
-      }
-    }
-    acc.add(v, bm, c);
-    if (TOP) {
-      if (bt == 0) {
-        // Every warp offers the q-th largest of its lanes' maxima: at least
-        // q * kLpWarps >= top columns reach the lowest offer.  From there the
-        // bound is raised, by halving, while `top` maxima still reach it.
-        const int q = (top + kLpWarps - 1) / kLpWarps;
-        uint32_t o = ord32(bm + 0.0f);
-        const uint32_t mine = o;
-        uint32_t w = __reduce_max_sync(0xffffffffu, o);
-        if (q > 1) {
-          const unsigned at = __ballot_sync(0xffffffffu, o == w);
-          if (lane == __ffs(at) - 1) o = 0;
-          w = __reduce_max_sync(0xffffffffu, o);
-        }
-        if (lane == 0) offer[warp] = w;
-        __syncthreads();
-        const uint32_t least = ord32(-3.402823466e38f);  // a column at -inf is never listed
-        uint32_t low = offer[0], high = offer[0];
-        for (int i = 1; i < kLpWarps; ++i) {
-          low = min(low, offer[i]);
-          high = max(high, offer[i]);
-        }
-        low = max(low, least);
-        for (int it = 0; it < 12 && low < high; ++it) {
-          const uint32_t mid = low + (high - low + 1) / 2;
-          const int n = __syncthreads_count(mine >= mid);
-          if (n >= top) {
-            low = mid;
-            if (n <= 2 * top) break;
-          } else {
-            high = mid - 1;
+        if (col < id && id < col + N && v + i * NT < v1) {  // the chosen one's own vector: t_after does not count what is before it
+          for (int j = 0; j < id - col; ++j) {
+            const float w = to_float(in[col + j]);
+            before += chosen > kNegInf ? w == chosen : -(w >= t_after);
           }
         }
-        thr = unord32(low);
       }
-      if (bm >= thr) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-          for (int j = 0; j < N; ++j)
-            if (v[i * N + j] >= thr) {
-              const int p = atomicAdd(&count, 1);
-              if (p < kLpCap)
-                list[p] = dkey(v[i * N + j], cu + ((bt * NV + i) * kLpThreads + tid) * N + j);
-            }
-      }
+      acc.add(e, bm, c);
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) x[i] = y[i];
+  }
+  if (edge >= 0) {
+    const float e[1] = {edge_value};
+    before += edge < id ? edge_value >= t_before : edge_value >= t_after;
+    acc.add(e, edge_value, c);
   }
 
   // the CTA's part of the row
@@ -488,16 +528,62 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprob_kernel(const LogprobArg
   p.ninf = __reduce_add_sync(0xffffffffu, acc.ninf);
   p.ntop = 0;
   if (lane == 0) parts[warp] = p;
-  __syncthreads();
 
   int ntop = 0;
   if (TOP) {
+    // Every warp offers the q-th largest of its maxima: q * kLpWarps >= top
+    // maxima reach the lowest offer.  From there the bound is raised by halving
+    // while `top` maxima still reach it.
+    const uint32_t mine = ord32(acc.m + 0.0f);
+    uint32_t o = mine;
+    uint32_t w = __reduce_max_sync(0xffffffffu, o);
+    if (top > kLpWarps) {
+      const unsigned at = __ballot_sync(0xffffffffu, o == w);
+      if (lane == __ffs(at) - 1) o = 0;
+      w = __reduce_max_sync(0xffffffffu, o);
+    }
+    if (lane == 0) offer[warp] = w;
+    __syncthreads();
+    const uint32_t least = ord32(kLowest);  // a column at -inf is never listed
+    uint32_t low = offer[lane % kLpWarps];
+    uint32_t high = ord32(parts[lane % kLpWarps].m);
+    low = max(__reduce_min_sync(0xffffffffu, low), least);
+    high = __reduce_max_sync(0xffffffffu, high);
+    for (int it = 0; it < 16 && low < high; ++it) {
+      const uint32_t mid = low + (high - low + 1) / 2;
+      const int n = __syncthreads_count(mine >= mid);
+      if (n >= top) {
+        low = mid;
+        if (n <= top + 4) break;
+      } else {
+        high = mid - 1;
+      }
+    }
+    const float thr = unord32(low);
+    if (mine >= low) hits[atomicAdd(&nhits, 1)] = static_cast<unsigned short>(tid);
+    if (edge_value >= thr) list[atomicAdd(&count, 1)] = dkey(edge_value, edge);
+    __syncthreads();
+    const int per = (v1 - v0 + NT - 1) / NT;  // vectors of a thread
+    for (int i = tid; i < nhits * per; i += NT) {
+      const int h = i / per;
+      const int v = v0 + (i - h * per) * NT + hits[h];
+      if (v >= v1) continue;
+      Vec<T> r;
+      r.raw = *reinterpret_cast<const uint4*>(vin + static_cast<long long>(v) * N);
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (r.get(j) >= thr) {
+          const int at = atomicAdd(&count, 1);
+          if (at < kLpCap) list[at] = dkey(r.get(j), head + v * N + j);
+        }
+    }
+    __syncthreads();
     int n = count;
     // Too many: the `top`-th of those that were kept is a bound that as many
     // columns reach; gather again from it on, in the order of the keys (distinct,
     // so at least kLpCap - top columns drop out each time).
     while (n > kLpCap) {
-      for (int i = tid; i < kLpCap; i += kLpThreads) {
+      for (int i = tid; i < kLpCap; i += NT) {
         int r = 0;
         const uint64_t k = list[i];
         for (int j = 0; j < kLpCap; ++j) r += list[j] < k;
@@ -507,7 +593,8 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprob_kernel(const LogprobArg
       const uint64_t bk = bound_key;
       if (tid == 0) count = 0;
       __syncthreads();
-      for (int col = lo + tid; col < hi; col += kLpThreads) {
+      const int lo = rankc == 0 ? 0 : head + v0 * N, hi = rankc == C - 1 ? a.vocab : head + v1 * N;
+      for (int col = lo + tid; col < hi; col += NT) {
         const float e = fmaxf(to_float(in[col]), kNegInf);
         const uint64_t k = dkey(e, col);
         if (e > kNegInf && k <= bk) {
@@ -520,14 +607,14 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprob_kernel(const LogprobArg
       __syncthreads();
     }
     ntop = min(n, top);
-    for (int i = tid; i < n; i += kLpThreads) {
+    for (int i = tid; i < n; i += NT) {
       int r = 0;
       const uint64_t k = list[i];
       for (int j = 0; j < n; ++j) r += list[j] < k;
       if (r < top) best[r] = k;
     }
-    __syncthreads();
   }
+  __syncthreads();
 
   LpPart mine;
   if (warp == 0) {
@@ -577,7 +664,7 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprob_kernel(const LogprobArg
   }
   if (TOP) {
     // a key's place: its own in its list, and what comes before it in the others
-    for (int i = tid; i < C * top; i += kLpThreads) {
+    for (int i = tid; i < C * top; i += NT) {
       const int l = i / top, at = i - l * top;
       if (at >= slots[l].ntop) continue;
       const uint64_t k = slot_keys[l * kLpMaxTop + at];
@@ -601,7 +688,7 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprob_kernel(const LogprobArg
     }
     int have = 0;
     for (int i = 0; i < C; ++i) have += slots[i].ntop;
-    for (int i = have + tid; i < top; i += kLpThreads) {
+    for (int i = have + tid; i < top; i += NT) {
       a.top_ids[static_cast<long long>(row) * top + i] = -1;
       a.top_logprobs[static_cast<long long>(row) * top + i] = kNegInf;
     }
@@ -611,13 +698,11 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprob_kernel(const LogprobArg
 template <class T>
 cudaError_t run_logprobs(LogprobArgs a, cudaStream_t s) {
   constexpr int N = Vec<T>::N;
-  // enough CTAs for the SMs, in slices of a batch (8192 columns) or more
+  // enough CTAs for the SMs, in slices of a batch or more
   int C = 1;
-  while (C < kLpMaxCluster && static_cast<long long>(C) * kLpThreads * kLpBatch < a.vocab &&
+  while (C < kLpMaxCluster && static_cast<long long>(C) * kLpThreads * kLpVecs * N < a.vocab &&
          static_cast<long long>(a.rows) * C < 148 * 4)
     C <<= 1;
-  const long long span = static_cast<long long>(a.vocab) + N - 1;
-  a.slice = static_cast<int>(((span + C - 1) / C + N - 1) / N * N);
   const long long grid = static_cast<long long>(a.rows) * C;
   if (grid > INT_MAX) return cudaErrorInvalidConfiguration;
   return a.top > 0 ? launch_chained(logprob_kernel<T, true>, static_cast<unsigned>(grid), kLpThreads, 0, C, s, a)
@@ -627,9 +712,9 @@ cudaError_t run_logprobs(LogprobArgs a, cudaStream_t s) {
 }  // namespace
 
 cudaError_t launch_process(ProcArgs a, int dtype, bool in_place, cudaStream_t s) {
-  if (dtype == kOpsF16) return pick_process<__half, false>(a, s);
-  if (dtype == kOpsBF16) return pick_process<__nv_bfloat16, false>(a, s);
-  return in_place ? pick_process<float, true>(a, s) : pick_process<float, false>(a, s);
+  if (dtype == kOpsF16) return run_process<__half, false>(a, s);
+  if (dtype == kOpsBF16) return run_process<__nv_bfloat16, false>(a, s);
+  return in_place ? run_process<float, true>(a, s) : run_process<float, false>(a, s);
 }
 
 cudaError_t launch_logprobs(LogprobArgs a, int dtype, cudaStream_t s) {

@@ -68,8 +68,10 @@ def _ops():
 
 
 def _rows(t, types, what):
-    """(rows, columns, row stride, type code) of a CUDA matrix with contiguous rows."""
-    if not t.is_cuda:
+    """(rows, columns, row stride, type code, device index) of a CUDA matrix with
+    contiguous rows."""
+    index = t.get_device()
+    if index < 0:
         raise VerboCudaError(f"{what} must be a CUDA tensor")
     code = types.get(t.dtype)
     if code is None:
@@ -80,14 +82,14 @@ def _rows(t, types, what):
     ld, step = t.stride()
     if step != 1 and cols > 1:
         raise VerboCudaError(f"{what}: rows must be contiguous (stride(1) == 1)")
-    return rows, cols, (ld if rows > 1 else max(cols, 1)), code
+    return rows, cols, (ld if rows > 1 else max(cols, 1)), code, index
 
 
-def _list(t, dtype, like, what, size=None):
-    """Device address of a contiguous CUDA tensor of one type on `like`'s device, or None."""
+def _list(t, dtype, index, what, size=None):
+    """Device address of a contiguous CUDA tensor of one type on a device, or None."""
     if t is None:
         return None
-    if not t.is_cuda or t.device != like.device:
+    if t.get_device() != index:
         raise VerboCudaError(f"{what} must be a CUDA tensor on the device of the rows")
     if t.dtype != dtype:
         raise VerboCudaError(f"{what} must be {str(dtype)[6:]}")
@@ -98,42 +100,39 @@ def _list(t, dtype, like, what, size=None):
     return t.data_ptr()
 
 
-class _On:
-    """Makes a device current while a call is made."""
-
-    __slots__ = ("torch", "device", "before")
-
-    def __init__(self, torch, device):
-        self.torch, self.device = torch, device.index
-
-    def __enter__(self):
-        self.before = self.torch.cuda.current_device()
-        if self.before != self.device:
-            self.torch.cuda.set_device(self.device)
-
-    def __exit__(self, *exc):
-        if self.before != self.device:
-            self.torch.cuda.set_device(self.before)
+def _call(fn, torch, index, *args):
+    """One library call with the device current (the calls on rows take the
+    current device's)."""
+    before = torch.cuda.current_device()
+    if before == index:
+        rc = fn(*args)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args)
+    if rc < 0:
+        raise _err()
 
 
-def _stream_of(torch, device, stream):
-    """The address of the call's stream (the current one of `device` if None)."""
+def _stream_of(torch, index, stream):
+    """The address of the call's stream (the device's current one if None)."""
     if stream is None:
-        return torch.cuda.current_stream(device).cuda_stream
+        return torch._C._cuda_getCurrentRawStream(index)
     at = getattr(stream, "device", None)
-    if at is not None and at != device:
+    if at is not None and at.index != index:
         raise VerboCudaError("stream must be one of the rows' device")
     return getattr(stream, "cuda_stream", stream)
 
 
-def _new(torch, device, stream, *sizes_and_types):
-    """New tensors that belong to the call's stream."""
-    if stream is None:
-        return [torch.empty(s, dtype=t, device=device) for s, t in sizes_and_types]
-    if not isinstance(stream, torch.cuda.Stream):
-        stream = torch.cuda.ExternalStream(stream, device=device)
-    with torch.cuda.stream(stream):
-        return [torch.empty(s, dtype=t, device=device) for s, t in sizes_and_types]
+def _new(torch, like, stream, rows, cols, dtype):
+    """A new matrix (or vector: cols None) that belongs to the call's stream."""
+    if stream is not None:
+        if not isinstance(stream, torch.cuda.Stream):
+            stream = torch.cuda.ExternalStream(stream, device=like.device)
+        with torch.cuda.stream(stream):
+            return _new(torch, like, None, rows, cols, dtype)
+    if cols is None:
+        return torch.empty(rows, dtype=dtype, device=like.device)
+    return torch.empty(rows, cols, dtype=dtype, device=like.device)
 
 
 def process_logits(logits, penalties=None, hist=None, hist_off=None, row_penalties=None, bias_ids=None, bias=None,
@@ -155,54 +154,56 @@ def process_logits(logits, penalties=None, hist=None, hist_off=None, row_penalti
     ``logits`` itself (float32): then only the columns that change are touched.
     Pass them to ``sample`` or ``Batch.step`` with repeat = 1."""
     lib, torch, types = _ops()
-    rows, cols, ld, code = _rows(logits, types, "logits")
+    rows, cols, ld, code, dev = _rows(logits, types, "logits")
     if vocab is None:
         vocab = cols
     elif not 0 < vocab <= cols:
         raise VerboCudaError("vocab must be in [1, columns of logits]")
-    at = _stream_of(torch, logits.device, stream)
+    at = _stream_of(torch, dev, stream)
     if out is None:
-        (out,) = _new(torch, logits.device, stream, ((rows, vocab), torch.float32))
+        out = _new(torch, logits, stream, rows, vocab, torch.float32)
         ld_out = vocab
+    elif out is logits and code == 0:
+        ld_out = ld
     else:
-        orows, ocols, ld_out, ocode = _rows(out, types, "out")
-        if ocode != 0 or orows != rows or ocols < vocab or out.device != logits.device:
+        orows, ocols, ld_out, ocode, odev = _rows(out, types, "out")
+        if ocode != 0 or orows != rows or ocols < vocab or odev != dev:
             raise VerboCudaError("out must be float32 with one row per row of logits, on their device")
-    ld_mask = 0
-    mp = None
+    mp, ld_mask = None, 0
     if mask is not None:
         if mask.dim() != 2 or mask.shape[0] not in (1, rows) or mask.shape[1] * 32 < vocab:
             raise VerboCudaError("mask must be [rows or 1, at least ceil(vocab / 32)]")
-        if not mask.is_cuda or mask.device != logits.device or mask.dtype != torch.int32:
+        if mask.get_device() != dev or mask.dtype != torch.int32:
             raise VerboCudaError("mask must be an int32 CUDA tensor on the device of the rows")
         if mask.shape[1] > 1 and mask.stride(1) != 1:
             raise VerboCudaError("mask: rows must be contiguous (stride(1) == 1)")
         mp = mask.data_ptr()
         if mask.shape[0] > 1:
             ld_mask = mask.stride(0)
-    if (bias_ids is None) != (bias is None) or (bias is None) != (bias_off is None):
-        raise VerboCudaError("bias_ids, bias and bias_off must all be given or all be None")
-    if bias is not None and bias_ids.numel() != bias.numel():
-        raise VerboCudaError("bias_ids and bias must have the same length")
-    if (hist is None) != (hist_off is None):
-        raise VerboCudaError("hist and hist_off must both be given or both be None")
-    if hist is not None and hist.numel() == 0:
-        hist = hist_off = None
-    if bias is not None and bias.numel() == 0:
-        bias_ids = bias = bias_off = None
-    i32, i64, f32 = torch.int32, torch.int64, torch.float32
-    pen = None
+    hp = op = rp = bi = bv = bo = pen = None
+    if hist is not None or hist_off is not None:
+        if hist is None or hist_off is None:
+            raise VerboCudaError("hist and hist_off must both be given or both be None")
+        hp = _list(hist, torch.int32, dev, "hist")
+        op = _list(hist_off, torch.int64, dev, "hist_off", rows + 1)
+        if hist.numel() == 0:
+            hp = op = None
+    if bias is not None or bias_ids is not None or bias_off is not None:
+        if bias is None or bias_ids is None or bias_off is None:
+            raise VerboCudaError("bias_ids, bias and bias_off must all be given or all be None")
+        bv = _list(bias, torch.float32, dev, "bias")
+        bi = _list(bias_ids, torch.int32, dev, "bias_ids", bias.numel())
+        bo = _list(bias_off, torch.int64, dev, "bias_off", rows + 1)
+        if bias.numel() == 0:
+            bi = bv = bo = None
     if penalties is not None:
-        pen = ctypes.byref(penalties._c())
-    elif row_penalties is not None:
-        pen = ctypes.byref(_Penalties(1.0, 0.0, 0.0, 0))
-    args = (logits.data_ptr(), code, rows, vocab, ld, pen, _list(row_penalties, f32, logits, "row_penalties", 3 * rows),
-            _list(hist, i32, logits, "hist"), _list(hist_off, i64, logits, "hist_off", rows + 1),
-            _list(bias_ids, i32, logits, "bias_ids"), _list(bias, f32, logits, "bias"),
-            _list(bias_off, i64, logits, "bias_off", rows + 1), mp, ld_mask, out.data_ptr(), ld_out, at)
-    with _On(torch, logits.device):
-        if lib.verbo_ops_process_logits(*args) < 0:
-            raise _err()
+        pen = penalties._c()
+    if row_penalties is not None:
+        rp = _list(row_penalties, torch.float32, dev, "row_penalties", 3 * rows)
+        if pen is None:
+            pen = _Penalties(1.0, 0.0, 0.0, 0)
+    _call(lib.verbo_ops_process_logits, torch, dev, logits.data_ptr(), code, rows, vocab, ld,
+          None if pen is None else ctypes.byref(pen), rp, hp, op, bi, bv, bo, mp, ld_mask, out.data_ptr(), ld_out, at)
     return out
 
 
@@ -218,25 +219,24 @@ def token_logprobs(logits, ids=None, top=0, temp=1.0, vocab=None, stream=None):
     ``top`` <= 32 columns of that order, (-1, -inf) where fewer have a
     probability.  A NaN counts as -inf."""
     lib, torch, types = _ops()
-    rows, cols, ld, code = _rows(logits, types, "logits")
+    rows, cols, ld, code, dev = _rows(logits, types, "logits")
     if vocab is None:
         vocab = cols
     elif not 0 < vocab <= cols:
         raise VerboCudaError("vocab must be in [1, columns of logits]")
-    dev = logits.device
     at = _stream_of(torch, dev, stream)
-    n = max(int(top), 0)
+    top = int(top)
+    n = max(top, 0)
     f32, i32 = torch.float32, torch.int32
-    tid, tlp = _new(torch, dev, stream, ((rows, n), i32), ((rows, n), f32))
-    lp = rank = None
-    if ids is not None:
-        lp, rank = _new(torch, dev, stream, ((rows,), f32), ((rows,), i32))
-    args = (logits.data_ptr(), code, rows, vocab, ld, temp, _list(ids, torch.int32, logits, "ids", rows),
-            None if lp is None else lp.data_ptr(), None if rank is None else rank.data_ptr(), int(top), tid.data_ptr(),
-            tlp.data_ptr(), at)
-    with _On(torch, dev):
-        if lib.verbo_ops_token_logprobs(*args) < 0:
-            raise _err()
+    tid, tlp = _new(torch, logits, stream, rows, n, i32), _new(torch, logits, stream, rows, n, f32)
+    if ids is None:
+        lp = rank = ip = lpp = rp = None
+    else:
+        ip = _list(ids, i32, dev, "ids", rows)
+        lp, rank = _new(torch, logits, stream, rows, None, f32), _new(torch, logits, stream, rows, None, i32)
+        lpp, rp = lp.data_ptr(), rank.data_ptr()
+    _call(lib.verbo_ops_token_logprobs, torch, dev, logits.data_ptr(), code, rows, vocab, ld, temp, ip, lpp, rp, top,
+          tid.data_ptr(), tlp.data_ptr(), at)
     return lp, rank, tid, tlp
 
 
@@ -309,19 +309,21 @@ class Q4Linear:
         torch = self._torch
         if self._h is None:
             raise VerboCudaError("the layer is closed")
-        n, cols, ldx, xt = _rows(x, self._types, "x")
-        if cols != self.ins or x.device != self.device:
+        n, cols, ldx, xt, dev = _rows(x, self._types, "x")
+        if cols != self.ins or dev != self.device.index:
             raise VerboCudaError(f"x must be [n, {self.ins}] on {self.device}")
-        at = _stream_of(torch, self.device, stream)
+        at = _stream_of(torch, dev, stream)
         if out is None:
-            yt = xt if dtype is None else self._types.get(dtype)
+            if dtype is None:
+                dtype = x.dtype
+            yt = self._types.get(dtype)
             if yt is None:
                 raise VerboCudaError("dtype must be float32, float16 or bfloat16")
-            (out,) = _new(torch, self.device, stream, ((n, self.outs), x.dtype if dtype is None else dtype))
+            out = _new(torch, x, stream, n, self.outs, dtype)
             ldy = self.outs
         else:
-            rows, ocols, ldy, yt = _rows(out, self._types, "out")
-            if rows != n or ocols != self.outs or out.device != self.device or (dtype is not None and dtype != out.dtype):
+            rows, ocols, ldy, yt, odev = _rows(out, self._types, "out")
+            if rows != n or ocols != self.outs or odev != dev or (dtype is not None and dtype != out.dtype):
                 raise VerboCudaError(f"out must be [n, {self.outs}] on {self.device}")
         if self._lib.verbo_ops_q4_matvec(self._h, x.data_ptr(), xt, n, ldx, out.data_ptr(), yt, ldy, at) < 0:
             raise _err()
