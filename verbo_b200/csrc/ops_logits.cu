@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "device.cuh"
 #include "ops.cuh"
@@ -331,16 +332,23 @@ cudaError_t run_process(ProcArgs a, cudaStream_t s) {
 // multiplied back.
 // The rank counts the columns v >= t, t the chosen value for columns before the
 // chosen one and the next larger float for those after it.
-// The first columns cost the pass nothing: of the threads' maxima, which it has
+// The first columns cost the pass little: of the threads' maxima, which it has
 // anyway, a bound T is taken that `top` of them reach, so that `top` columns do;
 // T is close to the `top`-th column itself, since two of the first columns
-// seldom meet in one thread.  The few threads whose maximum reaches T have their
-// columns read again (L2), and what reaches T is listed and ranked by counting.
-// A list that overflows (ties) is gathered anew with a sharper bound.
+// seldom meet in one thread.  The few batches whose maximum reaches T (kept in
+// shared memory) are read again, from L2, and what reaches T is listed and
+// ranked by counting.  A list that overflows (ties) is gathered anew with a
+// sharper bound.
+// Each thread copies its own vectors to shared memory (cp.async), two batches
+// ahead, and reads them back itself: no registers for what is in flight and no
+// barrier in the pass.
 constexpr int kLpThreads = 512;
 constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kLpVecs = 4;    // vectors per thread and batch
-constexpr int kLpCap = 2048;  // listed columns per CTA
+constexpr int kLpStages = 2;  // batches in flight
+constexpr int kLpGroups = 8;  // batches whose maxima are kept (the last: of all that follow)
+constexpr int kLpCap = 1024;  // listed columns per CTA
+constexpr int kLpOffers = 4;  // maxima a warp offers at most
 constexpr int kLpMaxCluster = 8;
 constexpr float kLowest = -3.402823466e38f;
 
@@ -362,37 +370,135 @@ __device__ __forceinline__ float lp_scaled(float s, float from, float m, float c
   return s > 0.0f && m != -kNegInf ? s * ex2((from - m) * c) : 0.0f;
 }
 
+// A value in T's own bits: the chosen column's, canonical (NaN as -inf, -0 as
+// 0), and the next larger value (of +inf: a NaN, which nothing reaches).
+template <class T>
+struct Bits;
+template <>
+struct Bits<float> {
+  using U = uint32_t;
+  static constexpr U kSign = 0x80000000u, kInf = 0x7f800000u, kNan = 0x7fffffffu;
+};
+template <>
+struct Bits<__half> {
+  using U = uint16_t;
+  static constexpr U kSign = 0x8000u, kInf = 0x7c00u, kNan = 0x7fffu;
+};
+template <>
+struct Bits<__nv_bfloat16> {
+  using U = uint16_t;
+  static constexpr U kSign = 0x8000u, kInf = 0x7f80u, kNan = 0x7fffu;
+};
+template <class T>
+__device__ __forceinline__ typename Bits<T>::U canon_bits(typename Bits<T>::U u) {
+  using B = Bits<T>;
+  if ((u & ~B::kSign) > B::kInf) return B::kSign | B::kInf;
+  return u == B::kSign ? 0 : u;
+}
+template <class T>
+__device__ __forceinline__ typename Bits<T>::U next_up(typename Bits<T>::U u) {
+  return u & Bits<T>::kSign ? u - 1 : u + 1;
+}
+
+// NV vectors of one thread.
+template <class T, int NV>
+struct LpBatch {
+  static constexpr int N = Vec<T>::N;
+  Vec<T> x[NV];
+  __device__ __forceinline__ const uint32_t& word(int i) const {  // i in [0, 4 NV)
+    const uint4& r = x[i >> 2].raw;
+    return (i & 3) == 0 ? r.x : (i & 3) == 1 ? r.y : (i & 3) == 2 ? r.z : r.w;
+  }
+  __device__ __forceinline__ float max() const {  // NaNs left out
+    if constexpr (sizeof(T) == 4) {
+      float m = kNegInf;
+#pragma unroll
+      for (int i = 0; i < 4 * NV; ++i) m = fmaxf(m, __uint_as_float(word(i)));
+      return m;
+    } else if constexpr (std::is_same_v<T, __half>) {
+      uint32_t m = 0xfc00fc00u;
+#pragma unroll
+      for (int i = 0; i < 4 * NV; ++i) asm("max.f16x2 %0, %0, %1;" : "+r"(m) : "r"(word(i)));
+      const __half2 h = *reinterpret_cast<const __half2*>(&m);
+      return fmaxf(__low2float(h), __high2float(h));
+    } else {
+      uint32_t m = 0xff80ff80u;
+#pragma unroll
+      for (int i = 0; i < 4 * NV; ++i) asm("max.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(word(i)));
+      return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
+    }
+  }
+  // how many of vector i's values reach the value of bits u
+  template <int I0, int I1>
+  __device__ __forceinline__ int reach(typename Bits<T>::U u) const {
+    if constexpr (sizeof(T) == 4) {
+      int n = 0;
+#pragma unroll
+      for (int i = 4 * I0; i < 4 * I1; ++i) n += __uint_as_float(word(i)) >= __uint_as_float(u);
+      return n;
+    } else if constexpr (std::is_same_v<T, __half>) {
+      const uint32_t t = u | static_cast<uint32_t>(u) << 16;
+      __half2 n = __floats2half2_rn(0.0f, 0.0f);  // counts up to 4 NV: exact
+#pragma unroll
+      for (int i = 4 * I0; i < 4 * I1; ++i)
+        n = __hadd2(n, __hge2(*reinterpret_cast<const __half2*>(&word(i)), *reinterpret_cast<const __half2*>(&t)));
+      return static_cast<int>(__low2float(n) + __high2float(n));
+    } else {
+      const uint32_t t = u | static_cast<uint32_t>(u) << 16;
+      __nv_bfloat162 n = __floats2bfloat162_rn(0.0f, 0.0f);
+#pragma unroll
+      for (int i = 4 * I0; i < 4 * I1; ++i)
+        n = __hadd2(n, __hge2(*reinterpret_cast<const __nv_bfloat162*>(&word(i)),
+                              *reinterpret_cast<const __nv_bfloat162*>(&t)));
+      return static_cast<int>(__low2float(n) + __high2float(n));
+    }
+  }
+  template <class F>
+  __device__ __forceinline__ void each(F&& f) const {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < N; ++j) f(x[i].get(j), j);
+  }
+};
+
 struct LpAcc {
   float m = kNegInf, s = 0.0f;
   int ninf = 0;
-  // bm: the maximum of x[0, n), which may hold NaNs (they count as -inf)
-  template <int n>
-  __device__ __forceinline__ void add(const float (&x)[n], float bm, float c) {
-    if (bm == -kNegInf) {  // +inf alone counts then
-#pragma unroll
-      for (int j = 0; j < n; ++j) ninf += x[j] == -kNegInf;
-      m = bm;
-    }
-    if (m == -kNegInf) return;
+  // bm: the maximum of the batch b, which may hold NaNs (they count as -inf)
+  template <class B>
+  __device__ __forceinline__ void add(const B& b, float bm, float c) {
     if (bm > m) {
       s = lp_scaled(s, m, bm, c);
       m = bm;
     }
-    if (m == kNegInf) return;
-    float t = 0.0f;
     if (fabsf(m) < 1e30f) {
-      const float b = -m * c;
-#pragma unroll
-      for (int j = 0; j < n; ++j) t += ex2(fmaf(x[j], c, b));
-      t *= ex2(fmaf(-m, c, -b));
+      const float o = -m * c;
+      float t[2] = {0.0f, 0.0f};
+      b.each([&](float v, int j) { t[j & 1] += ex2(fmaf(v, c, o)); });
+      t[0] = (t[0] + t[1]) * ex2(fmaf(-m, c, -o));
+      if (t[0] == t[0]) {
+        s += t[0];
+        return;
+      }
     }
-    // c m may overflow (rows masked with the type's lowest value), or a NaN was met
-    if (!(fabsf(m) < 1e30f && t == t)) {
-      t = 0.0f;
-#pragma unroll
-      for (int j = 0; j < n; ++j) t += ex2((fmaxf(x[j], kNegInf) - m) * c);
+    // rare: a NaN was met, or infinities, or c m may overflow (rows masked with
+    // the type's lowest value)
+    if (m == kNegInf) return;
+    if (m == -kNegInf) {  // +inf alone counts then
+      b.each([&](float v, int) { ninf += v == -kNegInf; });
+      return;
     }
+    float t = 0.0f;
+    b.each([&](float v, int) { t += ex2((fmaxf(v, kNegInf) - m) * c); });
     s += t;
+  }
+};
+struct LpOne {  // a single column
+  float v;
+  template <class F>
+  __device__ __forceinline__ void each(F&& f) const {
+    f(v, 0);
   }
 };
 
@@ -413,16 +519,18 @@ __device__ __forceinline__ uint4 all_neg_inf<__nv_bfloat16>() {
 
 template <class T, bool TOP>
 __global__ void __launch_bounds__(kLpThreads, 2) logprob_kernel(const LogprobArgs a) {
-  constexpr int N = Vec<T>::N, NV = kLpVecs, NT = kLpThreads;
-  constexpr int SUB = 16 / N;  // vectors whose terms are summed together
+  constexpr int N = Vec<T>::N, NT = kLpThreads, NV = kLpVecs;
+  extern __shared__ __align__(16) uint4 ring[];  // [kLpStages][NV][NT]
   __shared__ LpPart parts[kLpWarps];
   __shared__ LpPart slots[kLpMaxCluster];  // the leader's: one per CTA
   __shared__ uint64_t slot_keys[TOP ? kLpMaxCluster * kLpMaxTop : 1];
   __shared__ uint64_t list[TOP ? kLpCap : 1];
   __shared__ uint64_t best[TOP ? kLpMaxTop : 1];
-  __shared__ unsigned short hits[TOP ? NT : 1];
-  __shared__ uint32_t offer[kLpWarps];
+  __shared__ float group_max[TOP ? kLpGroups * NT : 1];
+  __shared__ unsigned short hits[TOP ? kLpGroups * NT : 1];  // group * NT + thread
+  __shared__ __align__(16) uint32_t offer[kLpWarps * kLpOffers];
   __shared__ int count, nhits;
+  __shared__ uint32_t bound;
   __shared__ uint64_t bound_key;
 
   cg::cluster_group cl = cg::this_cluster();
@@ -456,66 +564,90 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprob_kernel(const LogprobArg
     count = 0;
     nhits = 0;
   }
-  Vec<T> x[NV], y[NV];
-  auto load = [&](int v, Vec<T>(&to)[NV]) {
+  const int nfull = (v1 - v0) / (NV * NT), rest = v1 - v0 - nfull * (NV * NT);
+  const int nbatch = nfull + (rest > 0 ? 1 : 0);
+  const T* next = vin + static_cast<long long>(v0 + tid) * N;  // of the batch to be copied next
+  auto fetch = [&](int b) {
+    uint4* to = ring + (b % kLpStages) * (NV * NT) + tid;
+    if (b < nfull) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if (v + i * NT < v1)
-        to[i].raw = ld_stream16(vin + static_cast<long long>(v + i * NT) * N);
-      else
-        to[i].raw = all_neg_inf<T>();
+      for (int i = 0; i < NV; ++i) cp_async16(to + i * NT, next + i * NT * N);
+    } else if (b < nbatch) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (tid + i * NT < rest) cp_async16(to + i * NT, next + i * NT * N);
     }
+    next += NV * NT * N;
+    cp_async_commit();  // an empty group keeps the count
   };
-  load(v0 + tid, x);
+#pragma unroll
+  for (int b = 0; b < kLpStages; ++b) fetch(b);
   const float edge_value = edge >= 0 ? fmaxf(to_float(in[edge]), kNegInf) : kNegInf;
-  // thresholds of the rank; nothing reaches a NaN
-  const float nan = __uint_as_float(0x7fffffffu);
-  float chosen = kNegInf, t_before = nan, t_after = nan;
+  // thresholds of the rank
+  using U = typename Bits<T>::U;
+  float chosen = kNegInf;
+  U t_before = Bits<T>::kNan, t_after = Bits<T>::kNan;
   int before = 0;
   if (id >= 0) {
-    chosen = fmaxf(to_float(in[id]), kNegInf) + 0.0f;  // a NaN counts as -inf, -0 as 0
-    t_before = chosen;
-    t_after = __uint_as_float(chosen >= 0.0f ? __float_as_uint(chosen) + 1u : __float_as_uint(chosen) - 1u);
+    t_before = canon_bits<T>(reinterpret_cast<const U*>(in)[id]);
+    t_after = next_up<T>(t_before);
+    const U bits = t_before;
+    chosen = to_float(*reinterpret_cast<const T*>(&bits));
     if (chosen == kNegInf) {  // every column before it counts, NaN and -inf among them
-      t_before = nan;
+      t_before = Bits<T>::kNan;
       before = rankc == 0 && tid == 0 ? id : 0;
     }
   }
 
   LpAcc acc;
-  for (int v = v0 + tid; v < v1; v += NV * NT) {
-    if (v + NV * NT < v1) load(v + NV * NT, y);
+  for (int b = 0; b < nbatch; ++b) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kLpStages - 1) : "memory");
+    LpBatch<T, NV> x;
+    const uint4* from = ring + (b % kLpStages) * (NV * NT) + tid;
 #pragma unroll
-    for (int i0 = 0; i0 < NV; i0 += SUB) {
-      float e[SUB * N];
-      float bm = kNegInf;
+    for (int i = 0; i < NV; ++i) x.x[i].raw = from[i * NT];
+    if (b >= nfull) {
 #pragma unroll
-      for (int i = i0; i < i0 + SUB; ++i) {
-        const int col = head + (v + i * NT) * N;
-        const float t = col + N <= id ? t_before : t_after;
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-          const float w = x[i].get(j);
-          e[(i - i0) * N + j] = w;
-          bm = fmaxf(bm, w);
-          before += w >= t;
-        }
-        if (col < id && id < col + N && v + i * NT < v1) {  // the chosen one's own vector: t_after does not count what is before it
+      for (int i = 0; i < NV; ++i)
+        if (tid + i * NT >= rest) x.x[i].raw = all_neg_inf<T>();
+    }
+    fetch(b + kLpStages);
+    const float bm = x.max();
+    const int col0 = head + (v0 + b * (NV * NT)) * N;
+    if (id < col0) {
+      before += x.template reach<0, NV>(t_after);
+    } else if (id >= col0 + NV * NT * N) {
+      before += x.template reach<0, NV>(t_before);
+    } else {  // the batch that holds the chosen one
+      auto vector = [&](auto i) {
+        constexpr int I = decltype(i)::value;
+        const int col = col0 + (I * NT + tid) * N;
+        before += x.template reach<I, I + 1>(col + N <= id ? t_before : t_after);
+        // its vector: t_after does not count what is before it
+        if (col < id && id < col + N && I * NT + tid < v1 - v0 - b * (NV * NT)) {
           for (int j = 0; j < id - col; ++j) {
             const float w = to_float(in[col + j]);
-            before += chosen > kNegInf ? w == chosen : -(w >= t_after);
+            before += chosen > kNegInf ? w == chosen : -(w > kNegInf);
           }
         }
-      }
-      acc.add(e, bm, c);
+      };
+      vector(std::integral_constant<int, 0>{});
+      vector(std::integral_constant<int, 1>{});
+      vector(std::integral_constant<int, 2>{});
+      vector(std::integral_constant<int, 3>{});
+      static_assert(NV == 4, "one call per vector");
     }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) x[i] = y[i];
+    acc.add(x, bm, c);
+    if (TOP) {
+      float* at = &group_max[min(b, kLpGroups - 1) * NT + tid];
+      *at = b < kLpGroups ? bm : fmaxf(*at, bm);
+    }
   }
   if (edge >= 0) {
-    const float e[1] = {edge_value};
-    before += edge < id ? edge_value >= t_before : edge_value >= t_after;
-    acc.add(e, edge_value, c);
+    const U u = canon_bits<T>(reinterpret_cast<const U*>(in)[edge]);
+    const float t = to_float(*reinterpret_cast<const T*>(edge < id ? &t_before : &t_after));
+    before += to_float(*reinterpret_cast<const T*>(&u)) >= t;
+    acc.add(LpOne{edge_value}, edge_value, c);
   }
 
   // the CTA's part of the row
@@ -528,45 +660,62 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprob_kernel(const LogprobArg
   p.ninf = __reduce_add_sync(0xffffffffu, acc.ninf);
   p.ntop = 0;
   if (lane == 0) parts[warp] = p;
+  LpPart sum;  // in warp 0
+  auto total = [&]() {
+    const LpPart w = lane < kLpWarps ? parts[lane] : LpPart{kNegInf, 0.0f, 0, 0, 0};
+    sum.m = unord32(__reduce_max_sync(0xffffffffu, ord32(w.m + 0.0f)));
+    sum.s = lp_scaled(w.s, w.m, sum.m, c);
+#pragma unroll
+    for (int o = kLpWarps / 2; o > 0; o >>= 1) sum.s += __shfl_xor_sync(0xffffffffu, sum.s, o);
+    sum.rank = __reduce_add_sync(0xffffffffu, w.rank);
+    sum.ninf = __reduce_add_sync(0xffffffffu, w.ninf);
+  };
 
   int ntop = 0;
   if (TOP) {
-    // Every warp offers the q-th largest of its maxima: q * kLpWarps >= top
-    // maxima reach the lowest offer.  From there the bound is raised by halving
-    // while `top` maxima still reach it.
+    // Every warp offers its q largest maxima; the `top`-th of all offers is the
+    // bound (q * kLpWarps >= top of them, each of another thread).
     const uint32_t mine = ord32(acc.m + 0.0f);
+    const int q = min(kLpOffers, 2 * ((top + kLpWarps - 1) / kLpWarps));
     uint32_t o = mine;
-    uint32_t w = __reduce_max_sync(0xffffffffu, o);
-    if (top > kLpWarps) {
+    for (int i = 0; i < q; ++i) {
+      const uint32_t w = __reduce_max_sync(0xffffffffu, o);
       const unsigned at = __ballot_sync(0xffffffffu, o == w);
-      if (lane == __ffs(at) - 1) o = 0;
-      w = __reduce_max_sync(0xffffffffu, o);
-    }
-    if (lane == 0) offer[warp] = w;
-    __syncthreads();
-    const uint32_t least = ord32(kLowest);  // a column at -inf is never listed
-    uint32_t low = offer[lane % kLpWarps];
-    uint32_t high = ord32(parts[lane % kLpWarps].m);
-    low = max(__reduce_min_sync(0xffffffffu, low), least);
-    high = __reduce_max_sync(0xffffffffu, high);
-    for (int it = 0; it < 16 && low < high; ++it) {
-      const uint32_t mid = low + (high - low + 1) / 2;
-      const int n = __syncthreads_count(mine >= mid);
-      if (n >= top) {
-        low = mid;
-        if (n <= top + 4) break;
-      } else {
-        high = mid - 1;
+      if (lane == __ffs(at) - 1) {
+        offer[warp * q + i] = w;
+        o = 0;
       }
     }
-    const float thr = unord32(low);
-    if (mine >= low) hits[atomicAdd(&nhits, 1)] = static_cast<unsigned short>(tid);
-    if (edge_value >= thr) list[atomicAdd(&count, 1)] = dkey(edge_value, edge);
     __syncthreads();
-    const int per = (v1 - v0 + NT - 1) / NT;  // vectors of a thread
-    for (int i = tid; i < nhits * per; i += NT) {
-      const int h = i / per;
-      const int v = v0 + (i - h * per) * NT + hits[h];
+    if (warp == 0) total();
+    // the bound: an offer with fewer than `top` above it and `top` at or above it
+    if (tid >= 32 && tid < 32 + q * kLpWarps) {
+      const uint32_t w = offer[tid - 32];
+      int gt = 0, ge = 0;
+#pragma unroll 4
+      for (int j = 0; j < q * kLpWarps; j += 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(offer + j);
+        gt += (v.x > w) + (v.y > w) + (v.z > w) + (v.w > w);
+        ge += (v.x >= w) + (v.y >= w) + (v.z >= w) + (v.w >= w);
+      }
+      if (gt < top && top <= ge) bound = max(w, ord32(kLowest));  // a column at -inf is never listed
+    }
+    __syncthreads();
+    const uint32_t low = bound;
+    const float thr = unord32(low);
+    if (mine >= low) {
+      for (int g = 0; g < min(nbatch, kLpGroups); ++g)
+        if (group_max[g * NT + tid] >= thr) hits[atomicAdd(&nhits, 1)] = static_cast<unsigned short>(g * NT + tid);
+      if (edge_value >= thr) list[atomicAdd(&count, 1)] = dkey(edge_value, edge);
+    }
+    __syncthreads();
+    const int lastn = max(1, nbatch - kLpGroups + 1);  // batches of the last group
+    for (int i = tid; i < nhits * (NV * lastn); i += NT) {
+      const int h = lastn == 1 ? i / NV : i / (NV * lastn);
+      const int k = i - h * (NV * lastn);
+      const int g = hits[h] / NT;
+      if (k >= NV && g < kLpGroups - 1) continue;
+      const int v = v0 + (g * NV + k) * NT + hits[h] % NT;
       if (v >= v1) continue;
       Vec<T> r;
       r.raw = *reinterpret_cast<const uint4*>(vin + static_cast<long long>(v) * N);
@@ -616,25 +765,16 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprob_kernel(const LogprobArg
   }
   __syncthreads();
 
-  LpPart mine;
-  if (warp == 0) {
-    const LpPart w = lane < kLpWarps ? parts[lane] : LpPart{kNegInf, 0.0f, 0, 0, 0};
-    mine.m = unord32(__reduce_max_sync(0xffffffffu, ord32(w.m + 0.0f)));
-    mine.s = lp_scaled(w.s, w.m, mine.m, c);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mine.s += __shfl_xor_sync(0xffffffffu, mine.s, o);
-    mine.rank = __reduce_add_sync(0xffffffffu, w.rank);
-    mine.ninf = __reduce_add_sync(0xffffffffu, w.ninf);
-    mine.ntop = ntop;
-  }
+  if (!TOP && warp == 0) total();
+  sum.ntop = ntop;
   if (C > 1) {
     cluster_wait();
-    if (tid == 0) *cl.map_shared_rank(&slots[rankc], 0) = mine;
+    if (tid == 0) *cl.map_shared_rank(&slots[rankc], 0) = sum;
     if (TOP && tid < ntop) *cl.map_shared_rank(&slot_keys[rankc * kLpMaxTop + tid], 0) = best[tid];
     cluster_sync_all();
     if (rankc != 0) return;
   } else {
-    if (tid == 0) slots[0] = mine;
+    if (tid == 0) slots[0] = sum;
     if (TOP && tid < ntop) slot_keys[tid] = best[tid];
     __syncthreads();
   }
@@ -698,15 +838,17 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprob_kernel(const LogprobArg
 template <class T>
 cudaError_t run_logprobs(LogprobArgs a, cudaStream_t s) {
   constexpr int N = Vec<T>::N;
-  // enough CTAs for the SMs, in slices of a batch or more
+  // CTAs per row: one, or as many as give each SM one, with a batch each.
+  const long long batches = (a.vocab / N + kLpThreads * kLpVecs - 1) / (kLpThreads * kLpVecs);
   int C = 1;
-  while (C < kLpMaxCluster && static_cast<long long>(C) * kLpThreads * kLpVecs * N < a.vocab &&
-         static_cast<long long>(a.rows) * C < 148 * 4)
-    C <<= 1;
+  while (C < kLpMaxCluster && C < batches && static_cast<long long>(a.rows) * C < 148) C <<= 1;
   const long long grid = static_cast<long long>(a.rows) * C;
   if (grid > INT_MAX) return cudaErrorInvalidConfiguration;
-  return a.top > 0 ? launch_chained(logprob_kernel<T, true>, static_cast<unsigned>(grid), kLpThreads, 0, C, s, a)
-                   : launch_chained(logprob_kernel<T, false>, static_cast<unsigned>(grid), kLpThreads, 0, C, s, a);
+  constexpr int smem = kLpStages * kLpVecs * kLpThreads * 16;  // 64 KB
+  const auto kernel = a.top > 0 ? logprob_kernel<T, true> : logprob_kernel<T, false>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  return launch_chained(kernel, static_cast<unsigned>(grid), kLpThreads, smem, C, s, a);
 }
 
 }  // namespace
