@@ -94,8 +94,9 @@ VERBO_CUDA_API int verbo_ops_token_logprobs(const void* logits, int dtype, int r
    y = x W^T + b for a weight matrix of outs x ins in 4 bits with group scales:
      W[o][i] = s[o][g] * (q[o][i] - z[o][g]),  g = i / group
    The activations stay in their own type (the head of verbo_cuda_tail_*
-   quantises them, as the reference does): the products q - z times x are
-   exact, the sums fp32.  The same call gives the same bits; the order of a sum
+   quantises them, as the reference does): fp16 x is taken as it is, bf16 and
+   fp32 x to within 2^-24 of each value (or 2^-39 of its row's largest, for values
+   that much smaller); the products with q - z are exact, the sums fp32.  The same call gives the same bits; the order of a sum
    goes by n, so a row's last bits can differ between batches of other sizes. */
 typedef struct verbo_ops_q4 verbo_ops_q4;
 /* Lays the matrix out on `device` (host or device arrays, read before the
@@ -114,10 +115,16 @@ VERBO_CUDA_API verbo_ops_q4* verbo_ops_q4_new(int outs, int ins, int group, cons
                                               int device, void* stream);
 /* Waits for the device; a captured graph that uses the handle dies with it. */
 VERBO_CUDA_API void verbo_ops_q4_free(verbo_ops_q4* h);
+/* Largest n of a call. */
+#define VERBO_OPS_MAX_ROWS 65535
+/* Bytes of device memory that a call with n rows needs (16-byte aligned, its own
+   until the call's work is done; 0 for a few rows), or -1. */
+VERBO_CUDA_API long long verbo_ops_q4_workspace(const verbo_ops_q4* h, int x_type, int n);
 /* n rows x (row i at x + i*ldx, ins elements of x_type) -> n rows y (row i at
    y + i*ldy, outs elements of y_type), on the handle's device. */
 VERBO_CUDA_API int verbo_ops_q4_matvec(const verbo_ops_q4* h, const void* x, int x_type, int n, long long ldx, void* y,
-                                       int y_type, long long ldy, void* stream);
+                                       int y_type, long long ldy, void* workspace, long long workspace_bytes,
+                                       void* stream);
 
 #ifdef __cplusplus
 }

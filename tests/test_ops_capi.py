@@ -28,7 +28,7 @@ def test_exports_match_header(lib):
     out = subprocess.run(["nm", "-D", "--defined-only", str(build.LIB)], capture_output=True, text=True,
                          check=True).stdout
     assert sorted(ln.split()[-1] for ln in out.splitlines() if ln.split()[-1].startswith("verbo_ops_")) == declared
-    assert len(declared) == 6
+    assert len(declared) == 7
 
 
 def test_header_compiles_as_c(lib, tmp_path):
@@ -159,7 +159,8 @@ def test_q4_new_refusals(lib, kw, msg):
 
 
 def test_q4_null_handle(lib):
-    refused(lib, lib.verbo_ops_q4_matvec(None, 4, 0, 1, 64, 4, 0, 64, None), "NULL")
+    refused(lib, lib.verbo_ops_q4_matvec(None, 4, 0, 1, 64, 4, 0, 64, None, 0, None), "NULL")
+    refused(lib, lib.verbo_ops_q4_workspace(None, 0, 1), "NULL")
     lib.verbo_ops_q4_free(None)
 
 

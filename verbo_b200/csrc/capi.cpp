@@ -23,6 +23,7 @@
 
 #include "capi_guard.hpp"
 #include "kernels.cuh"
+#include "ops.cuh"
 #include "tail.cuh"
 #include "verbo_cuda.h"
 
@@ -431,6 +432,9 @@ VERBO_CUDA_API int verbo_cuda_check(void* stream) {
         cuda_ok(vb::tail_read_status(&tst, true), "tail status");
         if (tst & vb::kErrTailWait) fail("a logits-tail pipeline wait did not complete within the wait limit");
         if (tst) fail("tail device status " + std::to_string(tst));
+        unsigned ost = 0;
+        cuda_ok(vb::ops_read_status(&ost, true), "operator status");
+        if (ost & vb::kErrOpsWait) fail("a copy of a 4-bit product did not complete within the wait limit");
         if (st) fail("device status " + std::to_string(st));
         return 0;
       },

@@ -56,7 +56,8 @@ cudaError_t launch_logprobs(LogprobArgs a, int dtype, cudaStream_t s);
 //   1024 B  nibbles in the order in which the lanes of a warp feed them to
 //           mma.m16n8k16 (ops_q4.cu): two blocks of 32 lanes x 16 B
 //   then    the chunk's fp16 scales, [8 row pairs][sets][row g, row g + 8]
-//   then    its zero points (one byte each, the same order), if there are any
+//   then    its zero points (one byte each, the same order), if there are any,
+//           filled up to a multiple of 32 bytes
 // A set is `span` weights of one row that share a scale: gcd(group, 128).
 // Rows past outs and weights past ins have scale 0.
 constexpr int kQ4Rows = 16;
@@ -68,7 +69,7 @@ struct Q4Mat {
   int span;         // 32, 64 or 128
   int nkc;          // chunks per tile
   int ntile;
-  int chunk_bytes;  // 1024 + sets * 32 (+ sets * 16)
+  int chunk_bytes;
   bool zeros;
   const unsigned char* tiles;
   const float* bias;  // or null
@@ -79,13 +80,19 @@ struct Q4Args {
   int n;
   void* y;
   long long ldy;
+  void* workspace;  // q4_workspace_bytes, 16-byte aligned
 };
 // Fills in span, nkc, ntile, chunk_bytes from outs, ins, group, zeros.
 void q4_layout(Q4Mat& m);
 size_t q4_tiles_bytes(const Q4Mat& m);
+size_t q4_workspace_bytes(const Q4Mat& m, int n, int x_type);
 // Lays device arrays out into `tiles` (m.zeros: whether zeros is given).
 cudaError_t launch_q4_pack(const Q4Mat& m, const unsigned char* q, const uint16_t* s, const unsigned char* zeros,
                            unsigned char* tiles, cudaStream_t st);
 cudaError_t launch_q4(const Q4Mat& m, const Q4Args& a, int x_type, int y_type, cudaStream_t st);
+
+// Device-side failures of the operators (bounded waits that ran out).
+constexpr unsigned kErrOpsWait = 1u;
+cudaError_t ops_read_status(unsigned* st, bool clear);
 
 }  // namespace vb

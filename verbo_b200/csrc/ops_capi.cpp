@@ -62,11 +62,12 @@ void check_rows(const void* p, int type, int rows, int cols, long long ld, const
 
 // Whether two sets of rows can touch the same byte.  Rows of one pitch that
 // lie beside each other in it (two halves of one buffer) do not.
-bool overlap(const void* a, long long pa, long long la, const void* b, long long pb, long long lb, int rows) {
+bool overlap(const void* a, long long pa, long long la, const void* b, long long pb, long long lb, int rows_b,
+             int rows_a) {
   const char *x = static_cast<const char*>(a), *y = static_cast<const char*>(b);
-  const char *xe = x + (rows - 1) * pa + la, *ye = y + (rows - 1) * pb + lb;
+  const char *xe = x + (rows_a - 1) * pa + la, *ye = y + (rows_b - 1) * pb + lb;
   if (xe <= y || ye <= x) return false;
-  if (pa != pb) return true;
+  if (pa != pb || rows_a != rows_b) return true;
   const long long d = ((y - x) % pa + pa) % pa;
   return !(d >= la && d + lb <= pa);
 }
@@ -114,7 +115,7 @@ VERBO_CUDA_API int verbo_ops_process_logits(const void* logits, int dtype, int r
         if (in_place && (dtype != VERBO_OPS_F32 || (ld_out != ld && rows > 1)))
           fail("out may be logits only if they are F32 rows of the same stride");
         const long long size = vb::ops_type_size(dtype);
-        if (!in_place && overlap(logits, ld * size, vocab * size, out, ld_out * 4, vocab * 4ll, rows))
+        if (!in_place && overlap(logits, ld * size, vocab * size, out, ld_out * 4, vocab * 4ll, rows, rows))
           fail("out overlaps logits without being the same rows");
         vb::ProcArgs a{};
         a.logits = logits;
@@ -293,26 +294,49 @@ VERBO_CUDA_API void verbo_ops_q4_free(verbo_ops_q4* h) {
   if (h) q4_release(h);
 }
 
+VERBO_CUDA_API long long verbo_ops_q4_workspace(const verbo_ops_q4* h, int x_type, int n) {
+  return guard(
+      [&]() -> long long {
+        if (!h) fail("q4 handle is NULL");
+        check_type(x_type, "x_type");
+        if (n < 0 || n > VERBO_OPS_MAX_ROWS) fail("n must be in [0, " + std::to_string(VERBO_OPS_MAX_ROWS) + "]");
+        const DeviceScope scope(h->device);
+        return n == 0 ? 0 : static_cast<long long>(vb::q4_workspace_bytes(h->m, n, x_type));
+      },
+      -1);
+}
+
 VERBO_CUDA_API int verbo_ops_q4_matvec(const verbo_ops_q4* h, const void* x, int x_type, int n, long long ldx, void* y,
-                                       int y_type, long long ldy, void* stream) {
+                                       int y_type, long long ldy, void* workspace, long long workspace_bytes,
+                                       void* stream) {
   return guard(
       [&]() {
         if (!h) fail("q4 handle is NULL");
         check_type(x_type, "x_type");
         check_type(y_type, "y_type");
-        if (n < 0) fail("n must be >= 0");
+        if (n < 0 || n > VERBO_OPS_MAX_ROWS) fail("n must be in [0, " + std::to_string(VERBO_OPS_MAX_ROWS) + "]");
         if (n == 0) return 0;
         check_rows(x, x_type, n, h->m.ins, ldx, "x");
         check_rows(y, y_type, n, h->m.outs, ldy, "y");
-        const long long sx = vb::ops_type_size(x_type), sy = vb::ops_type_size(y_type);
-        if (overlap(x, ldx * sx, h->m.ins * sx, y, ldy * sy, h->m.outs * sy, n)) fail("y overlaps x");
         const DeviceScope scope(h->device);
+        const long long sx = vb::ops_type_size(x_type), sy = vb::ops_type_size(y_type);
+        if (overlap(x, ldx * sx, h->m.ins * sx, y, ldy * sy, h->m.outs * sy, n, n)) fail("y overlaps x");
+        const long long need = static_cast<long long>(vb::q4_workspace_bytes(h->m, n, x_type));
+        if (need) {
+          if (!workspace || workspace_bytes < need)
+            fail("the workspace must have " + std::to_string(need) + " bytes (verbo_ops_q4_workspace)");
+          check_aligned(workspace, 16, "workspace");
+          if (overlap(x, ldx * sx, h->m.ins * sx, workspace, need, need, 1, n) ||
+              overlap(y, ldy * sy, h->m.outs * sy, workspace, need, need, 1, n))
+            fail("workspace overlaps x or y");
+        }
         vb::Q4Args a{};
         a.x = x;
         a.ldx = ldx;
         a.n = n;
         a.y = y;
         a.ldy = ldy;
+        a.workspace = workspace;
         cuda_ok(vb::launch_q4(h->m, a, x_type, y_type, static_cast<cudaStream_t>(stream)), "kernel launch");
         return 0;
       },

@@ -1,5 +1,19 @@
 // Products with 4-bit weights (include/verbo_ops.h): y = x W^T + b with
-// W[o][i] = s[o][g] (q[o][i] - z[o][g]) and the activations in their own type.
+// W[o][i] = s[o][g] (q[o][i] - z[o][g]) and the activations at their own
+// precision.
+//
+// Both kernels feed mma.sync.m16n8k16 with fp16: A is a tile of 16 outputs with
+// the weights unpacked to q - z, exact, and B holds x as columns.  The products
+// are exact, a group's sum is fp32, and the group's scale multiplies that sum.
+//   fp16 x   is a column as it is.
+//   bf16 x   is a column times a power of two that takes the token's largest
+//            value to [2^14, 2^15): exact for all within 2^-31 of that value (8
+//            bits above 2^-24), and off by 2^-40 of it at most for the rest.
+//   fp32 x   is two columns, hi = fp16(v) and lo = fp16((v - hi) 2^11) of the
+//            same scaled v: each drops half a step of 11 bits, 2^-24 of v
+//            together, which is fp32's own rounding.
+// The sums are taken back by the inverse power.  Infinities and NaNs go through
+// hi as they are and do not count for the largest value.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -15,7 +29,9 @@ namespace {
 
 constexpr int kThreadsQ4 = 256;
 constexpr int kWarpsQ4 = kThreadsQ4 / 32;
-constexpr int kAhead = 4;  // chunks whose loads a warp keeps in flight
+constexpr int kAhead = 2;  // chunks whose loads a warp of q4_kernel keeps in flight
+
+__device__ unsigned g_ops_status;
 
 // ================================================================== pack ==
 // One thread per 32-bit word of the chunks' nibbles.  Word j of lane (g, t) =
@@ -24,8 +40,8 @@ constexpr int kAhead = 4;  // chunks whose loads a warp keeps in flight
 // k + 3 from k = 32 p + 8 t + 4 (j % 2).  (The sum over k has no order, so the
 // lane's share of a block is taken as 8 neighbouring weights, which lets x be
 // read as it lies.)  Nibbles, low to high: (g, k), (g+8, k), (g, k+2),
-// (g+8, k+2), (g, k+1), (g+8, k+1), (g, k+3), (g+8, k+3): four masks with
-// 0x000f000f at shifts 0, 4, 8, 12 give the pairs of a0, a1, a2, a3.
+// (g+8, k+2), (g, k+1), (g+8, k+1), (g, k+3), (g+8, k+3): masks with 0x000f000f
+// and 0x00f000f0 at shifts 0 and 8 give the pairs of a0, a1, a2, a3.
 __device__ __forceinline__ uint32_t q4_nibble(const Q4Mat& m, const unsigned char* q, int o, int i) {
   if (o >= m.outs || i >= m.ins) return 0;
   const int blk = i >> 5, e = i & 31;
@@ -64,7 +80,7 @@ __global__ void q4_pack_kernel(Q4Mat m, const unsigned char* __restrict__ q, con
   }
 }
 
-// ================================================================ matvec ==
+// ================================================================ pieces ==
 __device__ __forceinline__ uint4 ld_stream16(const void* p) {
   uint4 v;
   asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0,%1,%2,%3}, [%4];"
@@ -74,142 +90,220 @@ __device__ __forceinline__ uint4 ld_stream16(const void* p) {
 }
 
 // d = a b + d, or a b with START.
-template <bool BF16, bool START>
+template <bool START>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  const float c0 = START ? 0.0f : d[0], c1 = START ? 0.0f : d[1], c2 = START ? 0.0f : d[2], c3 = START ? 0.0f : d[3];
-  if (BF16)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%10,%11,%12,%13};"
+  if constexpr (START)
+    asm("{\n .reg .f32 z;\n mov.f32 z, 0f00000000;\n"
+        " mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {z,z,z,z};\n}"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%10,%11,%12,%13};"
-        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b, bool bf16) {
-  if (bf16) {
-    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&d);
-  }
-  const __half2 d = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&d);
+// (x, y) += s (px, py): the packed form of two fmas.
+__device__ __forceinline__ void fma2(float& x, float& y, uint64_t s, float px, float py) {
+  uint64_t a, p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(a) : "f"(x), "f"(y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(px), "f"(py));
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(a) : "l"(s), "l"(p));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a));
+}
+__device__ __forceinline__ uint64_t twice(float s) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %1};" : "=l"(d) : "f"(s));
+  return d;
 }
 
 // The zero points of rows g and g + 8 as unpack() wants them.
-template <bool BF16>
 struct Q4Zero {
   uint32_t g, h;
   __device__ __forceinline__ Q4Zero(uint32_t zg, uint32_t zh) {
-    zg |= zg << 16;
-    zh |= zh << 16;
-    g = (BF16 ? 0x43004300u : 0x64006400u) | zg;
-    h = BF16 ? 0x43004300u | zh : 0xd400d400u | (zh << 4);
+    g = 0x64006400u | zg | zg << 16;           // 1024 + z
+    h = 0xd400d400u | zh << 4 | zh << 20;      // -(64 + z)
   }
 };
 
 // A word's eight weights minus their zero points: the A fragment of one k-step,
 // exact.  0x6400 | q is the fp16 1024 + q, and with q four bits higher
-// 1024 + 16 q, of which a sixteenth minus (64 + z) is q - z; 0x4300 | q is the
-// bf16 128 + q, whose mantissa has no room for the second form.
-template <bool BF16>
-__device__ __forceinline__ void unpack(uint32_t w, const Q4Zero<BF16>& z, uint32_t (&a)[4]) {
-  if (BF16) {
-    a[0] = sub2((w & 0x000f000fu) | 0x43004300u, z.g, true);
-    a[1] = sub2(((w >> 4) & 0x000f000fu) | 0x43004300u, z.h, true);
-    a[2] = sub2(((w >> 8) & 0x000f000fu) | 0x43004300u, z.g, true);
-    a[3] = sub2(((w >> 12) & 0x000f000fu) | 0x43004300u, z.h, true);
-  } else {
-    const uint32_t v = w >> 8, sixteenth = 0x2c002c00u;
-    auto upper = [&](uint32_t u) {
-      u = (u & 0x00f000f0u) | 0x64006400u;
-      const __half2 d = __hfma2(*reinterpret_cast<const __half2*>(&u), *reinterpret_cast<const __half2*>(&sixteenth),
-                                *reinterpret_cast<const __half2*>(&z.h));
-      return *reinterpret_cast<const uint32_t*>(&d);
-    };
-    a[0] = sub2((w & 0x000f000fu) | 0x64006400u, z.g, false);
-    a[1] = upper(w);
-    a[2] = sub2((v & 0x000f000fu) | 0x64006400u, z.g, false);
-    a[3] = upper(v);
-  }
+// 1024 + 16 q, of which a sixteenth minus (64 + z) is q - z.
+__device__ __forceinline__ void unpack(uint32_t w, const Q4Zero& z, uint32_t (&a)[4]) {
+  const uint32_t v = w >> 8, sixteenth = 0x2c002c00u;
+  auto h2 = [](const uint32_t& u) -> const __half2& { return *reinterpret_cast<const __half2*>(&u); };
+  auto lower = [&](uint32_t u) {
+    u = (u & 0x000f000fu) | 0x64006400u;
+    const __half2 d = __hsub2(h2(u), h2(z.g));
+    return *reinterpret_cast<const uint32_t*>(&d);
+  };
+  auto upper = [&](uint32_t u) {
+    u = (u & 0x00f000f0u) | 0x64006400u;
+    const __half2 d = __hfma2(h2(u), h2(sixteenth), h2(z.h));
+    return *reinterpret_cast<const uint32_t*>(&d);
+  };
+  a[0] = lower(w);
+  a[1] = upper(w);
+  a[2] = lower(v);
+  a[3] = upper(v);
 }
+
+// A chunk's scales and zero points for rows g and g + 8.
+template <int SETS, bool ZP>
+struct Q4Tail {
+  uint32_t s[SETS];                     // two fp16 per set
+  uint32_t z[ZP ? (SETS + 1) / 2 : 1];  // two bytes per set
+  __device__ __forceinline__ void load(const unsigned char* p, int g) {
+    const unsigned char* sp = p + g * (4 * SETS);
+    if constexpr (SETS == 4) {
+      const uint4 v = *reinterpret_cast<const uint4*>(sp);
+      s[0] = v.x, s[1] = v.y, s[2] = v.z, s[3] = v.w;
+    } else if constexpr (SETS == 2) {
+      const uint2 v = *reinterpret_cast<const uint2*>(sp);
+      s[0] = v.x, s[1] = v.y;
+    } else {
+      s[0] = *reinterpret_cast<const uint32_t*>(sp);
+    }
+    if constexpr (ZP) {
+      const unsigned char* zp = p + 32 * SETS + g * (2 * SETS);
+      if constexpr (SETS == 4) {
+        const uint2 v = *reinterpret_cast<const uint2*>(zp);
+        z[0] = v.x, z[1] = v.y;
+      } else if constexpr (SETS == 2) {
+        z[0] = *reinterpret_cast<const uint32_t*>(zp);
+      } else {
+        z[0] = *reinterpret_cast<const uint16_t*>(zp);
+      }
+    }
+  }
+  __device__ __forceinline__ Q4Zero zero(int set) const {
+    if (!ZP) return Q4Zero(8u, 8u);
+    const uint32_t v = z[set >> 1] >> (16 * (set & 1));
+    return Q4Zero(v & 15u, (v >> 8) & 15u);
+  }
+  __device__ __forceinline__ float2 scale(int set) const {
+    return __half22float2(*reinterpret_cast<const __half2*>(&s[set]));
+  }
+};
 
 // What one lane holds of a chunk.
 template <int SETS, bool ZP>
-struct Q4Buf {
+struct Q4Buf : Q4Tail<SETS, ZP> {
+  uint4 w0, w1;
   __device__ __forceinline__ uint32_t word(int j) const {
     const uint4& w = j < 4 ? w0 : w1;
     return (j & 3) == 0 ? w.x : (j & 3) == 1 ? w.y : (j & 3) == 2 ? w.z : w.w;
   }
-  template <bool BF16>
-  __device__ __forceinline__ Q4Zero<BF16> zero(int set) const {
-    if (!ZP) return Q4Zero<BF16>(8u, 8u);
-    const uint32_t v = z[set >> 1] >> (16 * (set & 1));
-    return Q4Zero<BF16>(v & 15u, (v >> 8) & 15u);
-  }
-  __device__ __forceinline__ float2 scale(int set) const { return __half22float2(*reinterpret_cast<const __half2*>(&s[set])); }
-  uint4 w0, w1;
-  uint32_t s[SETS];                 // scales of rows g, g + 8 per set
-  uint32_t z[ZP ? (SETS + 1) / 2 : 1];  // zero points, two bytes per set
   __device__ __forceinline__ void load(const unsigned char* p, int lane) {
     w0 = ld_stream16(p + lane * 16);
     w1 = ld_stream16(p + 512 + lane * 16);
-    const unsigned char* sp = p + 1024 + (lane >> 2) * (4 * SETS);
-    if (SETS == 4) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(sp));
-      s[0] = v.x, s[1 % SETS] = v.y, s[2 % SETS] = v.z, s[3 % SETS] = v.w;
-    } else if (SETS == 2) {
-      const uint2 v = __ldg(reinterpret_cast<const uint2*>(sp));
-      s[0] = v.x, s[1 % SETS] = v.y;
-    } else {
-      s[0] = __ldg(reinterpret_cast<const unsigned*>(sp));
-    }
-    if (ZP) {
-      const unsigned char* zp = p + 1024 + 32 * SETS + (lane >> 2) * (2 * SETS);
-      if (SETS == 4) {
-        const uint2 v = __ldg(reinterpret_cast<const uint2*>(zp));
-        z[0] = v.x, z[(SETS + 1) / 2 - 1] = v.y;
-      } else if (SETS == 2) {
-        z[0] = __ldg(reinterpret_cast<const unsigned*>(zp));
-      } else {
-        z[0] = __ldg(reinterpret_cast<const unsigned short*>(zp));
-      }
-    }
+    Q4Tail<SETS, ZP>::load(p + 1024, lane >> 2);
   }
 };
 
 struct Q4Kernel {
   Q4Mat m;
-  const void* x;   // the pass's first row
+  const void* x;  // the pass's first row
   long long ldx;
-  int tokens;      // rows of x in this pass
-  int cols;        // columns of B: tokens, or 3 per token for fp32 x
-  int xstride;     // bytes from one column to the next in shared memory
+  int tokens;  // rows of x in this pass
   void* y;
   long long ldy;
   int y_type;
-  bool wide;  // 16-bit x whose rows start on 16 bytes
-  int kq;     // q4_tile_kernel: groups of warps along the inputs
+  bool wide;       // rows of x start on 16 bytes
+  int xstride;     // q4_kernel: bytes from one column to the next in shared memory
+  // q4_tile_kernel: x as q4_image_kernel lays it out, the factors that take its
+  // sums back (per token), and the groups of warps along the inputs
+  unsigned char* image;
+  float2* back;
+  int kq;
 };
 
-// Three bf16 that sum to v exactly; an infinity or a NaN goes through the first.
-__device__ __forceinline__ void split3(float v, uint16_t (&p)[3]) {
-  const uint32_t u = __float_as_uint(v);
-  if ((u & 0x7f800000u) == 0x7f800000u) {
-    p[0] = v != v ? 0x7fc0u : static_cast<uint16_t>(u >> 16);
-    p[1] = p[2] = 0;
-    return;
+template <int XT>
+constexpr int kPartsOf = XT == kOpsF32 ? 2 : 1;  // columns per token
+
+// Eight neighbouring values of a row (past `ins`: zeros).
+template <int XT>
+struct X8 {
+  using E = std::conditional_t<XT == kOpsF32, uint32_t, uint16_t>;
+  uint32_t v[XT == kOpsF32 ? 8 : 4];
+  __device__ __forceinline__ void load(const void* row, int k, int ins, bool wide) {
+    if (k >= ins) {  // ins is a multiple of 32
+#pragma unroll
+      for (uint32_t& w : v) w = 0;
+      return;
+    }
+    const E* p = static_cast<const E*>(row) + k;
+    if (wide) {
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(v) / 16); ++i) {
+        const uint4 u = reinterpret_cast<const uint4*>(p)[i];
+        v[4 * i] = u.x, v[4 * i + 1] = u.y, v[4 * i + 2] = u.z, v[4 * i + 3] = u.w;
+      }
+    } else if constexpr (XT == kOpsF32) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = p[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = p[2 * i] | static_cast<uint32_t>(p[2 * i + 1]) << 16;
+    }
   }
-  const float r = v - __uint_as_float(u & 0xffff0000u);
-  const float l = r - __uint_as_float(__float_as_uint(r) & 0xffff0000u);
-  p[0] = static_cast<uint16_t>(u >> 16);
-  p[1] = static_cast<uint16_t>(__float_as_uint(r) >> 16);
-  p[2] = static_cast<uint16_t>(__float_as_uint(l) >> 16);
-}
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (XT == kOpsF32)
+      return __uint_as_float(v[i]);
+    else if constexpr (XT == kOpsBF16)
+      return __uint_as_float((i & 1) ? v[i >> 1] & 0xffff0000u : v[i >> 1] << 16);
+    else
+      return __half2float(__ushort_as_half(static_cast<unsigned short>(v[i >> 1] >> (16 * (i & 1)))));
+  }
+  // the largest magnitude among the finite values, as bits
+  __device__ __forceinline__ uint32_t largest() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t u = __float_as_uint(get(i)) & 0x7fffffffu;
+      if (u < 0x7f800000u) m = max(m, u);
+    }
+    return m;
+  }
+  // the columns' 16 bytes
+  __device__ __forceinline__ void columns(float up, float up2, uint4& hi, uint4& lo) const {
+    if constexpr (XT == kOpsF16) {
+      hi = make_uint4(v[0], v[1], v[2], v[3]);
+    } else {
+      uint32_t h[4], l[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float a = get(2 * i) * up * up2, b = get(2 * i + 1) * up * up2;
+        const __half2 p = __floats2half2_rn(a, b);
+        h[i] = *reinterpret_cast<const uint32_t*>(&p);
+        const float2 q = __half22float2(p);
+        // of an infinity or a NaN nothing is left over
+        const __half2 r = __floats2half2_rn(fabsf(a) < __uint_as_float(0x7f800000u) ? (a - q.x) * 2048.0f : 0.0f,
+                                            fabsf(b) < __uint_as_float(0x7f800000u) ? (b - q.y) * 2048.0f : 0.0f);
+        l[i] = *reinterpret_cast<const uint32_t*>(&r);
+      }
+      hi = make_uint4(h[0], h[1], h[2], h[3]);
+      if (XT == kOpsF32) lo = make_uint4(l[0], l[1], l[2], l[3]);
+    }
+  }
+};
+
+// The power of two that takes a largest magnitude (as bits) to [2^14, 2^15), in
+// two factors that fp32 holds, and its inverse.
+struct Power {
+  float up, up2, down, down2;
+  __device__ __forceinline__ explicit Power(uint32_t largest) {
+    int e = 0;
+    if (largest) {
+      int x;
+      frexpf(__uint_as_float(largest), &x);  // value in [2^(x-1), 2^x)
+      e = 15 - x;
+    }
+    const int h = e / 2;
+    up = two(h), up2 = two(e - h), down = two(-h), down2 = two(h - e);
+  }
+  static __device__ __forceinline__ float two(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
+};
 
 __device__ __forceinline__ void q4_store(const Q4Kernel& a, int token, int o, float v) {
   const long long at = token * a.ldy + o;
@@ -221,25 +315,24 @@ __device__ __forceinline__ void q4_store(const Q4Kernel& a, int token, int o, fl
     static_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16_rn(v);
 }
 
-// The bound is reading the matrix once.  A tile is 16 outputs times all inputs;
-// a CTA takes a run of tiles and its warps equal shares of the run's chunks, so
-// each warp streams one contiguous piece of memory, kAhead chunks ahead, in
-// registers.  x lies in shared memory, one column after the other as in memory;
-// a lane's B fragment of two k-steps is 16 neighbouring bytes of a column
-// (columns 64 mod 128 bytes apart: the 8 lanes of a quarter warp hit 32 banks).
-// The weights are unpacked to q - z, exact in 16 bits, and mma.sync sums a
-// group's products in fp32; the group's scale multiplies that sum.  fp32 x is
-// cut into three bf16 parts of 8 bits each (24 bits: exact), three columns of B
-// that are added at the end.
-// A tile whose chunks fall to several warps is summed over the warps' partial
-// sums in shared memory, in the order of the warps.
-template <bool BF16, bool SPLIT, int NT, int SETS, bool ZP>
-__global__ void __launch_bounds__(kThreadsQ4, NT <= 2 ? 2 : 1) q4_kernel(const Q4Kernel a) {
-  constexpr int PER = SPLIT ? 2 : 8;  // tokens per 8 columns
-  extern __shared__ __align__(16) unsigned char smem_q4[];
+// ================================================================ matvec ==
+// Up to 8 columns.  The bound is reading the matrix once.  A tile is 16 outputs
+// times all inputs; a CTA takes a run of tiles and its warps equal shares of the
+// run's chunks, so each warp streams one contiguous piece of memory, kAhead
+// chunks ahead, in registers.  x lies in shared memory, one column after the
+// other as in memory; a lane's B fragment of two k-steps is 16 neighbouring
+// bytes of a column (columns 64 mod 128 bytes apart: the 8 lanes of a quarter
+// warp hit 32 banks).  A tile whose chunks fall to several warps is summed over
+// the warps' partial sums in shared memory, in the order of the warps.
+template <int XT, int SETS, bool ZP>
+__global__ void __launch_bounds__(kThreadsQ4, 2) q4_kernel(const Q4Kernel a) {
+  constexpr int PARTS = kPartsOf<XT>;
+  extern __shared__ __align__(128) unsigned char smem_q4[];
+  __shared__ uint32_t largest[8];
+  __shared__ float2 back[8];
   // slots: per warp the partial sums of its first tile, of its last, and one for
-  // the tile at hand; [NT][8 columns][16 rows] each
-  constexpr int SLOT = NT * 128;
+  // the tile at hand; [8 columns][16 rows] each
+  constexpr int SLOT = 128;
   float* slots = reinterpret_cast<float*>(smem_q4);
   unsigned char* xs = smem_q4 + 3 * kWarpsQ4 * SLOT * 4;
   const Q4Mat& m = a.m;
@@ -259,132 +352,118 @@ __global__ void __launch_bounds__(kThreadsQ4, NT <= 2 ? 2 : 1) q4_kernel(const Q
     if (first + i < last) buf[i].load(src + static_cast<long long>(i) * m.chunk_bytes, lane);
   src += static_cast<long long>(kAhead) * m.chunk_bytes;
 
+  grid_release();  // the next grid may start on its weights as SMs come free; it waits for this one's end as well
+  if (XT != kOpsF16 && tid < 8) largest[tid] = 0;
+  if (XT != kOpsF16) __syncthreads();
   grid_wait();  // the weights are the handle's; x comes from the grid before
   const int kp = m.nkc * kQ4Chunk;
-  if (SPLIT) {
-    const float* x = static_cast<const float*>(a.x);
-    for (int tok = 0; tok < a.tokens; ++tok)
-      for (int k = tid; k < kp; k += kThreadsQ4) {
-        uint16_t part[3];
-        split3(k < m.ins ? x[tok * a.ldx + k] : 0.0f, part);
-        unsigned char* at = xs + static_cast<size_t>(3 * tok) * a.xstride + 2 * k;
-#pragma unroll
-        for (int i = 0; i < 3; ++i) *reinterpret_cast<uint16_t*>(at + i * a.xstride) = part[i];
-      }
-  } else {
-    const uint16_t* x = static_cast<const uint16_t*>(a.x);
+  constexpr int ES = XT == kOpsF32 ? 4 : 2;
+  const char* x = static_cast<const char*>(a.x);
+  if (XT != kOpsF16) {
     for (int tok = 0; tok < a.tokens; ++tok) {
-      unsigned char* at = xs + static_cast<size_t>(tok) * a.xstride;
-      const uint16_t* row = x + tok * a.ldx;
-      for (int k = tid * 8; k < kp; k += kThreadsQ4 * 8) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (k < m.ins) {  // ins is a multiple of 32
-          if (a.wide) {
-            v = *reinterpret_cast<const uint4*>(row + k);
-          } else {
-            uint32_t w[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = row[k + 2 * j] | static_cast<uint32_t>(row[k + 2 * j + 1]) << 16;
-            v = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        }
-        *reinterpret_cast<uint4*>(at + 2 * k) = v;
+      uint32_t big = 0;
+      for (int k = tid * 8; k < m.ins; k += kThreadsQ4 * 8) {
+        X8<XT> v;
+        v.load(x + tok * a.ldx * ES, k, m.ins, a.wide);
+        big = max(big, v.largest());
       }
+      big = __reduce_max_sync(0xffffffffu, big);
+      if (lane == 0) atomicMax(&largest[tok], big);
+    }
+    __syncthreads();
+  }
+  for (int tok = 0; tok < a.tokens; ++tok) {
+    float up = 1.0f, up2 = 1.0f;
+    if (XT != kOpsF16) {
+      const Power p(largest[tok]);
+      up = p.up, up2 = p.up2;
+      if (tid == 0) back[tok] = make_float2(p.down, p.down2);
+    }
+    unsigned char* at = xs + static_cast<size_t>(PARTS * tok) * a.xstride;
+    for (int k = tid * 8; k < kp; k += kThreadsQ4 * 8) {
+      X8<XT> v;
+      v.load(x + tok * a.ldx * ES, k, m.ins, a.wide);
+      uint4 hi, lo;
+      v.columns(up, up2, hi, lo);
+      *reinterpret_cast<uint4*>(at + 2 * k) = hi;
+      if (PARTS == 2) *reinterpret_cast<uint4*>(at + a.xstride + 2 * k) = lo;
     }
   }
   __syncthreads();
 
-  // column of B that this lane reads in each group of 8 (past the last one: the
-  // last, whose sums are then not stored)
-  const unsigned char* xcol[NT];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    int c = SPLIT ? n * 6 + min(g, 5) : n * 8 + g;
-    xcol[n] = xs + static_cast<size_t>(min(c, a.cols - 1)) * a.xstride + t * 16;
-  }
-
-  float acc[NT][4];
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[n][i] = 0.0f;
+  // the column of B that this lane reads (past the last one: the last, whose sums
+  // are then not stored)
+  const unsigned char* xcol = xs + static_cast<size_t>(min(g, a.tokens * PARTS - 1)) * a.xstride + t * 16;
+  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 
   float* mine = slots + warp * 3 * SLOT;
-  auto spill = [&](float* slot) {  // acc -> [n][column][row]
+  auto spill = [&](float* slot) {  // acc -> [column][row]
+    slot[(2 * t) * 16 + g] = acc[0];
+    slot[(2 * t + 1) * 16 + g] = acc[1];
+    slot[(2 * t) * 16 + g + 8] = acc[2];
+    slot[(2 * t + 1) * 16 + g + 8] = acc[3];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      slot[n * 128 + (2 * t) * 16 + g] = acc[n][0];
-      slot[n * 128 + (2 * t + 1) * 16 + g] = acc[n][1];
-      slot[n * 128 + (2 * t) * 16 + g + 8] = acc[n][2];
-      slot[n * 128 + (2 * t + 1) * 16 + g + 8] = acc[n][3];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[n][i] = 0.0f;
-    }
+    for (int i = 0; i < 4; ++i) acc[i] = 0.0f;
+  };
+  // a token's sum in a slot
+  auto token_sum = [&](const float* slot, int tok, int r) {
+    const float* col = slot + tok * (PARTS * 16) + r;
+    return PARTS == 2 ? fmaf(col[16], 1.0f / 2048.0f, col[0]) : col[0];
   };
   auto finish = [&](int tile, int tok, int r, float v) {
     const int o = tile * kQ4Rows + r;
+    if (XT != kOpsF16) v = v * back[tok].x * back[tok].y;
     if (o < m.outs) q4_store(a, tok, o, m.bias ? v + m.bias[o] : v);
-  };
-  // one warp stores a whole tile out of a slot
-  auto store_tile = [&](int tile, const float* slot) {
-    for (int e = lane; e < a.tokens * 16; e += 32) {
-      const int tok = e >> 4, r = e & 15;
-      const float* col = slot + (tok / PER) * 128 + (tok % PER) * (SPLIT ? 3 : 1) * 16 + r;
-      finish(tile, tok, r, SPLIT ? col[0] + (col[16] + col[32]) : col[0]);
-    }
   };
 
   int kc = first % m.nkc, tile = tile0 + first / m.nkc;
-  const bool starts_inside = kc != 0;
-  bool first_part = starts_inside;  // the tile at hand began in an earlier warp's share
+  bool first_part = kc != 0;  // the tile at hand began in an earlier warp's share
+  const unsigned char* xk = xcol + kc * (kQ4Chunk * 2);
   for (int i0 = first; i0 < last; i0 += kAhead) {
 #pragma unroll
     for (int d = 0; d < kAhead; ++d) {
       if (i0 + d >= last) break;
       Q4Buf<SETS, ZP>& b = buf[d];
-      const int xoff = kc * (kQ4Chunk * 2);
 #pragma unroll
       for (int set = 0; set < SETS; ++set) {
         constexpr int BLK = 4 / SETS;  // 32-blocks per set
-        const Q4Zero<BF16> z = b.template zero<BF16>(set);
-        float part[NT][4];
+        const Q4Zero z = b.zero(set);
+        float part[4];
 #pragma unroll
         for (int p = set * BLK; p < (set + 1) * BLK; ++p) {
           uint32_t fa[2][4];
-          unpack<BF16>(b.word(2 * p), z, fa[0]);
-          unpack<BF16>(b.word(2 * p + 1), z, fa[1]);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const uint4 f = *reinterpret_cast<const uint4*>(xcol[n] + xoff + p * 64);
-            if (p == set * BLK)
-              mma16816<BF16, true>(part[n], fa[0], f.x, f.y);
-            else
-              mma16816<BF16, false>(part[n], fa[0], f.x, f.y);
-            mma16816<BF16, false>(part[n], fa[1], f.z, f.w);
+          unpack(b.word(2 * p), z, fa[0]);
+          unpack(b.word(2 * p + 1), z, fa[1]);
+          const uint4 f = *reinterpret_cast<const uint4*>(xk + p * 64);
+          if (p == set * BLK) {
+            mma16816<true>(part, fa[0], f.x, f.y);
+          } else {
+            mma16816<false>(part, fa[0], f.x, f.y);
           }
+          mma16816<false>(part, fa[1], f.z, f.w);
         }
         const float2 sc = b.scale(set);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          acc[n][0] = fmaf(sc.x, part[n][0], acc[n][0]);
-          acc[n][1] = fmaf(sc.x, part[n][1], acc[n][1]);
-          acc[n][2] = fmaf(sc.y, part[n][2], acc[n][2]);
-          acc[n][3] = fmaf(sc.y, part[n][3], acc[n][3]);
-        }
+        acc[0] = fmaf(sc.x, part[0], acc[0]);
+        acc[1] = fmaf(sc.x, part[1], acc[1]);
+        acc[2] = fmaf(sc.y, part[2], acc[2]);
+        acc[3] = fmaf(sc.y, part[3], acc[3]);
       }
       if (i0 + d + kAhead < last) b.load(src, lane);
       src += m.chunk_bytes;
+      xk += kQ4Chunk * 2;
       if (++kc == m.nkc) {
         if (first_part) {
           spill(mine);
           first_part = false;
-        } else {
+        } else {  // the whole tile is this warp's
           spill(mine + 2 * SLOT);
           __syncwarp();
-          store_tile(tile, mine + 2 * SLOT);
+          for (int e = lane; e < a.tokens * 16; e += 32)
+            finish(tile, e >> 4, e & 15, token_sum(mine + 2 * SLOT, e >> 4, e & 15));
           __syncwarp();
         }
         kc = 0;
+        xk = xcol;
         ++tile;
       }
     }
@@ -395,270 +474,334 @@ __global__ void __launch_bounds__(kThreadsQ4, NT <= 2 ? 2 : 1) q4_kernel(const Q
   __syncthreads();
 
   // tiles cut by a boundary between shares: summed by the warp in whose share they begin
-  if (last > first) {
-    const int end_tile = tile0 + last / m.nkc;  // the tile the share ends in
-    const int begin_at = (end_tile - tile0) * m.nkc;
-    if (last % m.nkc != 0 && begin_at >= first) {
-      for (int e = lane; e < a.tokens * 16; e += 32) {
-        const int tok = e >> 4, r = e & 15;
-        const int off = (tok / PER) * 128 + (tok % PER) * (SPLIT ? 3 : 1) * 16 + r;
-        float v = 0.0f;
-        for (int w = warp; w < kWarpsQ4; ++w) {
-          const int wf = static_cast<int>(static_cast<long long>(run) * w / kWarpsQ4);
-          const int wl = static_cast<int>(static_cast<long long>(run) * (w + 1) / kWarpsQ4);
-          if (wf >= begin_at + m.nkc) break;
-          if (wl <= wf) continue;
-          // its part of this tile: the last slot if the share ends inside the
-          // tile, the first slot if it ends at or past the tile's end
-          const float* col = slots + (w * 3 + (wl < begin_at + m.nkc ? 1 : 0)) * SLOT + off;
-          v += SPLIT ? col[0] + (col[16] + col[32]) : col[0];
-        }
-        finish(end_tile, tok, r, v);
+  const int end_tile = last / m.nkc, begin_at = end_tile * m.nkc;  // the tile the share ends in
+  if (last > first && last % m.nkc != 0 && begin_at >= first) {
+    for (int e = lane; e < a.tokens * 16; e += 32) {
+      float v = 0.0f;
+      for (int w = warp; w < kWarpsQ4; ++w) {
+        const int wf = static_cast<int>(static_cast<long long>(run) * w / kWarpsQ4);
+        const int wl = static_cast<int>(static_cast<long long>(run) * (w + 1) / kWarpsQ4);
+        if (wf >= begin_at + m.nkc) break;
+        if (wl <= wf) continue;
+        // its part of this tile: the last slot if the share ends inside the tile,
+        // the first slot if it ends at or past the tile's end
+        v += token_sum(slots + (w * 3 + (wl < begin_at + m.nkc ? 1 : 0)) * SLOT, e >> 4, e & 15);
       }
+      finish(tile0 + end_tile, e >> 4, e & 15, v);
     }
   }
 }
 
+// ================================================================= image ==
+// x for q4_tile_kernel, in passes of COLS columns: per chunk of 128 inputs, per
+// tile of 8 columns and per 32-block the 16 bytes that each lane's B fragments of
+// two k-steps are, so that a chunk is one contiguous copy and a fragment one
+// 16-byte load.  One CTA per token; also its factors back.
+template <int XT>
+__global__ void __launch_bounds__(256) q4_image_kernel(const Q4Kernel a, int cols) {
+  constexpr int PARTS = kPartsOf<XT>, ES = XT == kOpsF32 ? 4 : 2;
+  __shared__ uint32_t largest[8];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  grid_release();
+  grid_wait();
+  const int tok = blockIdx.x, per_pass = cols / PARTS;
+  const int pass = tok / per_pass, col = (tok - pass * per_pass) * PARTS;
+  const Q4Mat& m = a.m;
+  const char* row = static_cast<const char*>(a.x) + tok * a.ldx * ES;
+  float up = 1.0f, up2 = 1.0f;
+  if (XT != kOpsF16) {
+    uint32_t big = 0;
+    for (int k = tid * 8; k < m.ins; k += 256 * 8) {
+      X8<XT> v;
+      v.load(row, k, m.ins, a.wide);
+      big = max(big, v.largest());
+    }
+    big = __reduce_max_sync(0xffffffffu, big);
+    if (lane == 0) largest[warp] = big;
+    __syncthreads();
+    big = largest[lane & 7];
+    const Power p(__reduce_max_sync(0xffffffffu, big));
+    up = p.up, up2 = p.up2;
+    if (tid == 0) a.back[tok] = make_float2(p.down, p.down2);
+  } else if (tid == 0) {
+    a.back[tok] = make_float2(1.0f, 1.0f);
+  }
+  unsigned char* to = a.image + static_cast<size_t>(pass) * m.nkc * (cols * (kQ4Chunk * 2));
+  for (int u = tid; u < m.nkc * 16; u += 256) {  // 8 inputs each: chunk, block p, t
+    X8<XT> v;
+    v.load(row, u * 8, m.ins, a.wide);
+    uint4 hi, lo;
+    v.columns(up, up2, hi, lo);
+    unsigned char* at = to + static_cast<size_t>(u >> 4) * (cols * (kQ4Chunk * 2)) + (col >> 3) * 2048 +
+                        ((u >> 2) & 3) * 512 + (col & 7) * 64 + (u & 3) * 16;
+    *reinterpret_cast<uint4*>(at) = hi;
+    if (PARTS == 2) *reinterpret_cast<uint4*>(at + 64) = lo;  // the next column, of the same eight
+  }
+}
+
 // ================================================================= tiles ==
-// More columns than q4_kernel takes: the same products, with x streamed.  A CTA
-// is kq groups of warps that split the inputs among them; in a group each warp
-// has two tiles (32 outputs) at a time, and a chunk of x (128 inputs of every
-// column) is staged for the group by cp.async, three buffers deep, one named
-// barrier per chunk.  A warp's weights come straight to registers, a chunk
-// ahead.  Reading x again for every 32 * (8 / kq) outputs costs L2 as many bytes
-// as the weights at 16 * (8 / kq) * 2 columns.  A set's sums are scaled when it
-// ends, 64 inputs at most, so that the fragments of a set stay in registers.
-constexpr int kTileX = kQ4Chunk * 2 + 64;  // bytes of a column's chunk: 64 mod 128
-constexpr int kTileBufs = 3;
-constexpr int kTileRun = 2;  // tiles per warp at a time
+// More than 8 columns, or inputs too long for q4_kernel.  A CTA is kq groups of
+// warps that split the inputs among them; in a group each warp has a tile (16
+// outputs) times all columns at a time, its weights coming straight to registers,
+// two chunks ahead.  One thread of the group streams chunks of x (its image, one
+// bulk copy each) through a ring of stages (full / empty barriers).  A set's sums
+// are scaled when it ends, 64 inputs at most, so that its fragments stay in
+// registers; two column tiles go through the tensor pipe side by side.
+//
+// What bounds it is not memory but the pipes behind mma.sync: measured on B200, an
+// m16n8k16 takes 8.6 cycles of a quarter SM, and two of them (a group of 32) with
+// the four fmas of their scale 25.  tcgen05.mma does not help here: a group's sums
+// have to leave tensor memory before the next scale, 2 values per weight at 64
+// columns and groups of 32, and weights that are unpacked into tensor memory go
+// there at about 28 bytes per cycle and SM: a kernel built that way took 92 us for
+// 64 rows of a 151936 x 896 head in groups of 32 (this one 91) and 43 us for 16
+// (this one 35.5).
+constexpr int kTileStages = 4;
+// CTAs per SM.  More of them hide more, at fewer registers: 16 rows of a 151936 x
+// 896 head in groups of 32 took 35.5 us with three and 39 with two, of a 14336 x
+// 4096 matrix in groups of 64 (longer chains of fragments) 25 and 21.
+template <int NT, int SETS>
+constexpr int kTileCtas = NT <= 4 && SETS == 4 ? 3 : 2;
 
-__device__ __forceinline__ void cp_async16_or_zero(void* dst, const void* src, bool take) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(take ? 16 : 0)
-               : "memory");
+__device__ __forceinline__ void bulk_copy(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
 }
-__device__ __forceinline__ void group_sync(int id, int threads) {
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+__device__ __forceinline__ void mbar_arrive1(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// A wait with a limit of kWaitLimitNs; the timer is looked at now and then alone.
+__device__ __forceinline__ bool wait_limited(uint64_t* bar, uint32_t phase) {
+  if (mbar_try_wait(bar, phase)) return true;
+  uint64_t t0 = 0;
+  for (uint32_t i = 1;; ++i) {
+    if (mbar_try_wait(bar, phase)) return true;
+    if ((i & 255u) == 0) {
+      const uint64_t t = gtimer();
+      if (t0 == 0) t0 = t;
+      if (t - t0 > kWaitLimitNs) return false;
+    }
+  }
+}
+__device__ __forceinline__ Q4Zero zero_at(const unsigned char* p) {
+  const uint32_t v = *reinterpret_cast<const uint16_t*>(p);
+  return Q4Zero(v & 15u, v >> 8);
 }
 
-template <bool BF16, bool SPLIT, int NT, int SETS, bool ZP>
-__global__ void __launch_bounds__(kThreadsQ4, NT <= 2 ? 2 : 1) q4_tile_kernel(const Q4Kernel a) {
-  constexpr int COLS = NT * 8, R = kTileRun;
-  extern __shared__ __align__(16) unsigned char smem_q4[];
+template <int XT, int NT, int SETS, bool ZP>
+__global__ void __launch_bounds__(kThreadsQ4, kTileCtas<NT, SETS>) q4_tile_kernel(const Q4Kernel a) {
+  constexpr int PARTS = kPartsOf<XT>;
+  constexpr int XB = NT * 2048;  // a chunk of x
+  extern __shared__ __align__(128) unsigned char smem_q4[];
+  __shared__ uint64_t bars[kWarpsQ4][2 * kTileStages];  // per group: full, empty
+  __shared__ float2 back[NT * 8 / PARTS];
+  __shared__ int stop;
   const Q4Mat& m = a.m;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
-  const int wm_n = kWarpsQ4 / a.kq, kq = warp / wm_n, wm = warp % wm_n;
-  const int gthreads = wm_n * 32, gt = tid - kq * gthreads;
-  unsigned char* xs = smem_q4 + kq * (kTileBufs * COLS * kTileX);
-  float* red = reinterpret_cast<float*>(smem_q4 + a.kq * (kTileBufs * COLS * kTileX));
+  const int group = kWarpsQ4 / a.kq, kq = warp / group, wm = warp % group;
+  unsigned char* ring = smem_q4 + kq * (kTileStages * XB);
+  float* red = reinterpret_cast<float*>(smem_q4 + a.kq * (kTileStages * XB));
+  uint64_t* full = bars[kq];
+  uint64_t* empty = bars[kq] + kTileStages;
+  if (tid < a.kq * 2 * kTileStages)
+    mbar_init(&bars[tid / (2 * kTileStages)][tid % (2 * kTileStages)], tid % (2 * kTileStages) < kTileStages ? 1 : group);
+  if (tid == 0) stop = 0;
 
   const int tile0 = static_cast<int>(static_cast<long long>(m.ntile) * blockIdx.x / gridDim.x);
   const int tile1 = static_cast<int>(static_cast<long long>(m.ntile) * (blockIdx.x + 1) / gridDim.x);
   const int c0 = m.nkc * kq / a.kq, nc = m.nkc * (kq + 1) / a.kq - c0;
-  const int passes = (tile1 - tile0 + wm_n * R - 1) / (wm_n * R);
+  const int passes = (tile1 - tile0 + group - 1) / group;
   const int total = passes * nc;
+  const bool producer = wm == 0 && lane == 0;
+  __syncthreads();
 
-  auto stage = [&](int it) {  // chunk it % nc of x
-    if (it < total) {
-      unsigned char* to = xs + (it % kTileBufs) * (COLS * kTileX);
-      const int k0 = (c0 + it % nc) * kQ4Chunk;
-      if (SPLIT) {
-        const float* x = static_cast<const float*>(a.x);
-        for (int e = gt; e < a.tokens * (kQ4Chunk / 2); e += gthreads) {
-          const int tok = e / (kQ4Chunk / 2), k = 2 * (e % (kQ4Chunk / 2));
-          uint32_t h = 0, mi = 0, lo = 0;
-          if (k0 + k < m.ins) {
-            uint16_t p0[3], p1[3];
-            split3(x[tok * a.ldx + k0 + k], p0);
-            split3(x[tok * a.ldx + k0 + k + 1], p1);
-            h = p0[0] | static_cast<uint32_t>(p1[0]) << 16;
-            mi = p0[1] | static_cast<uint32_t>(p1[1]) << 16;
-            lo = p0[2] | static_cast<uint32_t>(p1[2]) << 16;
-          }
-          unsigned char* at = to + ((tok >> 1) * 8 + (tok & 1) * 3) * kTileX + 2 * k;
-          *reinterpret_cast<uint32_t*>(at) = h;
-          *reinterpret_cast<uint32_t*>(at + kTileX) = mi;
-          *reinterpret_cast<uint32_t*>(at + 2 * kTileX) = lo;
-        }
-      } else {
-        const uint16_t* x = static_cast<const uint16_t*>(a.x);
-        for (int e = gt; e < a.tokens * 16; e += gthreads) {
-          const int tok = e >> 4, k = k0 + 8 * (e & 15);
-          const uint16_t* from = x + tok * a.ldx + k;
-          unsigned char* at = to + tok * kTileX + 16 * (e & 15);
-          if (a.wide) {
-            cp_async16_or_zero(at, k < m.ins ? from : x, k < m.ins);
-          } else {
-            uint32_t w[4] = {0, 0, 0, 0};
-            if (k < m.ins) {
-#pragma unroll
-              for (int j = 0; j < 4; ++j) w[j] = from[2 * j] | static_cast<uint32_t>(from[2 * j + 1]) << 16;
-            }
-            *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        }
-      }
-    }
-    cp_async_commit();
-  };
-  Q4Buf<SETS, ZP> buf[2][R];
-  auto load = [&](int it, Q4Buf<SETS, ZP>(&b)[R]) {
-    if (it >= total) return;
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int tile = tile0 + (it / nc * wm_n + wm) * R + r;
-      if (tile < tile1) b[r].load(m.tiles + (static_cast<long long>(tile) * m.nkc + c0 + it % nc) * m.chunk_bytes, lane);
+  // the weights are the handle's; x comes from the grid before
+  Q4Buf<SETS, ZP> buf[2];
+  int load_tile = tile0 + wm, load_chunk = 0;
+  const unsigned char* load_at = m.tiles + (static_cast<long long>(load_tile) * m.nkc + c0) * m.chunk_bytes;
+  auto load = [&](Q4Buf<SETS, ZP>& b) {
+    if (load_tile < tile1) b.load(load_at, lane);
+    load_at += m.chunk_bytes;
+    if (++load_chunk == nc) {
+      load_chunk = 0;
+      load_tile += group;
+      load_at += (static_cast<long long>(group) * m.nkc - nc) * m.chunk_bytes;
     }
   };
-  load(0, buf[0]);
-  grid_wait();  // the weights are the handle's; x comes from the grid before
-  stage(0);
-  stage(1);
+  load(buf[0]);
+  load(buf[1]);
+  int put = 0, put_chunk = 0;  // the next chunk of x
+  auto inputs = [&]() {
+    const int s = put % kTileStages;
+    mbar_expect_tx(&full[s], XB);
+    bulk_copy(ring + s * XB, a.image + static_cast<size_t>(c0 + put_chunk) * XB, XB, &full[s]);
+    ++put;
+    if (++put_chunk == nc) put_chunk = 0;
+  };
+  grid_release();
+  grid_wait();
+  if (producer)
+    while (put < min(kTileStages, total)) inputs();
+  if (tid < a.tokens) back[tid] = a.back[tid];
+  __syncthreads();
 
-  // columns past the pass's last are not stored; they read the last column
-  int xcol[NT];
+  float acc[NT][4];
 #pragma unroll
   for (int n = 0; n < NT; ++n)
-    xcol[n] = (SPLIT ? n * 8 + min(g, 5) : min(n * 8 + g, a.tokens - 1)) * kTileX + t * 16;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[n][i] = 0.0f;
 
-  float acc[R][NT][4];
-#pragma unroll
-  for (int r = 0; r < R; ++r)
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[r][n][i] = 0.0f;
-
-  int chunk = 0, pass = 0;
+  bool ok = true;
+  int chunk = 0, tile = tile0 + wm;
   for (int it0 = 0; it0 < total; it0 += 2) {
 #pragma unroll
     for (int d = 0; d < 2; ++d) {
       const int it = it0 + d;
       if (it >= total) break;
-      load(it + 1, buf[d ^ 1]);
-      asm volatile("cp.async.wait_group 1;" ::: "memory");
-      group_sync(1 + kq, gthreads);  // the chunk is there, and the one before it is done with
-      stage(it + 2);
-      const unsigned char* xc = xs + (it % kTileBufs) * (COLS * kTileX);
-      const int first = tile0 + (pass * wm_n + wm) * R;
-      if (first < tile1) {
-        constexpr int PARTS = SETS < 2 ? 2 : SETS;  // scaled together: at most 64 inputs
-        constexpr int BLK = 4 / PARTS;
+      const int s = it % kTileStages;
+      // A wait that runs out ends the products of the warp, not its barriers, and
+      // nothing of the CTA is stored any more.
+      if (ok && !wait_limited(&full[s], (it / kTileStages) & 1)) {
+        ok = false;
+        stop = 1;
+      }
+      if (ok && tile < tile1) {
+        const unsigned char* xc = ring + s * XB + lane * 16;
+        constexpr int Q = SETS < 2 ? 2 : SETS;  // scaled together: at most 64 inputs
+        constexpr int BLK = 4 / Q;
+        constexpr int NP = NT < 2 ? NT : 2;  // column tiles side by side
 #pragma unroll
-        for (int q = 0; q < PARTS; ++q) {
-          const int set = q * SETS / PARTS;
-          uint32_t fa[R][2 * BLK][4];
-          float2 sc[R];
+        for (int q = 0; q < Q; ++q) {
+          const int set = q * SETS / Q;
+          const Q4Zero z = buf[d].zero(set);
+          uint32_t fa[2 * BLK][4];
 #pragma unroll
-          for (int r = 0; r < R; ++r) {
-            const Q4Zero<BF16> z = buf[d][r].template zero<BF16>(set);
+          for (int j = 0; j < 2 * BLK; ++j) unpack(buf[d].word(2 * BLK * q + j), z, fa[j]);
+          const float2 sc = buf[d].scale(set);
+          const uint64_t sg = twice(sc.x), sh = twice(sc.y);
 #pragma unroll
-            for (int j = 0; j < 2 * BLK; ++j) unpack<BF16>(buf[d][r].word(q * 2 * BLK + j), z, fa[r][j]);
-            sc[r] = buf[d][r].scale(set);
-          }
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            float part[R][4];
+          for (int n = 0; n < NT; n += NP) {
+            float part[NP][4];
 #pragma unroll
             for (int p = 0; p < BLK; ++p) {
-              const uint4 f = *reinterpret_cast<const uint4*>(xc + xcol[n] + (q * BLK + p) * 64);
+              uint4 f[NP];
 #pragma unroll
-              for (int r = 0; r < R; ++r) {
+              for (int u = 0; u < NP; ++u)
+                f[u] = *reinterpret_cast<const uint4*>(xc + (n + u) * 2048 + (q * BLK + p) * 512);
+#pragma unroll
+              for (int u = 0; u < NP; ++u) {
                 if (p == 0)
-                  mma16816<BF16, true>(part[r], fa[r][0], f.x, f.y);
+                  mma16816<true>(part[u], fa[0], f[u].x, f[u].y);
                 else
-                  mma16816<BF16, false>(part[r], fa[r][2 * p], f.x, f.y);
+                  mma16816<false>(part[u], fa[2 * p], f[u].x, f[u].y);
               }
 #pragma unroll
-              for (int r = 0; r < R; ++r) mma16816<BF16, false>(part[r], fa[r][2 * p + 1], f.z, f.w);
+              for (int u = 0; u < NP; ++u) mma16816<false>(part[u], fa[2 * p + 1], f[u].z, f[u].w);
             }
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-              acc[r][n][0] = fmaf(sc[r].x, part[r][0], acc[r][n][0]);
-              acc[r][n][1] = fmaf(sc[r].x, part[r][1], acc[r][n][1]);
-              acc[r][n][2] = fmaf(sc[r].y, part[r][2], acc[r][n][2]);
-              acc[r][n][3] = fmaf(sc[r].y, part[r][3], acc[r][n][3]);
+            for (int u = 0; u < NP; ++u) {
+              fma2(acc[n + u][0], acc[n + u][1], sg, part[u][0], part[u][1]);
+              fma2(acc[n + u][2], acc[n + u][3], sh, part[u][2], part[u][3]);
             }
           }
         }
       }
+      load(buf[d]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive1(&empty[s]);  // this warp has read the stage
+      // the stage that the group read a chunk ago takes the next chunk
+      if (producer && ok && it >= 1 && put < total) {
+        const int e = (it - 1) % kTileStages;
+        if (wait_limited(&empty[e], ((it - 1) / kTileStages) & 1)) {
+          inputs();
+        } else {
+          ok = false;
+          stop = 1;
+        }
+      }
       if (++chunk < nc) continue;
-      // the pass ends: the groups' sums are added in their order
+      // the tiles are through: the groups' sums are added in their order
       if (a.kq > 1) {
-        float* mine = red + ((kq - 1) * wm_n + wm) * (R * NT * 4 * 32) + lane;
+        float* mine = red + ((kq - 1) * group + wm) * (NT * 4 * 32) + lane;
         __syncthreads();
         if (kq > 0) {
 #pragma unroll
-          for (int r = 0; r < R; ++r)
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) mine[((r * NT + n) * 4 + i) * 32] = acc[r][n][i];
+            for (int i = 0; i < 4; ++i) mine[(n * 4 + i) * 32] = acc[n][i];
         }
         __syncthreads();
         if (kq == 0) {
           for (int o = 1; o < a.kq; ++o) {
-            const float* from = red + ((o - 1) * wm_n + wm) * (R * NT * 4 * 32) + lane;
+            const float* from = red + ((o - 1) * group + wm) * (NT * 4 * 32) + lane;
 #pragma unroll
-            for (int r = 0; r < R; ++r)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-              for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[r][n][i] += from[((r * NT + n) * 4 + i) * 32];
+              for (int i = 0; i < 4; ++i) acc[n][i] += from[(n * 4 + i) * 32];
           }
         }
       }
-      if (kq == 0) {
+      if (kq == 0 && ok && !*const_cast<volatile int*>(&stop) && tile < tile1) {
+        const int o = tile * kQ4Rows + g;
+        float bias[2] = {0.0f, 0.0f};
+        if (m.bias) {
+          if (o < m.outs) bias[0] = m.bias[o];
+          if (o + 8 < m.outs) bias[1] = m.bias[o + 8];
+        }
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
+        for (int n = 0; n < NT; ++n) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int o = (first + r) * kQ4Rows + g + 8 * h;
-            const bool in = first + r < tile1 && o < m.outs;
-            const float bias = in && m.bias ? m.bias[o] : 0.0f;
+          for (int u = 0; u < 2 / PARTS; ++u) {
+            const int tok = PARTS == 2 ? n * 4 + t : n * 8 + 2 * t + u;
+            if (tok >= a.tokens) continue;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              const float u = acc[r][n][2 * h], v = acc[r][n][2 * h + 1];
-              if (SPLIT) {  // columns 0, 1, 2 and 3, 4, 5 are the parts of one token each
-                const float u1 = __shfl_down_sync(0xffffffffu, u, 1), v1 = __shfl_down_sync(0xffffffffu, v, 1);
-                const float sum = t == 0 ? u + (v + u1) : v + (u1 + v1);
-                const int tok = 2 * n + t;
-                if (in && t < 2 && tok < a.tokens) q4_store(a, tok, o, sum + bias);
-              } else {
-                const int tok = n * 8 + 2 * t;
-                if (in && tok < a.tokens) q4_store(a, tok, o, u + bias);
-                if (in && tok + 1 < a.tokens) q4_store(a, tok + 1, o, v + bias);
-              }
+            for (int h = 0; h < 2; ++h) {
+              if (o + 8 * h >= m.outs) continue;
+              float v = PARTS == 2 ? fmaf(acc[n][2 * h + 1], 1.0f / 2048.0f, acc[n][2 * h]) : acc[n][2 * h + u];
+              if (XT != kOpsF16) v = v * back[tok].x * back[tok].y;
+              q4_store(a, tok, o + 8 * h, m.bias ? v + bias[h] : v);
             }
           }
         }
       }
 #pragma unroll
-      for (int r = 0; r < R; ++r)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[r][n][i] = 0.0f;
+        for (int i = 0; i < 4; ++i) acc[n][i] = 0.0f;
       chunk = 0;
-      ++pass;
+      tile += group;
     }
+  }
+  // No copy may be in flight when the CTA's shared memory goes away: those of
+  // every chunk that was waited for have come; after a wait that ran out, the
+  // rest is waited for, again with a limit.
+  if (!ok) {
+    atomicOr(&g_ops_status, kErrOpsWait);
+    if (producer)
+      for (int it = max(0, put - kTileStages); it < put; ++it)
+        (void)wait_limited(&full[it % kTileStages], (it / kTileStages) & 1);
   }
 }
 
+// SMs of the current device (the handle's, in the calls on one).
 int sm_count() {
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   return sms;
 }
 
-cudaError_t launch_q4_kernel(void (*kernel)(Q4Kernel), const Q4Kernel& a, int grid, int smem, cudaStream_t s) {
+template <class K, class... A>
+cudaError_t launch_chained(K kernel, int grid, int threads, int smem, cudaStream_t s, const A&... a) {
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
   }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kThreadsQ4);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute at{};
@@ -666,60 +809,94 @@ cudaError_t launch_q4_kernel(void (*kernel)(Q4Kernel), const Q4Kernel& a, int gr
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, a);
+  return cudaLaunchKernelEx(&cfg, kernel, a...);
 }
 
-template <bool BF16, bool SPLIT, int NT, int SETS, bool ZP>
-cudaError_t run_rows(const Q4Kernel& a, cudaStream_t s) {
-  const int smem = 3 * kWarpsQ4 * NT * 512 + a.cols * a.xstride;
-  const int per_sm = NT <= 2 && smem <= 110 * 1024 ? 2 : 1;
-  return launch_q4_kernel(q4_kernel<BF16, SPLIT, NT, SETS, ZP>, a, std::min(a.m.ntile, sm_count() * per_sm), smem, s);
+size_t back_bytes(int n) { return (static_cast<size_t>(n) * sizeof(float2) + 1023) & ~static_cast<size_t>(1023); }
+
+constexpr int kRowsSmem = 110 * 1024;  // two CTAs of q4_kernel per SM
+int rows_smem(const Q4Mat& m, int cols) { return 3 * kWarpsQ4 * 512 + cols * (m.nkc * kQ4Chunk * 2 + 64); }
+
+// How a call goes: q4_kernel at once, or q4_tile_kernel in passes of `cols` columns.
+struct Q4Plan {
+  bool tiles;
+  int cols, per_pass, passes;
+};
+Q4Plan plan_q4(const Q4Mat& m, int n, int x_type) {
+  const int per = x_type == kOpsF32 ? 2 : 1;
+  Q4Plan p{};
+  const long long cols = static_cast<long long>(n) * per;
+  p.tiles = cols > 8 || rows_smem(m, static_cast<int>(cols)) > kRowsSmem;
+  p.cols = cols <= 8 ? 8 : cols <= 16 ? 16 : cols <= 32 ? 32 : 64;
+  p.per_pass = p.cols / per;
+  p.passes = (n + p.per_pass - 1) / p.per_pass;
+  return p;
+}
+
+template <int XT, int SETS, bool ZP>
+cudaError_t run_rows(const Q4Kernel& a, int sms, cudaStream_t s) {
+  const int smem = rows_smem(a.m, a.tokens * kPartsOf<XT>);
+  return launch_chained(q4_kernel<XT, SETS, ZP>, std::min(a.m.ntile, sms * 2), kThreadsQ4, smem, s, a);
 }
 
 // Groups of warps along the inputs: the fewest that give every SM a CTA.
-template <bool BF16, bool SPLIT, int NT, int SETS, bool ZP>
-cudaError_t run_tiles(Q4Kernel a, cudaStream_t s) {
-  const int sms = sm_count();
-  auto ctas = [&](int kq) { return (a.m.ntile + kTileRun * kWarpsQ4 / kq - 1) / (kTileRun * kWarpsQ4 / kq); };
+template <int XT, int NT, int SETS, bool ZP>
+cudaError_t run_tiles(Q4Kernel a, int sms, cudaStream_t s) {
+  auto ctas = [&](int kq) { return (a.m.ntile + kWarpsQ4 / kq - 1) / (kWarpsQ4 / kq); };
   auto bytes = [&](int kq) {
-    return kq * kTileBufs * NT * 8 * kTileX + (kq - 1) * (kWarpsQ4 / kq) * kTileRun * NT * 512;
+    return kq * kTileStages * (NT * 2048) + (kq - 1) * (kWarpsQ4 / kq) * NT * 512;
   };
   a.kq = 1;
-  while (a.kq < kWarpsQ4 && 2 * a.kq <= a.m.nkc && ctas(a.kq) < sms && bytes(2 * a.kq) <= 220 * 1024) a.kq *= 2;
-  const int per_sm = NT <= 2 && bytes(a.kq) <= 110 * 1024 ? 2 : 1;
-  return launch_q4_kernel(q4_tile_kernel<BF16, SPLIT, NT, SETS, ZP>, a, std::min(ctas(a.kq), sms * per_sm), bytes(a.kq),
-                          s);
+  while (a.kq < kWarpsQ4 && 2 * a.kq <= a.m.nkc && ctas(a.kq) < 2 * sms && bytes(2 * a.kq) <= 220 * 1024) a.kq *= 2;
+  const int per_sm = std::max(1, std::min(kTileCtas<NT, SETS>, 226 * 1024 / (bytes(a.kq) + 2048)));
+  return launch_chained(q4_tile_kernel<XT, NT, SETS, ZP>, std::min(ctas(a.kq), sms * per_sm), kThreadsQ4, bytes(a.kq), s,
+                        a);
 }
 
-template <bool BF16, bool SPLIT, int NT, bool TILES>
-cudaError_t pick_sets(const Q4Kernel& a, cudaStream_t s) {
-  const int sets = kQ4Chunk / a.m.span;
-  auto run = [&](auto n, auto zp) {
-    if constexpr (TILES)
-      return run_tiles<BF16, SPLIT, NT, decltype(n)::value, decltype(zp)::value>(a, s);
-    else
-      return run_rows<BF16, SPLIT, NT, decltype(n)::value, decltype(zp)::value>(a, s);
-  };
+template <class F>
+cudaError_t with_sets(const Q4Mat& m, F&& f) {
   using std::integral_constant;
-  auto zeros = [&](auto n) {
-    return a.m.zeros ? run(n, integral_constant<bool, true>{}) : run(n, integral_constant<bool, false>{});
+  auto zeros = [&](auto sets) {
+    return m.zeros ? f(sets, integral_constant<bool, true>{}) : f(sets, integral_constant<bool, false>{});
   };
+  const int sets = kQ4Chunk / m.span;
   return sets == 4   ? zeros(integral_constant<int, 4>{})
          : sets == 2 ? zeros(integral_constant<int, 2>{})
                      : zeros(integral_constant<int, 1>{});
 }
 
-template <bool BF16, bool SPLIT>
-cudaError_t pick_cols(const Q4Kernel& a, bool tiles, cudaStream_t s) {
-  const int nt = (a.tokens + (SPLIT ? 1 : 7)) / (SPLIT ? 2 : 8);
-  if (!tiles) {
-    if (nt <= 1) return pick_sets<BF16, SPLIT, 1, false>(a, s);
-    return pick_sets<BF16, SPLIT, 2, false>(a, s);
+template <int XT>
+cudaError_t launch_typed(Q4Kernel a, const Q4Args& q, const Q4Plan& p, int sms, cudaStream_t st) {
+  if (!p.tiles) {
+    a.tokens = q.n;
+    return with_sets(a.m, [&](auto sets, auto zp) {
+      return run_rows<XT, decltype(sets)::value, decltype(zp)::value>(a, sms, st);
+    });
   }
-  if (nt <= 1) return pick_sets<BF16, SPLIT, 1, true>(a, s);
-  if (nt <= 2) return pick_sets<BF16, SPLIT, 2, true>(a, s);
-  if (nt <= 4) return pick_sets<BF16, SPLIT, 4, true>(a, s);
-  return pick_sets<BF16, SPLIT, 8, true>(a, s);
+  // the workspace: the factors, then the passes' images
+  unsigned char* w = static_cast<unsigned char*>(q.workspace);
+  const size_t image = static_cast<size_t>(a.m.nkc) * (p.cols * (kQ4Chunk * 2));
+  a.back = reinterpret_cast<float2*>(w);
+  a.image = w + back_bytes(q.n);
+  a.tokens = q.n;
+  cudaError_t e = launch_chained(q4_image_kernel<XT>, q.n, 256, 0, st, a, p.cols);
+  for (int i = 0; i < p.passes && e == cudaSuccess; ++i) {
+    Q4Kernel b = a;
+    const int first = i * p.per_pass;
+    b.tokens = std::min(p.per_pass, q.n - first);
+    b.y = static_cast<char*>(a.y) + first * q.ldy * ops_type_size(a.y_type);
+    b.back = a.back + first;
+    b.image = a.image + i * image;
+    e = with_sets(a.m, [&](auto sets, auto zp) {
+      constexpr int S = decltype(sets)::value;
+      constexpr bool Z = decltype(zp)::value;
+      return p.cols == 8    ? run_tiles<XT, 1, S, Z>(b, sms, st)
+             : p.cols == 16 ? run_tiles<XT, 2, S, Z>(b, sms, st)
+             : p.cols == 32 ? run_tiles<XT, 4, S, Z>(b, sms, st)
+                            : run_tiles<XT, 8, S, Z>(b, sms, st);
+    });
+  }
+  return e;
 }
 
 }  // namespace
@@ -729,10 +906,15 @@ void q4_layout(Q4Mat& m) {
   m.nkc = (m.ins + kQ4Chunk - 1) / kQ4Chunk;
   m.ntile = (m.outs + kQ4Rows - 1) / kQ4Rows;
   const int sets = kQ4Chunk / m.span;
-  m.chunk_bytes = 1024 + 32 * sets + (m.zeros ? 16 * sets : 0);
+  m.chunk_bytes = 1024 + 32 * sets + (m.zeros ? std::max(32, 16 * sets) : 0);
 }
 
 size_t q4_tiles_bytes(const Q4Mat& m) { return static_cast<size_t>(m.ntile) * m.nkc * m.chunk_bytes; }
+
+size_t q4_workspace_bytes(const Q4Mat& m, int n, int x_type) {
+  const Q4Plan p = plan_q4(m, n, x_type);
+  return p.tiles ? back_bytes(n) + static_cast<size_t>(p.passes) * m.nkc * (p.cols * (kQ4Chunk * 2)) : 0;
+}
 
 cudaError_t launch_q4_pack(const Q4Mat& m, const unsigned char* q, const uint16_t* s, const unsigned char* zeros,
                            unsigned char* tiles, cudaStream_t st) {
@@ -741,33 +923,28 @@ cudaError_t launch_q4_pack(const Q4Mat& m, const unsigned char* q, const uint16_
   return cudaGetLastError();
 }
 
-// Up to 8 columns (fp32: 16, 4 rows) whose x fits into shared memory take
-// q4_kernel; more, and the inputs that are too long for it, q4_tile_kernel in
-// passes of 64 columns (fp32: 16 rows).
 cudaError_t launch_q4(const Q4Mat& m, const Q4Args& q, int x_type, int y_type, cudaStream_t st) {
-  const bool split = x_type == kOpsF32;
-  const int per = split ? 2 : 8, parts = split ? 3 : 1;
   Q4Kernel a{};
   a.m = m;
-  a.xstride = m.nkc * kQ4Chunk * 2 + 64;
+  a.x = q.x;
   a.ldx = q.ldx;
+  a.y = q.y;
   a.ldy = q.ldy;
   a.y_type = y_type;
-  a.wide = reinterpret_cast<uintptr_t>(q.x) % 16 == 0 && q.ldx % 8 == 0;
-  const int nt = (q.n + per - 1) / per;
-  const bool tiles = nt > (split ? 2 : 1) || 3 * kWarpsQ4 * nt * 512 + q.n * parts * a.xstride > 110 * 1024;
-  const int most = 8 * per;
-  for (int i = 0; i < q.n; i += most) {
-    a.tokens = std::min(most, q.n - i);
-    a.cols = a.tokens * parts;
-    a.x = static_cast<const char*>(q.x) + i * q.ldx * ops_type_size(x_type);
-    a.y = static_cast<char*>(q.y) + i * q.ldy * ops_type_size(y_type);
-    const cudaError_t e = split                  ? pick_cols<true, true>(a, tiles, st)
-                          : x_type == kOpsBF16 ? pick_cols<true, false>(a, tiles, st)
-                                                 : pick_cols<false, false>(a, tiles, st);
-    if (e != cudaSuccess) return e;
-  }
-  return cudaSuccess;
+  a.wide = reinterpret_cast<uintptr_t>(q.x) % 16 == 0 && q.ldx * ops_type_size(x_type) % 16 == 0;
+  a.xstride = m.nkc * kQ4Chunk * 2 + 64;
+  const int sms = sm_count();
+  const Q4Plan p = plan_q4(m, q.n, x_type);
+  return x_type == kOpsF32    ? launch_typed<kOpsF32>(a, q, p, sms, st)
+         : x_type == kOpsBF16 ? launch_typed<kOpsBF16>(a, q, p, sms, st)
+                              : launch_typed<kOpsF16>(a, q, p, sms, st);
+}
+
+cudaError_t ops_read_status(unsigned* st, bool clear) {
+  cudaError_t e = cudaMemcpyFromSymbol(st, g_ops_status, sizeof(unsigned));
+  if (e != cudaSuccess || !clear || !*st) return e;
+  const unsigned z = 0;
+  return cudaMemcpyToSymbol(g_ops_status, &z, sizeof(unsigned));
 }
 
 }  // namespace vb

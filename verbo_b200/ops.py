@@ -59,7 +59,8 @@ def _ops():
             ("verbo_ops_token_logprobs", _I, [_P, _I, _I, _I, _L, ctypes.c_float, _P, _P, _P, _I, _P, _P, _P]),
             ("verbo_ops_q4_new", _P, [_I, _I, _I, _P, _P, _P, _P, _I, _P]),
             ("verbo_ops_q4_free", None, [_P]),
-            ("verbo_ops_q4_matvec", _I, [_P, _P, _I, _I, _L, _P, _I, _L, _P]),
+            ("verbo_ops_q4_workspace", _L, [_P, _I, _I]),
+            ("verbo_ops_q4_matvec", _I, [_P, _P, _I, _I, _L, _P, _I, _L, _P, _L, _P]),
         ):
             fn = getattr(lib, name)
             fn.restype, fn.argtypes = res, args
@@ -255,6 +256,7 @@ class Q4Linear:
         lib, torch, self._types = _ops()
         self._lib, self._torch = lib, torch
         self._h = None
+        self._need = {}  # workspace bytes by (rows, type)
 
         def hold(v, dtype, what):
             t = torch.as_tensor(v)
@@ -325,6 +327,15 @@ class Q4Linear:
             rows, ocols, ldy, yt, odev = _rows(out, self._types, "out")
             if rows != n or ocols != self.outs or odev != dev or (dtype is not None and dtype != out.dtype):
                 raise VerboCudaError(f"out must be [n, {self.outs}] on {self.device}")
-        if self._lib.verbo_ops_q4_matvec(self._h, x.data_ptr(), xt, n, ldx, out.data_ptr(), yt, ldy, at) < 0:
+        need = self._need.get((n, xt))
+        if need is None:
+            need = self._lib.verbo_ops_q4_workspace(self._h, xt, n)
+            if need < 0:
+                raise _err()
+            self._need[n, xt] = need
+        # the workspace belongs to the call's stream: freed here, it is reused behind the call
+        ws = _new(torch, x, stream, need, None, torch.uint8) if need else None
+        if self._lib.verbo_ops_q4_matvec(self._h, x.data_ptr(), xt, n, ldx, out.data_ptr(), yt, ldy,
+                                         ws.data_ptr() if need else None, need, at) < 0:
             raise _err()
         return out
