@@ -793,10 +793,13 @@ int sm_count() {
   return sms;
 }
 
+// limit: the most shared memory that calls of the kernel ask for.  The attribute
+// is set to it and not to the call's own size, which a call of another thread
+// could lower between here and the launch.
 template <class K, class... A>
-cudaError_t launch_chained(K kernel, int grid, int threads, int smem, cudaStream_t s, const A&... a) {
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+cudaError_t launch_chained(K kernel, int grid, int threads, int smem, int limit, cudaStream_t s, const A&... a) {
+  if (limit > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, limit);
     if (e != cudaSuccess) return e;
   }
   cudaLaunchConfig_t cfg{};
@@ -815,6 +818,7 @@ cudaError_t launch_chained(K kernel, int grid, int threads, int smem, cudaStream
 size_t back_bytes(int n) { return (static_cast<size_t>(n) * sizeof(float2) + 1023) & ~static_cast<size_t>(1023); }
 
 constexpr int kRowsSmem = 110 * 1024;  // two CTAs of q4_kernel per SM
+constexpr int kTileSmem = 220 * 1024;  // of q4_tile_kernel
 int rows_smem(const Q4Mat& m, int cols) { return 3 * kWarpsQ4 * 512 + cols * (m.nkc * kQ4Chunk * 2 + 64); }
 
 // How a call goes: q4_kernel at once, or q4_tile_kernel in passes of `cols` columns.
@@ -836,7 +840,7 @@ Q4Plan plan_q4(const Q4Mat& m, int n, int x_type) {
 template <int XT, int SETS, bool ZP>
 cudaError_t run_rows(const Q4Kernel& a, int sms, cudaStream_t s) {
   const int smem = rows_smem(a.m, a.tokens * kPartsOf<XT>);
-  return launch_chained(q4_kernel<XT, SETS, ZP>, std::min(a.m.ntile, sms * 2), kThreadsQ4, smem, s, a);
+  return launch_chained(q4_kernel<XT, SETS, ZP>, std::min(a.m.ntile, sms * 2), kThreadsQ4, smem, kRowsSmem, s, a);
 }
 
 // Groups of warps along the inputs: the fewest that give every SM a CTA.
@@ -847,10 +851,10 @@ cudaError_t run_tiles(Q4Kernel a, int sms, cudaStream_t s) {
     return kq * kTileStages * (NT * 2048) + (kq - 1) * (kWarpsQ4 / kq) * NT * 512;
   };
   a.kq = 1;
-  while (a.kq < kWarpsQ4 && 2 * a.kq <= a.m.nkc && ctas(a.kq) < 2 * sms && bytes(2 * a.kq) <= 220 * 1024) a.kq *= 2;
+  while (a.kq < kWarpsQ4 && 2 * a.kq <= a.m.nkc && ctas(a.kq) < 2 * sms && bytes(2 * a.kq) <= kTileSmem) a.kq *= 2;
   const int per_sm = std::max(1, std::min(kTileCtas<NT, SETS>, 226 * 1024 / (bytes(a.kq) + 2048)));
-  return launch_chained(q4_tile_kernel<XT, NT, SETS, ZP>, std::min(ctas(a.kq), sms * per_sm), kThreadsQ4, bytes(a.kq), s,
-                        a);
+  return launch_chained(q4_tile_kernel<XT, NT, SETS, ZP>, std::min(ctas(a.kq), sms * per_sm), kThreadsQ4, bytes(a.kq),
+                        kTileSmem, s, a);
 }
 
 template <class F>
@@ -879,7 +883,7 @@ cudaError_t launch_typed(Q4Kernel a, const Q4Args& q, const Q4Plan& p, int sms, 
   a.back = reinterpret_cast<float2*>(w);
   a.image = w + back_bytes(q.n);
   a.tokens = q.n;
-  cudaError_t e = launch_chained(q4_image_kernel<XT>, q.n, 256, 0, st, a, p.cols);
+  cudaError_t e = launch_chained(q4_image_kernel<XT>, q.n, 256, 0, 0, st, a, p.cols);
   for (int i = 0; i < p.passes && e == cudaSuccess; ++i) {
     Q4Kernel b = a;
     const int first = i * p.per_pass;
