@@ -85,7 +85,7 @@ constexpr int kProcSlice = kProcThreads * kProcCols;  // 4096
 constexpr int kProcHist = 4, kProcBias = 1;           // ids per thread in registers
 
 template <class T, bool LISTS, bool INPLACE>
-__global__ void __launch_bounds__(kProcThreads, 4) process_kernel(const ProcArgs a) {
+__global__ void __launch_bounds__(kProcThreads, !LISTS && INPLACE ? 8 : 4) process_kernel(const ProcArgs a) {
   constexpr int N = Vec<T>::N, NT = kProcThreads, V = kProcCols / N, S = kProcSlice;
   constexpr uint32_t kAll = (1u << N) - 1;
   constexpr int kNone = -(1 << 30);  // an id that lies in no slice
@@ -718,7 +718,10 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprob_kernel(const LogprobArg
       const int v = v0 + (g * NV + k) * NT + hits[h] % NT;
       if (v >= v1) continue;
       Vec<T> r;
-      r.raw = *reinterpret_cast<const uint4*>(vin + static_cast<long long>(v) * N);
+      if (nbatch <= kLpStages)  // still in the ring
+        r.raw = ring[(g * NV + k) * NT + hits[h] % NT];
+      else
+        r.raw = *reinterpret_cast<const uint4*>(vin + static_cast<long long>(v) * N);
 #pragma unroll
       for (int j = 0; j < N; ++j)
         if (r.get(j) >= thr) {

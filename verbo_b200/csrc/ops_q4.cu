@@ -543,23 +543,26 @@ __global__ void __launch_bounds__(256) q4_image_kernel(const Q4Kernel a, int col
 // More than 8 columns, or inputs too long for q4_kernel.  A CTA is kq groups of
 // warps that split the inputs among them; in a group each warp has a tile (16
 // outputs) times all columns at a time, its weights coming straight to registers,
-// two chunks ahead.  One thread of the group streams chunks of x (its image, one
+// half a chunk at a time.  One thread of the group streams chunks of x (its image, one
 // bulk copy each) through a ring of stages (full / empty barriers).  A set's sums
 // are scaled when it ends, 64 inputs at most, so that its fragments stay in
 // registers; two column tiles go through the tensor pipe side by side.
 //
 // What bounds it is not memory but the pipes behind mma.sync: measured on B200, an
 // m16n8k16 takes 8.6 cycles of a quarter SM, and two of them (a group of 32) with
-// the four fmas of their scale 25.  tcgen05.mma does not help here: a group's sums
-// have to leave tensor memory before the next scale, 2 values per weight at 64
-// columns and groups of 32, and weights that are unpacked into tensor memory go
-// there at about 28 bytes per cycle and SM: a kernel built that way took 92 us for
-// 64 rows of a 151936 x 896 head in groups of 32 (this one 91) and 43 us for 16
+// their load and the fmas of their scale 19.6: 37 us of the 85 that 64 rows of a
+// 151936 x 896 head take; unpacking and waiting make the rest.  tcgen05.mma does
+// not help here: a group's sums have to leave tensor memory before the next scale,
+// 2 values per weight at 64 columns and groups of 32, and weights that are unpacked
+// into tensor memory go there at about 28 bytes per cycle and SM: a kernel built
+// that way, five warps to 128 outputs, took 92 us for
+// 64 rows of a 151936 x 896 head in groups of 32 (this one 85) and 43 us for 16
 // (this one 35.5).
 constexpr int kTileStages = 4;
+constexpr int kTileAhead = 2;  // half chunks of weights in flight per warp (four: 0 to 2 us slower)
 // CTAs per SM.  More of them hide more, at fewer registers: 16 rows of a 151936 x
 // 896 head in groups of 32 took 35.5 us with three and 39 with two, of a 14336 x
-// 4096 matrix in groups of 64 (longer chains of fragments) 25 and 21.
+// 4096 matrix in groups of 64 (longer chains of fragments) 25.1 and 22.5.
 template <int NT, int SETS>
 constexpr int kTileCtas = NT <= 4 && SETS == 4 ? 3 : 2;
 
@@ -585,10 +588,36 @@ __device__ __forceinline__ bool wait_limited(uint64_t* bar, uint32_t phase) {
     }
   }
 }
-__device__ __forceinline__ Q4Zero zero_at(const unsigned char* p) {
-  const uint32_t v = *reinterpret_cast<const uint16_t*>(p);
-  return Q4Zero(v & 15u, v >> 8);
-}
+// What one lane holds of half a chunk: 64 inputs, one set or two.
+template <int SETS, bool ZP>
+struct Q4Half {
+  static constexpr int ND = SETS == 4 ? 2 : 1;
+  uint4 w;
+  uint32_t s[ND], z;
+  __device__ __forceinline__ uint32_t word(int j) const { return j == 0 ? w.x : j == 1 ? w.y : j == 2 ? w.z : w.w; }
+  // half h of the chunk at p
+  __device__ __forceinline__ void load(const unsigned char* p, int h, int lane) {
+    w = ld_stream16(p + h * 512 + lane * 16);
+    const unsigned char* tail = p + 1024;
+    const int set = (lane >> 2) * SETS + (SETS == 1 ? 0 : h * ND);
+    if constexpr (ND == 2) {
+      const uint2 v = __ldg(reinterpret_cast<const uint2*>(tail + set * 4));
+      s[0] = v.x, s[1] = v.y;
+      if constexpr (ZP) z = __ldg(reinterpret_cast<const unsigned*>(tail + 32 * SETS + set * 2));
+    } else {
+      s[0] = __ldg(reinterpret_cast<const unsigned*>(tail + set * 4));
+      if constexpr (ZP) z = __ldg(reinterpret_cast<const unsigned short*>(tail + 32 * SETS + set * 2));
+    }
+  }
+  __device__ __forceinline__ Q4Zero zero(int d) const {
+    if (!ZP) return Q4Zero(8u, 8u);
+    const uint32_t v = z >> (16 * d);
+    return Q4Zero(v & 15u, (v >> 8) & 15u);
+  }
+  __device__ __forceinline__ float2 scale(int d) const {
+    return __half22float2(*reinterpret_cast<const __half2*>(&s[d]));
+  }
+};
 
 template <int XT, int NT, int SETS, bool ZP>
 __global__ void __launch_bounds__(kThreadsQ4, kTileCtas<NT, SETS>) q4_tile_kernel(const Q4Kernel a) {
@@ -619,20 +648,21 @@ __global__ void __launch_bounds__(kThreadsQ4, kTileCtas<NT, SETS>) q4_tile_kerne
   __syncthreads();
 
   // the weights are the handle's; x comes from the grid before
-  Q4Buf<SETS, ZP> buf[2];
-  int load_tile = tile0 + wm, load_chunk = 0;
+  constexpr int AHEAD = kTileAhead;
+  Q4Half<SETS, ZP> buf[AHEAD];
+  int load_tile = tile0 + wm, load_half = 0;
   const unsigned char* load_at = m.tiles + (static_cast<long long>(load_tile) * m.nkc + c0) * m.chunk_bytes;
-  auto load = [&](Q4Buf<SETS, ZP>& b) {
-    if (load_tile < tile1) b.load(load_at, lane);
-    load_at += m.chunk_bytes;
-    if (++load_chunk == nc) {
-      load_chunk = 0;
+  auto load = [&](Q4Half<SETS, ZP>& b, int h) {  // h: load_half & 1
+    if (load_tile < tile1) b.load(load_at, h, lane);
+    if (h == 1) load_at += m.chunk_bytes;
+    if (++load_half == 2 * nc) {
+      load_half = 0;
       load_tile += group;
       load_at += (static_cast<long long>(group) * m.nkc - nc) * m.chunk_bytes;
     }
   };
-  load(buf[0]);
-  load(buf[1]);
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) load(buf[i], i & 1);
   int put = 0, put_chunk = 0;  // the next chunk of x
   auto inputs = [&]() {
     const int s = put % kTileStages;
@@ -656,31 +686,79 @@ __global__ void __launch_bounds__(kThreadsQ4, kTileCtas<NT, SETS>) q4_tile_kerne
 
   bool ok = true;
   int chunk = 0, tile = tile0 + wm;
-  for (int it0 = 0; it0 < total; it0 += 2) {
+  // The tiles are through: the groups' sums are added in their order.
+  auto finish = [&]() {
+    if (a.kq > 1) {
+      float* mine = red + ((kq - 1) * group + wm) * (NT * 4 * 32) + lane;
+      __syncthreads();
+      if (kq > 0) {
 #pragma unroll
-    for (int d = 0; d < 2; ++d) {
-      const int it = it0 + d;
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mine[(n * 4 + i) * 32] = acc[n][i];
+      }
+      __syncthreads();
+      if (kq == 0) {
+        for (int o = 1; o < a.kq; ++o) {
+          const float* from = red + ((o - 1) * group + wm) * (NT * 4 * 32) + lane;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[n][i] += from[(n * 4 + i) * 32];
+        }
+      }
+    }
+    if (kq == 0 && ok && !*const_cast<volatile int*>(&stop) && tile < tile1) {
+      const int o = tile * kQ4Rows + g;
+      float bias[2] = {0.0f, 0.0f};
+      if (m.bias) {
+        if (o < m.outs) bias[0] = m.bias[o];
+        if (o + 8 < m.outs) bias[1] = m.bias[o + 8];
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int u = 0; u < 2 / PARTS; ++u) {
+          const int tok = PARTS == 2 ? n * 4 + t : n * 8 + 2 * t + u;
+          if (tok >= a.tokens) continue;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (o + 8 * h >= m.outs) continue;
+            float v = PARTS == 2 ? fmaf(acc[n][2 * h + 1], 1.0f / 2048.0f, acc[n][2 * h]) : acc[n][2 * h + u];
+            if (XT != kOpsF16) v = v * back[tok].x * back[tok].y;
+            q4_store(a, tok, o + 8 * h, m.bias ? v + bias[h] : v);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[n][i] = 0.0f;
+  };
+  for (int it0 = 0; it0 < total; it0 += AHEAD / 2) {
+#pragma unroll
+    for (int d = 0; d < AHEAD; ++d) {
+      const int it = it0 + d / 2, half = d & 1;
       if (it >= total) break;
       const int s = it % kTileStages;
       // A wait that runs out ends the products of the warp, not its barriers, and
       // nothing of the CTA is stored any more.
-      if (ok && !wait_limited(&full[s], (it / kTileStages) & 1)) {
+      if (half == 0 && ok && !wait_limited(&full[s], (it / kTileStages) & 1)) {
         ok = false;
         stop = 1;
       }
       if (ok && tile < tile1) {
-        const unsigned char* xc = ring + s * XB + lane * 16;
-        constexpr int Q = SETS < 2 ? 2 : SETS;  // scaled together: at most 64 inputs
-        constexpr int BLK = 4 / Q;
-        constexpr int NP = NT < 2 ? NT : 2;  // column tiles side by side
+        const unsigned char* xc = ring + s * XB + half * 1024 + lane * 16;
+        constexpr int ND = Q4Half<SETS, ZP>::ND, BLK = 2 / ND;  // sets, 32-blocks of each
+        constexpr int NP = NT < 2 ? NT : 2;                      // column tiles side by side
 #pragma unroll
-        for (int q = 0; q < Q; ++q) {
-          const int set = q * SETS / Q;
-          const Q4Zero z = buf[d].zero(set);
+        for (int q = 0; q < ND; ++q) {
+          const Q4Zero z = buf[d].zero(q);
           uint32_t fa[2 * BLK][4];
 #pragma unroll
           for (int j = 0; j < 2 * BLK; ++j) unpack(buf[d].word(2 * BLK * q + j), z, fa[j]);
-          const float2 sc = buf[d].scale(set);
+          const float2 sc = buf[d].scale(q);
           const uint64_t sg = twice(sc.x), sh = twice(sc.y);
 #pragma unroll
           for (int n = 0; n < NT; n += NP) {
@@ -709,7 +787,8 @@ __global__ void __launch_bounds__(kThreadsQ4, kTileCtas<NT, SETS>) q4_tile_kerne
           }
         }
       }
-      load(buf[d]);
+      load(buf[d], half);
+      if (half == 0) continue;
       __syncwarp();
       if (lane == 0) mbar_arrive1(&empty[s]);  // this warp has read the stage
       // the stage that the group read a chunk ago takes the next chunk
@@ -722,57 +801,11 @@ __global__ void __launch_bounds__(kThreadsQ4, kTileCtas<NT, SETS>) q4_tile_kerne
           stop = 1;
         }
       }
-      if (++chunk < nc) continue;
-      // the tiles are through: the groups' sums are added in their order
-      if (a.kq > 1) {
-        float* mine = red + ((kq - 1) * group + wm) * (NT * 4 * 32) + lane;
-        __syncthreads();
-        if (kq > 0) {
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) mine[(n * 4 + i) * 32] = acc[n][i];
-        }
-        __syncthreads();
-        if (kq == 0) {
-          for (int o = 1; o < a.kq; ++o) {
-            const float* from = red + ((o - 1) * group + wm) * (NT * 4 * 32) + lane;
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) acc[n][i] += from[(n * 4 + i) * 32];
-          }
-        }
+      if (++chunk == nc) {
+        finish();
+        chunk = 0;
+        tile += group;
       }
-      if (kq == 0 && ok && !*const_cast<volatile int*>(&stop) && tile < tile1) {
-        const int o = tile * kQ4Rows + g;
-        float bias[2] = {0.0f, 0.0f};
-        if (m.bias) {
-          if (o < m.outs) bias[0] = m.bias[o];
-          if (o + 8 < m.outs) bias[1] = m.bias[o + 8];
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-#pragma unroll
-          for (int u = 0; u < 2 / PARTS; ++u) {
-            const int tok = PARTS == 2 ? n * 4 + t : n * 8 + 2 * t + u;
-            if (tok >= a.tokens) continue;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              if (o + 8 * h >= m.outs) continue;
-              float v = PARTS == 2 ? fmaf(acc[n][2 * h + 1], 1.0f / 2048.0f, acc[n][2 * h]) : acc[n][2 * h + u];
-              if (XT != kOpsF16) v = v * back[tok].x * back[tok].y;
-              q4_store(a, tok, o + 8 * h, m.bias ? v + bias[h] : v);
-            }
-          }
-        }
-      }
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[n][i] = 0.0f;
-      chunk = 0;
-      tile += group;
     }
   }
   // No copy may be in flight when the CTA's shared memory goes away: those of
