@@ -255,9 +255,19 @@ struct X8 {
     else
       return __half2float(__ushort_as_half(static_cast<unsigned short>(v[i >> 1] >> (16 * (i & 1)))));
   }
-  // the largest magnitude among the finite values, as bits
+  // the largest magnitude among the finite values, as bits of a float
   __device__ __forceinline__ uint32_t largest() const {
     uint32_t m = 0;
+    if constexpr (XT == kOpsF32) {
+#pragma unroll
+      for (uint32_t u : v) m = max(m, u & 0x7fffffffu);
+    } else {
+#pragma unroll
+      for (uint32_t u : v) m = __vmaxu2(m, u & 0x7fff7fffu);
+      m = XT == kOpsBF16 ? max(m << 16, m & 0xffff0000u) : 0;
+    }
+    if (m < 0x7f800000u) return m;
+    m = 0;  // an infinity or a NaN is among them
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const uint32_t u = __float_as_uint(get(i)) & 0x7fffffffu;
@@ -273,7 +283,11 @@ struct X8 {
       uint32_t h[4], l[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float a = get(2 * i) * up * up2, b = get(2 * i + 1) * up * up2;
+        float a = get(2 * i) * up, b = get(2 * i + 1) * up;
+        if (up2 != 1.0f) {
+          a *= up2;
+          b *= up2;
+        }
         const __half2 p = __floats2half2_rn(a, b);
         h[i] = *reinterpret_cast<const uint32_t*>(&p);
         const float2 q = __half22float2(p);
@@ -288,8 +302,8 @@ struct X8 {
   }
 };
 
-// The power of two that takes a largest magnitude (as bits) to [2^14, 2^15), in
-// two factors that fp32 holds, and its inverse.
+// The power of two that takes a largest magnitude (as bits) to [2^14, 2^15), and
+// its inverse, each in two factors that fp32 holds, the second mostly 1.
 struct Power {
   float up, up2, down, down2;
   __device__ __forceinline__ explicit Power(uint32_t largest) {
@@ -299,7 +313,7 @@ struct Power {
       frexpf(__uint_as_float(largest), &x);  // value in [2^(x-1), 2^x)
       e = 15 - x;
     }
-    const int h = e / 2;
+    const int h = e > 120 || e < -120 ? e / 2 : e;
     up = two(h), up2 = two(e - h), down = two(-h), down2 = two(h - e);
   }
   static __device__ __forceinline__ float two(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
@@ -356,38 +370,45 @@ __global__ void __launch_bounds__(kThreadsQ4, 2) q4_kernel(const Q4Kernel a) {
   if (XT != kOpsF16 && tid < 8) largest[tid] = 0;
   if (XT != kOpsF16) __syncthreads();
   grid_wait();  // the weights are the handle's; x comes from the grid before
+  // x: eight inputs per thread at a time, a few loads in flight; the warps are dealt
+  // to the tokens in equal numbers (of 3, 5, 6 and 7 tokens some warps have none)
+  constexpr int ES = XT == kOpsF32 ? 4 : 2, FLY = 4;
   const int kp = m.nkc * kQ4Chunk;
-  constexpr int ES = XT == kOpsF32 ? 4 : 2;
-  const char* x = static_cast<const char*>(a.x);
+  const int deal = a.tokens <= 1 ? 8 : a.tokens <= 2 ? 4 : a.tokens <= 4 ? 2 : 1;  // warps per token
+  const int tok = warp / deal, k0 = ((warp % deal) * 32 + lane) * 8, dk = deal * 256;
+  const char* row = static_cast<const char*>(a.x) + tok * a.ldx * ES;
+  auto each_unit = [&](auto&& f) {
+    for (int k = k0; k < kp; k += FLY * dk) {
+      X8<XT> v[FLY];
+#pragma unroll
+      for (int i = 0; i < FLY; ++i) v[i].load(row, k + i * dk, m.ins, a.wide);
+#pragma unroll
+      for (int i = 0; i < FLY; ++i)
+        if (k + i * dk < kp) f(v[i], k + i * dk);
+    }
+  };
   if (XT != kOpsF16) {
-    for (int tok = 0; tok < a.tokens; ++tok) {
+    if (tok < a.tokens) {
       uint32_t big = 0;
-      for (int k = tid * 8; k < m.ins; k += kThreadsQ4 * 8) {
-        X8<XT> v;
-        v.load(x + tok * a.ldx * ES, k, m.ins, a.wide);
-        big = max(big, v.largest());
-      }
+      each_unit([&](const X8<XT>& v, int) { big = max(big, v.largest()); });
       big = __reduce_max_sync(0xffffffffu, big);
       if (lane == 0) atomicMax(&largest[tok], big);
     }
     __syncthreads();
   }
-  for (int tok = 0; tok < a.tokens; ++tok) {
-    float up = 1.0f, up2 = 1.0f;
+  if (tok < a.tokens) {
+    Power p(0);
     if (XT != kOpsF16) {
-      const Power p(largest[tok]);
-      up = p.up, up2 = p.up2;
-      if (tid == 0) back[tok] = make_float2(p.down, p.down2);
+      p = Power(largest[tok]);
+      if (k0 == 0) back[tok] = make_float2(p.down, p.down2);
     }
     unsigned char* at = xs + static_cast<size_t>(PARTS * tok) * a.xstride;
-    for (int k = tid * 8; k < kp; k += kThreadsQ4 * 8) {
-      X8<XT> v;
-      v.load(x + tok * a.ldx * ES, k, m.ins, a.wide);
+    each_unit([&](const X8<XT>& v, int k) {
       uint4 hi, lo;
-      v.columns(up, up2, hi, lo);
+      v.columns(p.up, p.up2, hi, lo);
       *reinterpret_cast<uint4*>(at + 2 * k) = hi;
       if (PARTS == 2) *reinterpret_cast<uint4*>(at + a.xstride + 2 * k) = lo;
-    }
+    });
   }
   __syncthreads();
 
