@@ -203,9 +203,9 @@ struct Q4Buf : Q4Tail<SETS, ZP> {
 
 struct Q4Kernel {
   Q4Mat m;
-  const void* x;  // the pass's first row
+  const void* x;
   long long ldx;
-  int tokens;  // rows of x in this pass
+  int tokens;  // rows of x
   void* y;
   long long ldy;
   int y_type;
@@ -216,6 +216,7 @@ struct Q4Kernel {
   unsigned char* image;
   float2* back;
   int kq;
+  int per_pass;  // tokens of a pass; blockIdx.y is the pass
 };
 
 template <int XT>
@@ -571,15 +572,14 @@ __global__ void __launch_bounds__(256) q4_image_kernel(const Q4Kernel a, int col
 //
 // What bounds it is not memory but the pipes behind mma.sync: measured on B200, an
 // m16n8k16 takes 8.6 cycles of a quarter SM, and two of them (a group of 32) with
-// their load and the fmas of their scale 19.6: 37 us of the 85 that 64 rows of a
+// their load and the fmas of their scale 19.6: 37 us of the 86 that 64 rows of a
 // 151936 x 896 head take; unpacking and waiting make the rest.  tcgen05.mma does
 // not help here: a group's sums have to leave tensor memory before the next scale,
 // 2 values per weight at 64 columns and groups of 32, and weights that are unpacked
-// into tensor memory go there at about 28 bytes per cycle and SM: a kernel built
-// that way, five warps to 128 outputs, took 92 us for
-// 64 rows of a 151936 x 896 head in groups of 32 (this one 85) and 43 us for 16
-// (this one 35.5).
-constexpr int kTileStages = 4;
+// into tensor memory went there at about 25 bytes per cycle and SM: a kernel built
+// that way, five warps to 128 outputs, took 92 us for 64 rows of a 151936 x 896 head
+// in groups of 32 (this one 86) and 43 us for 16 (this one 36).
+constexpr int kTileStages = 3;
 constexpr int kTileAhead = 2;  // half chunks of weights in flight per warp (four: 0 to 2 us slower)
 // CTAs per SM.  More of them hide more, at fewer registers: 16 rows of a 151936 x
 // 896 head in groups of 32 took 35.5 us with three and 39 with two, of a 14336 x
@@ -666,6 +666,8 @@ __global__ void __launch_bounds__(kThreadsQ4, kTileCtas<NT, SETS>) q4_tile_kerne
   const int passes = (tile1 - tile0 + group - 1) / group;
   const int total = passes * nc;
   const bool producer = wm == 0 && lane == 0;
+  const int tok0 = blockIdx.y * a.per_pass, tokens = min(a.per_pass, a.tokens - tok0);
+  const unsigned char* image = a.image + static_cast<size_t>(blockIdx.y) * m.nkc * XB;
   __syncthreads();
 
   // the weights are the handle's; x comes from the grid before
@@ -688,7 +690,7 @@ __global__ void __launch_bounds__(kThreadsQ4, kTileCtas<NT, SETS>) q4_tile_kerne
   auto inputs = [&]() {
     const int s = put % kTileStages;
     mbar_expect_tx(&full[s], XB);
-    bulk_copy(ring + s * XB, a.image + static_cast<size_t>(c0 + put_chunk) * XB, XB, &full[s]);
+    bulk_copy(ring + s * XB, image + static_cast<size_t>(c0 + put_chunk) * XB, XB, &full[s]);
     ++put;
     if (++put_chunk == nc) put_chunk = 0;
   };
@@ -696,7 +698,7 @@ __global__ void __launch_bounds__(kThreadsQ4, kTileCtas<NT, SETS>) q4_tile_kerne
   grid_wait();
   if (producer)
     while (put < min(kTileStages, total)) inputs();
-  if (tid < a.tokens) back[tid] = a.back[tid];
+  if (tid < tokens) back[tid] = a.back[tok0 + tid];
   __syncthreads();
 
   float acc[NT][4];
@@ -741,13 +743,13 @@ __global__ void __launch_bounds__(kThreadsQ4, kTileCtas<NT, SETS>) q4_tile_kerne
 #pragma unroll
         for (int u = 0; u < 2 / PARTS; ++u) {
           const int tok = PARTS == 2 ? n * 4 + t : n * 8 + 2 * t + u;
-          if (tok >= a.tokens) continue;
+          if (tok >= tokens) continue;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             if (o + 8 * h >= m.outs) continue;
             float v = PARTS == 2 ? fmaf(acc[n][2 * h + 1], 1.0f / 2048.0f, acc[n][2 * h]) : acc[n][2 * h + u];
             if (XT != kOpsF16) v = v * back[tok].x * back[tok].y;
-            q4_store(a, tok, o + 8 * h, m.bias ? v + bias[h] : v);
+            q4_store(a, tok0 + tok, o + 8 * h, m.bias ? v + bias[h] : v);
           }
         }
       }
@@ -851,13 +853,13 @@ int sm_count() {
 // is set to it and not to the call's own size, which a call of another thread
 // could lower between here and the launch.
 template <class K, class... A>
-cudaError_t launch_chained(K kernel, int grid, int threads, int smem, int limit, cudaStream_t s, const A&... a) {
+cudaError_t launch_chained(K kernel, dim3 grid, int threads, int smem, int limit, cudaStream_t s, const A&... a) {
   if (limit > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, limit);
     if (e != cudaSuccess) return e;
   }
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid);
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
@@ -875,19 +877,43 @@ constexpr int kRowsSmem = 110 * 1024;  // two CTAs of q4_kernel per SM
 constexpr int kTileSmem = 220 * 1024;  // of q4_tile_kernel
 int rows_smem(const Q4Mat& m, int cols) { return 3 * kWarpsQ4 * 512 + cols * (m.nkc * kQ4Chunk * 2 + 64); }
 
-// How a call goes: q4_kernel at once, or q4_tile_kernel in passes of `cols` columns.
+// CTAs of q4_tile_kernel along the outputs, and their shared memory, with kq groups
+// of warps and `cols` columns.
+int tile_ctas(const Q4Mat& m, int kq) { return (m.ntile + kWarpsQ4 / kq - 1) / (kWarpsQ4 / kq); }
+int tile_smem(int kq, int cols) { return kq * kTileStages * (cols * 256) + (kq - 1) * (kWarpsQ4 / kq) * cols * 64; }
+bool tile_fits(const Q4Mat& m, int kq, int cols) {
+  return kq <= kWarpsQ4 && kq <= m.nkc && tile_smem(kq, cols) <= kTileSmem;
+}
+
+// How a call goes: q4_kernel, or q4_tile_kernel in passes of `cols` columns with kq
+// groups of warps.  The columns go in one pass, up to 64 of them; but where that
+// leaves SMs without a CTA (few outputs), in more passes, which run side by side
+// and each unpack the weights: 28 fp32 rows of a 2145 x 7328 matrix took 42 us in
+// one pass and 22.7 in four.
 struct Q4Plan {
   bool tiles;
-  int cols, per_pass, passes;
+  int cols, per_pass, passes, kq;
 };
-Q4Plan plan_q4(const Q4Mat& m, int n, int x_type) {
+Q4Plan plan_q4(const Q4Mat& m, int n, int x_type, int sms) {
   const int per = x_type == kOpsF32 ? 2 : 1;
   Q4Plan p{};
   const long long cols = static_cast<long long>(n) * per;
   p.tiles = cols > 8 || rows_smem(m, static_cast<int>(cols)) > kRowsSmem;
-  p.cols = cols <= 8 ? 8 : cols <= 16 ? 16 : cols <= 32 ? 32 : 64;
-  p.per_pass = p.cols / per;
-  p.passes = (n + p.per_pass - 1) / p.per_pass;
+  if (!p.tiles) return p;
+  auto set = [&](int c) {
+    p.cols = c;
+    p.per_pass = c / per;
+    p.passes = (n + p.per_pass - 1) / p.per_pass;
+    int most = 1;
+    while (tile_fits(m, 2 * most, c)) most *= 2;
+    return static_cast<long long>(tile_ctas(m, most)) * p.passes;
+  };
+  int c = cols <= 8 ? 8 : cols <= 16 ? 16 : cols <= 32 ? 32 : 64;
+  while (set(c) < sms && c > 8) c /= 2;
+  // the fewest groups that give the SMs 3/2 CTAs each: more of them take more shared
+  // memory (64 rows of 4096 x 4096: 17.3 us, and 27 with two CTAs each asked for)
+  p.kq = 1;
+  while (static_cast<long long>(tile_ctas(m, p.kq)) * p.passes * 2 < 3 * sms && tile_fits(m, 2 * p.kq, p.cols)) p.kq *= 2;
   return p;
 }
 
@@ -897,18 +923,12 @@ cudaError_t run_rows(const Q4Kernel& a, int sms, cudaStream_t s) {
   return launch_chained(q4_kernel<XT, SETS, ZP>, std::min(a.m.ntile, sms * 2), kThreadsQ4, smem, kRowsSmem, s, a);
 }
 
-// Groups of warps along the inputs: the fewest that give every SM a CTA.
 template <int XT, int NT, int SETS, bool ZP>
-cudaError_t run_tiles(Q4Kernel a, int sms, cudaStream_t s) {
-  auto ctas = [&](int kq) { return (a.m.ntile + kWarpsQ4 / kq - 1) / (kWarpsQ4 / kq); };
-  auto bytes = [&](int kq) {
-    return kq * kTileStages * (NT * 2048) + (kq - 1) * (kWarpsQ4 / kq) * NT * 512;
-  };
-  a.kq = 1;
-  while (a.kq < kWarpsQ4 && 2 * a.kq <= a.m.nkc && ctas(a.kq) < 2 * sms && bytes(2 * a.kq) <= kTileSmem) a.kq *= 2;
-  const int per_sm = std::max(1, std::min(kTileCtas<NT, SETS>, 226 * 1024 / (bytes(a.kq) + 2048)));
-  return launch_chained(q4_tile_kernel<XT, NT, SETS, ZP>, std::min(ctas(a.kq), sms * per_sm), kThreadsQ4, bytes(a.kq),
-                        kTileSmem, s, a);
+cudaError_t run_tiles(const Q4Kernel& a, const Q4Plan& p, int sms, cudaStream_t s) {
+  const int smem = tile_smem(a.kq, p.cols);
+  const int per_sm = std::max(1, std::min(kTileCtas<NT, SETS>, 226 * 1024 / (smem + 2048)));
+  const int ctas = std::min(tile_ctas(a.m, a.kq), std::max(1, sms * per_sm / p.passes));
+  return launch_chained(q4_tile_kernel<XT, NT, SETS, ZP>, dim3(ctas, p.passes), kThreadsQ4, smem, kTileSmem, s, a);
 }
 
 template <class F>
@@ -933,28 +953,21 @@ cudaError_t launch_typed(Q4Kernel a, const Q4Args& q, const Q4Plan& p, int sms, 
   }
   // the workspace: the factors, then the passes' images
   unsigned char* w = static_cast<unsigned char*>(q.workspace);
-  const size_t image = static_cast<size_t>(a.m.nkc) * (p.cols * (kQ4Chunk * 2));
   a.back = reinterpret_cast<float2*>(w);
   a.image = w + back_bytes(q.n);
   a.tokens = q.n;
-  cudaError_t e = launch_chained(q4_image_kernel<XT>, q.n, 256, 0, 0, st, a, p.cols);
-  for (int i = 0; i < p.passes && e == cudaSuccess; ++i) {
-    Q4Kernel b = a;
-    const int first = i * p.per_pass;
-    b.tokens = std::min(p.per_pass, q.n - first);
-    b.y = static_cast<char*>(a.y) + first * q.ldy * ops_type_size(a.y_type);
-    b.back = a.back + first;
-    b.image = a.image + i * image;
-    e = with_sets(a.m, [&](auto sets, auto zp) {
-      constexpr int S = decltype(sets)::value;
-      constexpr bool Z = decltype(zp)::value;
-      return p.cols == 8    ? run_tiles<XT, 1, S, Z>(b, sms, st)
-             : p.cols == 16 ? run_tiles<XT, 2, S, Z>(b, sms, st)
-             : p.cols == 32 ? run_tiles<XT, 4, S, Z>(b, sms, st)
-                            : run_tiles<XT, 8, S, Z>(b, sms, st);
-    });
-  }
-  return e;
+  a.per_pass = p.per_pass;
+  a.kq = p.kq;
+  const cudaError_t e = launch_chained(q4_image_kernel<XT>, q.n, 256, 0, 0, st, a, p.cols);
+  if (e != cudaSuccess) return e;
+  return with_sets(a.m, [&](auto sets, auto zp) {
+    constexpr int S = decltype(sets)::value;
+    constexpr bool Z = decltype(zp)::value;
+    return p.cols == 8    ? run_tiles<XT, 1, S, Z>(a, p, sms, st)
+           : p.cols == 16 ? run_tiles<XT, 2, S, Z>(a, p, sms, st)
+           : p.cols == 32 ? run_tiles<XT, 4, S, Z>(a, p, sms, st)
+                          : run_tiles<XT, 8, S, Z>(a, p, sms, st);
+  });
 }
 
 }  // namespace
@@ -970,7 +983,7 @@ void q4_layout(Q4Mat& m) {
 size_t q4_tiles_bytes(const Q4Mat& m) { return static_cast<size_t>(m.ntile) * m.nkc * m.chunk_bytes; }
 
 size_t q4_workspace_bytes(const Q4Mat& m, int n, int x_type) {
-  const Q4Plan p = plan_q4(m, n, x_type);
+  const Q4Plan p = plan_q4(m, n, x_type, sm_count());
   return p.tiles ? back_bytes(n) + static_cast<size_t>(p.passes) * m.nkc * (p.cols * (kQ4Chunk * 2)) : 0;
 }
 
@@ -992,7 +1005,7 @@ cudaError_t launch_q4(const Q4Mat& m, const Q4Args& q, int x_type, int y_type, c
   a.wide = reinterpret_cast<uintptr_t>(q.x) % 16 == 0 && q.ldx * ops_type_size(x_type) % 16 == 0;
   a.xstride = m.nkc * kQ4Chunk * 2 + 64;
   const int sms = sm_count();
-  const Q4Plan p = plan_q4(m, q.n, x_type);
+  const Q4Plan p = plan_q4(m, q.n, x_type, sms);
   return x_type == kOpsF32    ? launch_typed<kOpsF32>(a, q, p, sms, st)
          : x_type == kOpsBF16 ? launch_typed<kOpsBF16>(a, q, p, sms, st)
                               : launch_typed<kOpsF16>(a, q, p, sms, st);
