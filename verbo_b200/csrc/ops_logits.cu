@@ -79,6 +79,14 @@ __device__ __forceinline__ int row_shift(const T* row) {
 // the window stay in registers over the slices, and the next slice's logits
 // and mask words are on their way while a slice is counted and stored.
 // In place nothing of the row is loaded but columns that change.
+//
+// The bound is memory: the row in, the row out, the mask's bits.  Four CTAs of 256
+// threads per SM with 16 columns per thread on their way; a slice of 4096 columns
+// has 16 KB of counters, so that lists cost no occupancy.  Measured on B200: 512
+// fp32 rows of 151936 with up to 1024 ids each 111 us, 5.6 TB/s (86% of the card's
+// copy rate); 256 bf16 rows with ids, biases and masks 49 us, 4.9 TB/s; 512 rows
+// masked in place 102 us, of which a third of the columns is written.  One slice
+// per CTA and the window read again for each took 160 and 92 us.
 constexpr int kProcThreads = 256;
 constexpr int kProcCols = 16;                         // columns per thread and slice
 constexpr int kProcSlice = kProcThreads * kProcCols;  // 4096
@@ -342,6 +350,14 @@ cudaError_t run_process(ProcArgs a, cudaStream_t s) {
 // Each thread copies its own vectors to shared memory (cp.async), two batches
 // ahead, and reads them back itself: no registers for what is in flight and no
 // barrier in the pass.
+//
+// Measured on B200: 512 fp32 rows of 151936 in 53 us, 5.9 TB/s (90% of the card's
+// copy rate).  256 bf16 rows with the 20 first take 26 us, 3.0 TB/s: about ten
+// instructions a column and an exponential unit of 16 lanes (9 us alone) bound it,
+// and 256 rows leave 40 of 148 SMs half empty; two CTAs a row (a cluster's
+// barriers, every first column found twice) take 34.7.  Clusters serve the few rows
+// that would leave SMs without work: one row of 49152 with the 5 first 9.2 us, 5.4
+// without them.
 constexpr int kLpThreads = 512;
 constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kLpVecs = 4;    // vectors per thread and batch

@@ -339,6 +339,15 @@ __device__ __forceinline__ void q4_store(const Q4Kernel& a, int token, int o, fl
 // bytes of a column (columns 64 mod 128 bytes apart: the 8 lanes of a quarter
 // warp hit 32 banks).  A tile whose chunks fall to several warps is summed over
 // the warps' partial sums in shared memory, in the order of the warps.
+//
+// Measured on B200: a 151936 x 896 matrix in groups of 32 times one fp32 row 20.5
+// us, 3.8 TB/s (57% of the card's copy rate): reading alone would take 11.8.  A
+// chunk costs a warp about 190 instructions, 72 of them the unpacking, and its
+// eight mma with their scaling 100 cycles of a quarter SM, against 198 in which memory
+// delivers it.  About 4 us are start and end: 4096 x 4096 takes 6.4 us, 896 x 896
+// 4.  Sixteen warps for small matrices, three CTAs per SM or more chunks ahead
+// changed nothing or lost.  8 bf16 rows of 14336 x 4096 take 16.5 us, most of the
+// difference to one row in laying x out in every CTA.
 template <int XT, int SETS, bool ZP>
 __global__ void __launch_bounds__(kThreadsQ4, 2) q4_kernel(const Q4Kernel a) {
   constexpr int PARTS = kPartsOf<XT>;

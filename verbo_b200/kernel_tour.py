@@ -27,6 +27,12 @@ the rows of every sampling step are larger than the 126 MB L2:
            tail_head_f32_kernel); the tcgen05 head at 256 rows
            (VERBO_CUDA_TAIL_TCGEN05=1, tail_head_tc_kernel)
 
+  process  verbo_ops_process_logits, 256 x 151936 with 256 ids each and a mask,
+           and a mask alone in place (process_kernel)
+  logprobs verbo_ops_token_logprobs, 256 x 151936 with the 20 first (logprob_kernel)
+  q4       verbo_ops_q4_matvec, 151936 x 896 at 1 and 64 fp32 rows (q4_kernel;
+           q4_image_kernel, q4_tile_kernel)
+
 Between steps a one-element torch fill marks the boundary in a launch list,
 and every input is made before the first step, so the only other kernels in
 a capture are those markers (and the fill that creates the marker).  Each
@@ -78,6 +84,11 @@ def main() -> None:
         q, s, norm = tw.with_dtype(dt).make_head()
         heads[dt] = vb.Tail(dt, q, s, norm, tw.eps)
     hid = torch.from_numpy(tw.make_hidden_np(256)).to(dev)
+    q, s, _ = tw.with_dtype("q4").make_head()
+    layer = vb.Q4Linear(q, s.view(np.float16))
+    px = c3[1].clone()
+    mask = torch.randint(-2**31, 2**31, (1, (px.shape[1] + 31) // 32), device=dev).int()
+    lids = torch.zeros(px.shape[0], dtype=torch.int32, device=dev)
     ncols = c5[0].vocab // 8
     cv = torch.empty(8, 512, 64, dtype=torch.float32, device=dev)
     ci = torch.empty(8, 512, 64, dtype=torch.int32, device=dev)
@@ -137,6 +148,12 @@ def main() -> None:
     os.environ["VERBO_CUDA_TAIL_TCGEN05"] = "1"
     step("tail q8 x256 tcgen05", lambda: heads["q8"].logits(hid))
     del os.environ["VERBO_CUDA_TAIL_TCGEN05"]
+    step("process", lambda: vb.process_logits(c3[1], vb.Penalties(1.1, 0.2, 0.1), hist=c3[2], hist_off=c3[3], mask=mask))
+    step("process in place", lambda: vb.process_logits(px, mask=mask, out=px))
+    step("logprobs", lambda: vb.token_logprobs(c3[1], lids, top=20))
+    step("q4 matvec x1", lambda: layer.matvec(hid[:1]))
+    step("q4 matvec x64", lambda: layer.matvec(hid[:64]))
+    layer.close()
     for t in heads.values():
         t.close()
     batch.close()
