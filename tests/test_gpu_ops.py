@@ -504,6 +504,16 @@ def test_q4_refusals_on_device(vb):
                dict(out=x[:, :8]), dict(out=torch.zeros(2, 8, device="cuda"), dtype=F16)):
         with pytest.raises(vb.VerboCudaError):
             layer.matvec(x, **kw)
+    # a workspace that is missing, too small or in the way
+    lib, many = layer._lib, torch.zeros(40, 64, device="cuda")
+    y = torch.zeros(40, 8, device="cuda")
+    need = lib.verbo_ops_q4_workspace(layer._h, 0, 40)
+    assert need > 0 and lib.verbo_ops_q4_workspace(layer._h, 0, 1) == 0
+    assert lib.verbo_ops_q4_workspace(layer._h, 0, 65536) == -1 and lib.verbo_ops_q4_workspace(layer._h, 7, 1) == -1
+    ws = torch.zeros(need, dtype=torch.uint8, device="cuda")
+    for at, size in ((None, need), (ws.data_ptr(), need - 1), (ws.data_ptr() + 4, need), (y.data_ptr(), need)):
+        assert lib.verbo_ops_q4_matvec(layer._h, many.data_ptr(), 0, 40, 64, y.data_ptr(), 0, 8, at, size, None) == -1
+        assert "workspace" in lib.verbo_cuda_last_error().decode()
     layer.close()
     with pytest.raises(vb.VerboCudaError):
         layer.matvec(x)
@@ -609,3 +619,79 @@ def test_calls_on_several_streams(vb):
     for i, t in enumerate(got):
         for u, v in zip(t, want[i % 4]):
             assert torch.equal(u, v)
+
+
+def test_calls_from_several_threads(vb):
+    """Threads of their own streams, calls of other sizes at once."""
+    import threading
+
+    g = np.random.default_rng(24)
+    q, s, _, _, w = make_q4(g, 3000, 2048, 64, False, False)
+    layer = vb.Q4Linear(q, s, group=64)
+    sizes = (1, 3, 8, 12, 40)
+    x = [torch.randn(n, 2048, device="cuda").half() for n in sizes]
+    want = [(layer.matvec(t), *vb.token_logprobs(layer.matvec(t), top=3)[2:]) for t in x]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        st = torch.cuda.Stream()
+        for _ in range(30):
+            y = layer.matvec(x[i], stream=st)
+            got = (y, *vb.token_logprobs(y, top=3, stream=st)[2:])
+            st.synchronize()
+            if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(sizes))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+def test_layer_freed_during_a_capture(vb):
+    """Garbage collection frees a layer whenever it likes: not into a capture."""
+    g = np.random.default_rng(25)
+    q, s, _, _, w = make_q4(g, 64, 64, 32, False, False)
+    layer, other = vb.Q4Linear(q, s), vb.Q4Linear(q, s)
+    x = torch.randn(2, 64, device="cuda")
+    want = layer.matvec(x).clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = layer.matvec(x)
+        other.close()
+    graph.replay()
+    assert torch.equal(y, want)
+
+
+def test_sampler_after_a_layer_on_one_stream(vb):
+    """The layers and the sampler's kernels start early on one another's heels; each
+    step has to see what the one before wrote."""
+    g = np.random.default_rng(26)
+    q, s, _, _, w = make_q4(g, 20000, 256, 32, False, False)
+    layer = vb.Q4Linear(q, s)
+    xs = [torch.randn(4, 256, device="cuda") for _ in range(20)]
+    lg = torch.empty(4, 20000, device="cuda")
+    hist = torch.randint(0, 20000, (4 * 32,), device="cuda", dtype=torch.int32)
+    off = torch.arange(5, device="cuda") * 32
+    o = vb.Sampling(temp=0.0, repeat=1.2, repeat_last=32)
+    mask = torch.randint(-2**31, 2**31 - 1, (4, 625), device="cuda").int()
+
+    def step(x):
+        layer.matvec(x, out=lg)
+        vb.process_logits(lg, mask=mask, out=lg)
+        ids = vb.sample(lg, o, hist=hist, hist_off=off)
+        return ids, *vb.token_logprobs(lg, ids, top=2)
+
+    want = []
+    for x in xs:
+        want.append([t.clone() for t in step(x)])
+        torch.cuda.synchronize()
+    for _ in range(5):
+        got = [step(x) for x in xs]
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(u, v) for u, v in zip(a, b))

@@ -224,13 +224,18 @@ class Staged {
   const void* view_ = nullptr;
 };
 
+// A language with garbage collection may free a handle while a stream of this
+// thread is being captured: freeing is no part of the capture.
 void q4_release(verbo_ops_q4* h) {
   int before = 0;
   const bool known = cudaGetDevice(&before) == cudaSuccess;
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  const bool relaxed = cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess;
   cudaSetDevice(h->device);
   cudaFree(h->d_tiles);
   cudaFree(h->d_bias);
   if (known) cudaSetDevice(before);
+  if (relaxed) cudaThreadExchangeStreamCaptureMode(&mode);
   delete h;
 }
 

@@ -53,11 +53,18 @@ __device__ __forceinline__ float Vec<__nv_bfloat16>::get(int i) const {
   return __uint_as_float((i & 1) ? (w[i >> 1] & 0xffff0000u) : (w[i >> 1] << 16));
 }
 
+// Not the read-only path: a kernel that is launched programmatically has begun
+// before the grid whose rows it reads has ended.
 __device__ __forceinline__ uint4 ld_stream16(const void* p) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0,%1,%2,%3}, [%4];"
+  asm volatile("ld.global.L1::no_allocate.L2::256B.v4.u32 {%0,%1,%2,%3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint32_t ld_word(const uint32_t* p) {
+  uint32_t v;
+  asm volatile("ld.global.u32 %0, [%1];" : "=r"(v) : "l"(p));
   return v;
 }
 
@@ -120,8 +127,8 @@ __global__ void __launch_bounds__(kProcThreads, !LISTS && INPLACE ? 8 : 4) proce
         if (!INPLACE) x[i].raw = ld_stream16(in + c);
         if (mask) {
           const uint32_t* w = mask + (c >> 5);
-          ml[i] = __ldg(w);
-          mh[i] = (c & 31) + N > 32 ? __ldg(w + 1) : 0u;
+          ml[i] = ld_word(w);
+          mh[i] = (c & 31) + N > 32 ? ld_word(w + 1) : 0u;
         }
       }
     }
@@ -282,7 +289,7 @@ __global__ void __launch_bounds__(kProcThreads, !LISTS && INPLACE ? 8 : 4) proce
       } else if (c + N > 0 && c < a.vocab) {  // the row's ragged ends
         for (int j = max(0, -c); j < min(N, a.vocab - c); ++j) {
           const int k = lists ? cnt[p + j] : 0;
-          const bool allowed = !mask || ((__ldg(mask + ((c + j) >> 5)) >> ((c + j) & 31)) & 1u);
+          const bool allowed = !mask || ((mask[(c + j) >> 5] >> ((c + j) & 31)) & 1u);
           if (INPLACE && allowed && k == 0) continue;
           float v = to_float(in[c + j]);
           if (k) {
