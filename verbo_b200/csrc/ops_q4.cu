@@ -577,17 +577,17 @@ __global__ void __launch_bounds__(256) q4_image_kernel(const Q4Kernel a, int col
 // half a chunk at a time.  One thread of the group streams chunks of x (its image, one
 // bulk copy each) through a ring of stages (full / empty barriers).  A set's sums
 // are scaled when it ends, 64 inputs at most, so that its fragments stay in
-// registers; two column tiles go through the tensor pipe side by side.
+// registers; up to four column tiles go through the tensor pipe side by side.
 //
 // What bounds it is not memory but the pipes behind mma.sync: measured on B200, an
 // m16n8k16 takes 8.6 cycles of a quarter SM, and two of them (a group of 32) with
-// their load and the fmas of their scale 19.6: 37 us of the 86 that 64 rows of a
+// their load and the fmas of their scale 19.6: 37 us of the 81 that 64 rows of a
 // 151936 x 896 head take; unpacking and waiting make the rest.  tcgen05.mma does
 // not help here: a group's sums have to leave tensor memory before the next scale,
 // 2 values per weight at 64 columns and groups of 32, and weights that are unpacked
 // into tensor memory went there at about 25 bytes per cycle and SM: a kernel built
 // that way, five warps to 128 outputs, took 92 us for 64 rows of a 151936 x 896 head
-// in groups of 32 (this one 86) and 43 us for 16 (this one 36).
+// in groups of 32 (this one 81) and 43 us for 16 (this one 36).
 constexpr int kTileStages = 3;
 constexpr int kTileAhead = 2;  // half chunks of weights in flight per warp (four: 0 to 2 us slower)
 // CTAs per SM.  More of them hide more, at fewer registers: 16 rows of a 151936 x
@@ -783,7 +783,7 @@ __global__ void __launch_bounds__(kThreadsQ4, kTileCtas<NT, SETS>) q4_tile_kerne
       if (ok && tile < tile1) {
         const unsigned char* xc = ring + s * XB + half * 1024 + lane * 16;
         constexpr int ND = Q4Half<SETS, ZP>::ND, BLK = 2 / ND;  // sets, 32-blocks of each
-        constexpr int NP = NT < 2 ? NT : 2;                      // column tiles side by side
+        constexpr int NP = NT < 4 ? NT : 4;                      // column tiles side by side
 #pragma unroll
         for (int q = 0; q < ND; ++q) {
           const Q4Zero z = buf[d].zero(q);
@@ -920,7 +920,7 @@ Q4Plan plan_q4(const Q4Mat& m, int n, int x_type, int sms) {
   int c = cols <= 8 ? 8 : cols <= 16 ? 16 : cols <= 32 ? 32 : 64;
   while (set(c) < sms && c > 8) c /= 2;
   // the fewest groups that give the SMs 3/2 CTAs each: more of them take more shared
-  // memory (64 rows of 4096 x 4096: 17.3 us, and 27 with two CTAs each asked for)
+  // memory (64 rows of 4096 x 4096: 16.6 us, and 27 with two CTAs each asked for)
   p.kq = 1;
   while (static_cast<long long>(tile_ctas(m, p.kq)) * p.passes * 2 < 3 * sms && tile_fits(m, 2 * p.kq, p.cols)) p.kq *= 2;
   return p;
