@@ -695,3 +695,42 @@ def test_sampler_after_a_layer_on_one_stream(vb):
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+def test_rows_beyond_32_bits(vb):
+    """Rows more than 2^31 elements apart."""
+    ld, vocab = 2**31 + 9, 4000
+    buf = torch.zeros(ld + vocab, dtype=BF16, device="cuda")
+    x = buf.as_strided((2, vocab), (ld, 1))
+    x.copy_(torch.randn(2, vocab, device="cuda"))
+    near = x.contiguous()
+    assert torch.equal(vb.process_logits(x), near.float())
+    ids = np.array([17, 3999])
+    check_logprobs(vb, x, ids, 5, 1.0)
+    g = np.random.default_rng(30)
+    q, s, _, _, w = make_q4(g, 48, 3200, 128, False, False)
+    layer = vb.Q4Linear(q, s, group=128)
+    assert torch.equal(layer.matvec(x[:, :3200]), layer.matvec(near[:, :3200].contiguous()))
+    far = torch.zeros(2**31 // 2 + 9 + 64, device="cuda").as_strided((2, 48), (2**31 // 2 + 9, 1))
+    layer.matvec(near[:, :3200].contiguous(), out=far, dtype=F32)
+    check_q4(far.contiguous(), near[:, :3200], w, None)
+
+
+def test_many_short_rows(vb):
+    rows, vocab = 70001, 37
+    g = np.random.default_rng(31)
+    x = g.standard_normal((rows, vocab)).astype(np.float32)
+    allowed = g.random((rows, vocab)) < 0.6
+    out = vb.process_logits(dev(x), mask=dev(words(allowed))).cpu().numpy()
+    np.testing.assert_array_equal(out, np.where(allowed, x, NEG))
+    ids = g.integers(0, vocab, rows)
+    lp, rank, tid, tlp = vb.token_logprobs(dev(out), dev(ids.astype(np.int32)), top=2)
+    v = out.astype(np.float64)
+    with np.errstate(divide="ignore"):
+        want = v - np.log(np.exp(v).sum(1, keepdims=True))
+    check_lp(lp.cpu().numpy()[allowed.any(1)], want[np.arange(rows), ids][allowed.any(1)])
+    mine = v[np.arange(rows), ids][:, None]
+    before = (v > mine) | ((v == mine) & (np.arange(vocab) < ids[:, None]))
+    np.testing.assert_array_equal(rank.cpu().numpy(), before.sum(1))
+    first = v.argmax(1)
+    np.testing.assert_array_equal(tid.cpu().numpy()[:, 0], np.where(allowed.any(1), first, -1))

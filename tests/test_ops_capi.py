@@ -51,7 +51,7 @@ def process(lib, **kw):
     a = dict(logits=1 << 20, dtype=F32, rows=2, vocab=8, ld=8, opts=vb.Penalties(1.1), row=None, hist=None, off=None,
              bias_ids=None, bias=None, bias_off=None, mask=None, ld_mask=0, out=1 << 24, ld_out=8)
     a.update(kw)
-    o = a["opts"]._c() if a["opts"] is not None else None
+    o = a["opts"]
     return lib.verbo_ops_process_logits(a["logits"], a["dtype"], a["rows"], a["vocab"], a["ld"],
                                         ctypes.byref(o) if o is not None else None, a["row"], a["hist"], a["off"],
                                         a["bias_ids"], a["bias"], a["bias_off"], a["mask"], a["ld_mask"], a["out"],

@@ -10,7 +10,6 @@ checked here and in the C ABI; both raise ``VerboCudaError``.
 from __future__ import annotations
 
 import ctypes
-from dataclasses import dataclass
 
 from . import VerboCudaError, _err, load_library
 
@@ -21,25 +20,20 @@ _I = ctypes.c_int
 _L = ctypes.c_longlong
 
 
-class _Penalties(ctypes.Structure):
-    _fields_ = [("repeat", ctypes.c_float), ("frequency", ctypes.c_float), ("presence", ctypes.c_float),
-                ("last", ctypes.c_int)]
-
-
-@dataclass
-class Penalties:
+class Penalties(ctypes.Structure):
     """Penalties on the ids of a row's history: ``repeat`` is that of ``Sampling``
     (v > 0 ? v / repeat : v * repeat), then ``frequency`` times the number of
     occurrences and ``presence`` once are subtracted.  ``last`` is the window:
-    the last ``last`` ids, all of them if <= 0."""
+    the last ``last`` ids, all of them if <= 0.  (verbo_ops_penalties itself.)"""
 
-    repeat: float = 1.0
-    frequency: float = 0.0
-    presence: float = 0.0
-    last: int = 0
+    _fields_ = [("repeat", ctypes.c_float), ("frequency", ctypes.c_float), ("presence", ctypes.c_float),
+                ("last", ctypes.c_int)]
 
-    def _c(self) -> _Penalties:
-        return _Penalties(self.repeat, self.frequency, self.presence, self.last)
+    def __init__(self, repeat: float = 1.0, frequency: float = 0.0, presence: float = 0.0, last: int = 0):
+        super().__init__(repeat, frequency, presence, last)
+
+    def __repr__(self):
+        return f"Penalties(repeat={self.repeat}, frequency={self.frequency}, presence={self.presence}, last={self.last})"
 
 
 _state = None
@@ -53,8 +47,8 @@ def _ops():
 
         lib = load_library()
         for name, res, args in (
-            ("verbo_ops_default_penalties", _Penalties, []),
-            ("verbo_ops_process_logits", _I, [_P, _I, _I, _I, _L, ctypes.POINTER(_Penalties), _P, _P, _P, _P, _P, _P, _P,
+            ("verbo_ops_default_penalties", Penalties, []),
+            ("verbo_ops_process_logits", _I, [_P, _I, _I, _I, _L, ctypes.POINTER(Penalties), _P, _P, _P, _P, _P, _P, _P,
                                               _L, _P, _L, _P]),
             ("verbo_ops_token_logprobs", _I, [_P, _I, _I, _I, _L, ctypes.c_float, _P, _P, _P, _I, _P, _P, _P]),
             ("verbo_ops_q4_new", _P, [_I, _I, _I, _P, _P, _P, _P, _I, _P]),
@@ -104,8 +98,7 @@ def _list(t, dtype, index, what, size=None):
 def _call(fn, torch, index, *args):
     """One library call with the device current (the calls on rows take the
     current device's)."""
-    before = torch.cuda.current_device()
-    if before == index:
+    if torch.cuda.current_device() == index:
         rc = fn(*args)
     else:
         with torch.cuda.device(index):
@@ -172,15 +165,17 @@ def process_logits(logits, penalties=None, hist=None, hist_off=None, row_penalti
             raise VerboCudaError("out must be float32 with one row per row of logits, on their device")
     mp, ld_mask = None, 0
     if mask is not None:
-        if mask.dim() != 2 or mask.shape[0] not in (1, rows) or mask.shape[1] * 32 < vocab:
+        shape = mask.shape
+        if len(shape) != 2 or (shape[0] != rows and shape[0] != 1) or shape[1] * 32 < vocab:
             raise VerboCudaError("mask must be [rows or 1, at least ceil(vocab / 32)]")
         if mask.get_device() != dev or mask.dtype != torch.int32:
             raise VerboCudaError("mask must be an int32 CUDA tensor on the device of the rows")
-        if mask.shape[1] > 1 and mask.stride(1) != 1:
+        stride = mask.stride()
+        if stride[1] != 1 and shape[1] > 1:
             raise VerboCudaError("mask: rows must be contiguous (stride(1) == 1)")
         mp = mask.data_ptr()
-        if mask.shape[0] > 1:
-            ld_mask = mask.stride(0)
+        if shape[0] > 1:
+            ld_mask = stride[0]
     hp = op = rp = bi = bv = bo = pen = None
     if hist is not None or hist_off is not None:
         if hist is None or hist_off is None:
@@ -198,11 +193,13 @@ def process_logits(logits, penalties=None, hist=None, hist_off=None, row_penalti
         if bias.numel() == 0:
             bi = bv = bo = None
     if penalties is not None:
-        pen = penalties._c()
+        if not isinstance(penalties, Penalties):
+            raise VerboCudaError("penalties must be Penalties")
+        pen = penalties
     if row_penalties is not None:
         rp = _list(row_penalties, torch.float32, dev, "row_penalties", 3 * rows)
         if pen is None:
-            pen = _Penalties(1.0, 0.0, 0.0, 0)
+            pen = Penalties(1.0, 0.0, 0.0, 0)
     _call(lib.verbo_ops_process_logits, torch, dev, logits.data_ptr(), code, rows, vocab, ld,
           None if pen is None else ctypes.byref(pen), rp, hp, op, bi, bv, bo, mp, ld_mask, out.data_ptr(), ld_out, at)
     return out
