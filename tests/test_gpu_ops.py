@@ -734,3 +734,27 @@ def test_many_short_rows(vb):
     np.testing.assert_array_equal(rank.cpu().numpy(), before.sum(1))
     first = v.argmax(1)
     np.testing.assert_array_equal(tid.cpu().numpy()[:, 0], np.where(allowed.any(1), first, -1))
+
+
+def test_the_rings_wait_gives_up(vb, tmp_path):
+    """The wait of the 4-bit products' ring on a barrier that nothing arrives on ends
+    after its limit, and the context goes on."""
+    import ctypes
+    import subprocess
+    from pathlib import Path
+
+    from verbo_b200 import build
+
+    root = Path(__file__).resolve().parent.parent
+    so = tmp_path / "libops_wait.so"
+    subprocess.run([build.nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-O2", "-std=c++17", "-shared",
+                    "-Xcompiler", "-fPIC", f"-I{root / 'verbo_b200' / 'csrc'}", "-o", str(so),
+                    str(root / "tests" / "cpp" / "ops_wait_timeout.cu")], check=True, capture_output=True)
+    lib = ctypes.CDLL(str(so))
+    gave_up, waited, limit = ctypes.c_uint(7), ctypes.c_ulonglong(0), ctypes.c_ulonglong(0)
+    assert lib.run_ops_wait_timeout(ctypes.byref(gave_up), ctypes.byref(waited), ctypes.byref(limit)) == 0
+    assert gave_up.value == 1
+    assert limit.value <= waited.value < 20 * limit.value
+    x = torch.randn(2, 64, device="cuda")
+    assert torch.equal(vb.process_logits(x), x)
+    vb.check()

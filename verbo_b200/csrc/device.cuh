@@ -102,6 +102,20 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t phase)
   }
   return true;
 }
+// The same with the timer, which is slow to read, looked at now and then alone:
+// for waits that are short and many.
+__device__ __forceinline__ bool mbar_wait_limited(uint64_t* bar, uint32_t phase) {
+  if (mbar_try_wait(bar, phase)) return true;
+  uint64_t t0 = 0;
+  for (uint32_t i = 1;; ++i) {
+    if (mbar_try_wait(bar, phase)) return true;
+    if ((i & 255u) == 0) {
+      const uint64_t t = gtimer();
+      if (t0 == 0) t0 = t;
+      if (t - t0 > kWaitLimitNs) return false;
+    }
+  }
+}
 // Global -> this CTA's shared memory, completion counted on `bar` in bytes.
 // Both addresses 16-byte aligned, bytes a multiple of 16.  Never multicast.
 __device__ __forceinline__ void bulk_g2s(void* dst_smem, const void* src_gmem, uint32_t bytes, uint64_t* bar,

@@ -605,19 +605,7 @@ __device__ __forceinline__ void bulk_copy(void* dst, const void* src, uint32_t b
 __device__ __forceinline__ void mbar_arrive1(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-// A wait with a limit of kWaitLimitNs; the timer is looked at now and then alone.
-__device__ __forceinline__ bool wait_limited(uint64_t* bar, uint32_t phase) {
-  if (mbar_try_wait(bar, phase)) return true;
-  uint64_t t0 = 0;
-  for (uint32_t i = 1;; ++i) {
-    if (mbar_try_wait(bar, phase)) return true;
-    if ((i & 255u) == 0) {
-      const uint64_t t = gtimer();
-      if (t0 == 0) t0 = t;
-      if (t - t0 > kWaitLimitNs) return false;
-    }
-  }
-}
+
 // What one lane holds of half a chunk: 64 inputs, one set or two.
 template <int SETS, bool ZP>
 struct Q4Half {
@@ -717,7 +705,7 @@ __global__ void __launch_bounds__(kThreadsQ4, kTileCtas<NT, SETS>) q4_tile_kerne
     for (int i = 0; i < 4; ++i) acc[n][i] = 0.0f;
 
   bool ok = true;
-  int chunk = 0, tile = tile0 + wm;
+  int chunk = 0, tile = tile0 + wm, limit = total;  // limit: the chunks of x to copy
   // The tiles are through: the groups' sums are added in their order.
   auto finish = [&]() {
     if (a.kq > 1) {
@@ -774,13 +762,13 @@ __global__ void __launch_bounds__(kThreadsQ4, kTileCtas<NT, SETS>) q4_tile_kerne
       const int it = it0 + d / 2, half = d & 1;
       if (it >= total) break;
       const int s = it % kTileStages;
-      // A wait that runs out ends the products of the warp, not its barriers, and
-      // nothing of the CTA is stored any more.
-      if (half == 0 && ok && !wait_limited(&full[s], (it / kTileStages) & 1)) {
+      // After a wait that ran out the warp goes on without waiting (its lanes stay
+      // together, and the barriers are met), but nothing of the CTA is stored.
+      if (half == 0 && ok && !mbar_wait_limited(&full[s], (it / kTileStages) & 1)) {
         ok = false;
         stop = 1;
       }
-      if (ok && tile < tile1) {
+      if (tile < tile1) {
         const unsigned char* xc = ring + s * XB + half * 1024 + lane * 16;
         constexpr int ND = Q4Half<SETS, ZP>::ND, BLK = 2 / ND;  // sets, 32-blocks of each
         constexpr int NP = NT < 4 ? NT : 4;                      // column tiles side by side
@@ -824,12 +812,12 @@ __global__ void __launch_bounds__(kThreadsQ4, kTileCtas<NT, SETS>) q4_tile_kerne
       __syncwarp();
       if (lane == 0) mbar_arrive1(&empty[s]);  // this warp has read the stage
       // the stage that the group read a chunk ago takes the next chunk
-      if (producer && ok && it >= 1 && put < total) {
-        const int e = (it - 1) % kTileStages;
-        if (wait_limited(&empty[e], ((it - 1) / kTileStages) & 1)) {
+      // (a refill that does not come off is the last one: the full waits then run out)
+      if (producer && ok && it >= 1 && put < limit) {
+        if (mbar_wait_limited(&empty[(it - 1) % kTileStages], ((it - 1) / kTileStages) & 1)) {
           inputs();
         } else {
-          ok = false;
+          limit = put;
           stop = 1;
         }
       }
@@ -847,7 +835,7 @@ __global__ void __launch_bounds__(kThreadsQ4, kTileCtas<NT, SETS>) q4_tile_kerne
     atomicOr(&g_ops_status, kErrOpsWait);
     if (producer)
       for (int it = max(0, put - kTileStages); it < put; ++it)
-        (void)wait_limited(&full[it % kTileStages], (it / kTileStages) & 1);
+        (void)mbar_wait_limited(&full[it % kTileStages], (it / kTileStages) & 1);
   }
 }
 
