@@ -95,7 +95,7 @@ VERBO_CUDA_API int verbo_ops_token_logprobs(const void* logits, int dtype, int r
      W[o][i] = s[o][g] * (q[o][i] - z[o][g]),  g = i / group
    The activations stay in their own type (the head of verbo_cuda_tail_*
    quantises them, as the reference does): fp16 x is taken as it is, bf16 and
-   fp32 x to within 2^-24 of each value (or 2^-39 of its row's largest, for values
+   fp32 x to within 2^-23 of each value (or 2^-39 of its row's largest, for values
    that much smaller); the products with q - z are exact, the sums fp32.  The same call gives the same bits; the order of a sum
    goes by n, so a row's last bits can differ between batches of other sizes. */
 typedef struct verbo_ops_q4 verbo_ops_q4;

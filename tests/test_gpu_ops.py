@@ -7,7 +7,8 @@ eps(t) / 2 that of an output type t.
   * process: five roundings (the penalty, f * c, two subtractions, the bias),
     each of at most u times the value it rounds: u times the sum of the five
     magnitudes.
-  * q4: the products are exact; K additions and one multiplication by a scale,
+  * q4: x is met to within 2u of each value, the products are exact; K additions
+    and one multiplication by a scale,
     in fp32 in the tensor core's order, whose additions may truncate: at most
     2u each, of partial sums no larger than A = sum |w x| (+ |b|); then the
     output's rounding.  Norm-wise, K/16 + K/32 + 16 roundings (an instruction
@@ -441,8 +442,8 @@ def test_q4_each_weight_lands_in_its_place(vb):
             np.testing.assert_array_equal(y.double().cpu().numpy().T, w)
 
 
-def test_q4_fp32_inputs_keep_their_24_bits(vb):
-    """fp32 x of widely spread sizes, and what is not a number."""
+def test_q4_inputs_of_all_sizes(vb):
+    """x of widely spread sizes, last places of fp32, and what is not a number."""
     g = np.random.default_rng(4)
     q, s, _, _, w = make_q4(g, 40, 64, 32, False, False)
     layer = vb.Q4Linear(q, s)

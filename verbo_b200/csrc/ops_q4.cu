@@ -8,10 +8,10 @@
 //   fp16 x   is a column as it is.
 //   bf16 x   is a column times a power of two that takes the token's largest
 //            value to [2^14, 2^15): exact for all within 2^-31 of that value (8
-//            bits above 2^-24), and off by 2^-40 of it at most for the rest.
+//            bits above 2^-24), and off by 2^-39 of it at most for the rest.
 //   fp32 x   is two columns, hi = fp16(v) and lo = fp16((v - hi) 2^11) of the
-//            same scaled v: each drops half a step of 11 bits, 2^-24 of v
-//            together, which is fp32's own rounding.
+//            same scaled v: v - hi is at most 2^12 of v's last places, of which lo
+//            holds 11 bits, so v is met to within one of its last places (2^-23).
 // The sums are taken back by the inverse power.  Infinities and NaNs go through
 // hi as they are and do not count for the largest value.
 #include <cuda_bf16.h>
@@ -42,11 +42,18 @@ __device__ unsigned g_ops_status;
 // read as it lies.)  Nibbles, low to high: (g, k), (g+8, k), (g, k+2),
 // (g+8, k+2), (g, k+1), (g+8, k+1), (g, k+3), (g+8, k+3): masks with 0x000f000f
 // and 0x00f000f0 at shifts 0 and 8 give the pairs of a0, a1, a2, a3.
-__device__ __forceinline__ uint32_t q4_nibble(const Q4Mat& m, const unsigned char* q, int o, int i) {
+// Four neighbouring weights of output o from input i on (a multiple of 4) as the
+// low halves of four bytes.
+__device__ __forceinline__ uint32_t q4_four(const Q4Mat& m, const unsigned char* q, int o, int i) {
   if (o >= m.outs || i >= m.ins) return 0;
-  const int blk = i >> 5, e = i & 31;
-  const unsigned char b = q[static_cast<size_t>(o) * (m.ins / 2) + blk * 16 + (e & 15)];
-  return e < 16 ? b & 15u : b >> 4;
+  const int e = i & 31;
+  const unsigned char* p = q + static_cast<size_t>(o) * (m.ins / 2) + (i >> 5) * 16 + (e & 15);
+  uint32_t v;
+  if ((reinterpret_cast<uintptr_t>(q) & 3) == 0)
+    v = *reinterpret_cast<const uint32_t*>(p);
+  else
+    v = p[0] | p[1] << 8 | p[2] << 16 | static_cast<uint32_t>(p[3]) << 24;
+  return (e < 16 ? v : v >> 4) & 0x0f0f0f0fu;
 }
 
 __global__ void q4_pack_kernel(Q4Mat m, const unsigned char* __restrict__ q, const uint16_t* __restrict__ s,
@@ -63,10 +70,10 @@ __global__ void q4_pack_kernel(Q4Mat m, const unsigned char* __restrict__ q, con
       const int g = lane >> 2, t = lane & 3;
       const int k = kc * kQ4Chunk + 32 * (j >> 1) + 8 * t + 4 * (j & 1);
       const int r = tile * kQ4Rows + g;
-      uint32_t v = 0;
-      const int dk[8] = {0, 0, 2, 2, 1, 1, 3, 3};
-#pragma unroll
-      for (int n = 0; n < 8; ++n) v |= q4_nibble(m, q, r + 8 * (n & 1), k + dk[n]) << (4 * n);
+      // k, k + 1, k + 2, k + 3 of row g to nibbles 0, 4, 2, 6, of row g + 8 to 1, 5, 3, 7
+      const uint32_t lo = q4_four(m, q, r, k), up = q4_four(m, q, r + 8, k);
+      const uint32_t both = lo | up << 4;
+      const uint32_t v = __byte_perm(both, 0, 0x3120);
       reinterpret_cast<uint32_t*>(dst)[w] = v;
     }
     if (w < 16 * sets) {  // [g][set][row g, row g + 8]
