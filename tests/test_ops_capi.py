@@ -85,6 +85,12 @@ def process(lib, **kw):
     (dict(opts=vb.Penalties(1.0, 0.0, float("nan"))), "presence"),
     (dict(mask=4, ld_mask=1, vocab=40, ld=40, ld_out=40), "ld_mask"),
     (dict(mask=6), "aligned"),
+    (dict(row=6), "row_penalties must be aligned"),
+    (dict(hist=6, off=8), "hist must be aligned"),
+    (dict(hist=4, off=4), "hist_off must be aligned"),
+    (dict(bias=4, bias_ids=5, bias_off=8), "bias_ids must be aligned"),
+    (dict(bias=6, bias_ids=4, bias_off=8), "bias must be aligned"),
+    (dict(bias=4, bias_ids=4, bias_off=4), "bias_off must be aligned"),
     (dict(dtype=BF16, out=1 << 20), "out may be logits"),
     (dict(out=1 << 20, ld_out=9), "out may be logits"),
     (dict(out=(1 << 20) + 4), "overlaps"),
@@ -118,6 +124,11 @@ def logprobs(lib, **kw):
     (dict(ld=4), "stride"),
     (dict(logits=None), "NULL"),
     (dict(dtype=F16, logits=(1 << 20) + 1), "aligned"),
+    (dict(ids=5), "ids must be aligned"),
+    (dict(lp=6), "logprob must be aligned"),
+    (dict(rank=7), "rank must be aligned"),
+    (dict(top=1, tid=6, tlp=4), "top_ids must be aligned"),
+    (dict(top=1, tid=4, tlp=6), "top_logprobs must be aligned"),
     (dict(temp=0.0), "temp"),
     (dict(temp=-1.0), "temp"),
     (dict(temp=float("nan")), "temp"),

@@ -111,6 +111,12 @@ VERBO_CUDA_API int verbo_ops_process_logits(const void* logits, int dtype, int r
         check_rows(logits, dtype, rows, vocab, ld, "logits");
         check_rows(out, VERBO_OPS_F32, rows, vocab, ld_out, "out");
         check_aligned(mask, 4, "mask");
+        check_aligned(row_penalties, 4, "row_penalties");
+        check_aligned(hist, 4, "hist");
+        check_aligned(hist_off, 8, "hist_off");
+        check_aligned(bias_ids, 4, "bias_ids");
+        check_aligned(bias, 4, "bias");
+        check_aligned(bias_off, 8, "bias_off");
         const bool in_place = static_cast<const void*>(out) == logits;
         if (in_place && (dtype != VERBO_OPS_F32 || (ld_out != ld && rows > 1)))
           fail("out may be logits only if they are F32 rows of the same stride");
@@ -162,6 +168,11 @@ VERBO_CUDA_API int verbo_ops_token_logprobs(const void* logits, int dtype, int r
         check_rows(logits, dtype, rows, vocab, ld, "logits");
         if (ids && (!logprob || !rank)) fail("logprob and rank must not be NULL when ids are given");
         if (top > 0 && (!top_ids || !top_logprobs)) fail("top_ids and top_logprobs must not be NULL when top > 0");
+        check_aligned(ids, 4, "ids");
+        check_aligned(logprob, 4, "logprob");
+        check_aligned(rank, 4, "rank");
+        check_aligned(top_ids, 4, "top_ids");
+        check_aligned(top_logprobs, 4, "top_logprobs");
         if (!ids && top == 0) return 0;
         vb::LogprobArgs a{};
         a.logits = logits;
