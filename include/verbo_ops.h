@@ -80,12 +80,12 @@ VERBO_CUDA_API int verbo_ops_process_logits(const void* logits, int dtype, int r
                 written.  logprob[r] is its log-probability, rank[r] the number
                 of columns before it in the sampler's order (value descending,
                 index ascending).  An id outside [0, vocab): -inf and -1.
-   top          0..32: the `top` first columns of that order that have a
-                probability, top_ids and top_logprobs [rows][top]; where fewer
-                have one, the rest is (-1, -inf).
+   top          0..32: the `top` first columns of that order whose values are
+                above -inf, top_ids and top_logprobs [rows][top]; where there
+                are fewer, the rest is (-1, -inf).
    A NaN counts as -inf, as in verbo_cuda_sample; -0 equals +0.  A row of -inf
    alone has no probabilities: its log-probabilities are -inf.  Columns at
-   +inf share the whole probability.  temp in [1e-4, 1e4]. */
+   +inf share the whole probability (the others' logarithm is -inf).  temp in [1e-4, 1e4]. */
 VERBO_CUDA_API int verbo_ops_token_logprobs(const void* logits, int dtype, int rows, int vocab, long long ld,
                                             float temp, const int* ids, float* logprob, int* rank, int top,
                                             int* top_ids, float* top_logprobs, void* stream);
@@ -96,8 +96,9 @@ VERBO_CUDA_API int verbo_ops_token_logprobs(const void* logits, int dtype, int r
    The activations stay in their own type (the head of verbo_cuda_tail_*
    quantises them, as the reference does): fp16 x is taken as it is, bf16 and
    fp32 x to within 2^-23 of each value (or 2^-39 of its row's largest, for values
-   that much smaller); the products with q - z are exact, the sums fp32.  The same call gives the same bits; the order of a sum
-   goes by n, so a row's last bits can differ between batches of other sizes. */
+   that much smaller); the products with q - z are exact, the sums fp32.  The same
+   call gives the same bits; the order of a sum goes by n, so a row's last bits can
+   differ between batches of other sizes. */
 typedef struct verbo_ops_q4 verbo_ops_q4;
 /* Lays the matrix out on `device` (host or device arrays, read before the
    call returns; work on device arrays is ordered after `stream`).

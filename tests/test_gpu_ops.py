@@ -235,7 +235,8 @@ def test_process_refusals_on_device(vb):
            dict(hist=h.cpu(), hist_off=o), dict(mask=torch.zeros(2, 1, dtype=torch.int32, device="cuda")),
            dict(mask=torch.zeros(3, 2, dtype=torch.int32, device="cuda")), dict(mask=torch.zeros(2, 2, device="cuda")),
            dict(out=torch.zeros(1, 64, device="cuda")), dict(out=x.half()), dict(out=x[:, 1:], vocab=63), dict(vocab=65),
-           dict(row_penalties=torch.ones(2, 2, device="cuda")), dict(bias=torch.zeros(1, device="cuda"))]
+           dict(row_penalties=torch.ones(2, 2, device="cuda")), dict(row_penalties=torch.ones(3, 2, device="cuda")),
+           dict(bias=torch.zeros(1, device="cuda"))]
     for kw in bad:
         with pytest.raises(vb.VerboCudaError):
             vb.process_logits(x, **kw)
@@ -340,6 +341,17 @@ def test_logprobs_hard_rows(vb, vocab):
         for ids in (np.full(16, vocab // 2), np.zeros(16, int), np.full(16, vocab - 1)):
             for top in (0, 1, 20, 32):
                 check_logprobs(vb, t, ids, top, 1.0)
+
+
+def test_logprobs_differences_beyond_fp32(vb):
+    """Values whose difference fp32 does not hold, and a temperature that makes a
+    number of it again.  Three roundings of the result's own size: 3u."""
+    x = np.array([[3e38, -3e38, 1.0, -1e38], [-3.4e38, 3.4e38, NEG, 1e30]], np.float32)
+    for temp in (2.0, 10.0, 1e4):
+        _, _, tid, tlp = vb.token_logprobs(dev(x), top=4, temp=temp)
+        _, _, wtid, wtlp = plain_logprobs(x, None, 4, temp)
+        np.testing.assert_array_equal(tid.cpu().numpy(), wtid)
+        np.testing.assert_allclose(tlp.double().cpu().numpy(), wtlp, rtol=3 * U * (1 + 2.0 ** -20), atol=0)
 
 
 def test_logprobs_ids_outside_and_none(vb):

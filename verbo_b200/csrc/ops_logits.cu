@@ -822,7 +822,8 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprob_kernel(const LogprobArg
   auto logp = [&](float v) {
     if (v == kNegInf) return kNegInf;
     if (v == m) return -ls;
-    return __fdiv_rn(v - m, a.temp) - ls;
+    // halves: the difference of two large values of opposite sign stays finite
+    return __fdiv_rn(0.5f * v - 0.5f * m, 0.5f * a.temp) - ls;
   };
   if (tid == 0 && a.ids) {
     a.logprob[row] = id >= 0 ? logp(chosen) : kNegInf;

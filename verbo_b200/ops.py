@@ -198,6 +198,8 @@ def process_logits(logits, penalties=None, hist=None, hist_off=None, row_penalti
         pen = penalties
     if row_penalties is not None:
         rp = _list(row_penalties, torch.float32, dev, "row_penalties", 3 * rows)
+        if row_penalties.dim() != 2 or row_penalties.shape[0] != rows:
+            raise VerboCudaError("row_penalties must be [rows, 3]")
         if pen is None:
             pen = Penalties(1.0, 0.0, 0.0, 0)
     _call(lib.verbo_ops_process_logits, torch, dev, logits.data_ptr(), code, rows, vocab, ld,
@@ -214,8 +216,8 @@ def token_logprobs(logits, ids=None, top=0, temp=1.0, vocab=None, stream=None):
     the number of columns before it in the sampler's order (value descending,
     id ascending); both None without ids; -inf and -1 for an id outside
     [0, vocab).  top_ids int32 and top_logprobs float32 [rows, top]: the first
-    ``top`` <= 32 columns of that order, (-1, -inf) where fewer have a
-    probability.  A NaN counts as -inf."""
+    ``top`` <= 32 columns of that order, (-1, -inf) where fewer are above
+    -inf.  A NaN counts as -inf."""
     lib, torch, types = _ops()
     rows, cols, ld, code, dev = _rows(logits, types, "logits")
     if vocab is None:
