@@ -495,26 +495,27 @@ struct LpAcc {
       s = lp_scaled(s, m, bm, c);
       m = bm;
     }
-    if (fabsf(m) < 1e30f) {
-      const float o = -m * c;
+    if (fabsf(m) < -kNegInf) {
+      // fma(c, m, o) is the rounding of c m, exactly, and at most 2^6 below 2^31:
+      // neither 2^(c v + o) nor the factor that takes it back leaves fp32's range.
+      // A larger c m (rows masked with large finite values) counts the columns at m:
+      // one step of fp32 below it (2^-24 |m| at least) is a factor of 2^-128.  So
+      // does the power of two that takes |m| to [2^30, 2^31), where it is 2^-64.
+      float k = c;
+      if (fabsf(m * c) >= 2147483648.0f)
+        k = __uint_as_float((284u << 23) - (__float_as_uint(m) & 0x7f800000u));
+      const float o = -m * k;
       float t[2] = {0.0f, 0.0f};
-      b.each([&](float v, int j) { t[j & 1] += ex2(fmaf(v, c, o)); });
-      t[0] = (t[0] + t[1]) * ex2(fmaf(-m, c, -o));
-      if (t[0] == t[0]) {
-        s += t[0];
-        return;
+      b.each([&](float v, int j) { t[j & 1] += ex2(fmaf(v, k, o)); });
+      t[0] = (t[0] + t[1]) * ex2(fmaf(-m, k, -o));
+      if (t[0] != t[0]) {  // rare: a NaN was met
+        t[0] = 0.0f;
+        b.each([&](float v, int) { t[0] += ex2((fmaxf(v, kNegInf) - m) * c); });
       }
-    }
-    // rare: a NaN was met, or infinities, or c m may overflow (rows masked with
-    // the type's lowest value)
-    if (m == kNegInf) return;
-    if (m == -kNegInf) {  // +inf alone counts then
+      s += t[0];
+    } else if (m == -kNegInf) {  // +inf alone counts then
       b.each([&](float v, int) { ninf += v == -kNegInf; });
-      return;
     }
-    float t = 0.0f;
-    b.each([&](float v, int) { t += ex2((fmaxf(v, kNegInf) - m) * c); });
-    s += t;
   }
 };
 struct LpOne {  // a single column
