@@ -103,3 +103,29 @@ def test_logprobs_of_large_values_at_low_temperatures(vb, dtype):
     x = x.to(dtype)
     for temp in (1e-4, 2.5e-4, 1e-3):
         check_logprobs(vb, x, torch.arange(rows, device="cuda") * 7, 5, temp, 3)
+
+
+# ==================================================================== q4 ==
+def make_q4(g, outs, ins, group, zeros):
+    """(q, s, zeros, the matrix in 64 bits)."""
+    q = g.integers(0, 256, (outs, ins // 2), dtype=np.uint8)
+    cells = (outs, -(-ins // group))
+    s = (np.abs(g.standard_normal(cells)) * 0.01 + 1e-4).astype(np.float16)
+    z = g.integers(0, 16, cells, dtype=np.uint8) if zeros else None
+    b = q.reshape(outs, ins // 32, 16)
+    w = np.concatenate([b & 15, b >> 4], axis=2).reshape(outs, ins).astype(np.float64)
+    at = np.arange(ins) // group
+    return q, s, z, (w - (8 if z is None else z[:, at])) * s.astype(np.float64)[:, at]
+
+
+@pytest.mark.parametrize("group", [64, 96, 4096, 2**31 - 32, 2**31 - 64, 2**31 - 128])
+def test_q4_groups_longer_than_a_row(vb, group):
+    """One scale per row, whatever the group's length.  One-hot rows read the matrix
+    back, exactly."""
+    g = np.random.default_rng(5)
+    for ins in (64, 32):
+        q, s, z, w = make_q4(g, 50, ins, group, True)
+        assert s.shape == (50, 1)
+        layer = vb.Q4Linear(q, s, zeros=z, group=group)
+        y = layer.matvec(torch.eye(ins, device="cuda"))
+        np.testing.assert_array_equal(y.double().cpu().numpy().T, w)

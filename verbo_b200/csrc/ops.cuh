@@ -66,6 +66,7 @@ constexpr int kQ4MaxIns = 32768;
 constexpr int kQ4MaxOuts = 1 << 22;
 struct Q4Mat {
   int outs, ins, group;
+  int groups;       // of a row
   int span;         // 32, 64 or 128
   int nkc;          // chunks per tile
   int ntile;
@@ -82,7 +83,7 @@ struct Q4Args {
   long long ldy;
   void* workspace;  // q4_workspace_bytes, 16-byte aligned
 };
-// Fills in span, nkc, ntile, chunk_bytes from outs, ins, group, zeros.
+// Fills in groups, span, nkc, ntile, chunk_bytes from outs, ins, group, zeros.
 void q4_layout(Q4Mat& m);
 size_t q4_tiles_bytes(const Q4Mat& m);
 size_t q4_workspace_bytes(const Q4Mat& m, int n, int x_type);

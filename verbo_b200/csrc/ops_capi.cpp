@@ -279,8 +279,7 @@ VERBO_CUDA_API verbo_ops_q4* verbo_ops_q4_new(int outs, int ins, int group, cons
           h->m.group = group;
           h->m.zeros = zeros != nullptr;
           vb::q4_layout(h->m);
-          const size_t groups = (static_cast<size_t>(ins) + group - 1) / group;
-          const size_t cells = static_cast<size_t>(outs) * groups;
+          const size_t cells = static_cast<size_t>(outs) * h->m.groups;
           cuda_ok(cudaMalloc(&h->d_tiles, vb::q4_tiles_bytes(h->m)), "cudaMalloc weights");
           {
             const Staged dq(q, static_cast<size_t>(outs) * (ins / 2), device, st);
