@@ -18,6 +18,8 @@ __all__ = ["Penalties", "process_logits", "token_logprobs", "Q4Linear"]
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _L = ctypes.c_longlong
+_INT_MAX = 2**31 - 1  # what ctypes takes for an int it cuts to 32 bits, without an error
+_MAX_TOP = 32
 
 
 class Penalties(ctypes.Structure):
@@ -30,6 +32,8 @@ class Penalties(ctypes.Structure):
                 ("last", ctypes.c_int)]
 
     def __init__(self, repeat: float = 1.0, frequency: float = 0.0, presence: float = 0.0, last: int = 0):
+        if not -_INT_MAX - 1 <= last <= _INT_MAX:
+            raise VerboCudaError("last must be in [-2147483648, 2147483647]")
         super().__init__(repeat, frequency, presence, last)
 
     def __repr__(self):
@@ -65,15 +69,17 @@ def _ops():
 def _rows(t, types, what):
     """(rows, columns, row stride, type code, device index) of a CUDA matrix with
     contiguous rows."""
+    if t.dim() != 2:
+        raise VerboCudaError(f"{what} must have two dimensions")
+    rows, cols = t.shape
+    if rows > _INT_MAX or cols > _INT_MAX:
+        raise VerboCudaError(f"{what} must have at most {_INT_MAX} rows and columns")
     index = t.get_device()
     if index < 0:
         raise VerboCudaError(f"{what} must be a CUDA tensor")
     code = types.get(t.dtype)
     if code is None:
         raise VerboCudaError(f"{what} must be float32, float16 or bfloat16")
-    if t.dim() != 2:
-        raise VerboCudaError(f"{what} must have two dimensions")
-    rows, cols = t.shape
     ld, step = t.stride()
     if step != 1 and cols > 1:
         raise VerboCudaError(f"{what}: rows must be contiguous (stride(1) == 1)")
@@ -219,16 +225,17 @@ def token_logprobs(logits, ids=None, top=0, temp=1.0, vocab=None, stream=None):
     ``top`` <= 32 columns of that order, (-1, -inf) where fewer are above
     -inf.  A NaN counts as -inf."""
     lib, torch, types = _ops()
+    top = int(top)
+    if not 0 <= top <= _MAX_TOP:
+        raise VerboCudaError(f"top must be in [0, {_MAX_TOP}]")
     rows, cols, ld, code, dev = _rows(logits, types, "logits")
     if vocab is None:
         vocab = cols
     elif not 0 < vocab <= cols:
         raise VerboCudaError("vocab must be in [1, columns of logits]")
     at = _stream_of(torch, dev, stream)
-    top = int(top)
-    n = max(top, 0)
     f32, i32 = torch.float32, torch.int32
-    tid, tlp = _new(torch, logits, stream, rows, n, i32), _new(torch, logits, stream, rows, n, f32)
+    tid, tlp = _new(torch, logits, stream, rows, top, i32), _new(torch, logits, stream, rows, top, f32)
     if ids is None:
         lp = rank = ip = lpp = rp = None
     else:
@@ -271,8 +278,10 @@ class Q4Linear:
         device = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
         self.device = torch.device("cuda", torch.cuda.current_device() if device.index is None else device.index)
         self.outs, self.ins, self.group = q.shape[0], 2 * q.shape[1], int(group)
-        if self.group < 1:
-            raise VerboCudaError("group must be a multiple of 32, at least 32")
+        if not 1 <= self.group <= _INT_MAX:
+            raise VerboCudaError("group must be a multiple of 32 in [32, 2^31)")
+        if max(self.outs, self.ins) > _INT_MAX:
+            raise VerboCudaError(f"q must have at most {_INT_MAX} rows and weights of a row")
         cells = (self.outs, -(-self.ins // self.group))
         s = hold(s, torch.float16, "s")
         zeros = None if zeros is None else hold(zeros, torch.uint8, "zeros")
