@@ -27,8 +27,12 @@ auto guard(F&& fn, decltype(fn()) fail) -> decltype(fn()) {
 
 [[noreturn]] inline void fail(const std::string& m) { throw std::runtime_error("verbo_cuda: " + m); }
 
+// The runtime keeps a failed call's error until somebody takes it: taken here, or the
+// next launch of the thread, which looks for errors that way, would answer with it.
 inline void cuda_ok(cudaError_t e, const char* what) {
-  if (e != cudaSuccess) fail(std::string(what) + ": " + cudaGetErrorString(e));
+  if (e == cudaSuccess) return;
+  (void)cudaGetLastError();
+  fail(std::string(what) + ": " + cudaGetErrorString(e));
 }
 
 }  // namespace vb
