@@ -101,7 +101,8 @@ VERBO_CUDA_API int verbo_ops_token_logprobs(const void* logits, int dtype, int r
    differ between batches of other sizes. */
 typedef struct verbo_ops_q4 verbo_ops_q4;
 /* Lays the matrix out on `device` (host or device arrays, read before the
-   call returns; work on device arrays is ordered after `stream`).
+   call returns; work on device arrays is ordered after `stream`).  Refused on a
+   stream that is being captured, whose capture goes on.
    q      outs x ins/2 bytes, the reference's Q4 rows (src/kernels.hpp:13-23):
           byte j of a 32-block holds element j in its low half and element
           j+16 in its high half

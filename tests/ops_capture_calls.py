@@ -43,7 +43,42 @@ def a_failed_call():
     return out
 
 
+def a_layer():
+    """Refused on the captured stream; beside it, on another stream or from another
+    thread, it is made.  The capture goes on."""
+    import threading
+
+    x = torch.ones(8, device="cuda")
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    out, made = {}, []
+
+    def beside():
+        made.append(layer())
+
+    def capture():
+        with torch.cuda.graph(graph):
+            y = x + 1
+            out["inside"] = said(layer)
+            with torch.cuda.stream(side):
+                out["other stream"] = said(beside)
+            t = threading.Thread(target=lambda: out.update({"other thread": said(beside)}))
+            t.start()
+            t.join()
+            made.append(y * 2)
+
+    out["capture"] = said(capture)
+    graph.replay()
+    a, b, y = made
+    torch.cuda.synchronize()
+    out["replayed"] = bool((y == 4).all())
+    eye = torch.eye(64, device="cuda")
+    out["read"] = [bool(((m.matvec(eye) / 0.01).abs() <= 8.01).all()) for m in (a, b)]
+    vb.check()
+    return out
+
+
 if __name__ == "__main__":
     layer()
     torch.cuda.synchronize()
-    print(json.dumps({"a_failed_call": a_failed_call}[sys.argv[1]]()))
+    print(json.dumps({"a_failed_call": a_failed_call, "a_layer": a_layer}[sys.argv[1]]()))

@@ -30,3 +30,10 @@ def test_a_failed_call_leaves_nothing_behind(cuda_lib):
     got = worker(cuda_lib, "a_failed_call")
     assert got["inside"].startswith("VerboCudaError")
     assert got["next layer"] == "" and got["next check"] == ""
+
+
+def test_a_layer_made_during_a_capture(cuda_lib):
+    got = worker(cuda_lib, "a_layer")
+    assert "being captured" in got["inside"]
+    assert got["other stream"] == "" and got["other thread"] == "" and got["capture"] == ""
+    assert got["replayed"] and got["read"] == [True, True]

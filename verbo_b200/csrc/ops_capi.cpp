@@ -43,6 +43,23 @@ class DeviceScope {
   bool changed_ = false;
 };
 
+// While a stream is being captured, CUDA refuses allocations and waits to the
+// capturing thread (and to all threads, for some captures) and ends the capture.
+// Those of a handle are no part of it: this thread's calls are let through.
+class BesideCaptures {
+ public:
+  BesideCaptures() { changed_ = cudaThreadExchangeStreamCaptureMode(&mode_) == cudaSuccess; }
+  ~BesideCaptures() {
+    if (changed_) cudaThreadExchangeStreamCaptureMode(&mode_);
+  }
+  BesideCaptures(const BesideCaptures&) = delete;
+  BesideCaptures& operator=(const BesideCaptures&) = delete;
+
+ private:
+  cudaStreamCaptureMode mode_ = cudaStreamCaptureModeRelaxed;
+  bool changed_ = false;
+};
+
 void check_type(int t, const char* what) {
   if (t != VERBO_OPS_F32 && t != VERBO_OPS_F16 && t != VERBO_OPS_BF16)
     fail(std::string(what) + " must be VERBO_OPS_F32, VERBO_OPS_F16 or VERBO_OPS_BF16");
@@ -235,18 +252,15 @@ class Staged {
   const void* view_ = nullptr;
 };
 
-// A language with garbage collection may free a handle while a stream of this
-// thread is being captured: freeing is no part of the capture.
+// A language with garbage collection may free a handle during a capture.
 void q4_release(verbo_ops_q4* h) {
   int before = 0;
   const bool known = cudaGetDevice(&before) == cudaSuccess;
-  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-  const bool relaxed = cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess;
+  const BesideCaptures beside;
   cudaSetDevice(h->device);
   cudaFree(h->d_tiles);
   cudaFree(h->d_bias);
   if (known) cudaSetDevice(before);
-  if (relaxed) cudaThreadExchangeStreamCaptureMode(&mode);
   delete h;
 }
 
@@ -271,6 +285,14 @@ VERBO_CUDA_API verbo_ops_q4* verbo_ops_q4_new(int outs, int ins, int group, cons
         if (device < 0 || device >= n) fail("no CUDA device " + std::to_string(device));
         const DeviceScope scope(device);
         const cudaStream_t st = static_cast<cudaStream_t>(stream);
+        cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+        const cudaError_t e = cudaStreamIsCapturing(st, &capture);
+        if (e != cudaErrorStreamCaptureImplicit) cuda_ok(e, "stream");
+        if (e != cudaSuccess || capture != cudaStreamCaptureStatusNone) {
+          (void)cudaGetLastError();
+          fail("a layer cannot be made on a stream that is being captured");
+        }
+        const BesideCaptures beside;
         auto* h = new verbo_ops_q4();
         h->device = device;
         try {
