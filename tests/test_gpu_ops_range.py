@@ -269,3 +269,38 @@ def test_q4_of_prompts(vb, n, outs, ins):
     for dtype in (F32, BF16):
         x = torch.from_numpy(g.standard_normal((n, ins)).astype(np.float32)).cuda().to(dtype)
         check_q4(layer.matvec(x), x, w, None)
+
+
+def test_the_sampler_right_behind_a_layer(vb):
+    """A layer's grid lets the next one start early; each of the sampler's paths and
+    the tail has to wait for the layer's rows, without a kernel between them."""
+    g = np.random.default_rng(27)
+    vocab = 40000
+    q, s, z, w = make_q4(g, vocab, 256, 32, False)
+    layer = vb.Q4Linear(q, s)
+    rows = 6
+    xs = [torch.randn(rows, 256, device="cuda") for _ in range(12)]
+    lg = torch.empty(rows, vocab, device="cuda")
+    hist = torch.randint(0, vocab, (rows * 32,), device="cuda", dtype=torch.int32)
+    off = torch.arange(rows + 1, device="cuda") * 32
+    for o in (vb.Sampling(temp=0.0), vb.Sampling(temp=0.0, repeat=1.3, repeat_last=32), vb.Sampling(temp=0.9, top_k=40),
+              vb.Sampling(temp=0.9, top_k=40, repeat=1.3, repeat_last=32), vb.Sampling(temp=0.8, top_k=300),
+              vb.Sampling(temp=1.0, top_k=0, top_p=0.9)):
+        kw = dict(hist=hist, hist_off=off) if o.repeat != 1 else {}
+
+        def step(x, rng):
+            layer.matvec(x, out=lg)
+            return vb.sample(lg, o, rng=rng, **kw).clone()
+
+        first = torch.from_numpy(np.array(vb.seed_states(range(1, rows + 1)), np.uint64).view(np.int64)).cuda()
+        rng = first.clone()
+        want = []
+        for x in xs:
+            want.append(step(x, rng))
+            torch.cuda.synchronize()
+        for _ in range(5):
+            rng = first.clone()
+            got = [step(x, rng) for x in xs]
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), o
+    vb.check()

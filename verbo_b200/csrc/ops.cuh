@@ -11,6 +11,15 @@ namespace vb {
 enum OpsType { kOpsF32 = 0, kOpsF16 = 1, kOpsBF16 = 2 };
 inline int ops_type_size(int t) { return t == kOpsF32 ? 4 : 2; }
 
+// SMs of the current device (the handle's, in the calls on one).
+inline int sm_count() {
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return 148;  // a B200's; the launch that follows says what is wrong
+  return sms;
+}
+
 // ------------------------------------------------------------ process -----
 struct ProcArgs {
   const void* logits;

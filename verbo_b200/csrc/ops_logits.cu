@@ -327,7 +327,7 @@ cudaError_t launch_chained(K kernel, unsigned grid, int threads, size_t smem, in
 template <class T, bool INPLACE>
 cudaError_t run_process(ProcArgs a, cudaStream_t s) {
   const long long slices = (static_cast<long long>(a.vocab) + Vec<T>::N - 1 + kProcSlice - 1) / kProcSlice;
-  long long per = std::max(1ll, std::min(8ll, a.rows * slices / (148 * 4 * 4)));
+  long long per = std::max(1ll, std::min(8ll, a.rows * slices / (sm_count() * 4 * 4)));
   a.part_cols = static_cast<int>(per) * kProcSlice;
   a.parts = static_cast<int>((slices + per - 1) / per);
   const long long grid = static_cast<long long>(a.rows) * a.parts;
@@ -868,8 +868,9 @@ cudaError_t run_logprobs(LogprobArgs a, cudaStream_t s) {
   constexpr int N = Vec<T>::N;
   // CTAs per row: one, or as many as give each SM one, with a batch each.
   const long long batches = (a.vocab / N + kLpThreads * kLpVecs - 1) / (kLpThreads * kLpVecs);
+  const int sms = sm_count();
   int C = 1;
-  while (C < kLpMaxCluster && C < batches && static_cast<long long>(a.rows) * C < 148) C <<= 1;
+  while (C < kLpMaxCluster && C < batches && static_cast<long long>(a.rows) * C < sms) C <<= 1;
   const long long grid = static_cast<long long>(a.rows) * C;
   if (grid > INT_MAX) return cudaErrorInvalidConfiguration;
   constexpr int smem = kLpStages * kLpVecs * kLpThreads * 16;  // 64 KB

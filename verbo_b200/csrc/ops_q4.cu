@@ -845,13 +845,6 @@ __global__ void __launch_bounds__(kThreadsQ4, kTileCtas<NT, SETS>) q4_tile_kerne
   }
 }
 
-// SMs of the current device (the handle's, in the calls on one).
-int sm_count() {
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms;
-}
-
 // limit: the most shared memory that calls of the kernel ask for.  The attribute
 // is set to it and not to the call's own size, which a call of another thread
 // could lower between here and the launch.
@@ -994,7 +987,7 @@ size_t q4_workspace_bytes(const Q4Mat& m, int n, int x_type) {
 cudaError_t launch_q4_pack(const Q4Mat& m, const unsigned char* q, const uint16_t* s, const unsigned char* zeros,
                            unsigned char* tiles, cudaStream_t st) {
   const long long nchunk = static_cast<long long>(m.ntile) * m.nkc;
-  q4_pack_kernel<<<static_cast<unsigned>(std::min(nchunk, 148ll * 64)), 256, 0, st>>>(m, q, s, zeros, tiles);
+  q4_pack_kernel<<<static_cast<unsigned>(std::min(nchunk, sm_count() * 64ll)), 256, 0, st>>>(m, q, s, zeros, tiles);
   return cudaGetLastError();
 }
 
