@@ -75,7 +75,6 @@ constexpr int kQ4MaxIns = 32768;
 constexpr int kQ4MaxOuts = 1 << 22;
 struct Q4Mat {
   int outs, ins, group;
-  int groups;       // of a row
   int span;         // 32, 64 or 128
   int nkc;          // chunks per tile
   int ntile;
@@ -84,6 +83,8 @@ struct Q4Mat {
   const unsigned char* tiles;
   const float* bias;  // or null
 };
+// Scales of a row, without the sum ins + group: group is anything up to 2^31.
+__host__ __device__ inline int q4_groups(const Q4Mat& m) { return (m.ins - 1) / m.group + 1; }
 struct Q4Args {
   const void* x;
   long long ldx;
@@ -92,7 +93,7 @@ struct Q4Args {
   long long ldy;
   void* workspace;  // q4_workspace_bytes, 16-byte aligned
 };
-// Fills in groups, span, nkc, ntile, chunk_bytes from outs, ins, group, zeros.
+// Fills in span, nkc, ntile, chunk_bytes from outs, ins, group, zeros.
 void q4_layout(Q4Mat& m);
 size_t q4_tiles_bytes(const Q4Mat& m);
 size_t q4_workspace_bytes(const Q4Mat& m, int n, int x_type);

@@ -301,7 +301,7 @@ VERBO_CUDA_API verbo_ops_q4* verbo_ops_q4_new(int outs, int ins, int group, cons
           h->m.group = group;
           h->m.zeros = zeros != nullptr;
           vb::q4_layout(h->m);
-          const size_t cells = static_cast<size_t>(outs) * h->m.groups;
+          const size_t cells = static_cast<size_t>(outs) * vb::q4_groups(h->m);
           cuda_ok(cudaMalloc(&h->d_tiles, vb::q4_tiles_bytes(h->m)), "cudaMalloc weights");
           {
             const Staged dq(q, static_cast<size_t>(outs) * (ins / 2), device, st);

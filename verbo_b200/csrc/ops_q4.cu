@@ -60,6 +60,7 @@ __global__ void q4_pack_kernel(Q4Mat m, const unsigned char* __restrict__ q, con
                                const unsigned char* __restrict__ z, unsigned char* __restrict__ tiles) {
   const long long nchunk = static_cast<long long>(m.ntile) * m.nkc;
   const int sets = kQ4Chunk / m.span;
+  const int groups = q4_groups(m);
   for (long long c = blockIdx.x; c < nchunk; c += gridDim.x) {
     const int tile = static_cast<int>(c / m.nkc), kc = static_cast<int>(c % m.nkc);
     unsigned char* dst = tiles + c * m.chunk_bytes;
@@ -79,7 +80,7 @@ __global__ void q4_pack_kernel(Q4Mat m, const unsigned char* __restrict__ q, con
       const int g = w / (2 * sets), set = (w / 2) % sets, o = tile * kQ4Rows + g + 8 * (w & 1);
       const int i = kc * kQ4Chunk + set * m.span;
       const bool in = o < m.outs && i < m.ins;
-      const size_t at = in ? static_cast<size_t>(o) * m.groups + i / m.group : 0;
+      const size_t at = in ? static_cast<size_t>(o) * groups + i / m.group : 0;
       reinterpret_cast<uint16_t*>(dst + 1024)[w] = in ? s[at] : uint16_t(0);
       if (m.zeros) dst[1024 + 32 * sets + w] = in ? z[at] & 15 : 0;
     }
@@ -969,7 +970,6 @@ cudaError_t launch_typed(Q4Kernel a, const Q4Args& q, const Q4Plan& p, int sms, 
 }  // namespace
 
 void q4_layout(Q4Mat& m) {
-  m.groups = (m.ins - 1) / m.group + 1;  // group may be anything up to 2^31
   m.span = m.group % 128 == 0 ? 128 : m.group % 64 == 0 ? 64 : 32;
   m.nkc = (m.ins + kQ4Chunk - 1) / kQ4Chunk;
   m.ntile = (m.outs + kQ4Rows - 1) / kQ4Rows;
