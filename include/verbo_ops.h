@@ -123,7 +123,9 @@ VERBO_CUDA_API void verbo_ops_q4_free(verbo_ops_q4* h);
    until the call's work is done; 0 for a few rows), or -1. */
 VERBO_CUDA_API long long verbo_ops_q4_workspace(const verbo_ops_q4* h, int x_type, int n);
 /* n rows x (row i at x + i*ldx, ins elements of x_type) -> n rows y (row i at
-   y + i*ldy, outs elements of y_type), on the handle's device. */
+   y + i*ldy, outs elements of y_type), on the handle's device.  If a copy inside the
+   kernel has not come after a second, the call ends with y written in part only, and
+   verbo_cuda_check() fails with it. */
 VERBO_CUDA_API int verbo_ops_q4_matvec(const verbo_ops_q4* h, const void* x, int x_type, int n, long long ldx, void* y,
                                        int y_type, long long ldy, void* workspace, long long workspace_bytes,
                                        void* stream);

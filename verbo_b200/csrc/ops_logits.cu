@@ -91,9 +91,14 @@ __device__ __forceinline__ int row_shift(const T* row) {
 // threads per SM with 16 columns per thread on their way; a slice of 4096 columns
 // has 16 KB of counters, so that lists cost no occupancy.  Measured on B200: 512
 // fp32 rows of 151936 with up to 1024 ids each 111 us, 5.6 TB/s (86% of the card's
-// copy rate); 256 bf16 rows with ids, biases and masks 49 us, 4.9 TB/s; 512 rows
-// masked in place 102 us, of which a third of the columns is written.  One slice
+// copy rate); 256 bf16 rows with ids, biases and masks 49 us, 4.9 TB/s.  One slice
 // per CTA and the window read again for each took 160 and 92 us.
+// 512 rows masked in place, a third of them free, a third nearly and a third with
+// few columns left, take 48 us: 25 to look through the masks (issue slots 72%
+// busy), the rest for the stores.  Those of masked columns beside allowed ones are
+// 4 bytes each: half of all columns masked at random takes 206 us, all of them 59.
+// The window's ids beyond the first 1024 are read again for each slice: 64 rows with
+// 32768 ids each take 70 us.
 constexpr int kProcThreads = 256;
 constexpr int kProcCols = 16;                         // columns per thread and slice
 constexpr int kProcSlice = kProcThreads * kProcCols;  // 4096

@@ -600,6 +600,9 @@ constexpr int kTileAhead = 2;  // half chunks of weights in flight per warp (fou
 // CTAs per SM.  More of them hide more, at fewer registers: 16 rows of a 151936 x
 // 896 head in groups of 32 took 35.5 us with three and 39 with two, of a 14336 x
 // 4096 matrix in groups of 64 (longer chains of fragments) 25.1 and 22.5.
+// The widest forms (NT 8; NT 4 and 2 with four sets) spill 4 to 44 bytes of registers a
+// thread.  How much goes by little: one more int in Q4Kernel made it 64 bytes in the
+// loop of 64 rows of that head, which then took 140 us in place of 81.
 template <int NT, int SETS>
 constexpr int kTileCtas = NT <= 4 && SETS == 4 ? 3 : 2;
 
@@ -770,7 +773,9 @@ __global__ void __launch_bounds__(kThreadsQ4, kTileCtas<NT, SETS>) q4_tile_kerne
       if (it >= total) break;
       const int s = it % kTileStages;
       // After a wait that ran out the warp goes on without waiting (its lanes stay
-      // together, and the barriers are met), but nothing of the CTA is stored.
+      // together, and the barriers are met), but stores no tile any more, nor do
+      // warps that see `stop`.  Tiles that were through before are in y: the call's
+      // y is partly written then, and the status says so.
       if (half == 0 && ok && !mbar_wait_limited(&full[s], (it / kTileStages) & 1)) {
         ok = false;
         stop = 1;
