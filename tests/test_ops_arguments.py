@@ -2,6 +2,9 @@
 refused, not taken modulo 2^32."""
 from __future__ import annotations
 
+import copy
+import pickle
+
 import pytest
 
 import verbo_b200 as vb
@@ -40,3 +43,12 @@ def test_rows_and_columns(shape):
         vb.process_logits(x)
     with pytest.raises(vb.VerboCudaError, match="2147483647"):
         vb.token_logprobs(x, top=1)
+
+
+@pytest.mark.parametrize("how", [copy.copy, copy.deepcopy, pickle.dumps], ids=["copy", "deepcopy", "pickle"])
+def test_a_layer_is_not_copied(how):
+    """A second object with the handle would free it a second time."""
+    layer = object.__new__(vb.Q4Linear)
+    layer._h = None
+    with pytest.raises(TypeError, match="Q4Linear"):
+        how(layer)

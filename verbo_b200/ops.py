@@ -256,7 +256,10 @@ class Q4Linear:
     [outs, ceil(ins / group)]; zeros: uint8 [outs, ceil(ins / group)] with values
     0..15, or None for 8 everywhere; bias: float32 [outs] or None.  Each a numpy
     array or a tensor of any device; they are read before the constructor
-    returns.  W[o, i] = s[o, i // group] * (q[o, i] - zeros[o, i // group])."""
+    returns.  W[o, i] = s[o, i // group] * (q[o, i] - zeros[o, i // group]).
+
+    Keep a layer as long as the CUDA graphs that were captured with it.  It cannot
+    be copied or pickled: its weights belong to one object."""
 
     def __init__(self, q, s, zeros=None, bias=None, group: int = 32, device=None):
         lib, torch, self._types = _ops()
@@ -300,6 +303,9 @@ class Q4Linear:
         if not h:
             raise _err()
         self._h = h
+
+    def __reduce_ex__(self, protocol):
+        raise TypeError("a Q4Linear cannot be copied or pickled")
 
     def close(self):
         if getattr(self, "_h", None):
