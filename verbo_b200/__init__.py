@@ -22,6 +22,8 @@ Entry points
 ``Q4Linear``        products with 4-bit weights and group scales (ops.py)
 ``process_logits``  penalties, biases and masks on logits rows, before the pick (ops.py)
 ``token_logprobs``  log-probabilities and ranks of tokens, after it (ops.py)
+``beam_select``     beam search: the best continuations of each request's beams (beam.py)
+``beam_reorder``    the beams' states in the order of the chosen parents (beam.py)
 """
 from __future__ import annotations
 
@@ -33,7 +35,7 @@ from typing import Optional, Sequence
 
 __all__ = ["Sampling", "Sampler", "VerboCudaError", "load_library", "sample", "sample_noalloc", "full_vocab_fallbacks", "shard_topk", "merge_sample",
            "seed_states", "check", "version", "ROW_STATS_FIELDS", "Batch", "Server", "Tail", "Comm",
-           "Penalties", "process_logits", "token_logprobs", "Q4Linear"]
+           "Penalties", "process_logits", "token_logprobs", "Q4Linear", "beam_select", "beam_reorder"]
 __version__ = "0.1.0"
 
 _HERE = Path(__file__).resolve().parent
@@ -648,3 +650,4 @@ class Tail:
 
 
 from .ops import Penalties, Q4Linear, process_logits, token_logprobs  # noqa: E402
+from .beam import beam_reorder, beam_select  # noqa: E402

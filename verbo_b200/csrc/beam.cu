@@ -1,0 +1,635 @@
+// Beam search's operators (include/verbo_beam.h): the best continuations of each
+// request's beams, and the beams' states in the order of the chosen parents.
+#include <climits>
+#include <type_traits>
+
+#include "beam.cuh"
+#include "device.cuh"
+#include "ops.cuh"
+#include "opsdev.cuh"
+
+namespace vb {
+namespace {
+
+// ================================================================ select ==
+// value(b, i) = score[b] + (x[b][i] - lse[b]),  lse[b] = m + log sum_j e^(x[b][j] - m)
+//
+// Two beams' candidates are ordered by their values, so the sums have to be exact
+// to well below the distance of two candidates: fp32's 1e-7 would swap a pair
+// now and then.  The terms are fp32 but without a common error (the factor log2(e)
+// is taken in two parts, so a term is off by its own roundings alone, which cancel
+// in the sum), eight of them are added in fp32 and the rest in 64 bits.  A sum goes by
+// the columns alone, not by where a row lies in memory: equal rows have equal sums
+// to the last bit, and equal candidates are ordered by their beams.
+//
+// One pass over a row finds the sum and its first `take` columns (the bound from
+// the threads' maxima, as in logprob_kernel); a cluster of CTAs shares a row where
+// the rows are few.  A second, small kernel joins the beams of a request: a lane
+// keeps the head of a beam's list, and the largest is taken `take` times.
+constexpr int kSelThreads = 512;
+constexpr int kSelWarps = kSelThreads / 32;
+constexpr int kSelVecs = 4;                         // vectors per thread and batch
+constexpr int kSelStages = 2;                       // batches in flight
+constexpr int kSelWarpVecs = kSelVecs * 32;         // a warp's vectors lie side by side
+constexpr int kSelSlots = kSelWarpVecs + 1;         // one more for rows off the 16-byte grid
+constexpr int kSelBatch = kSelVecs * kSelThreads;
+constexpr int kSelGroups = 8;  // batches whose maxima are kept (the last: of all that follow)
+constexpr int kSelCap = 1024;  // listed columns per CTA
+constexpr int kSelOffers = 8;  // maxima a warp offers at most
+constexpr int kSelMaxCluster = 8;
+constexpr float kSelLowest = -3.402823466e38f;
+// log2(e) = kLog2eHi + kLog2eLo to 2^-49
+constexpr double kLog2e = 1.4426950408889634;
+constexpr float kLog2eHi = static_cast<float>(kLog2e);
+constexpr float kLog2eLo = static_cast<float>(kLog2e - static_cast<double>(kLog2eHi));
+
+// What a row leaves for the second kernel, before its keys.
+struct SelRow {
+  double lse;  // of a row with columns at +inf: the logarithm of their number
+  int n;       // keys
+  int inf;
+};
+
+struct SelPart {
+  double s;  // sum of e^(x - m)
+  float m;
+  int ninf;
+};
+
+__device__ __forceinline__ void cp_async16_part(void* dst, const void* src, int bytes) {  // the rest is zero
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
+}
+
+template <class T>
+struct SelBatch {
+  static constexpr int N = Vec<T>::N, NV = kSelVecs;
+  Vec<T> x[NV];
+  __device__ __forceinline__ uint32_t word(int i) const {  // i in [0, 4 NV)
+    const uint4& r = x[i >> 2].raw;
+    return (i & 3) == 0 ? r.x : (i & 3) == 1 ? r.y : (i & 3) == 2 ? r.z : r.w;
+  }
+  __device__ __forceinline__ float max() const {  // NaNs left out
+    if constexpr (sizeof(T) == 4) {
+      float m = kNegInf;
+#pragma unroll
+      for (int i = 0; i < 4 * NV; ++i) m = fmaxf(m, __uint_as_float(word(i)));
+      return m;
+    } else if constexpr (std::is_same_v<T, __half>) {
+      uint32_t m = 0xfc00fc00u;
+#pragma unroll
+      for (int i = 0; i < 4 * NV; ++i) asm("max.f16x2 %0, %0, %1;" : "+r"(m) : "r"(word(i)));
+      const __half2 h = *reinterpret_cast<const __half2*>(&m);
+      return fmaxf(__low2float(h), __high2float(h));
+    } else {
+      uint32_t m = 0xff80ff80u;
+#pragma unroll
+      for (int i = 0; i < 4 * NV; ++i) asm("max.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(word(i)));
+      return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
+    }
+  }
+  // sum of e^(x - ref), NaNs left out
+  __device__ __forceinline__ double sum(float ref) const {
+    float part[NV * N / 8];
+#pragma unroll
+    for (int c = 0; c < NV * N / 8; ++c) {
+      float t = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float d = x[(c * 8 + j) / N].get((c * 8 + j) % N) - ref;
+        t += ex2(fmaf(d, kLog2eHi, d * kLog2eLo));
+      }
+      part[c] = t;
+    }
+    double s = 0.0;
+#pragma unroll
+    for (int c = 0; c < NV * N / 8; c += 2) s += static_cast<double>(part[c]) + static_cast<double>(part[c + 1]);
+    if (s != s) {  // rare: a NaN was met
+      s = 0.0;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const float d = fmaxf(x[i].get(j), kNegInf) - ref;
+          s += static_cast<double>(ex2(fmaf(d, kLog2eHi, d * kLog2eLo)));
+        }
+    }
+    return s;
+  }
+  __device__ __forceinline__ int count_inf() const {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < N; ++j) n += x[i].get(j) == -kNegInf;
+    return n;
+  }
+};
+
+__device__ __forceinline__ double shfl_xor_double(double v, int o) { return __shfl_xor_sync(0xffffffffu, v, o); }
+
+// e^x in 64 bits of a difference of maxima; 0 where there is no sum to scale.
+__device__ __forceinline__ double sel_scaled(double s, float from, float m) {
+  return s > 0.0 ? s * exp(static_cast<double>(from) - static_cast<double>(m)) : 0.0;
+}
+
+// SHIFT: a row need not begin on the 16-byte grid; a thread joins its vector from
+// two that its warp copied.
+template <class T, bool SHIFT>
+__global__ void __launch_bounds__(kSelThreads, 2) beam_rows_kernel(const BeamSelectArgs a) {
+  constexpr int N = Vec<T>::N, NT = kSelThreads, NV = kSelVecs, SLOTS = SHIFT ? kSelSlots : kSelWarpVecs;
+  extern __shared__ __align__(16) uint4 ring[];  // [kSelStages][kSelWarps][SLOTS]
+  __shared__ SelPart parts[kSelWarps];
+  __shared__ SelPart slots[kSelMaxCluster];  // the leader's: one per CTA
+  __shared__ int slot_n[kSelMaxCluster];
+  __shared__ uint64_t slot_keys[kSelMaxCluster * kBeamMaxTake];
+  __shared__ uint64_t list[kSelCap];
+  __shared__ uint64_t best[kBeamMaxTake];
+  __shared__ float group_max[kSelGroups * NT];
+  __shared__ unsigned short hits[kSelGroups * NT];  // group * NT + thread
+  __shared__ __align__(16) uint32_t offer[kSelWarps * kSelOffers];
+  __shared__ int count, nhits;
+  __shared__ uint32_t bound;
+  __shared__ uint64_t bound_key;
+
+  cg::cluster_group cl = cg::this_cluster();
+  const int C = cl.num_blocks();
+  const int rankc = cl.block_rank();
+  if (C > 1) cluster_arrive();  // every CTA of the cluster has started before one writes to the leader
+  const int row = blockIdx.x / C;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) {
+    count = 0;
+    nhits = 0;
+    bound = 0xffffffffu;
+  }
+  grid_wait();
+  grid_release();
+  const int top = a.take;
+  const T* in = static_cast<const T*>(a.logits) + row * a.ld;
+  const bool dead = !(a.scores[row] > kNegInf);  // no candidates: the row is not read (the same in the whole cluster)
+  const int shift = SHIFT ? static_cast<int>(reinterpret_cast<uintptr_t>(in) & 15) : 0;  // bytes
+  const char* grid = reinterpret_cast<const char*>(in) - shift;
+  const long long last = static_cast<long long>(a.vocab) * sizeof(T) + shift;  // the row's end, from `grid`
+  // vectors are counted by columns, whatever the row's place
+  const int nvec = dead ? 0 : (a.vocab + N - 1) / N;
+  const int v0 = static_cast<int>(static_cast<long long>(nvec) * rankc / C);
+  const int v1 = static_cast<int>(static_cast<long long>(nvec) * (rankc + 1) / C);
+  const int nbatch = (v1 - v0 + kSelBatch - 1) / kSelBatch;
+
+  auto copy = [&](uint4* to, int v) {  // the 16 bytes at v of the row's grid
+    const long long at = static_cast<long long>(v) * 16;
+    const int bytes = static_cast<int>(last - at < 16 ? (last - at > 0 ? last - at : 0) : 16);
+    if (SHIFT && v == 0) {  // what lies before the row is not read
+      T* t = reinterpret_cast<T*>(to);
+      const int first = shift / static_cast<int>(sizeof(T));
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (j >= first && j * static_cast<int>(sizeof(T)) < bytes) t[j] = in[j - first];
+    } else {
+      cp_async16_part(to, bytes > 0 ? grid + at : grid + 16 * (v0 + 1) - 16, bytes);
+    }
+  };
+  auto fetch = [&](int b) {
+    if (b < nbatch) {
+      uint4* to = ring + ((b % kSelStages) * kSelWarps + warp) * SLOTS;
+      const int v = v0 + b * kSelBatch + warp * kSelWarpVecs;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (v + i * 32 + lane < v1 + (SHIFT ? 1 : 0)) copy(to + i * 32 + lane, v + i * 32 + lane);
+      if (SHIFT && lane == 0 && v + kSelWarpVecs < v1 + 1) copy(to + kSelWarpVecs, v + kSelWarpVecs);
+    }
+    cp_async_commit();  // an empty group keeps the count
+  };
+#pragma unroll
+  for (int b = 0; b < kSelStages; ++b) fetch(b);
+
+  float ref = kNegInf, mx = kNegInf;
+  double sum = 0.0;
+  int ninf = 0;
+  for (int b = 0; b < nbatch; ++b) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kSelStages - 1) : "memory");
+    if (SHIFT) __syncwarp();
+    SelBatch<T> x;
+    const uint4* from = ring + ((b % kSelStages) * kSelWarps + warp) * SLOTS + lane;
+    const int vb = v0 + b * kSelBatch + warp * kSelWarpVecs + lane;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (SHIFT) {
+        const uint4 p = from[i * 32], q = from[i * 32 + 1];
+        uint32_t w[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
+        if (shift & 8) {
+#pragma unroll
+          for (int j = 0; j < 6; ++j) w[j] = w[j + 2];
+        }
+        if (shift & 4) {
+#pragma unroll
+          for (int j = 0; j < 5; ++j) w[j] = w[j + 1];
+        }
+        const int bits = (shift & 3) * 8;
+        x.x[i].raw = make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
+                                __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+      } else {
+        x.x[i].raw = from[i * 32];
+      }
+      // the row's last, short vector, and those behind the part
+      const int v = vb + i * 32;
+      if (v >= v1) {
+        x.x[i].raw = all_neg_inf<T>();
+      } else if (v == nvec - 1 && a.vocab % N) {
+        const int have = a.vocab % N;
+        uint4 r = x.x[i].raw;
+        const uint4 none = all_neg_inf<T>();
+        uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          constexpr int P = N / 4;  // columns of a word
+          if (j * P >= have)
+            w[j] = none.x;
+          else if (P == 2 && j * P + 1 >= have)
+            w[j] = (w[j] & 0xffffu) | (none.x & 0xffff0000u);
+        }
+        x.x[i].raw = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+    if (SHIFT) __syncwarp();
+    fetch(b + kSelStages);
+    const float bm = x.max();
+    mx = fmaxf(mx, bm);
+    if (bm == -kNegInf) {
+      ninf += x.count_inf();
+    } else if (bm > kNegInf) {
+      // The first maximum is kept: terms may be above 1, but not by more than 2^64.
+      if (ref == kNegInf) {
+        ref = bm;
+      } else if (bm - ref > 44.0f) {
+        sum = sel_scaled(sum, ref, bm);
+        ref = bm;
+      }
+      sum += x.sum(ref);
+    }
+    float* at = &group_max[min(b, kSelGroups - 1) * NT + tid];
+    *at = b < kSelGroups ? bm : fmaxf(*at, bm);
+  }
+
+  // the CTA's part of the row
+  SelPart p;
+  p.m = unord32(__reduce_max_sync(0xffffffffu, ord32(mx + 0.0f)));
+  p.s = fabsf(p.m) < -kNegInf ? sel_scaled(sum, ref, p.m) : 0.0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) p.s += shfl_xor_double(p.s, o);
+  p.ninf = __reduce_add_sync(0xffffffffu, ninf);
+  if (lane == 0) parts[warp] = p;
+
+  // Every warp offers its q largest maxima; the `top`-th of all offers is the
+  // bound (q * kSelWarps >= top of them, each of another thread).
+  const uint32_t mine = ord32(mx + 0.0f);
+  const int q = min(kSelOffers, 2 * ((top + kSelWarps - 1) / kSelWarps));
+  uint32_t o = mine;
+  for (int i = 0; i < q; ++i) {
+    const uint32_t w = __reduce_max_sync(0xffffffffu, o);
+    const unsigned at = __ballot_sync(0xffffffffu, o == w);
+    if (lane == __ffs(at) - 1) {
+      offer[warp * q + i] = w;
+      o = 0;
+    }
+  }
+  __syncthreads();
+  SelPart total;  // in warp 0
+  if (warp == 0) {
+    const SelPart w = lane < kSelWarps ? parts[lane] : SelPart{0.0, kNegInf, 0};
+    total.m = unord32(__reduce_max_sync(0xffffffffu, ord32(w.m + 0.0f)));
+    total.s = fabsf(total.m) < -kNegInf ? sel_scaled(w.s, w.m, total.m) : 0.0;
+#pragma unroll
+    for (int i = kSelWarps / 2; i > 0; i >>= 1) total.s += shfl_xor_double(total.s, i);
+    total.ninf = __reduce_add_sync(0xffffffffu, w.ninf);
+  }
+  // the bound: an offer with fewer than `top` above it and `top` at or above it
+  if (tid >= 32 && tid < 32 + q * kSelWarps) {
+    const uint32_t w = offer[tid - 32];
+    int gt = 0, ge = 0;
+#pragma unroll 4
+    for (int j = 0; j < q * kSelWarps; j += 4) {
+      const uint4 v = *reinterpret_cast<const uint4*>(offer + j);
+      gt += (v.x > w) + (v.y > w) + (v.z > w) + (v.w > w);
+      ge += (v.x >= w) + (v.y >= w) + (v.z >= w) + (v.w >= w);
+    }
+    if (gt < top && top <= ge) bound = max(w, ord32(kSelLowest));  // a column at -inf is no candidate
+  }
+  __syncthreads();
+  const uint32_t low = bound;
+  const float thr = unord32(low);
+  if (mine >= low) {
+    for (int g = 0; g < min(nbatch, kSelGroups); ++g)
+      if (group_max[g * NT + tid] >= thr) hits[atomicAdd(&nhits, 1)] = static_cast<unsigned short>(g * NT + tid);
+  }
+  __syncthreads();
+  const int lastn = max(1, nbatch - kSelGroups + 1);  // batches of the last group
+  for (int i = tid; i < nhits * (NV * lastn); i += NT) {
+    const int h = lastn == 1 ? i / NV : i / (NV * lastn);
+    const int k = i - h * (NV * lastn);
+    const int g = hits[h] / NT, t = hits[h] % NT;
+    if (k >= NV && g < kSelGroups - 1) continue;
+    const int v = v0 + (g + k / NV) * kSelBatch + (t >> 5) * kSelWarpVecs + (k % NV) * 32 + (t & 31);
+    if (v >= v1) continue;
+    const int col = v * N, have = min(N, a.vocab - col);
+    if (!SHIFT && have == N) {
+      Vec<T> r;
+      r.raw = *reinterpret_cast<const uint4*>(in + col);
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (r.get(j) >= thr) {
+          const int at = atomicAdd(&count, 1);
+          if (at < kSelCap) list[at] = dkey(r.get(j), col + j);
+        }
+    } else {
+      for (int j = 0; j < have; ++j) {
+        const float e = to_float(in[col + j]);
+        if (e >= thr) {
+          const int at = atomicAdd(&count, 1);
+          if (at < kSelCap) list[at] = dkey(e, col + j);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  int n = count;
+  // Too many: the `top`-th of those that were kept is a bound that as many
+  // columns reach; gather again from it on, in the order of the keys (distinct,
+  // so at least kSelCap - top columns drop out each time).
+  while (n > kSelCap) {
+    for (int i = tid; i < kSelCap; i += NT) {
+      int r = 0;
+      const uint64_t k = list[i];
+      for (int j = 0; j < kSelCap; ++j) r += list[j] < k;
+      if (r == top - 1) bound_key = k;
+    }
+    __syncthreads();
+    const uint64_t bk = bound_key;
+    if (tid == 0) count = 0;
+    __syncthreads();
+    const int hi = min(a.vocab, v1 * N);
+    for (int col = v0 * N + tid; col < hi; col += NT) {
+      const float e = fmaxf(to_float(in[col]), kNegInf);
+      const uint64_t k = dkey(e, col);
+      if (e > kNegInf && k <= bk) {
+        const int at = atomicAdd(&count, 1);
+        if (at < kSelCap) list[at] = k;
+      }
+    }
+    __syncthreads();
+    n = count;
+    __syncthreads();
+  }
+  const int ntop = min(n, top);
+  for (int i = tid; i < n; i += NT) {
+    int r = 0;
+    const uint64_t k = list[i];
+    for (int j = 0; j < n; ++j) r += list[j] < k;
+    if (r < top) best[r] = k;
+  }
+  __syncthreads();
+
+  if (C > 1) {
+    cluster_wait();
+    if (tid == 0) {
+      *cl.map_shared_rank(&slots[rankc], 0) = total;
+      *cl.map_shared_rank(&slot_n[rankc], 0) = ntop;
+    }
+    if (tid < ntop) *cl.map_shared_rank(&slot_keys[rankc * kBeamMaxTake + tid], 0) = best[tid];
+    cluster_sync_all();
+    if (rankc != 0) return;
+  } else {
+    if (tid == 0) {
+      slots[0] = total;
+      slot_n[0] = ntop;
+    }
+    if (tid < ntop) slot_keys[tid] = best[tid];
+    __syncthreads();
+  }
+
+  // the leader: the row's sum, and a key's place: its own in its list and what
+  // comes before it in the others
+  uint64_t* keys = static_cast<uint64_t*>(a.workspace) + static_cast<long long>(row) * (top + 2);
+  float m = kNegInf;
+  int inf = 0, have = 0;
+  for (int i = 0; i < C; ++i) {
+    m = fmaxf(m, slots[i].m);
+    inf += slots[i].ninf;
+    have += slot_n[i];
+  }
+  if (tid == 0) {
+    double s = 0.0;
+    if (m != -kNegInf)
+      for (int i = 0; i < C; ++i) s += sel_scaled(slots[i].s, slots[i].m, m);
+    SelRow r;
+    r.inf = inf > 0;
+    r.lse = inf > 0 ? log(static_cast<double>(inf)) : static_cast<double>(m) + log(s);
+    r.n = min(top, inf > 0 ? min(inf, have) : have);
+    *reinterpret_cast<SelRow*>(keys) = r;
+  }
+  for (int i = tid; i < C * top; i += NT) {
+    const int l = i / top, at = i - l * top;
+    if (at >= slot_n[l]) continue;
+    const uint64_t k = slot_keys[l * kBeamMaxTake + at];
+    int r = at;
+    for (int c = 0; c < C; ++c) {
+      if (c == l) continue;
+      int b = 0, e = slot_n[c];
+      while (b < e) {
+        const int h = (b + e) >> 1;
+        if (slot_keys[c * kBeamMaxTake + h] < k)
+          b = h + 1;
+        else
+          e = h;
+      }
+      r += b;
+    }
+    if (r < top) keys[2 + r] = k;
+  }
+}
+
+// Order-preserving code of a value in 64 bits (no NaN); larger value, larger code.
+__device__ __forceinline__ uint64_t ord64(double v) {
+  const uint64_t b = static_cast<uint64_t>(__double_as_longlong(v + 0.0));
+  return b & 0x8000000000000000ull ? ~b : b | 0x8000000000000000ull;
+}
+__device__ __forceinline__ double unord64(uint64_t o) {
+  return __longlong_as_double(static_cast<long long>(o & 0x8000000000000000ull ? o & 0x7fffffffffffffffull : ~o));
+}
+
+constexpr int kJoinThreads = 256;
+
+// One CTA per request.  Codes of the lists' values in shared memory, then warp 0
+// takes the largest head `take` times; equal values go by the beam.  A code of 0
+// is no value's: the end of a list.
+__global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const BeamSelectArgs a) {
+  extern __shared__ uint64_t codes[];  // [beams][take + 1], then tokens [beams][take]
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int K = a.beams, top = a.take;
+  uint32_t* toks = reinterpret_cast<uint32_t*>(codes + K * (top + 1));
+  grid_wait();
+  grid_release();
+  const int req = blockIdx.x;
+  const uint64_t* ws = static_cast<const uint64_t*>(a.workspace) + static_cast<long long>(req) * K * (top + 2);
+  for (int i = tid; i < K * (top + 1); i += kJoinThreads) {
+    const int b = i / (top + 1), j = i - b * (top + 1);
+    const uint64_t* keys = ws + static_cast<long long>(b) * (top + 2);
+    const SelRow r = *reinterpret_cast<const SelRow*>(keys);
+    const float score = a.scores[static_cast<long long>(req) * K + b];
+    uint64_t code = 0;
+    if (score > kNegInf && j < r.n) {
+      const uint64_t k = keys[2 + j];
+      const double lp = r.inf ? -r.lse : static_cast<double>(dval(k)) - r.lse;
+      const double v = static_cast<double>(score) + lp;
+      if (v > -static_cast<double>(__int_as_float(0x7f800000))) code = ord64(v);
+      toks[b * top + j] = did(k);
+    }
+    codes[i] = code;
+  }
+  __syncthreads();
+  if (tid >= 32) return;
+  int at = 0;
+  uint64_t head = lane < K ? codes[lane * (top + 1)] : 0;
+  const long long out = static_cast<long long>(req) * top;
+  for (int i = 0; i < top; ++i) {
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(head >> 32));
+    const uint32_t low = static_cast<uint32_t>(head >> 32) == hi ? static_cast<uint32_t>(head) : 0u;
+    const uint32_t lo = __reduce_max_sync(0xffffffffu, low);
+    const unsigned who =
+        __ballot_sync(0xffffffffu, static_cast<uint32_t>(head >> 32) == hi && static_cast<uint32_t>(head) == lo);
+    if (hi == 0 && lo == 0) {  // no candidates are left
+      for (int j = i + lane; j < top; j += 32) {
+        a.out_scores[out + j] = kNegInf;
+        a.parents[out + j] = -1;
+        a.tokens[out + j] = -1;
+      }
+      return;
+    }
+    if (lane == __ffs(who) - 1) {
+      a.out_scores[out + i] = static_cast<float>(unord64(head));
+      a.parents[out + i] = lane;
+      a.tokens[out + i] = static_cast<int>(toks[lane * top + at]);
+      ++at;
+      head = codes[lane * (top + 1) + at];
+    }
+  }
+}
+
+template <class T, bool SHIFT>
+cudaError_t run_select(const BeamSelectArgs& a, cudaStream_t s) {
+  // CTAs per row: one, or as many as give each SM one, with a batch each.
+  const long long batches = (a.vocab / Vec<T>::N + kSelBatch - 1) / kSelBatch;
+  const long long rows = static_cast<long long>(a.requests) * a.beams;
+  const int sms = sm_count();
+  int C = 1;
+  while (C < kSelMaxCluster && C < batches && rows * C < sms) C <<= 1;
+  const long long grid = rows * C;
+  if (grid > INT_MAX) return cudaErrorInvalidConfiguration;
+  constexpr int smem = kSelStages * kSelWarps * (SHIFT ? kSelSlots : kSelWarpVecs) * 16;
+  const auto kernel = beam_rows_kernel<T, SHIFT>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  e = launch_chained(kernel, static_cast<unsigned>(grid), kSelThreads, smem, C, s, a);
+  if (e != cudaSuccess) return e;
+  const size_t lists = static_cast<size_t>(a.beams) * ((a.take + 1) * 8 + a.take * 4);
+  return launch_chained(beam_join_kernel, static_cast<unsigned>(a.requests), kJoinThreads, lists, 1, s, a);
+}
+
+template <class T>
+cudaError_t run_select(const BeamSelectArgs& a, cudaStream_t s) {
+  const bool on_grid = reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 &&
+                       (static_cast<long long>(a.requests) * a.beams == 1 || a.ld % Vec<T>::N == 0);
+  return on_grid ? run_select<T, false>(a, s) : run_select<T, true>(a, s);
+}
+
+// =============================================================== reorder ==
+// state[r][k] <- state[r][parent[r][k]] in place.  A thread owns one column (W
+// bytes) of a request's rows: it reads all rows' parents at that column, then
+// writes them, so nothing is read after it was written and no copy is kept.
+// Rows that are their own parents are neither read nor written.
+constexpr int kReorderThreads = 256;
+
+template <int W>
+struct Piece;
+template <>
+struct Piece<16> {
+  using type = uint4;
+};
+template <>
+struct Piece<4> {
+  using type = uint32_t;
+};
+template <>
+struct Piece<1> {
+  using type = unsigned char;
+};
+
+template <int K, int W>
+__global__ void __launch_bounds__(kReorderThreads) beam_reorder_kernel(const BeamReorderArgs a) {
+  using P = typename Piece<W>::type;
+  grid_wait();
+  grid_release();
+  int t = 0;
+  while (t + 1 < a.n && blockIdx.x >= a.first[t + 1]) ++t;
+  const unsigned i = blockIdx.x - a.first[t];
+  const unsigned req = i / a.chunks[t];
+  const long long col = (static_cast<long long>(i - req * a.chunks[t]) * kReorderThreads + threadIdx.x) * W;
+  const BeamState st = a.states[t];
+  if (col >= st.row_bytes) return;
+  const int* parents = a.parents + req * a.ld_parents;
+  char* at = static_cast<char*>(st.data) + static_cast<long long>(req) * a.beams * st.stride_bytes + col;
+  int from[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    from[k] = k < a.beams ? parents[k] : k;
+    if (from[k] < 0 || from[k] >= a.beams) from[k] = k;
+  }
+  P v[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+    if (from[k] != k) v[k] = *reinterpret_cast<const P*>(at + from[k] * st.stride_bytes);
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+    if (from[k] != k) *reinterpret_cast<P*>(at + k * st.stride_bytes) = v[k];
+}
+
+template <int W>
+cudaError_t run_reorder(const BeamReorderArgs& a, unsigned grid, cudaStream_t s) {
+  if (a.beams <= 4) return launch_chained(beam_reorder_kernel<4, W>, grid, kReorderThreads, 0, 1, s, a);
+  if (a.beams <= 8) return launch_chained(beam_reorder_kernel<8, W>, grid, kReorderThreads, 0, 1, s, a);
+  if (a.beams <= 16) return launch_chained(beam_reorder_kernel<16, W>, grid, kReorderThreads, 0, 1, s, a);
+  return launch_chained(beam_reorder_kernel<32, W>, grid, kReorderThreads, 0, 1, s, a);
+}
+
+}  // namespace
+
+size_t beam_workspace_bytes(int rows, int take) {
+  static_assert(sizeof(SelRow) == 16, "a row's record is two keys long");
+  return static_cast<size_t>(rows) * (take + 2) * 8;
+}
+
+cudaError_t launch_beam_select(const BeamSelectArgs& a, int dtype, cudaStream_t s) {
+  if (dtype == kOpsF16) return run_select<__half>(a, s);
+  if (dtype == kOpsBF16) return run_select<__nv_bfloat16>(a, s);
+  return run_select<float>(a, s);
+}
+
+cudaError_t launch_beam_reorder(BeamReorderArgs a, int requests, int width, cudaStream_t s) {
+  unsigned long long ctas = 0;
+  for (int i = 0; i < a.n; ++i) {
+    const long long per = static_cast<long long>(kReorderThreads) * width;
+    const long long chunks = (a.states[i].row_bytes + per - 1) / per;
+    if (chunks > INT_MAX) return cudaErrorInvalidConfiguration;
+    a.first[i] = static_cast<unsigned>(ctas);
+    a.chunks[i] = static_cast<unsigned>(chunks);
+    ctas += static_cast<unsigned long long>(chunks) * requests;
+    if (ctas > INT_MAX) return cudaErrorInvalidConfiguration;
+  }
+  if (ctas == 0) return cudaSuccess;
+  const unsigned grid = static_cast<unsigned>(ctas);
+  if (width == 16) return run_reorder<16>(a, grid, s);
+  if (width == 4) return run_reorder<4>(a, grid, s);
+  return run_reorder<1>(a, grid, s);
+}
+
+}  // namespace vb

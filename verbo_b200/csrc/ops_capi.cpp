@@ -5,6 +5,7 @@
 #include <cmath>
 #include <string>
 
+#include "capi_checks.hpp"
 #include "capi_guard.hpp"
 #include "ops.cuh"
 #include "verbo_ops.h"
@@ -18,9 +19,13 @@ struct verbo_ops_q4 {
 
 namespace {
 
+using vb::check_aligned;
+using vb::check_rows;
+using vb::check_type;
 using vb::cuda_ok;
 using vb::fail;
 using vb::guard;
+using vb::overlap;
 
 // The calls on a handle run on its device and leave the caller's current.
 class DeviceScope {
@@ -59,35 +64,6 @@ class BesideCaptures {
   cudaStreamCaptureMode mode_ = cudaStreamCaptureModeRelaxed;
   bool changed_ = false;
 };
-
-void check_type(int t, const char* what) {
-  if (t != VERBO_OPS_F32 && t != VERBO_OPS_F16 && t != VERBO_OPS_BF16)
-    fail(std::string(what) + " must be VERBO_OPS_F32, VERBO_OPS_F16 or VERBO_OPS_BF16");
-}
-
-void check_aligned(const void* p, int size, const char* what) {
-  if (reinterpret_cast<uintptr_t>(p) % static_cast<unsigned>(size))
-    fail(std::string(what) + " must be aligned to its elements");
-}
-
-void check_rows(const void* p, int type, int rows, int cols, long long ld, const char* what) {
-  if (!p) fail(std::string(what) + " must not be NULL");
-  check_aligned(p, vb::ops_type_size(type), what);
-  if (ld < cols) fail(std::string(what) + ": the row stride must be at least the row's length");
-  if (ld > (1ll << 62) / (static_cast<long long>(rows) * 4)) fail(std::string(what) + ": the row stride is too large");
-}
-
-// Whether two sets of rows can touch the same byte.  Rows of one pitch that
-// lie beside each other in it (two halves of one buffer) do not.
-bool overlap(const void* a, long long pa, long long la, const void* b, long long pb, long long lb, int rows_b,
-             int rows_a) {
-  const char *x = static_cast<const char*>(a), *y = static_cast<const char*>(b);
-  const char *xe = x + (rows_a - 1) * pa + la, *ye = y + (rows_b - 1) * pb + lb;
-  if (xe <= y || ye <= x) return false;
-  if (pa != pb || rows_a != rows_b) return true;
-  const long long d = ((y - x) % pa + pa) % pa;
-  return !(d >= la && d + lb <= pa);
-}
 
 }  // namespace
 

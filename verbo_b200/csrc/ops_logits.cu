@@ -1,67 +1,16 @@
 // Logits operators around the sampler (include/verbo_ops.h): penalties, biases
 // and masks before the pick, log-probabilities after it.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
 #include <algorithm>
 #include <climits>
 #include <type_traits>
 
 #include "device.cuh"
 #include "ops.cuh"
+#include "opsdev.cuh"
 
 namespace vb {
 namespace {
 
-constexpr float kNegInf = -__builtin_huge_valf();
-
-template <class T>
-__device__ __forceinline__ float to_float(T v);
-template <>
-__device__ __forceinline__ float to_float(float v) {
-  return v;
-}
-template <>
-__device__ __forceinline__ float to_float(__half v) {
-  return __half2float(v);
-}
-template <>
-__device__ __forceinline__ float to_float(__nv_bfloat16 v) {
-  return __bfloat162float(v);
-}
-
-// Elements of a 16-byte vector as floats.
-template <class T>
-struct Vec {
-  static constexpr int N = 16 / sizeof(T);
-  uint4 raw;
-  __device__ __forceinline__ float get(int i) const;
-};
-template <>
-__device__ __forceinline__ float Vec<float>::get(int i) const {
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-  return __uint_as_float(w[i]);
-}
-template <>
-__device__ __forceinline__ float Vec<__half>::get(int i) const {
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-  return __half2float(__ushort_as_half(static_cast<unsigned short>(w[i >> 1] >> (16 * (i & 1)))));
-}
-template <>
-__device__ __forceinline__ float Vec<__nv_bfloat16>::get(int i) const {
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-  return __uint_as_float((i & 1) ? (w[i >> 1] & 0xffff0000u) : (w[i >> 1] << 16));
-}
-
-// Not the read-only path: a kernel that is launched programmatically has begun
-// before the grid whose rows it reads has ended.
-__device__ __forceinline__ uint4 ld_stream16(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.L1::no_allocate.L2::256B.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
-}
 __device__ __forceinline__ uint32_t ld_word(const uint32_t* p) {
   uint32_t v;
   asm volatile("ld.global.u32 %0, [%1];" : "=r"(v) : "l"(p));
@@ -309,25 +258,6 @@ __global__ void __launch_bounds__(kProcThreads, !LISTS && INPLACE ? 8 : 4) proce
   }
 }
 
-template <class K, class A>
-cudaError_t launch_chained(K kernel, unsigned grid, int threads, size_t smem, int cluster, cudaStream_t s, const A& a) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim.x = cluster;
-  at[1].val.clusterDim.y = 1;
-  at[1].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = cluster > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kernel, a);
-}
-
 // Parts of as many slices as leave at least four waves of CTAs, 8 at most.
 template <class T, bool INPLACE>
 cudaError_t run_process(ProcArgs a, cudaStream_t s) {
@@ -386,12 +316,6 @@ struct LpPart {
   int ninf;    // columns at +inf
   int ntop;    // keys in the slot
 };
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 // s seen from another maximum m >= the one it was taken at.
 __device__ __forceinline__ float lp_scaled(float s, float from, float m, float c) {
@@ -530,21 +454,6 @@ struct LpOne {  // a single column
     f(v, 0);
   }
 };
-
-template <class T>
-__device__ __forceinline__ uint4 all_neg_inf();
-template <>
-__device__ __forceinline__ uint4 all_neg_inf<float>() {
-  return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u);
-}
-template <>
-__device__ __forceinline__ uint4 all_neg_inf<__half>() {
-  return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u);
-}
-template <>
-__device__ __forceinline__ uint4 all_neg_inf<__nv_bfloat16>() {
-  return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
-}
 
 template <class T, bool TOP>
 __global__ void __launch_bounds__(kLpThreads, 2) logprob_kernel(const LogprobArgs a) {
