@@ -24,6 +24,7 @@ Entry points
 ``token_logprobs``  log-probabilities and ranks of tokens, after it (ops.py)
 ``beam_select``     beam search: the best continuations of each request's beams (beam.py)
 ``beam_reorder``    the beams' states in the order of the chosen parents (beam.py)
+``PagedCache``      keys and values in 8 bits, in pages that rows share: reserve, fork, free, compact, append, attend (cache.py)
 """
 from __future__ import annotations
 
@@ -35,7 +36,8 @@ from typing import Optional, Sequence
 
 __all__ = ["Sampling", "Sampler", "VerboCudaError", "load_library", "sample", "sample_noalloc", "full_vocab_fallbacks", "shard_topk", "merge_sample",
            "seed_states", "check", "version", "ROW_STATS_FIELDS", "Batch", "Server", "Tail", "Comm",
-           "Penalties", "process_logits", "token_logprobs", "Q4Linear", "beam_select", "beam_reorder"]
+           "Penalties", "process_logits", "token_logprobs", "Q4Linear", "beam_select", "beam_reorder",
+           "PagedCache"]
 __version__ = "0.1.0"
 
 _HERE = Path(__file__).resolve().parent
@@ -651,3 +653,4 @@ class Tail:
 
 from .ops import Penalties, Q4Linear, process_logits, token_logprobs  # noqa: E402
 from .beam import beam_reorder, beam_select  # noqa: E402
+from .cache import PagedCache  # noqa: E402

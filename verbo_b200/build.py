@@ -20,10 +20,12 @@ CSRC = PKG / "csrc"
 LIB_DIR = PKG / "_lib"
 LIB = LIB_DIR / "libverbo_cuda.so"
 SOURCES = [CSRC / "kernels.cu", CSRC / "nucleus.cu", CSRC / "tail.cu", CSRC / "ops_logits.cu", CSRC / "ops_q4.cu",
-           CSRC / "beam.cu", CSRC / "capi.cpp", CSRC / "ops_capi.cpp", CSRC / "beam_capi.cpp"]
+           CSRC / "beam.cu", CSRC / "cache_pages.cu", CSRC / "cache_attend.cu", CSRC / "capi.cpp", CSRC / "ops_capi.cpp",
+           CSRC / "beam_capi.cpp", CSRC / "cache_capi.cpp"]
 HEADERS = [CSRC / "device.cuh", CSRC / "kernels.cuh", CSRC / "rowdev.cuh", CSRC / "tail.cuh",
-           CSRC / "ops.cuh", CSRC / "opsdev.cuh", CSRC / "beam.cuh", CSRC / "capi_guard.hpp", CSRC / "capi_checks.hpp",
-           ROOT / "include" / "verbo_cuda.h", ROOT / "include" / "verbo_ops.h", ROOT / "include" / "verbo_beam.h"]
+           CSRC / "ops.cuh", CSRC / "opsdev.cuh", CSRC / "beam.cuh", CSRC / "cache.cuh", CSRC / "capi_guard.hpp",
+           CSRC / "capi_checks.hpp", ROOT / "include" / "verbo_cuda.h", ROOT / "include" / "verbo_ops.h",
+           ROOT / "include" / "verbo_beam.h", ROOT / "include" / "verbo_cache.h"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
