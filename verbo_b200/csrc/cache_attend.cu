@@ -30,10 +30,12 @@ namespace {
 
 constexpr int kAttWarps = 8;
 constexpr int kAttThreads = kAttWarps * 32;
-constexpr int kAttRows = 8;      // query rows of a tile: heads that share a token, times steps
-constexpr int kAttFlush = 8;     // blocks between two transfers of the sums
-constexpr int kAttStages = 6;    // blocks in flight per warp, at most
-constexpr float kUp = 14.0f;     // weights are held times 2^14: fp16's subnormals begin at 2^-28 of the largest
+constexpr int kAttRows = 8;    // query rows of a tile: heads that share a token, times steps
+constexpr int kAttPair = 2;    // blocks of a step
+constexpr int kAttFlush = 4;   // steps between two transfers of the sums
+constexpr int kAttStages = 3;  // steps whose copies are in flight
+constexpr int kAttHeads = 64;  // blocks that are known ahead, per warp
+constexpr float kUp = 14.0f;   // weights are held times 2^14: fp16's subnormals begin at 2^-28 of the largest
 constexpr double kLog2e = 1.4426950408889634;
 
 struct AttendArgs {
@@ -53,11 +55,11 @@ struct AttendArgs {
   int tiles;      // of kAttRows query rows
   int teams;      // warps that share a part of the blocks, one tile each: grid warps / tiles
   int least;      // blocks that a warp takes at least
-  int stages;
   int q_type, out_type;
+  bool wide_q, wide_out;  // 16 bytes at a time
   float c_hi, c_lo;  // scale * log2(e)
   float* parts;      // [teams][tiles][2][part_floats]
-  long long* first;  // [rows + 1] blocks before each row
+  int* first;        // [rows + 1] blocks before each row
 };
 __host__ __device__ inline int part_floats(int dim) { return kAttRows * (dim + 2); }
 
@@ -107,22 +109,74 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 __device__ __forceinline__ void cp_async16_if(uint32_t dst, const void* src, bool take) {  // zeros otherwise
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+
+// 16 elements from `p` on, as floats.
+__device__ __forceinline__ void load16(const void* p, long long i, int type, bool wide, float (&x)[16]) {
+  if (!wide) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) x[j] = load_any(p, i + j, type);
+  } else if (type == kOpsF32) {
+    const float4* v = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float4 y = v[j];
+      x[4 * j] = y.x, x[4 * j + 1] = y.y, x[4 * j + 2] = y.z, x[4 * j + 3] = y.w;
+    }
+  } else {
+    const uint4* v = reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(p) + i);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint4 y = v[j];
+      const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float2 f;
+        if (type == kOpsF16)
+          f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+        else
+          f = make_float2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
+        x[8 * j + 2 * k] = f.x, x[8 * j + 2 * k + 1] = f.y;
+      }
+    }
+  }
+}
+__device__ __forceinline__ void store16(void* p, long long i, int type, bool wide, const float (&x)[16]) {
+  if (!wide) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) store_any(p, i + j, type, x[j]);
+  } else if (type == kOpsF32) {
+    float4* v = reinterpret_cast<float4*>(static_cast<float*>(p) + i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
+  } else {
+    uint4* v = reinterpret_cast<uint4*>(static_cast<unsigned short*>(p) + i);
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (type == kOpsF16) {
+        w[j] = two_halves(x[2 * j], x[2 * j + 1]);
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
+        w[j] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    v[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    v[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
 }
 
 // Blocks of 16 tokens before each row, in shared memory (rows + 1), by the CTA.
-__device__ __forceinline__ void scan_rows(const AttendArgs& a, long long* first, long long* ws) {
-  long long base = 0;
+__device__ __forceinline__ void scan_rows(const AttendArgs& a, int* first, int* ws) {
+  int base = 0;
   for (int r0 = 0; r0 < a.rows; r0 += kAttThreads) {
     const int r = r0 + threadIdx.x;
-    long long n = 0;
+    int n = 0;
     if (r < a.rows) {
       const int len = max(0, min(a.lens[r], a.width * a.page));
-      n = (len + kCacheBlock - 1) / kCacheBlock;
+      n = len / kCacheBlock + (len % kCacheBlock > 0);
     }
-    long long total;
-    const long long at = block_excl_scan<long long, kAttThreads>(n, ws, &total);
+    int total;
+    const int at = block_excl_scan<int, kAttThreads>(n, ws, &total);
     if (r < a.rows) first[r] = base + at;
     base += total;
     __syncthreads();
@@ -131,40 +185,47 @@ __device__ __forceinline__ void scan_rows(const AttendArgs& a, long long* first,
   __syncthreads();
 }
 
-struct __align__(16) SlotHead {
+// What is known of a block before it is copied.
+struct __align__(16) BlockHead {
   float ks, vs;
-  int valid;
-  int pad;
+  int valid;  // tokens, 0 where there is no page
+  int block;  // of the layer's pool
 };
 
-// DP: the head dimension filled up with zeros.  Shared memory per warp: `stages`
-// slots of a block's keys and values, rows of DP bytes whose 16-byte chunks are
+// DP: the head dimension filled up with zeros.  Shared memory per warp: kAttStages
+// steps of two blocks' keys and values, rows of DP bytes whose 16-byte chunks are
 // exchanged so that the fragment loads below meet no bank twice.
 template <int DP>
+struct AttShape {
+  static constexpr int kBlock = 16 * DP;                   // bytes of a block's keys, and of its values
+  static constexpr int kStep = kAttPair * 2 * kBlock;      // of a step
+  static constexpr int kRing = kAttStages * kStep;
+  static constexpr int kWarp = kRing + kAttHeads * static_cast<int>(sizeof(BlockHead));
+};
+
+template <int DP>
 __global__ void __launch_bounds__(kAttThreads, DP == 64 ? 2 : 1) cache_attend_kernel(const AttendArgs a) {
-  constexpr int NJ = DP / 8;            // output tiles of 8 dims
-  constexpr int KS = DP / 16;           // steps of 16 dims
-  constexpr int CH = DP / 32;           // chunks that a lane copies of a block's keys
-  constexpr int BLOCK_BYTES = 16 * DP;  // of keys, and of values
-  constexpr int OWN = DP / 4;           // output dims of a lane
+  using S = AttShape<DP>;
+  constexpr int NJ = DP / 8;   // output tiles of 8 dims
+  constexpr int KS = DP / 16;  // steps of 16 dims
+  constexpr int CH = DP / 32;  // chunks that a lane copies of a block's keys
+  constexpr int OWN = DP / 4;  // output dims of a lane
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ long long scan_ws[kAttWarps];
+  __shared__ int scan_ws[kAttWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
-  unsigned char* ring = smem + static_cast<size_t>(warp) * a.stages * (2 * BLOCK_BYTES + sizeof(SlotHead));
-  SlotHead* heads_at = reinterpret_cast<SlotHead*>(ring + static_cast<size_t>(a.stages) * 2 * BLOCK_BYTES);
-  long long* first =
-      reinterpret_cast<long long*>(smem + static_cast<size_t>(kAttWarps) * a.stages * (2 * BLOCK_BYTES + sizeof(SlotHead)));
+  unsigned char* ring = smem + warp * S::kWarp;
+  BlockHead* known = reinterpret_cast<BlockHead*>(ring + S::kRing);
+  int* first = reinterpret_cast<int*>(smem + kAttWarps * S::kWarp);
   if (a.dim < DP)  // the filled-up dims stay zero
-    for (int i = lane; i < a.stages * 2 * BLOCK_BYTES / 16; i += 32)
-      reinterpret_cast<uint4*>(ring)[i] = make_uint4(0, 0, 0, 0);
+    for (int i = lane; i < S::kRing / 16; i += 32) reinterpret_cast<uint4*>(ring)[i] = make_uint4(0, 0, 0, 0);
   grid_wait();
   grid_release();
   scan_rows(a, first, scan_ws);
   if (blockIdx.x == 0)
     for (int r = tid; r <= a.rows; r += kAttThreads) a.first[r] = first[r];
 
-  const long long all = first[a.rows] * a.heads;
+  const long long all = static_cast<long long>(first[a.rows]) * a.heads;
   const long long each = blocks_each(a, all);
   const int id = warp * gridDim.x + blockIdx.x;  // few blocks go to as many SMs as there are
   const int team = id / a.tiles, tile = id - team * a.tiles;
@@ -190,8 +251,23 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 ? 2 : 1) cache_attend_ke
       const int line = tok >> 1, place = ((tok & 1) << 2) | col;
       to_v[i] = line * 128 + ((place ^ ((line & 3) << 1)) << 4);
     }
+    to_v[i] += S::kBlock;
   }
-  const uint32_t ring_at = smem_u32(ring), heads_smem = smem_u32(heads_at);
+  const uint32_t ring_at = smem_u32(ring);
+  const long long block_bytes = 16ll * a.dim;
+  // and where it reads fragments: keys of token g (and g + 8), values of tokens 2 t, 2 t + 1 (and + 8)
+  uint32_t at_k0, at_k1, at_v0, at_v1;
+  if (DP == 128) {
+    const int flip = (g & 1) << 2;
+    at_k0 = g * 128 + ((t ^ flip) << 4);
+    at_k1 = g * 128 + (((t + 4) ^ flip) << 4);
+    at_v0 = S::kBlock + 2 * t * 128 + ((g ^ (t << 1)) << 4);
+    at_v1 = at_v0 + 128;
+  } else {
+    at_k0 = at_k1 = g * 64 + (t << 4);
+    at_v0 = S::kBlock + t * 128 + (((g >> 1) ^ (t << 1)) << 4) + (g & 1) * 8;
+    at_v1 = S::kBlock + t * 128 + (((4 | (g >> 1)) ^ (t << 1)) << 4) + (g & 1) * 8;
+  }
 
   int row;
   {
@@ -208,71 +284,86 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 ? 2 : 1) cache_attend_ke
   }
   int part = 0;  // parts that this warp has written
   while (i0 < i1) {
-    while (first[row + 1] * a.heads <= i0) ++row;
-    const int nb = static_cast<int>(first[row + 1] - first[row]);
-    const long long in_row = i0 - first[row] * a.heads;
+    while (static_cast<long long>(first[row + 1]) * a.heads <= i0) ++row;
+    const int nb = first[row + 1] - first[row];
+    const long long in_row = i0 - static_cast<long long>(first[row]) * a.heads;
     const int head = static_cast<int>(in_row / nb);
     const int b0 = static_cast<int>(in_row - static_cast<long long>(head) * nb);
     const int n = static_cast<int>(min(static_cast<long long>(nb - b0), i1 - i0));
     const int len = max(0, min(a.lens[row], a.width * a.page));
     const int* pages = a.table + static_cast<long long>(row) * a.width;
+    const int steps = (n + 1) / 2;
 
-    // ---- copies, `stages` blocks ahead
-    int page_ids = -1;  // of 32 blocks, one per lane
+    // ---- copies, kAttStages - 1 steps ahead
+    int slot_in = 0;
     auto fetch = [&](int j) {
-      if (j < n) {
-        if ((j & 31) == 0) {
-          const int b = b0 + j + lane;
-          page_ids = b < nb ? pages[(b * kCacheBlock) / a.page] : -1;
-        }
-        int pid = __shfl_sync(0xffffffffu, page_ids, j & 31);
-        const int b = b0 + j;
-        int valid = min(kCacheBlock, len - b * kCacheBlock);
-        if (pid < 0 || pid >= a.pages) {
-          pid = 0;
-          valid = 0;
-        }
-        const int inside = (b * kCacheBlock) % a.page;
-        const long long at = static_cast<long long>(pid) * a.heads + head;
-        const long long from = (at * a.page + inside) * a.dim + lane * 16;
-        const int slot = j % a.stages;
-        const uint32_t to = ring_at + slot * 2 * BLOCK_BYTES;
-#pragma unroll
-        for (int i = 0; i < CH; ++i)
-          if (token_of[i] < 16) {
-            const bool take = token_of[i] < valid;
-            cp_async16_if(to + to_k[i], a.k + from + i * 512, take);
-            cp_async16_if(to + BLOCK_BYTES + to_v[i], a.v + from + i * 512, take);
+      if (j < steps) {
+        if ((j & 15) == 0) {  // the next 32 blocks: one per lane
+          const int i = 2 * j + lane, b = b0 + i;
+          BlockHead h{0.0f, 0.0f, 0, -1};
+          if (i < n) {
+            const int at = b * kCacheBlock;
+            const int pid = pages[at / a.page];
+            if (pid >= 0 && pid < a.pages) {
+              h.block = (pid * a.heads + head) * (a.page / kCacheBlock) + (at % a.page) / kCacheBlock;
+              h.ks = a.k_scale[h.block];
+              h.vs = a.v_scale[h.block];
+              h.valid = min(kCacheBlock, len - at);
+            }
           }
-        const long long sc = at * (a.page / kCacheBlock) + inside / kCacheBlock;
-        if (lane == 0) {
-          cp_async4(heads_smem + slot * sizeof(SlotHead), a.k_scale + sc);
-          cp_async4(heads_smem + slot * sizeof(SlotHead) + 4, a.v_scale + sc);
-          heads_at[slot].valid = valid;
+          __syncwarp();
+          known[i & (kAttHeads - 1)] = h;
+          __syncwarp();
+        }
+        const uint32_t to = ring_at + slot_in * S::kStep;
+#pragma unroll
+        for (int u = 0; u < kAttPair; ++u) {
+          const int2 h = *reinterpret_cast<const int2*>(&known[(2 * j + u) & (kAttHeads - 1)].valid);
+          const long long from = max(h.y, 0) * block_bytes + lane * 16;
+          const unsigned char* fk = a.k + from;
+          const unsigned char* fv = a.v + from;
+#pragma unroll
+          for (int i = 0; i < CH; ++i)
+            if (token_of[i] < 16) {
+              const bool take = token_of[i] < h.x;
+              cp_async16_if(to + u * 2 * S::kBlock + to_k[i], fk + i * 512, take);
+              cp_async16_if(to + u * 2 * S::kBlock + to_v[i], fv + i * 512, take);
+            }
         }
       }
+      slot_in = slot_in == kAttStages - 1 ? 0 : slot_in + 1;
       cp_async_commit();
     };
-    for (int j = 0; j < a.stages - 1; ++j) fetch(j);
+#pragma unroll
+    for (int j = 0; j < kAttStages - 1; ++j) fetch(j);
 
     // ---- the queries of this lane's row: row g of the tile, its own dims
     const int r = tile * kAttRows + g;  // step r / group, head r % group
     const bool live = r < a.steps * a.group;
     const int step = live ? r / a.group : 0;
-    const long long q_at = (static_cast<long long>(row) * a.steps + step) * a.ld_q +
-                           static_cast<long long>(head * a.group + (live ? r - step * a.group : 0)) * a.hd_q;
+    const int q_head = head * a.group + (live ? r - step * a.group : 0);
+    const long long q_token = static_cast<long long>(row) * a.steps + step;
     uint32_t qa[KS][4];
-    float row_scale;
+    float c_hi, c_lo;  // the row's factors
     {
       float x[OWN];
-#pragma unroll
-      for (int i = 0; i < OWN; ++i) {
-        const int d = (i / 16) * 64 + t * 16 + (i % 16);
-        x[i] = live && d < a.dim ? load_any(a.q, q_at + d, a.q_type) : 0.0f;
-      }
       float most = 0.0f;
 #pragma unroll
-      for (int i = 0; i < OWN; ++i) most = fmaxf(most, fabsf(x[i]));
+      for (int i = 0; i < OWN / 16; ++i) {
+        const int d = i * 64 + t * 16;
+        float y[16];
+        if (live && d < a.dim) {
+          load16(a.q, q_token * a.ld_q + q_head * a.hd_q + d, a.q_type, a.wide_q, y);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 16; ++k) y[k] = 0.0f;
+        }
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          x[16 * i + k] = y[k];
+          most = fmaxf(most, fabsf(y[k]));
+        }
+      }
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
       // the row times 2^e has its largest element in [2^14, 2^15)
@@ -280,7 +371,9 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 ? 2 : 1) cache_attend_ke
       if (e < -113) e = 0;  // inf or NaN
       e = min(e, 126);
       const float up = __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
-      row_scale = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+      const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+      c_hi = a.c_hi * down;
+      c_lo = a.c_lo * down;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         const float* y = x + 4 * s;
@@ -291,6 +384,7 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 ? 2 : 1) cache_attend_ke
       }
     }
     const int end = len - (a.steps - 1 - step);  // places that the row sees
+    const int all_see = len - (a.steps - 1);     // places that every row sees
 
     float acc[NJ][4], sum[NJ][2];
 #pragma unroll
@@ -298,8 +392,7 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 ? 2 : 1) cache_attend_ke
       acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
       sum[j][0] = sum[j][1] = 0.0f;
     }
-    float m = kNegInf, l = 0.0f, vref = 0.0f;
-    int since = 0;
+    float m = kNegInf, l = 0.0f, vref = 0.0f, vinv = 0.0f;
     auto flush = [&]() {
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
@@ -307,64 +400,69 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 ? 2 : 1) cache_attend_ke
         sum[j][1] += acc[j][1] + acc[j][3];
         acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
       }
-      since = 0;
     };
 
-    for (int j = 0; j < n; ++j) {
-      fetch(j + a.stages - 1);
-      // all but the newest stages - 1 groups are here
-      if (a.stages == 6)
-        asm volatile("cp.async.wait_group 5;" ::: "memory");
-      else if (a.stages == 5)
-        asm volatile("cp.async.wait_group 4;" ::: "memory");
-      else
-        asm volatile("cp.async.wait_group 3;" ::: "memory");
+    int slot = 0;
+    for (int j = 0; j < steps; ++j) {
+      fetch(j + kAttStages - 1);
+      asm volatile("cp.async.wait_group %0;" ::"n"(kAttStages - 1) : "memory");
       __syncwarp();
-      const int slot = j % a.stages;
-      const unsigned char* kt = ring + slot * 2 * BLOCK_BYTES;
-      const unsigned char* vt = kt + BLOCK_BYTES;
-      const SlotHead sh = heads_at[slot];
+      const unsigned char* at = ring + slot * S::kStep;
+      slot = slot == kAttStages - 1 ? 0 : slot + 1;
+      BlockHead h[kAttPair];
+#pragma unroll
+      for (int u = 0; u < kAttPair; ++u) h[u] = known[(2 * j + u) & (kAttHeads - 1)];
 
-      // scores: tokens 8 h + g are the columns, this lane has columns 2 t and 2 t + 1
-      float sc[2][4];
+      // scores: tokens 8 i + g are the columns, this lane has columns 2 t and 2 t + 1
+      float sc[2 * kAttPair][4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        sc[h][0] = sc[h][1] = sc[h][2] = sc[h][3] = 0.0f;
-        const int tok = 8 * h + g;
+      for (int i = 0; i < 2 * kAttPair; ++i) {
+        sc[i][0] = sc[i][1] = sc[i][2] = sc[i][3] = 0.0f;
+        const unsigned char* kt = at + (i >> 1) * 2 * S::kBlock + (i & 1) * 8 * DP;
+        uint32_t w[KS];
+        const uint4 x = *reinterpret_cast<const uint4*>(kt + at_k0);
+        w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
         if (DP == 128) {
-          const int flip = (tok & 1) << 2;
-          const uint4 x = *reinterpret_cast<const uint4*>(kt + tok * 128 + ((t ^ flip) << 4));
-          const uint4 y = *reinterpret_cast<const uint4*>(kt + tok * 128 + (((t + 4) ^ flip) << 4));
-          const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+          const uint4 y = *reinterpret_cast<const uint4*>(kt + at_k1);
+          w[KS - 4] = y.x, w[KS - 3] = y.y, w[KS - 2] = y.z, w[KS - 1] = y.w;
+        }
 #pragma unroll
-          for (int s = 0; s < KS; ++s) mma16816(sc[h], qa[s], codes_lo(w[s]), codes_hi(w[s]));
-        } else {
-          const uint4 x = *reinterpret_cast<const uint4*>(kt + tok * 64 + (t << 4));
-          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        for (int s = 0; s < KS; ++s) mma16816(sc[i], qa[s], codes_lo(w[s]), codes_hi(w[s]));
+      }
+      float p[2 * kAttPair][2];
 #pragma unroll
-          for (int s = 0; s < KS; ++s) mma16816(sc[h], qa[s], codes_lo(w[s]), codes_hi(w[s]));
+      for (int u = 0; u < kAttPair; ++u) {
+        const float f_hi = c_hi * h[u].ks, f_lo = c_lo * h[u].ks;
+#pragma unroll
+        for (int i = 2 * u; i < 2 * u + 2; ++i)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float x = sc[i][k] + sc[i][k + 2];
+            p[i][k] = fmaf(x, f_hi, x * f_lo);
+          }
+      }
+      const int place = (b0 + 2 * j) * kCacheBlock;
+      if (h[0].valid + h[1].valid < 2 * kCacheBlock || place + 2 * kCacheBlock > all_see) {
+#pragma unroll
+        for (int u = 0; u < kAttPair; ++u) {
+          const int lim = min(h[u].valid, end - place - u * kCacheBlock);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              if (8 * i + 2 * t + k >= lim) p[2 * u + i][k] = kNegInf;
         }
       }
-      const int lim = min(sh.valid, end - (b0 + j) * kCacheBlock);
-      const float f = row_scale * sh.ks;
-      float p[2][2];
       float mx = kNegInf;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float x = (sc[h][i] + sc[h][i + 2]) * f;
-          const float y = fmaf(x, a.c_hi, x * a.c_lo);
-          p[h][i] = 8 * h + 2 * t + i < lim ? y : kNegInf;
-          mx = fmaxf(mx, p[h][i]);
-        }
+      for (int i = 0; i < 2 * kAttPair; ++i) mx = fmaxf(mx, fmaxf(p[i][0], p[i][1]));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float vnew = sh.valid > 0 ? fmaxf(vref, fabsf(sh.vs)) : vref;
-      if (__any_sync(0xffffffffu, mx > m || vnew != vref)) {
-        const float mn = fmaxf(m, mx);
+      const float vmax = fmaxf(fabsf(h[0].vs), fabsf(h[1].vs));  // 0 where there is no page
+      if (__any_sync(0xffffffffu, mx > m || vmax > vref)) {
+        const float mn = fmaxf(m, mx), vn = fmaxf(vref, vmax);
         const float alpha = m > kNegInf ? ex2(m - mn) : 0.0f;
-        const float both = vnew != vref ? (vref > 0.0f ? alpha * __fdiv_rn(vref, vnew) : 0.0f) : alpha;
+        const float both = vn > vref ? alpha * __fdiv_rn(vref, vn) : alpha;
 #pragma unroll
         for (int i = 0; i < NJ; ++i) {
           acc[i][0] *= both, acc[i][1] *= both, acc[i][2] *= both, acc[i][3] *= both;
@@ -372,49 +470,51 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 ? 2 : 1) cache_attend_ke
         }
         l *= alpha;
         m = mn;
-        vref = vnew;
+        if (vn > vref) vinv = __fdiv_rn(1.0f, vn);
+        vref = vn;
       }
       const float base = m > kNegInf ? m - kUp : 0.0f;
-      const float ratio = vref > 0.0f && sh.valid > 0 ? __fdiv_rn(sh.vs, vref) : 0.0f;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int i = 0; i < 2 * kAttPair; ++i)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) p[i][k] = ex2(p[i][k] - base);
+      l += ((p[0][0] + p[0][1]) + (p[1][0] + p[1][1])) + ((p[2][0] + p[2][1]) + (p[3][0] + p[3][1]));
+
+#pragma unroll
+      for (int u = 0; u < kAttPair; ++u) {
+        const float ratio = h[u].vs * vinv;
+        uint32_t pa[4];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          p[h][i] = ex2(p[h][i] - base);
-          l += p[h][i];
-          p[h][i] *= ratio;
+          const float x = p[2 * u + i][0] * ratio, y = p[2 * u + i][1] * ratio;
+          pa[2 * i] = two_halves(x, y);
+          pa[2 * i + 1] = two_rests(x, y, pa[2 * i]);
         }
-      uint32_t pa[4];
-      pa[0] = two_halves(p[0][0], p[0][1]);
-      pa[1] = two_rests(p[0][0], p[0][1], pa[0]);
-      pa[2] = two_halves(p[1][0], p[1][1]);
-      pa[3] = two_rests(p[1][0], p[1][1], pa[2]);
-
-      // values: this lane has tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9 at the dims g DP / 8 ...
-      constexpr int W = DP / 32;  // words of a token
-      uint32_t v[4][W];
+        // values: this lane has tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9 at the dims g DP / 8 ...
+        constexpr int W = DP / 32;  // words of a token
+        uint32_t v[4][W];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int tok = 2 * t + (i & 1) + 8 * (i >> 1);
-        if (DP == 128) {
-          const uint4 x = *reinterpret_cast<const uint4*>(vt + tok * 128 + ((g ^ (((tok >> 1) & 3) << 1)) << 4));
-          v[i][0] = x.x, v[i][1] = x.y, v[i][W - 2] = x.z, v[i][W - 1] = x.w;
-        } else {
-          const int line = tok >> 1, place = ((tok & 1) << 2) | (g >> 1);
-          const uint2 x = *reinterpret_cast<const uint2*>(vt + line * 128 + ((place ^ ((line & 3) << 1)) << 4) + (g & 1) * 8);
-          v[i][0] = x.x, v[i][1] = x.y;
+        for (int i = 0; i < 4; ++i) {
+          const unsigned char* vt = at + u * 2 * S::kBlock + (i >> 1) * 8 * DP + (i & 1 ? at_v1 : at_v0);
+          if (DP == 128) {
+            const uint4 x = *reinterpret_cast<const uint4*>(vt);
+            v[i][0] = x.x, v[i][1] = x.y, v[i][W - 2] = x.z, v[i][W - 1] = x.w;
+          } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(vt);
+            v[i][0] = x.x, v[i][1] = x.y;
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          const uint32_t a0 = __byte_perm(v[0][w], v[1][w], 0x5140), a1 = __byte_perm(v[0][w], v[1][w], 0x7362);
+          const uint32_t c0 = __byte_perm(v[2][w], v[3][w], 0x5140), c1 = __byte_perm(v[2][w], v[3][w], 0x7362);
+          mma16816(acc[4 * w], pa, codes_lo(a0), codes_lo(c0));
+          mma16816(acc[4 * w + 1], pa, codes_hi(a0), codes_hi(c0));
+          mma16816(acc[4 * w + 2], pa, codes_lo(a1), codes_lo(c1));
+          mma16816(acc[4 * w + 3], pa, codes_hi(a1), codes_hi(c1));
         }
       }
-#pragma unroll
-      for (int w = 0; w < W; ++w) {
-        const uint32_t a0 = __byte_perm(v[0][w], v[1][w], 0x5140), a1 = __byte_perm(v[0][w], v[1][w], 0x7362);
-        const uint32_t c0 = __byte_perm(v[2][w], v[3][w], 0x5140), c1 = __byte_perm(v[2][w], v[3][w], 0x7362);
-        mma16816(acc[4 * w], pa, codes_lo(a0), codes_lo(c0));
-        mma16816(acc[4 * w + 1], pa, codes_hi(a0), codes_hi(c0));
-        mma16816(acc[4 * w + 2], pa, codes_lo(a1), codes_lo(c1));
-        mma16816(acc[4 * w + 3], pa, codes_hi(a1), codes_hi(c1));
-      }
-      if (++since == kAttFlush) flush();
+      if ((j & (kAttFlush - 1)) == kAttFlush - 1) flush();
       __syncwarp();  // the slot may be filled again
     }
     cp_async_wait_all();
@@ -424,37 +524,34 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 ? 2 : 1) cache_attend_ke
 
     // this lane's dims: OWN t + i, from the tiles i % NJ and the columns 2 t, 2 t + 1
     const bool whole = n == nb;
-    if (whole) {
-      if (live) {
-        const float inv = l > 0.0f || l != l ? __fdiv_rn(vref, l) : 0.0f;
-        const long long o = (static_cast<long long>(row) * a.steps + step) * a.ld_out +
-                            static_cast<long long>(head * a.group + r - step * a.group) * a.hd_out;
+    const float by = whole ? (l > 0.0f || l != l ? __fdiv_rn(vref, l) : 0.0f) : vref;
+    float* to = whole ? nullptr
+                      : a.parts + ((static_cast<long long>(team) * a.tiles + tile) * 2 + part) * part_floats(a.dim);
 #pragma unroll
-        for (int i = 0; i < OWN; ++i) {
-          const int d = OWN * t + i;
-          if (d < a.dim) store_any(a.out, o + d, a.out_type, sum[i % NJ][i / NJ] * inv);
-        }
-      }
-    } else {
-      float* to = a.parts + ((static_cast<long long>(team) * a.tiles + tile) * 2 + part) * part_floats(a.dim);
+    for (int i = 0; i < OWN / 16; ++i) {
+      const int d = OWN * t + 16 * i;
+      float y[16];
 #pragma unroll
-      for (int i = 0; i < OWN; ++i) {
-        const int d = OWN * t + i;
-        if (d < a.dim) to[g * a.dim + d] = sum[i % NJ][i / NJ] * vref;
-      }
-      if (t == 0) {
-        to[kAttRows * a.dim + g] = m;
-        to[kAttRows * a.dim + kAttRows + g] = l;
-      }
+      for (int k = 0; k < 16; ++k) y[k] = sum[(16 * i + k) % NJ][(16 * i + k) / NJ] * by;
+      if (d >= a.dim) continue;
+      if (!whole)
+        store16(to, g * a.dim + d, kOpsF32, true, y);
+      else if (live)
+        store16(a.out, q_token * a.ld_out + q_head * a.hd_out + d, a.out_type, a.wide_out, y);
+    }
+    if (!whole && t == 0) {
+      to[kAttRows * a.dim + g] = m;
+      to[kAttRows * a.dim + kAttRows + g] = l;
     }
     part = 1;
     i0 += n;
   }
 }
 
-constexpr int kJoinThreads = 128;
+constexpr int kJoinThreads = 256;
+constexpr int kJoinAhead = 4;  // parts of a warp that are loaded at once
 
-// One CTA per (row, head, tile, query row): the parts of its blocks joined, in their
+// One CTA per (row, head, query row): the parts of its blocks joined, in their
 // order; nothing to do where one warp had them all.
 __global__ void __launch_bounds__(kJoinThreads) cache_attend_join_kernel(const AttendArgs a) {
   constexpr int W = kJoinThreads / 32, PER = VERBO_CACHE_MAX_DIM / 32;
@@ -470,32 +567,51 @@ __global__ void __launch_bounds__(kJoinThreads) cache_attend_join_kernel(const A
   const int step = qr / a.group;
   const long long o = (static_cast<long long>(row) * a.steps + step) * a.ld_out +
                       static_cast<long long>(head * a.group + qr - step * a.group) * a.hd_out;
-  const long long nb = a.first[row + 1] - a.first[row];
+  const int f0 = a.first[row], nb = a.first[row + 1] - f0, all = a.first[a.rows];
   if (nb == 0) {  // an empty row
     for (int d = threadIdx.x; d < a.dim; d += kJoinThreads) store_any(a.out, o + d, a.out_type, 0.0f);
     return;
   }
-  const long long each = blocks_each(a, a.first[a.rows] * a.heads);
-  const long long f = a.first[row] * a.heads + head * nb, e = f + nb - 1;
+  const long long each = blocks_each(a, static_cast<long long>(all) * a.heads);
+  const long long f = static_cast<long long>(f0) * a.heads + static_cast<long long>(head) * nb, e = f + nb - 1;
   const int w0 = static_cast<int>(f / each), w1 = static_cast<int>(e / each);
   if (w0 == w1) return;
   float m = kNegInf, l = 0.0f, x[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) x[i] = 0.0f;
-  for (int w = w0 + warp; w <= w1; w += W) {
-    const int which = w * each < f;  // its second part, after the end of another
-    const float* from = a.parts + ((static_cast<long long>(w) * a.tiles + tile) * 2 + which) * part_floats(a.dim);
-    const float pm = from[kAttRows * a.dim + g], pl = from[kAttRows * a.dim + kAttRows + g];
-    float y[PER];
+  for (int w = w0 + warp; w <= w1; w += W * kJoinAhead) {
+    float pm[kJoinAhead], pl[kJoinAhead], y[kJoinAhead][PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) y[i] = lane + 32 * i < a.dim ? from[g * a.dim + lane + 32 * i] : 0.0f;
-    if (pm == kNegInf && pl == 0.0f) continue;
-    const float mn = fmaxf(m, pm);
-    const float u = m > kNegInf ? ex2(m - mn) : 0.0f, t = pm > kNegInf ? ex2(pm - mn) : 1.0f;
+    for (int u = 0; u < kJoinAhead; ++u) {
+      const int v = w + u * W;
+      pm[u] = kNegInf;
+      pl[u] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) y[u][i] = 0.0f;
+      if (v > w1) continue;
+      const int which = v * each < f;  // its second part, after the end of another
+      const float* from = a.parts + ((static_cast<long long>(v) * a.tiles + tile) * 2 + which) * part_floats(a.dim);
+      pm[u] = from[kAttRows * a.dim + g];
+      pl[u] = from[kAttRows * a.dim + kAttRows + g];
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (lane + 32 * i < a.dim) y[u][i] = from[g * a.dim + lane + 32 * i];
+    }
+    float mn = m;
+#pragma unroll
+    for (int u = 0; u < kJoinAhead; ++u) mn = fmaxf(mn, pm[u]);
+    const float s = m > kNegInf ? ex2(m - mn) : 1.0f;
     m = mn;
-    l = l * u + pl * t;
+    l *= s;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) x[i] = x[i] * u + y[i] * t;
+    for (int i = 0; i < PER; ++i) x[i] *= s;
+#pragma unroll
+    for (int u = 0; u < kJoinAhead; ++u) {
+      const float t = pm[u] > kNegInf ? ex2(pm[u] - mn) : 1.0f;  // a part that sees nothing is zeros, or NaNs
+      l += pl[u] * t;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) x[i] += y[u][i] * t;
+    }
   }
   if (lane == 0) {
     ms[warp] = m;
@@ -505,11 +621,12 @@ __global__ void __launch_bounds__(kJoinThreads) cache_attend_join_kernel(const A
   for (int i = 0; i < PER; ++i) os[warp][lane + 32 * i] = x[i];
   __syncthreads();
   float mn = kNegInf;
+#pragma unroll
   for (int w = 0; w < W; ++w) mn = fmaxf(mn, ms[w]);
   float total = 0.0f, u[W];
 #pragma unroll
   for (int w = 0; w < W; ++w) {
-    u[w] = ms[w] > kNegInf ? ex2(ms[w] - mn) : (ls[w] != ls[w] ? 1.0f : 0.0f);
+    u[w] = ms[w] > kNegInf ? ex2(ms[w] - mn) : 1.0f;
     total += ls[w] * u[w];
   }
   const float inv = total > 0.0f || total != total ? __fdiv_rn(1.0f, total) : 0.0f;
@@ -524,31 +641,31 @@ __global__ void __launch_bounds__(kJoinThreads) cache_attend_join_kernel(const A
 constexpr int kAttMaxSmem = 227 * 1024;
 
 struct Plan {
-  int dp, grid, stages, tiles, teams, least;
+  int dp, grid, tiles, teams, least;
   size_t smem, parts_bytes;
 };
 Plan plan(const verbo_cache& c, int heads, int steps) {
   Plan p{};
   p.dp = c.dim <= 64 ? 64 : 128;
-  const int per_sm = p.dp == 64 ? 2 : 1;
+  p.smem = static_cast<size_t>(kAttWarps) * (p.dp == 64 ? AttShape<64>::kWarp : AttShape<128>::kWarp) +
+           (static_cast<size_t>(c.rows) + 1) * 4;
+  // small heads leave room for two CTAs an SM, unless there are very many rows
+  const int per_sm = p.dp == 64 && 2 * (p.smem + 1024) <= kAttMaxSmem + 1024 ? 2 : 1;
   p.grid = sm_count() * per_sm;
   p.tiles = (steps * (heads / c.heads) + kAttRows - 1) / kAttRows;
   p.teams = std::max(1, p.grid * kAttWarps / p.tiles);
   p.least = 2;
-  const size_t rows = (static_cast<size_t>(c.rows) + 1) * 8;
-  const size_t slot = static_cast<size_t>(kAttWarps) * (32 * p.dp + sizeof(SlotHead));
-  const size_t room = (kAttMaxSmem - 1024 * (per_sm - 1)) / per_sm - 512;
-  p.stages = std::min<int>(kAttStages, static_cast<int>((room - rows) / slot));
-  p.smem = p.stages * slot + rows;
   p.parts_bytes = static_cast<size_t>(p.teams) * p.tiles * 2 * part_floats(c.dim) * 4;
   return p;
 }
 
 template <int DP>
 cudaError_t run_attend(const AttendArgs& a, const Plan& p, cudaStream_t s) {
+  static_assert(kAttWarps * AttShape<128>::kWarp + (VERBO_CACHE_MAX_ROWS + 1) * 4 + 64 <= kAttMaxSmem, "shared memory");
   const auto kernel = cache_attend_kernel<DP>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             DP == 64 ? kAttMaxSmem / 2 : kAttMaxSmem - 1024);
+  const cudaError_t e =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           kAttWarps * AttShape<DP>::kWarp + (VERBO_CACHE_MAX_ROWS + 1) * 4);
   if (e != cudaSuccess) return e;
   return launch_chained(kernel, static_cast<unsigned>(p.grid), kAttThreads, p.smem, 1, s, a);
 }
@@ -556,7 +673,7 @@ cudaError_t run_attend(const AttendArgs& a, const Plan& p, cudaStream_t s) {
 }  // namespace
 
 size_t cache_attend_bytes(const verbo_cache& c, int heads, int steps) {
-  return (plan(c, heads, steps).parts_bytes + (static_cast<size_t>(c.rows) + 1) * 8 + 15) / 16 * 16;
+  return (plan(c, heads, steps).parts_bytes + (static_cast<size_t>(c.rows) + 1) * 4 + 15) / 16 * 16;
 }
 
 cudaError_t launch_cache_attend(const verbo_cache& c, int layer, const CacheQuery& x, int q_type, int out_type,
@@ -587,14 +704,19 @@ cudaError_t launch_cache_attend(const verbo_cache& c, int layer, const CacheQuer
   a.tiles = p.tiles;
   a.teams = p.teams;
   a.least = p.least;
-  a.stages = p.stages;
   a.q_type = q_type;
   a.out_type = out_type;
   const double f = static_cast<double>(x.scale) * kLog2e;
   a.c_hi = static_cast<float>(f);
   a.c_lo = static_cast<float>(f - static_cast<double>(a.c_hi));
   a.parts = static_cast<float*>(x.workspace);
-  a.first = reinterpret_cast<long long*>(static_cast<char*>(x.workspace) + p.parts_bytes);
+  a.first = reinterpret_cast<int*>(static_cast<char*>(x.workspace) + p.parts_bytes);
+  const auto wide = [](const void* p, long long ld, long long hd, int type) {
+    const int n = type == kOpsF32 ? 4 : 8;  // elements of 16 bytes
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % n == 0 && hd % n == 0;
+  };
+  a.wide_q = wide(x.q, x.ld_q, x.hd_q, q_type);
+  a.wide_out = wide(x.out, x.ld_out, x.hd_out, out_type);
   const long long joins = static_cast<long long>(c.rows) * c.heads * x.steps * a.group;
   if (joins > INT_MAX) return cudaErrorInvalidConfiguration;
   const cudaError_t e = p.dp == 64 ? run_attend<64>(a, p, s) : run_attend<128>(a, p, s);

@@ -48,6 +48,11 @@ void check_sizes(const verbo_cache* c) {
   if (c->page % VERBO_CACHE_BLOCK) fail("page must be a multiple of 16");
   check_number(c->rows, 0, VERBO_CACHE_MAX_ROWS, "rows");
   check_number(c->width, 1, INT_MAX / c->page, "width");
+  // blocks are counted in 32 bits: those of a layer, and those of all tables
+  const long long per = c->page / VERBO_CACHE_BLOCK;
+  if (static_cast<long long>(c->pages) * c->heads * per > INT_MAX)
+    fail("pages * heads * page / 16 must be below 2^31");
+  if (static_cast<long long>(c->rows) * c->width * per > INT_MAX) fail("rows * width * page / 16 must be below 2^31");
 }
 
 struct CacheRanges {
