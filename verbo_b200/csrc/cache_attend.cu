@@ -35,6 +35,9 @@ constexpr int kAttPair = 2;    // blocks of a step
 constexpr int kAttFlush = 4;   // steps between two transfers of the sums
 constexpr int kAttStages = 3;  // steps whose copies are in flight
 constexpr int kAttHeads = 64;  // blocks that are known ahead, per warp
+// What the beginning and the end of a (row, head) cost a warp, in blocks: parts are
+// equal with it counted.  64 rows of up to 8192 tokens without it: KAPPA us.
+constexpr int kAttStart = 4;
 constexpr float kUp = 14.0f;   // weights are held times 2^14: fp16's subnormals begin at 2^-28 of the largest
 constexpr double kLog2e = 1.4426950408889634;
 
@@ -165,7 +168,8 @@ __device__ __forceinline__ void store16(void* p, long long i, int type, bool wid
   }
 }
 
-// Blocks of 16 tokens before each row, in shared memory (rows + 1), by the CTA.
+// Blocks of 16 tokens before each row, kAttStart more for each row that has any, in
+// shared memory (rows + 1), by the CTA.
 __device__ __forceinline__ void scan_rows(const AttendArgs& a, int* first, int* ws) {
   int base = 0;
   for (int r0 = 0; r0 < a.rows; r0 += kAttThreads) {
@@ -173,7 +177,7 @@ __device__ __forceinline__ void scan_rows(const AttendArgs& a, int* first, int* 
     int n = 0;
     if (r < a.rows) {
       const int len = max(0, min(a.lens[r], a.width * a.page));
-      n = len / kCacheBlock + (len % kCacheBlock > 0);
+      n = len > 0 ? (len - 1) / kCacheBlock + 1 + kAttStart : 0;
     }
     int total;
     const int at = block_excl_scan<int, kAttThreads>(n, ws, &total);
@@ -285,11 +289,17 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 ? 2 : 1) cache_attend_ke
   int part = 0;  // parts that this warp has written
   while (i0 < i1) {
     while (static_cast<long long>(first[row + 1]) * a.heads <= i0) ++row;
-    const int nb = first[row + 1] - first[row];
+    const int counted = first[row + 1] - first[row], nb = counted - kAttStart;
     const long long in_row = i0 - static_cast<long long>(first[row]) * a.heads;
-    const int head = static_cast<int>(in_row / nb);
-    const int b0 = static_cast<int>(in_row - static_cast<long long>(head) * nb);
-    const int n = static_cast<int>(min(static_cast<long long>(nb - b0), i1 - i0));
+    const int head = static_cast<int>(in_row / counted);
+    const int c0 = static_cast<int>(in_row - static_cast<long long>(head) * counted);
+    const int c1 = static_cast<int>(min(static_cast<long long>(counted), c0 + (i1 - i0)));
+    i0 += c1 - c0;
+    const int b0 = max(0, c0 - kAttStart), n = max(0, c1 - kAttStart) - b0;
+    if (n == 0) {  // its start alone
+      part = 1;
+      continue;
+    }
     const int len = max(0, min(a.lens[row], a.width * a.page));
     const int* pages = a.table + static_cast<long long>(row) * a.width;
     const int steps = (n + 1) / 2;
@@ -544,97 +554,103 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 ? 2 : 1) cache_attend_ke
       to[kAttRows * a.dim + kAttRows + g] = l;
     }
     part = 1;
-    i0 += n;
   }
 }
 
 constexpr int kJoinThreads = 256;
-constexpr int kJoinAhead = 4;  // parts of a warp that are loaded at once
 
-// One CTA per (row, head, query row): the parts of its blocks joined, in their
-// order; nothing to do where one warp had them all.
+// One CTA per (row, head, tile): the parts of its blocks joined, in their order;
+// nothing to do where one warp had them all.  A warp takes every eighth part, all
+// query rows of it.
 __global__ void __launch_bounds__(kJoinThreads) cache_attend_join_kernel(const AttendArgs a) {
-  constexpr int W = kJoinThreads / 32, PER = VERBO_CACHE_MAX_DIM / 32;
-  __shared__ float ms[W], ls[W], os[W][VERBO_CACHE_MAX_DIM];
+  constexpr int W = kJoinThreads / 32, R = kAttRows;
+  extern __shared__ float4 os[];  // [W][R][dim / 4]
+  __shared__ float ms[W][R], ls[W][R];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int q_rows = a.steps * a.group;
-  const int qr = blockIdx.x % q_rows;
-  const int head = blockIdx.x / q_rows % a.heads;
-  const int row = blockIdx.x / q_rows / a.heads;
-  const int tile = qr / kAttRows, g = qr % kAttRows;
+  const int tile = blockIdx.x % a.tiles;
+  const int head = blockIdx.x / a.tiles % a.heads;
+  const int row = blockIdx.x / a.tiles / a.heads;
   grid_wait();
   grid_release();
-  const int step = qr / a.group;
+  const int f0 = a.first[row], counted = a.first[row + 1] - f0;
+  const int quads = a.dim / 4;
+  // this thread's part of the output: a query row, four dims
+  const int qr = tile * R + warp, step = qr / a.group;
+  const bool live = qr < a.steps * a.group && lane < quads;
   const long long o = (static_cast<long long>(row) * a.steps + step) * a.ld_out +
-                      static_cast<long long>(head * a.group + qr - step * a.group) * a.hd_out;
-  const int f0 = a.first[row], nb = a.first[row + 1] - f0, all = a.first[a.rows];
-  if (nb == 0) {  // an empty row
-    for (int d = threadIdx.x; d < a.dim; d += kJoinThreads) store_any(a.out, o + d, a.out_type, 0.0f);
-    return;
-  }
-  const long long each = blocks_each(a, static_cast<long long>(all) * a.heads);
-  const long long f = static_cast<long long>(f0) * a.heads + static_cast<long long>(head) * nb, e = f + nb - 1;
-  const int w0 = static_cast<int>(f / each), w1 = static_cast<int>(e / each);
-  if (w0 == w1) return;
-  float m = kNegInf, l = 0.0f, x[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) x[i] = 0.0f;
-  for (int w = w0 + warp; w <= w1; w += W * kJoinAhead) {
-    float pm[kJoinAhead], pl[kJoinAhead], y[kJoinAhead][PER];
-#pragma unroll
-    for (int u = 0; u < kJoinAhead; ++u) {
-      const int v = w + u * W;
-      pm[u] = kNegInf;
-      pl[u] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) y[u][i] = 0.0f;
-      if (v > w1) continue;
-      const int which = v * each < f;  // its second part, after the end of another
-      const float* from = a.parts + ((static_cast<long long>(v) * a.tiles + tile) * 2 + which) * part_floats(a.dim);
-      pm[u] = from[kAttRows * a.dim + g];
-      pl[u] = from[kAttRows * a.dim + kAttRows + g];
-#pragma unroll
-      for (int i = 0; i < PER; ++i)
-        if (lane + 32 * i < a.dim) y[u][i] = from[g * a.dim + lane + 32 * i];
+                      static_cast<long long>(head * a.group + qr - step * a.group) * a.hd_out + 4 * lane;
+  float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (counted > 0) {
+    const long long all = static_cast<long long>(a.first[a.rows]) * a.heads;
+    const long long each = blocks_each(a, all);
+    const long long f = static_cast<long long>(f0) * a.heads + static_cast<long long>(head) * counted;
+    int w0, w1;
+    if (all < INT_MAX) {
+      w0 = static_cast<int>(f + kAttStart) / static_cast<int>(each);
+      w1 = static_cast<int>(f + counted - 1) / static_cast<int>(each);
+    } else {
+      w0 = static_cast<int>((f + kAttStart) / each);
+      w1 = static_cast<int>((f + counted - 1) / each);
     }
-    float mn = m;
+    if (w0 == w1) return;  // teams w0 to w1 have blocks of it
+    float m[R], l[R];
+    float4 x[R];
 #pragma unroll
-    for (int u = 0; u < kJoinAhead; ++u) mn = fmaxf(mn, pm[u]);
-    const float s = m > kNegInf ? ex2(m - mn) : 1.0f;
-    m = mn;
-    l *= s;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) x[i] *= s;
-#pragma unroll
-    for (int u = 0; u < kJoinAhead; ++u) {
-      const float t = pm[u] > kNegInf ? ex2(pm[u] - mn) : 1.0f;  // a part that sees nothing is zeros, or NaNs
-      l += pl[u] * t;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) x[i] += y[u][i] * t;
+    for (int i = 0; i < R; ++i) {
+      m[i] = kNegInf;
+      l[i] = 0.0f;
+      x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
+    for (int w = w0 + warp; w <= w1; w += W) {
+      const int which = w * each < f;  // its second part, after the end of another
+      const float* from = a.parts + ((static_cast<long long>(w) * a.tiles + tile) * 2 + which) * part_floats(a.dim);
+      const float ml = lane < 2 * R ? from[R * a.dim + lane] : 0.0f;
+      float4 v[R];
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+        v[i] = lane < quads ? reinterpret_cast<const float4*>(from)[i * quads + lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        const float pm = __shfl_sync(0xffffffffu, ml, i), pl = __shfl_sync(0xffffffffu, ml, R + i);
+        const float mn = fmaxf(m[i], pm);
+        const float s = m[i] > kNegInf ? ex2(m[i] - mn) : 1.0f;
+        const float t = pm > kNegInf ? ex2(pm - mn) : 1.0f;  // a part that sees nothing is zeros, or NaNs
+        m[i] = mn;
+        l[i] = l[i] * s + pl * t;
+        x[i].x = x[i].x * s + v[i].x * t;
+        x[i].y = x[i].y * s + v[i].y * t;
+        x[i].z = x[i].z * s + v[i].z * t;
+        x[i].w = x[i].w * s + v[i].w * t;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      if (lane < quads) os[(warp * R + i) * quads + lane] = x[i];
+      if (lane == i) {
+        ms[warp][i] = m[i];
+        ls[warp][i] = l[i];
+      }
+    }
+    __syncthreads();
+    const int used = min(W, w1 - w0 + 1);
+    float mn = kNegInf, total = 0.0f;
+    for (int w = 0; w < used; ++w) mn = fmaxf(mn, ms[w][warp]);
+    for (int w = 0; w < used; ++w) {
+      const float t = ms[w][warp] > kNegInf ? ex2(ms[w][warp] - mn) : 1.0f;
+      total += ls[w][warp] * t;
+      if (lane < quads) {
+        const float4 v = os[(w * R + warp) * quads + lane];
+        y.x += v.x * t, y.y += v.y * t, y.z += v.z * t, y.w += v.w * t;
+      }
+    }
+    const float inv = total > 0.0f || total != total ? __fdiv_rn(1.0f, total) : 0.0f;
+    y.x *= inv, y.y *= inv, y.z *= inv, y.w *= inv;
   }
-  if (lane == 0) {
-    ms[warp] = m;
-    ls[warp] = l;
-  }
-#pragma unroll
-  for (int i = 0; i < PER; ++i) os[warp][lane + 32 * i] = x[i];
-  __syncthreads();
-  float mn = kNegInf;
-#pragma unroll
-  for (int w = 0; w < W; ++w) mn = fmaxf(mn, ms[w]);
-  float total = 0.0f, u[W];
-#pragma unroll
-  for (int w = 0; w < W; ++w) {
-    u[w] = ms[w] > kNegInf ? ex2(ms[w] - mn) : 1.0f;
-    total += ls[w] * u[w];
-  }
-  const float inv = total > 0.0f || total != total ? __fdiv_rn(1.0f, total) : 0.0f;
-  for (int d = threadIdx.x; d < a.dim; d += kJoinThreads) {
-    float y = 0.0f;
-#pragma unroll
-    for (int w = 0; w < W; ++w) y += os[w][d] * u[w];
-    store_any(a.out, o + d, a.out_type, y * inv);
+  if (live) {  // an empty row's are zeros
+    store_any(a.out, o, a.out_type, y.x);
+    store_any(a.out, o + 1, a.out_type, y.y);
+    store_any(a.out, o + 2, a.out_type, y.z);
+    store_any(a.out, o + 3, a.out_type, y.w);
   }
 }
 
@@ -717,11 +733,12 @@ cudaError_t launch_cache_attend(const verbo_cache& c, int layer, const CacheQuer
   };
   a.wide_q = wide(x.q, x.ld_q, x.hd_q, q_type);
   a.wide_out = wide(x.out, x.ld_out, x.hd_out, out_type);
-  const long long joins = static_cast<long long>(c.rows) * c.heads * x.steps * a.group;
+  const long long joins = static_cast<long long>(c.rows) * c.heads * p.tiles;
   if (joins > INT_MAX) return cudaErrorInvalidConfiguration;
   const cudaError_t e = p.dp == 64 ? run_attend<64>(a, p, s) : run_attend<128>(a, p, s);
   if (e != cudaSuccess) return e;
-  return launch_chained(cache_attend_join_kernel, static_cast<unsigned>(joins), kJoinThreads, 0, 1, s, a);
+  return launch_chained(cache_attend_join_kernel, static_cast<unsigned>(joins), kJoinThreads,
+                        static_cast<size_t>(kJoinThreads / 32) * kAttRows * c.dim * 4, 1, s, a);
 }
 
 }  // namespace vb

@@ -52,7 +52,7 @@ void check_sizes(const verbo_cache* c) {
   const long long per = c->page / VERBO_CACHE_BLOCK;
   if (static_cast<long long>(c->pages) * c->heads * per > INT_MAX)
     fail("pages * heads * page / 16 must be below 2^31");
-  if (static_cast<long long>(c->rows) * c->width * per > INT_MAX) fail("rows * width * page / 16 must be below 2^31");
+  if (static_cast<long long>(c->rows) * (c->width * per + 16) > INT_MAX) fail("rows * width * page / 16 must be below 2^31");
 }
 
 struct CacheRanges {
