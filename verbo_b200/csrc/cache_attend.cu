@@ -113,6 +113,10 @@ __device__ __forceinline__ void cp_async16_if(uint32_t dst, const void* src, boo
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
 }
 
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+
 // 16 elements from `p` on, as floats.
 __device__ __forceinline__ void load16(const void* p, long long i, int type, bool wide, float (&x)[16]) {
   if (!wide) {
@@ -306,23 +310,25 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 ? 2 : 1) cache_attend_ke
 
     // ---- copies, kAttStages - 1 steps ahead
     int slot_in = 0;
+    int next_page = lane < n ? pages[(b0 + lane) * kCacheBlock / a.page] : -1;
     auto fetch = [&](int j) {
       if (j < steps) {
         if ((j & 15) == 0) {  // the next 32 blocks: one per lane
-          const int i = 2 * j + lane, b = b0 + i;
-          BlockHead h{0.0f, 0.0f, 0, -1};
-          if (i < n) {
-            const int at = b * kCacheBlock;
-            const int pid = pages[at / a.page];
-            if (pid >= 0 && pid < a.pages) {
-              h.block = (pid * a.heads + head) * (a.page / kCacheBlock) + (at % a.page) / kCacheBlock;
-              h.ks = a.k_scale[h.block];
-              h.vs = a.v_scale[h.block];
-              h.valid = min(kCacheBlock, len - at);
-            }
-          }
+          const int i = 2 * j + lane, at = (b0 + i) * kCacheBlock;
+          const int pid = next_page;
+          next_page = i + 32 < n ? pages[(at + 32 * kCacheBlock) / a.page] : -1;
+          BlockHead* h = &known[i & (kAttHeads - 1)];
+          int2 v = make_int2(0, -1);
           __syncwarp();
-          known[i & (kAttHeads - 1)] = h;
+          if (i < n && pid >= 0 && pid < a.pages) {
+            v.y = (pid * a.heads + head) * (a.page / kCacheBlock) + (at % a.page) / kCacheBlock;
+            v.x = min(kCacheBlock, len - at);
+            cp_async4(smem_u32(&h->ks), a.k_scale + v.y);
+            cp_async4(smem_u32(&h->vs), a.v_scale + v.y);
+          } else {
+            h->ks = h->vs = 0.0f;
+          }
+          *reinterpret_cast<int2*>(&h->valid) = v;
           __syncwarp();
         }
         const uint32_t to = ring_at + slot_in * S::kStep;
@@ -544,9 +550,10 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 ? 2 : 1) cache_attend_ke
 #pragma unroll
       for (int k = 0; k < 16; ++k) y[k] = sum[(16 * i + k) % NJ][(16 * i + k) / NJ] * by;
       if (d >= a.dim) continue;
+      if (!live) continue;
       if (!whole)
         store16(to, g * a.dim + d, kOpsF32, true, y);
-      else if (live)
+      else
         store16(a.out, q_token * a.ld_out + q_head * a.hd_out + d, a.out_type, a.wide_out, y);
     }
     if (!whole && t == 0) {
@@ -557,31 +564,33 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 ? 2 : 1) cache_attend_ke
   }
 }
 
-constexpr int kJoinThreads = 256;
+// Warps of a join's CTA: one round trip to memory does it where there are few parts to
+// a (row, head), or many of these; few of them are split over most of the card's warps.
+constexpr int kJoinFew = 4, kJoinMany = 16;
+constexpr int kJoinRows = 4;  // query rows of a CTA
 
-// One CTA per (row, head, tile): the parts of its blocks joined, in their order;
-// nothing to do where one warp had them all.  A warp takes every eighth part, all
-// query rows of it.
-__global__ void __launch_bounds__(kJoinThreads) cache_attend_join_kernel(const AttendArgs a) {
-  constexpr int W = kJoinThreads / 32, R = kAttRows;
+// One CTA per (row, head, half a tile): the parts of its blocks joined, in their
+// order; nothing to do where one warp had them all.  A warp takes every W-th part.
+template <int W>
+__global__ void __launch_bounds__(W * 32) cache_attend_join_kernel(const AttendArgs a) {
+  constexpr int R = kJoinRows, H = kAttRows / R, AHEAD = 2;
   extern __shared__ float4 os[];  // [W][R][dim / 4]
   __shared__ float ms[W][R], ls[W][R];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int tile = blockIdx.x % a.tiles;
-  const int head = blockIdx.x / a.tiles % a.heads;
-  const int row = blockIdx.x / a.tiles / a.heads;
+  const int half = blockIdx.x % H;
+  const int tile = blockIdx.x / H % a.tiles;
+  const int head = blockIdx.x / (H * a.tiles) % a.heads;
+  const int row = blockIdx.x / (H * a.tiles) / a.heads;
   grid_wait();
   grid_release();
-  const int f0 = a.first[row], counted = a.first[row + 1] - f0;
+  const int rows = min(R, a.steps * a.group - tile * kAttRows - half * R);  // of this CTA
+  if (rows <= 0) return;
+  const int f0 = a.first[row], counted = a.first[row + 1] - f0, blocks = a.first[a.rows];
   const int quads = a.dim / 4;
-  // this thread's part of the output: a query row, four dims
-  const int qr = tile * R + warp, step = qr / a.group;
-  const bool live = qr < a.steps * a.group && lane < quads;
-  const long long o = (static_cast<long long>(row) * a.steps + step) * a.ld_out +
-                      static_cast<long long>(head * a.group + qr - step * a.group) * a.hd_out + 4 * lane;
-  float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float total = 0.0f;
+  int used = 0;
   if (counted > 0) {
-    const long long all = static_cast<long long>(a.first[a.rows]) * a.heads;
+    const long long all = static_cast<long long>(blocks) * a.heads;
     const long long each = blocks_each(a, all);
     const long long f = static_cast<long long>(f0) * a.heads + static_cast<long long>(head) * counted;
     int w0, w1;
@@ -593,6 +602,7 @@ __global__ void __launch_bounds__(kJoinThreads) cache_attend_join_kernel(const A
       w1 = static_cast<int>((f + counted - 1) / each);
     }
     if (w0 == w1) return;  // teams w0 to w1 have blocks of it
+    used = min(W, w1 - w0 + 1);
     float m[R], l[R];
     float4 x[R];
 #pragma unroll
@@ -601,27 +611,38 @@ __global__ void __launch_bounds__(kJoinThreads) cache_attend_join_kernel(const A
       l[i] = 0.0f;
       x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
-    for (int w = w0 + warp; w <= w1; w += W) {
-      const int which = w * each < f;  // its second part, after the end of another
-      const float* from = a.parts + ((static_cast<long long>(w) * a.tiles + tile) * 2 + which) * part_floats(a.dim);
-      const float ml = lane < 2 * R ? from[R * a.dim + lane] : 0.0f;
-      float4 v[R];
+    for (int w = w0 + warp; w <= w1; w += W * AHEAD) {
+      float ml[AHEAD];
+      float4 v[AHEAD][R];
 #pragma unroll
-      for (int i = 0; i < R; ++i)
-        v[i] = lane < quads ? reinterpret_cast<const float4*>(from)[i * quads + lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int u = 0; u < AHEAD; ++u) {
+        const int at = w + u * W;
+        const int which = at * each < f;  // its second part, after the end of another
+        const float* from = a.parts + ((static_cast<long long>(at) * a.tiles + tile) * 2 + which) * part_floats(a.dim);
+        ml[u] = lane < R ? kNegInf : 0.0f;
+        if (at <= w1 && lane < 2 * R && lane % R < rows)
+          ml[u] = from[kAttRows * a.dim + lane / R * kAttRows + half * R + lane % R];
 #pragma unroll
-      for (int i = 0; i < R; ++i) {
-        const float pm = __shfl_sync(0xffffffffu, ml, i), pl = __shfl_sync(0xffffffffu, ml, R + i);
-        const float mn = fmaxf(m[i], pm);
-        const float s = m[i] > kNegInf ? ex2(m[i] - mn) : 1.0f;
-        const float t = pm > kNegInf ? ex2(pm - mn) : 1.0f;  // a part that sees nothing is zeros, or NaNs
-        m[i] = mn;
-        l[i] = l[i] * s + pl * t;
-        x[i].x = x[i].x * s + v[i].x * t;
-        x[i].y = x[i].y * s + v[i].y * t;
-        x[i].z = x[i].z * s + v[i].z * t;
-        x[i].w = x[i].w * s + v[i].w * t;
+        for (int i = 0; i < R; ++i)
+          v[u][i] = at <= w1 && i < rows && lane < quads
+                        ? reinterpret_cast<const float4*>(from)[(half * R + i) * quads + lane]
+                        : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       }
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          const float pm = __shfl_sync(0xffffffffu, ml[u], i), pl = __shfl_sync(0xffffffffu, ml[u], R + i);
+          const float mn = fmaxf(m[i], pm);
+          const float s = m[i] > kNegInf ? ex2(m[i] - mn) : 1.0f;
+          const float t = pm > kNegInf ? ex2(pm - mn) : 1.0f;  // a part that sees nothing is zeros, or NaNs
+          m[i] = mn;
+          l[i] = l[i] * s + pl * t;
+          x[i].x = x[i].x * s + v[u][i].x * t;
+          x[i].y = x[i].y * s + v[u][i].y * t;
+          x[i].z = x[i].z * s + v[u][i].z * t;
+          x[i].w = x[i].w * s + v[u][i].w * t;
+        }
     }
 #pragma unroll
     for (int i = 0; i < R; ++i) {
@@ -632,26 +653,29 @@ __global__ void __launch_bounds__(kJoinThreads) cache_attend_join_kernel(const A
       }
     }
     __syncthreads();
-    const int used = min(W, w1 - w0 + 1);
-    float mn = kNegInf, total = 0.0f;
-    for (int w = 0; w < used; ++w) mn = fmaxf(mn, ms[w][warp]);
-    for (int w = 0; w < used; ++w) {
-      const float t = ms[w][warp] > kNegInf ? ex2(ms[w][warp] - mn) : 1.0f;
-      total += ls[w][warp] * t;
-      if (lane < quads) {
-        const float4 v = os[(w * R + warp) * quads + lane];
-        y.x += v.x * t, y.y += v.y * t, y.z += v.z * t, y.w += v.w * t;
-      }
+  }
+  // a warp to a query row, four dims to a lane
+  if (warp >= rows) return;
+  float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // an empty row's
+  float mn = kNegInf;
+  for (int w = 0; w < used; ++w) mn = fmaxf(mn, ms[w][warp]);
+  for (int w = 0; w < used; ++w) {
+    const float t = ms[w][warp] > kNegInf ? ex2(ms[w][warp] - mn) : 1.0f;
+    total += ls[w][warp] * t;
+    if (lane < quads) {
+      const float4 v = os[(w * R + warp) * quads + lane];
+      y.x += v.x * t, y.y += v.y * t, y.z += v.z * t, y.w += v.w * t;
     }
-    const float inv = total > 0.0f || total != total ? __fdiv_rn(1.0f, total) : 0.0f;
-    y.x *= inv, y.y *= inv, y.z *= inv, y.w *= inv;
   }
-  if (live) {  // an empty row's are zeros
-    store_any(a.out, o, a.out_type, y.x);
-    store_any(a.out, o + 1, a.out_type, y.y);
-    store_any(a.out, o + 2, a.out_type, y.z);
-    store_any(a.out, o + 3, a.out_type, y.w);
-  }
+  if (lane >= quads) return;
+  const float inv = total > 0.0f || total != total ? __fdiv_rn(1.0f, total) : 0.0f;
+  const int qr = tile * kAttRows + half * R + warp, step = qr / a.group;
+  const long long o = (static_cast<long long>(row) * a.steps + step) * a.ld_out +
+                      static_cast<long long>(head * a.group + qr - step * a.group) * a.hd_out + 4 * lane;
+  store_any(a.out, o, a.out_type, y.x * inv);
+  store_any(a.out, o + 1, a.out_type, y.y * inv);
+  store_any(a.out, o + 2, a.out_type, y.z * inv);
+  store_any(a.out, o + 3, a.out_type, y.w * inv);
 }
 
 constexpr int kAttMaxSmem = 227 * 1024;
@@ -733,12 +757,16 @@ cudaError_t launch_cache_attend(const verbo_cache& c, int layer, const CacheQuer
   };
   a.wide_q = wide(x.q, x.ld_q, x.hd_q, q_type);
   a.wide_out = wide(x.out, x.ld_out, x.hd_out, out_type);
-  const long long joins = static_cast<long long>(c.rows) * c.heads * p.tiles;
+  const long long joins = static_cast<long long>(c.rows) * c.heads * p.tiles * (kAttRows / kJoinRows);
   if (joins > INT_MAX) return cudaErrorInvalidConfiguration;
   const cudaError_t e = p.dp == 64 ? run_attend<64>(a, p, s) : run_attend<128>(a, p, s);
   if (e != cudaSuccess) return e;
-  return launch_chained(cache_attend_join_kernel, static_cast<unsigned>(joins), kJoinThreads,
-                        static_cast<size_t>(kJoinThreads / 32) * kAttRows * c.dim * 4, 1, s, a);
+  const size_t smem = static_cast<size_t>(kJoinRows) * c.dim * 4;  // of a warp
+  if (joins >= 2 * sm_count())
+    return launch_chained(cache_attend_join_kernel<kJoinFew>, static_cast<unsigned>(joins), kJoinFew * 32,
+                          kJoinFew * smem, 1, s, a);
+  return launch_chained(cache_attend_join_kernel<kJoinMany>, static_cast<unsigned>(joins), kJoinMany * 32,
+                        kJoinMany * smem, 1, s, a);
 }
 
 }  // namespace vb
