@@ -34,7 +34,7 @@ extern "C" {
                  candidates.  Of a row with columns at +inf those alone are,
                  with -log(their number).
    scores        requests*beams floats: the beams' summed log-probabilities.  A
-                 beam at -inf (or NaN) has no candidates and its row is not read;
+                 beam at -inf (or NaN) has no candidates, whatever its row holds;
                  so a request's first step, when all its beams hold the same
                  prompt, has 0 for one of them and -inf for the others.
    take          1..64.

@@ -32,10 +32,9 @@ constexpr int kSelVecs = 4;                         // vectors per thread and ba
 constexpr int kSelStages = 2;                       // batches in flight
 constexpr int kSelWarpVecs = kSelVecs * 32;         // a warp's vectors lie side by side
 constexpr int kSelSlots = kSelWarpVecs + 1;         // one more for rows off the 16-byte grid
-constexpr int kSelBatch = kSelVecs * kSelThreads;
-constexpr int kSelGroups = 8;  // batches whose maxima are kept (the last: of all that follow)
+constexpr int kSelGroups = 10;  // groups of batches whose maxima are kept
 constexpr int kSelCap = 1024;  // listed columns per CTA
-constexpr int kSelOffers = 8;  // maxima a warp offers at most
+constexpr int kSelOffers = 32;  // maxima a warp offers at most
 constexpr int kSelMaxCluster = 8;
 constexpr float kSelLowest = -3.402823466e38f;
 // log2(e) = kLog2eHi + kLog2eLo to 2^-49
@@ -52,7 +51,7 @@ struct SelRow {
 
 struct SelPart {
   double s;  // sum of e^(x - m)
-  float m;
+  float m;   // the reference
   int ninf;
 };
 
@@ -127,9 +126,9 @@ struct SelBatch {
 
 __device__ __forceinline__ double shfl_xor_double(double v, int o) { return __shfl_xor_sync(0xffffffffu, v, o); }
 
-// e^x in 64 bits of a difference of maxima; 0 where there is no sum to scale.
+// A sum of e^(x - from), seen from another reference.
 __device__ __forceinline__ double sel_scaled(double s, float from, float m) {
-  return s > 0.0 ? s * exp(static_cast<double>(from) - static_cast<double>(m)) : 0.0;
+  return from == m || !(s > 0.0) ? s : s * exp(static_cast<double>(from) - static_cast<double>(m));
 }
 
 // SHIFT: a row need not begin on the 16-byte grid; a thread joins its vector from
@@ -155,7 +154,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) beam_rows_kernel(const BeamSel
   const int C = cl.num_blocks();
   const int rankc = cl.block_rank();
   if (C > 1) cluster_arrive();  // every CTA of the cluster has started before one writes to the leader
-  const int row = blockIdx.x / C;
+  const int row = blockIdx.x >> (__ffs(C) - 1);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) {
     count = 0;
@@ -166,15 +165,22 @@ __global__ void __launch_bounds__(kSelThreads, 2) beam_rows_kernel(const BeamSel
   grid_release();
   const int top = a.take;
   const T* in = static_cast<const T*>(a.logits) + row * a.ld;
-  const bool dead = !(a.scores[row] > kNegInf);  // no candidates: the row is not read (the same in the whole cluster)
+  const float score = a.scores[row];
   const int shift = SHIFT ? static_cast<int>(reinterpret_cast<uintptr_t>(in) & 15) : 0;  // bytes
   const char* grid = reinterpret_cast<const char*>(in) - shift;
   const long long last = static_cast<long long>(a.vocab) * sizeof(T) + shift;  // the row's end, from `grid`
   // vectors are counted by columns, whatever the row's place
-  const int nvec = dead ? 0 : (a.vocab + N - 1) / N;
-  const int v0 = static_cast<int>(static_cast<long long>(nvec) * rankc / C);
-  const int v1 = static_cast<int>(static_cast<long long>(nvec) * (rankc + 1) / C);
-  const int nbatch = (v1 - v0 + kSelBatch - 1) / kSelBatch;
+  const int nvec = (a.vocab + N - 1) / N;
+  const int cbits = __ffs(C) - 1;  // C is a power of two, and eight times the vectors are below 2^31
+  const int v0 = nvec * rankc >> cbits;
+  const int v1 = nvec * (rankc + 1) >> cbits;
+  // vectors of a thread and batch: fewer where a part is short, so that all warps have some
+  const int nv = min(NV, (v1 - v0 + NT - 1) / NT);
+  const int step = nv * NT, mine0 = warp * nv * 32;  // of a batch; this warp's place in one
+  int nbatch = nv == NV ? (v1 - v0 + NV * NT - 1) / (NV * NT) : v1 > v0;
+  // batches of whole vectors: neither they nor, off the grid, the 16 bytes after them
+  // reach the row's end
+  const int whole = nv == NV ? (v1 - v0 - (SHIFT ? 2 : rankc == C - 1 && a.vocab % N ? 1 : 0)) / (NV * NT) : 0;
 
   auto copy = [&](uint4* to, int v) {  // the 16 bytes at v of the row's grid
     const long long at = static_cast<long long>(v) * 16;
@@ -189,29 +195,37 @@ __global__ void __launch_bounds__(kSelThreads, 2) beam_rows_kernel(const BeamSel
       cp_async16_part(to, bytes > 0 ? grid + at : grid + 16 * (v0 + 1) - 16, bytes);
     }
   };
+  const char* next = grid + (static_cast<long long>(v0) + mine0 + lane) * 16;  // of the batch to be copied next
   auto fetch = [&](int b) {
-    if (b < nbatch) {
-      uint4* to = ring + ((b % kSelStages) * kSelWarps + warp) * SLOTS;
-      const int v = v0 + b * kSelBatch + warp * kSelWarpVecs;
+    uint4* to = ring + ((b % kSelStages) * kSelWarps + warp) * SLOTS;
+    if (b < whole && !(SHIFT && v0 == 0 && b == 0)) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) cp_async16(to + i * 32 + lane, next + i * 512);
+      if (SHIFT && lane == 0) cp_async16(to + kSelWarpVecs, next + kSelWarpVecs * 16);
+    } else if (b < nbatch) {
+      const int v = v0 + b * step + mine0;
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        if (v + i * 32 + lane < v1 + (SHIFT ? 1 : 0)) copy(to + i * 32 + lane, v + i * 32 + lane);
-      if (SHIFT && lane == 0 && v + kSelWarpVecs < v1 + 1) copy(to + kSelWarpVecs, v + kSelWarpVecs);
+        if (i < nv && v + i * 32 + lane < v1 + (SHIFT ? 1 : 0)) copy(to + i * 32 + lane, v + i * 32 + lane);
+      if (SHIFT && lane == 0 && v + nv * 32 < v1 + 1) copy(to + nv * 32, v + nv * 32);
     }
+    next += kSelVecs * NT * 16;
     cp_async_commit();  // an empty group keeps the count
   };
 #pragma unroll
   for (int b = 0; b < kSelStages; ++b) fetch(b);
+  if (!(score > kNegInf)) nbatch = 0;  // no candidates (the same in the whole cluster): nothing else is read
 
-  float ref = kNegInf, mx = kNegInf;
+  const int per_group = max(1, (nbatch + kSelGroups - 1) / kSelGroups);
+  float ref = kNegInf, mx = kNegInf, gm = kNegInf;
   double sum = 0.0;
-  int ninf = 0;
+  int ninf = 0, group = 0, in_group = 0;
   for (int b = 0; b < nbatch; ++b) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kSelStages - 1) : "memory");
     if (SHIFT) __syncwarp();
     SelBatch<T> x;
     const uint4* from = ring + ((b % kSelStages) * kSelWarps + warp) * SLOTS + lane;
-    const int vb = v0 + b * kSelBatch + warp * kSelWarpVecs + lane;
+    const int vb = v0 + b * step + mine0 + lane;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if (SHIFT) {
@@ -231,34 +245,45 @@ __global__ void __launch_bounds__(kSelThreads, 2) beam_rows_kernel(const BeamSel
       } else {
         x.x[i].raw = from[i * 32];
       }
-      // the row's last, short vector, and those behind the part
-      const int v = vb + i * 32;
-      if (v >= v1) {
-        x.x[i].raw = all_neg_inf<T>();
-      } else if (v == nvec - 1 && a.vocab % N) {
-        const int have = a.vocab % N;
-        uint4 r = x.x[i].raw;
-        const uint4 none = all_neg_inf<T>();
-        uint32_t w[4] = {r.x, r.y, r.z, r.w};
+    }
+    if (b >= whole) {  // the row's last, short vector, and what lies behind the part
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          constexpr int P = N / 4;  // columns of a word
-          if (j * P >= have)
-            w[j] = none.x;
-          else if (P == 2 && j * P + 1 >= have)
-            w[j] = (w[j] & 0xffffu) | (none.x & 0xffff0000u);
+      for (int i = 0; i < NV; ++i) {
+        const int v = vb + i * 32;
+        if (i >= nv || v >= v1) {
+          x.x[i].raw = all_neg_inf<T>();
+        } else if (v == nvec - 1 && a.vocab % N) {
+          const int have = a.vocab % N;
+          const uint4 r = x.x[i].raw, none = all_neg_inf<T>();
+          uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            constexpr int P = N / 4;  // columns of a word
+            if (j * P >= have)
+              w[j] = none.x;
+            else if (P == 2 && j * P + 1 >= have)
+              w[j] = (w[j] & 0xffffu) | (none.x & 0xffff0000u);
+          }
+          x.x[i].raw = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        x.x[i].raw = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
     if (SHIFT) __syncwarp();
     fetch(b + kSelStages);
     const float bm = x.max();
     mx = fmaxf(mx, bm);
+    if (b == 0) {
+      const uint32_t w = __reduce_max_sync(0xffffffffu, ord32(bm + 0.0f));
+      if (lane == 0) offer[warp] = w;
+      __syncthreads();
+      ref = unord32(__reduce_max_sync(0xffffffffu, lane < kSelWarps ? offer[lane] : 0u));
+      if (ref == -kNegInf) ref = kNegInf;
+    }
     if (bm == -kNegInf) {
       ninf += x.count_inf();
     } else if (bm > kNegInf) {
-      // The first maximum is kept: terms may be above 1, but not by more than 2^64.
+      // The first batch's maximum is kept, the CTA's: terms may be above 1, but not by
+      // more than 2^64.
       if (ref == kNegInf) {
         ref = bm;
       } else if (bm - ref > 44.0f) {
@@ -267,23 +292,30 @@ __global__ void __launch_bounds__(kSelThreads, 2) beam_rows_kernel(const BeamSel
       }
       sum += x.sum(ref);
     }
-    float* at = &group_max[min(b, kSelGroups - 1) * NT + tid];
-    *at = b < kSelGroups ? bm : fmaxf(*at, bm);
+    gm = fmaxf(gm, bm);
+    if (++in_group == per_group || b == nbatch - 1) {
+      group_max[group * NT + tid] = gm;
+      gm = kNegInf;
+      in_group = 0;
+      ++group;
+    }
   }
 
-  // the CTA's part of the row
+  // the CTA's part of the row: sums of one reference are added as they are
   SelPart p;
-  p.m = unord32(__reduce_max_sync(0xffffffffu, ord32(mx + 0.0f)));
-  p.s = fabsf(p.m) < -kNegInf ? sel_scaled(sum, ref, p.m) : 0.0;
+  p.m = unord32(__reduce_max_sync(0xffffffffu, ord32(ref + 0.0f)));
+  p.s = sel_scaled(sum, ref, p.m);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) p.s += shfl_xor_double(p.s, o);
   p.ninf = __reduce_add_sync(0xffffffffu, ninf);
   if (lane == 0) parts[warp] = p;
 
   // Every warp offers its q largest maxima; the `top`-th of all offers is the
-  // bound (q * kSelWarps >= top of them, each of another thread).
+  // bound: `top` columns reach it, each of another thread.  The warps that have
+  // columns offer twice as many in all; where there are not enough, all is listed.
   const uint32_t mine = ord32(mx + 0.0f);
-  const int q = min(kSelOffers, 2 * ((top + kSelWarps - 1) / kSelWarps));
+  const int busy = nbatch > 1 ? kSelWarps : max(1, min(kSelWarps, (v1 - v0 + nv * 32 - 1) / max(1, nv * 32)));
+  const int q = nbatch > 1 ? (2 * top + kSelWarps - 1) / kSelWarps : min(kSelOffers, (2 * top + busy - 1) / busy);
   uint32_t o = mine;
   for (int i = 0; i < q; ++i) {
     const uint32_t w = __reduce_max_sync(0xffffffffu, o);
@@ -298,14 +330,14 @@ __global__ void __launch_bounds__(kSelThreads, 2) beam_rows_kernel(const BeamSel
   if (warp == 0) {
     const SelPart w = lane < kSelWarps ? parts[lane] : SelPart{0.0, kNegInf, 0};
     total.m = unord32(__reduce_max_sync(0xffffffffu, ord32(w.m + 0.0f)));
-    total.s = fabsf(total.m) < -kNegInf ? sel_scaled(w.s, w.m, total.m) : 0.0;
+    total.s = sel_scaled(w.s, w.m, total.m);
 #pragma unroll
     for (int i = kSelWarps / 2; i > 0; i >>= 1) total.s += shfl_xor_double(total.s, i);
     total.ninf = __reduce_add_sync(0xffffffffu, w.ninf);
   }
   // the bound: an offer with fewer than `top` above it and `top` at or above it
-  if (tid >= 32 && tid < 32 + q * kSelWarps) {
-    const uint32_t w = offer[tid - 32];
+  for (int i = tid; i < q * kSelWarps; i += NT) {
+    const uint32_t w = offer[i];
     int gt = 0, ge = 0;
 #pragma unroll 4
     for (int j = 0; j < q * kSelWarps; j += 4) {
@@ -319,17 +351,17 @@ __global__ void __launch_bounds__(kSelThreads, 2) beam_rows_kernel(const BeamSel
   const uint32_t low = bound;
   const float thr = unord32(low);
   if (mine >= low) {
-    for (int g = 0; g < min(nbatch, kSelGroups); ++g)
+    for (int g = 0; g < group; ++g)
       if (group_max[g * NT + tid] >= thr) hits[atomicAdd(&nhits, 1)] = static_cast<unsigned short>(g * NT + tid);
   }
   __syncthreads();
-  const int lastn = max(1, nbatch - kSelGroups + 1);  // batches of the last group
-  for (int i = tid; i < nhits * (NV * lastn); i += NT) {
-    const int h = lastn == 1 ? i / NV : i / (NV * lastn);
-    const int k = i - h * (NV * lastn);
+  // a thread to a vector of the groups that were hit: read again, from L2
+  const int per_hit = per_group * nv;
+  for (int i = tid; i < nhits * per_hit; i += NT) {
+    const int h = i / per_hit, k = i - h * per_hit;
     const int g = hits[h] / NT, t = hits[h] % NT;
-    if (k >= NV && g < kSelGroups - 1) continue;
-    const int v = v0 + (g + k / NV) * kSelBatch + (t >> 5) * kSelWarpVecs + (k % NV) * 32 + (t & 31);
+    const int kb = nv == NV ? k / NV : k / nv;
+    const int v = v0 + (g * per_group + kb) * step + (t >> 5) * nv * 32 + (k - kb * nv) * 32 + (t & 31);
     if (v >= v1) continue;
     const int col = v * N, have = min(N, a.vocab - col);
     if (!SHIFT && have == N) {
@@ -419,8 +451,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) beam_rows_kernel(const BeamSel
   }
   if (tid == 0) {
     double s = 0.0;
-    if (m != -kNegInf)
-      for (int i = 0; i < C; ++i) s += sel_scaled(slots[i].s, slots[i].m, m);
+    for (int i = 0; i < C; ++i) s += sel_scaled(slots[i].s, slots[i].m, m);
     SelRow r;
     r.inf = inf > 0;
     r.lse = inf > 0 ? log(static_cast<double>(inf)) : static_cast<double>(m) + log(s);
@@ -518,7 +549,7 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const BeamSelec
 template <class T, bool SHIFT>
 cudaError_t run_select(const BeamSelectArgs& a, cudaStream_t s) {
   // CTAs per row: one, or as many as give each SM one, with a batch each.
-  const long long batches = (a.vocab / Vec<T>::N + kSelBatch - 1) / kSelBatch;
+  const long long batches = (a.vocab / Vec<T>::N + kSelVecs * kSelThreads - 1) / (kSelVecs * kSelThreads);
   const long long rows = static_cast<long long>(a.requests) * a.beams;
   const int sms = sm_count();
   int C = 1;
