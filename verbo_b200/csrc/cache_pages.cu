@@ -455,7 +455,7 @@ struct AppendArgs {
   int layer;
   int slots;  // blocks that are looked at
   int per;    // of a row, without offsets
-  bool wide;  // four elements at a time
+  bool wide;  // 16 bytes at a time
 };
 constexpr int kAppendThreads = 256;
 
@@ -471,32 +471,46 @@ __device__ __forceinline__ float2 from_codes(uint32_t two) {  // the low 16 bits
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
+// Eight elements as they lie, and as floats.
 template <class T>
-__device__ __forceinline__ float4 load4(const T* p, bool wide) {
-  if (!wide) return make_float4(to_float(p[0]), to_float(p[1]), to_float(p[2]), to_float(p[3]));
-  if constexpr (sizeof(T) == 4) {
-    return *reinterpret_cast<const float4*>(p);
-  } else {
-    const uint2 r = *reinterpret_cast<const uint2*>(p);
-    const T* t = reinterpret_cast<const T*>(&r);
-    return make_float4(to_float(t[0]), to_float(t[1]), to_float(t[2]), to_float(t[3]));
+struct Eight {
+  uint4 raw[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p, bool wide) {
+    if (wide) {
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) raw[i] = reinterpret_cast<const uint4*>(p)[i];
+    } else if constexpr (sizeof(T) == 4) {
+      const uint32_t* u = reinterpret_cast<const uint32_t*>(p);
+      raw[0] = make_uint4(u[0], u[1], u[2], u[3]);
+      raw[1] = make_uint4(u[4], u[5], u[6], u[7]);
+    } else {
+      const unsigned short* u = reinterpret_cast<const unsigned short*>(p);
+      raw[0] = make_uint4(u[0] | static_cast<uint32_t>(u[1]) << 16, u[2] | static_cast<uint32_t>(u[3]) << 16,
+                          u[4] | static_cast<uint32_t>(u[5]) << 16, u[6] | static_cast<uint32_t>(u[7]) << 16);
+    }
   }
-}
+  __device__ __forceinline__ float get(int i) const {
+    constexpr int N = Vec<T>::N;
+    Vec<T> v;
+    v.raw = raw[i / N];
+    return v.get(i % N);
+  }
+};
 
 __device__ __forceinline__ float divided(float x, float s, float inv) {
   return inv != 0.0f ? x * inv : __fdiv_rn(x, s);
 }
 
 template <class T>
-__global__ void __launch_bounds__(kAppendThreads) cache_append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, sizeof(T) == 2 ? 3 : 2) cache_append_kernel(const AppendArgs a) {
   const verbo_cache& c = a.c;
   grid_wait();
   grid_release();
   const int lane = threadIdx.x & 31;
-  const long long w = static_cast<long long>(blockIdx.x) * (kAppendThreads / 32) + (threadIdx.x >> 5);
-  const int slot = static_cast<int>(w / (c.heads * 2));
+  const unsigned w = blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5);
+  const int slot = static_cast<int>(w / (c.heads * 2u));
   if (slot >= a.slots) return;
-  const int rest = static_cast<int>(w - static_cast<long long>(slot) * (c.heads * 2));
+  const int rest = static_cast<int>(w - slot * (c.heads * 2u));
   const int head = rest >> 1;
   const bool value = rest & 1;
 
@@ -504,14 +518,16 @@ __global__ void __launch_bounds__(kAppendThreads) cache_append_kernel(const Appe
   int row, j;
   long long t0, t1;
   if (a.x.off) {
-    // row r's slots begin at off[r] / 16 + 2 r: as many as it can have blocks
-    int lo = 0, hi = c.rows - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (a.x.off[mid] / kCacheBlock + 2ll * mid <= slot)
-        lo = mid;
-      else
-        hi = mid - 1;
+    // row r's slots begin at off[r] / 16 + 2 r: as many as it can have blocks.  The last
+    // row that begins at or before this one, 32 rows looked at in one round trip.
+    int lo = 0, count = c.rows;
+    while (count > 1) {
+      const int each = (count + 31) / 32, r = lo + lane * each;
+      const bool before = lane * each < count && a.x.off[r] / kCacheBlock + 2ll * r <= slot;
+      const unsigned which = __ballot_sync(0xffffffffu, before) | 1u;
+      const int at = (31 - __clz(which)) * each;
+      lo += at;
+      count = min(each, count - at);
     }
     row = lo;
     t0 = max(0ll, min(a.x.off[row], static_cast<long long>(a.x.tokens)));
@@ -530,30 +546,49 @@ __global__ void __launch_bounds__(kAppendThreads) cache_append_kernel(const Appe
   const long long lo = max(begin, static_cast<long long>(start));
   const long long hi = min(begin + kCacheBlock, start + (t1 - t0));
   if (lo >= hi || begin >= static_cast<long long>(c.width) * c.page) return;
-  const int id = c.table[static_cast<long long>(row) * c.width + begin / c.page];
+  const long long ld = value ? a.x.ld_v : a.x.ld_k;
+  const T* x = static_cast<const T*>(value ? a.x.v : a.x.k) + head * (value ? a.x.hd_v : a.x.hd_k) +
+               (t0 + (lo - start)) * ld;
+  // a lane takes eight elements of a token, of every `side`-th one
+  const int eights = c.dim / 8, side = 32 / eights;
+  const int tok = lane / eights, col = (lane - tok * eights) * 8;
+  const int n = tok < side ? static_cast<int>(hi - lo) : 0;
+  constexpr int MOST = 8;  // of a lane, if two tokens lie side by side; up to 128 dims
+  Eight<T> e[MOST];
+#pragma unroll
+  for (int i = 0; i < MOST; ++i)
+    if (tok + i * side < n) e[i].load(x + (tok + i * side) * ld + col, a.wide);
+  const int place = static_cast<int>(begin);
+  const int id = c.table[static_cast<long long>(row) * c.width + place / c.page];
   if (!is_page(c, id)) return;
-  const int inside = static_cast<int>(begin % c.page);
+  const int inside = place % c.page;
   const long long at = (static_cast<long long>(a.layer) * c.pages + id) * c.heads + head;
   uint32_t* codes = reinterpret_cast<uint32_t*>((value ? c.v : c.k) + (at * c.page + inside) * c.dim);
   float* scale = (value ? c.v_scale : c.k_scale) + at * (c.page / kCacheBlock) + inside / kCacheBlock;
   const bool held = begin < start;
   const float had = held ? *scale : 0.0f;
 
-  const long long ld = value ? a.x.ld_v : a.x.ld_k;
-  const T* x = static_cast<const T*>(value ? a.x.v : a.x.k) + head * (value ? a.x.hd_v : a.x.hd_k) +
-               (t0 + (lo - start)) * ld;
-  const int quads = c.dim / 4;  // of a token
-  const int n = static_cast<int>(hi - lo) * quads;
   float most = 0.0f;
-  auto take = [&](float v) {
-    v = fabsf(v);
-    if (v <= 3.402823466e38f) most = fmaxf(most, v);  // finite ones
-  };
-  for (int i = lane; i < n; i += 32) {
-    const float4 v = load4(x + (i / quads) * ld + (i % quads) * 4, a.wide);
-    take(v.x), take(v.y), take(v.z), take(v.w);
-  }
+#pragma unroll
+  for (int i = 0; i < MOST; ++i)
+    if (tok + i * side < n) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) most = fmaxf(most, fabsf(e[i].get(k)));  // NaNs left out
+    }
   most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+  if (most > 3.402823466e38f) {  // rare: infinities are left out too
+    most = 0.0f;
+#pragma unroll
+    for (int i = 0; i < MOST; ++i)
+      if (tok + i * side < n) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float v = fabsf(e[i].get(k));
+          most = fmaxf(most, v <= 3.402823466e38f ? v : 0.0f);
+        }
+      }
+    most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+  }
   // most = 1.m 2^(e - 127); 448 = 1.75 * 2^8
   const uint32_t bits = __float_as_uint(most);
   const int q = max(static_cast<int>(bits >> 23) - ((bits & 0x7fffffu) > 0x600000u ? 134 : 135), -64);
@@ -563,18 +598,29 @@ __global__ void __launch_bounds__(kAppendThreads) cache_append_kernel(const Appe
   const uint32_t sb = __float_as_uint(s);
   const float inv = (sb & 0x7fffffu) == 0 && sb < (247u << 23) ? __uint_as_float((254u << 23) - sb) : 0.0f;
   if (held && s != had) {
-    for (int i = lane; i < static_cast<int>(lo - begin) * quads; i += 32) {
+    for (int i = lane; i < static_cast<int>(lo - begin) * (c.dim / 4); i += 32) {
       const uint32_t old = codes[i];
       const float2 u = from_codes(old), v = from_codes(old >> 16);
       codes[i] = to_codes(divided(u.x * had, s, inv), divided(u.y * had, s, inv), divided(v.x * had, s, inv),
                           divided(v.y * had, s, inv));
     }
   }
-  codes += static_cast<int>(lo - begin) * quads;
-  for (int i = lane; i < n; i += 32) {
-    const float4 v = load4(x + (i / quads) * ld + (i % quads) * 4, a.wide);
-    codes[i] = to_codes(divided(v.x, s, inv), divided(v.y, s, inv), divided(v.z, s, inv), divided(v.w, s, inv));
-  }
+  unsigned char* to = reinterpret_cast<unsigned char*>(codes) + (static_cast<int>(lo - begin) + tok) * c.dim + col;
+  auto store = [&](auto&& coded) {
+#pragma unroll
+    for (int i = 0; i < MOST; ++i)
+      if (tok + i * side < n) {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = coded(e[i].get(k));
+        *reinterpret_cast<uint2*>(to + i * side * c.dim) =
+            make_uint2(to_codes(v[0], v[1], v[2], v[3]), to_codes(v[4], v[5], v[6], v[7]));
+      }
+  };
+  if (inv != 0.0f)
+    store([&](float v) { return v * inv; });
+  else
+    store([&](float v) { return __fdiv_rn(v, s); });
   if (lane == 0 && !(held && s == had)) *scale = s;
 }
 
@@ -582,11 +628,11 @@ template <class T>
 cudaError_t run_append(AppendArgs a, cudaStream_t s) {
   const long long warps = static_cast<long long>(a.slots) * a.c.heads * 2;
   const long long grid = (warps + kAppendThreads / 32 - 1) / (kAppendThreads / 32);
-  if (grid > INT_MAX) return cudaErrorInvalidConfiguration;
-  // four elements at once where every group of them is aligned
+  if (warps > INT_MAX) return cudaErrorInvalidConfiguration;
+  // eight elements at once where every group of them is aligned to 16 bytes
   const long long all = a.x.ld_k | a.x.hd_k | a.x.ld_v | a.x.hd_v;
-  a.wide = all % 4 == 0 && reinterpret_cast<uintptr_t>(a.x.k) % (4 * sizeof(T)) == 0 &&
-           reinterpret_cast<uintptr_t>(a.x.v) % (4 * sizeof(T)) == 0;
+  a.wide = all % Vec<T>::N == 0 && reinterpret_cast<uintptr_t>(a.x.k) % 16 == 0 &&
+           reinterpret_cast<uintptr_t>(a.x.v) % 16 == 0;
   return launch_chained(cache_append_kernel<T>, static_cast<unsigned>(grid), kAppendThreads, 0, 1, s, a);
 }
 
