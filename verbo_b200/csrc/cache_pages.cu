@@ -120,115 +120,97 @@ struct ReserveArgs {
   int* status;
 };
 constexpr int kReserveThreads = 1024;
-constexpr int kReservePer = VERBO_CACHE_MAX_ROWS / kReserveThreads;
 
-// One CTA for all rows (4 of them a thread).  What a row needs is known when the
+// One CTA for all rows, a thread to a row.  What a row needs is known when the
 // rows before it are counted that write into the same page: with r references and
 // i such rows, the row copies the page if r - i > 1.  Then pages are dealt out
-// through the scan of the needs, one thread to a page.
+// through the scan of the needs, one thread to a page.  Latency alone counts: the
+// chain is lengths, tables, references, and the list of free pages.
 __global__ void __launch_bounds__(kReserveThreads) cache_reserve_kernel(const ReserveArgs a) {
-  extern __shared__ int smem[];  // last [rows], first [rows], copied [rows], then pre [chunks + 1]
-  __shared__ int ws[kReserveThreads / 32];
-  __shared__ long long wide_ws[kReserveThreads / 32];
+  constexpr int NT = kReserveThreads;
+  extern __shared__ __align__(16) int smem[];  // last, len, more, first, copied [rows + 3 each], then pre [chunks + 1]
+  __shared__ int ws[NT / 32];
+  __shared__ long long wide_ws[NT / 32];
   __shared__ int narrow;
   const verbo_cache& c = a.c;
   const int rows = c.rows, page = c.page, tid = threadIdx.x, chunks = chunks_of(c);
-  int* last = smem;
-  int* first = last + rows;
-  int* copied = first + rows;
-  int* pre = copied + rows;
+  const int most = c.width * page, pitch = (rows + 3) / 4 * 4;
+  int* last = smem;            // the shared page that a row writes into, -1: none
+  int* len = last + pitch;
+  int* more = len + pitch;
+  int* first = more + pitch;   // needs before the row
+  int* copied = first + pitch; // 1 + its place among the copies, 0: none
+  int* pre = copied + pitch;
   if (tid == 0) narrow = INT_MAX;
   __syncthreads();
   grid_wait();
   grid_release();
-  const int total_free = scan_counts<kReserveThreads>(a.w, chunks, pre, ws);
 
-  int len[kReservePer], more[kReservePer], need[kReservePer], refs[kReservePer];
-#pragma unroll
-  for (int i = 0; i < kReservePer; ++i) {
-    const int r = tid * kReservePer + i;
-    len[i] = more[i] = need[i] = refs[i] = 0;
-    if (r >= rows) continue;
-    len[i] = length_of(c, r);
-    more[i] = max(0, a.add[r]);
-    if (more[i] > c.width * page - len[i]) {
-      atomicMin(&narrow, r);
-      more[i] = 0;
+  for (int r = tid; r < pitch; r += NT) {
+    int p = -1, n = 0, m = 0, shared = 0;
+    if (r < rows) {
+      n = length_of(c, r);
+      m = max(0, a.add[r]);
+      if (m > most - n) {
+        atomicMin(&narrow, r);
+        m = 0;
+      }
+      if (m > 0 && n % page > 0) {
+        p = c.table[static_cast<long long>(r) * c.width + n / page];
+        if (!is_page(c, p)) p = -1;
+      }
+      if (p >= 0) shared = c.refs[p];
+      if (shared < 2) p = -1;
     }
-    int p = -1;
-    if (more[i] > 0 && len[i] % page > 0) p = c.table[static_cast<long long>(r) * c.width + len[i] / page];
-    if (!is_page(c, p)) p = -1;
-    if (p >= 0) refs[i] = c.refs[p];
     last[r] = p;
+    len[r] = n;
+    more[r] = m;
+    copied[r] = shared;
   }
-  __syncthreads();
-  int mine = 0;
-#pragma unroll
-  for (int i = 0; i < kReservePer; ++i) {
-    const int r = tid * kReservePer + i;
-    if (r >= rows) continue;
-    bool copy = false;
-    if (refs[i] > 1) {
+  const int total_free = scan_counts<NT>(a.w, chunks, pre, ws);
+  // a row needs up to 2^27 pages: sums in 64 bits, the copies' in the upper half
+  long long sum = 0;
+  for (int r0 = 0; r0 < rows; r0 += NT) {
+    const int r = r0 + tid;
+    long long need = 0;
+    if (r < rows) {
       const int p = last[r];
-      int before = 0;
-      for (int j = 0; j < r; ++j) before += last[j] == p;
-      copy = refs[i] - before > 1;
+      bool copy = false;
+      if (p >= 0) {
+        int before = 0;
+        const int4* q = reinterpret_cast<const int4*>(last);
+        for (int j = 0; j < r / 4; ++j) {
+          const int4 v = q[j];
+          before += (v.x == p) + (v.y == p) + (v.z == p) + (v.w == p);
+        }
+        for (int j = r / 4 * 4; j < r; ++j) before += last[j] == p;
+        copy = copied[r] - before > 1;
+      }
+      const int n = len[r], m = more[r];
+      need = copy + (m > 0 ? pages_for(n + m, page) - pages_for(n, page) : 0) + (static_cast<long long>(copy) << 40);
     }
-    copied[r] = copy;
-    need[i] = copy + (more[i] > 0 ? pages_for(len[i] + more[i], page) - pages_for(len[i], page) : 0);
-    mine += need[i];
+    long long total;
+    const long long at = sum + block_excl_scan<long long, NT>(need, wide_ws, &total);
+    if (r < rows) {
+      first[r] = static_cast<int>(min(at & ((1ll << 40) - 1), static_cast<long long>(INT_MAX)));
+      copied[r] = need >> 40 ? static_cast<int>(at >> 40) + 1 : 0;
+    }
+    sum += total;
+    __syncthreads();
   }
-  // a row needs up to 2^27 pages: sums in 64 bits, cut to what a call can still refuse
-  long long sum;
-  long long at64 = block_excl_scan<long long, kReserveThreads>(static_cast<long long>(mine), wide_ws, &sum);
-  const int total = static_cast<int>(min(sum, static_cast<long long>(INT_MAX)));
-#pragma unroll
-  for (int i = 0; i < kReservePer; ++i) {
-    const int r = tid * kReservePer + i;
-    if (r < rows) first[r] = static_cast<int>(min(at64, static_cast<long long>(INT_MAX)));
-    at64 += need[i];
-  }
-  __syncthreads();
+  const int total = static_cast<int>(min(sum & ((1ll << 40) - 1), static_cast<long long>(INT_MAX)));
   const int status = narrow != INT_MAX ? -(narrow + 1) : total > total_free ? total - total_free : 0;
   if (tid == 0) {
     *a.status = status;
-    if (status) a.w.head[0] = 0;
+    a.w.head[0] = status ? 0 : static_cast<int>(sum >> 40);
   }
-  if (status) {
-#pragma unroll
-    for (int i = 0; i < kReservePer; ++i) {
-      const int r = tid * kReservePer + i;
-      if (r < rows) a.start[r] = -1;
-    }
-    return;
+  for (int r = tid; r < rows; r += NT) {
+    const int m = status ? 0 : more[r];
+    a.start[r] = m > 0 ? len[r] : -1;
+    if (m > 0) c.lens[r] = len[r] + m;
   }
-  // the pages that are copied, in the order of the rows
-  int ncopy = 0;
-#pragma unroll
-  for (int i = 0; i < kReservePer; ++i) {
-    const int r = tid * kReservePer + i;
-    if (r < rows) ncopy += copied[r];
-  }
-  int copies;
-  int at = block_excl_scan<int, kReserveThreads>(ncopy, ws, &copies);
-  if (tid == 0) a.w.head[0] = copies;
-#pragma unroll
-  for (int i = 0; i < kReservePer; ++i) {
-    const int r = tid * kReservePer + i;
-    if (r >= rows) continue;
-    if (copied[r]) {
-      const int to = free_page(a.w, chunks, pre, first[r]);
-      a.w.src[at] = last[r];
-      a.w.dst[at] = to;
-      ++at;
-      atomicSub(&c.refs[last[r]], 1);
-      c.refs[to] = 1;
-      c.table[static_cast<long long>(r) * c.width + len[i] / page] = to;
-    }
-    a.start[r] = more[i] > 0 ? len[i] : -1;
-  }
-  // the others, one thread to a page
-  for (int i = tid; i < total; i += kReserveThreads) {
+  if (status) return;
+  for (int i = tid; i < total; i += NT) {
     int lo = 0, hi = rows - 1;
     while (lo < hi) {  // the last row whose pages begin at or before i
       const int mid = (lo + hi + 1) >> 1;
@@ -237,17 +219,17 @@ __global__ void __launch_bounds__(kReserveThreads) cache_reserve_kernel(const Re
       else
         hi = mid - 1;
     }
-    const int k = i - first[lo] - copied[lo];
-    if (k < 0) continue;  // the copied page
     const int to = free_page(a.w, chunks, pre, i);
+    const int k = i - first[lo] - (copied[lo] > 0);
+    int at = pages_for(len[lo], page) + k;
+    if (k < 0) {  // a copy of the row's last page
+      at = len[lo] / page;
+      a.w.src[copied[lo] - 1] = last[lo];
+      a.w.dst[copied[lo] - 1] = to;
+      atomicSub(&c.refs[last[lo]], 1);
+    }
     c.refs[to] = 1;
-    c.table[static_cast<long long>(lo) * c.width + pages_for(length_of(c, lo), page) + k] = to;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kReservePer; ++i) {
-    const int r = tid * kReservePer + i;
-    if (r < rows && more[i] > 0) c.lens[r] = len[i] + more[i];
+    c.table[static_cast<long long>(lo) * c.width + at] = to;
   }
 }
 
@@ -408,7 +390,15 @@ __global__ void __launch_bounds__(kForkThreads) cache_fork_kernel(const ForkArgs
   for (int k = 0; k < K; ++k) most = max(most, used[k]);
   int* t = c.table + static_cast<long long>(group) * K * c.width;
   for (int j = rank * kForkThreads + tid; j < most; j += C * kForkThreads) {
-    for (int k = 0; k < K; ++k) tile[k * kForkThreads + tid] = j < used[k] ? t[static_cast<long long>(k) * c.width + j] : -1;
+    for (int k0 = 0; k0 < K; k0 += 8) {  // eight rows' entries on their way
+      int v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        v[k] = k0 + k < K && j < used[k0 + k] ? t[static_cast<long long>(k0 + k) * c.width + j] : -1;
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k0 + k < K) tile[(k0 + k) * kForkThreads + tid] = v[k];
+    }
     for (int k = 0; k < K; ++k) {
       const int old = tile[k * kForkThreads + tid];
       const int now = from[k] < 0 ? -1 : tile[from[k] * kForkThreads + tid];
@@ -654,9 +644,9 @@ cudaError_t launch_cache_reserve(const verbo_cache& c, const int* add, int* star
   cudaError_t e = launch_chained(cache_scan_kernel, static_cast<unsigned>(chunks_of(c)), kScanThreads, 0, 1, s,
                                  ScanArgs{c, w});
   if (e != cudaSuccess) return e;
-  const size_t smem = (3 * static_cast<size_t>(c.rows) + chunks_of(c) + 1) * 4;
+  const size_t smem = (5 * ((static_cast<size_t>(c.rows) + 3) / 4 * 4) + chunks_of(c) + 1) * 4;
   e = cudaFuncSetAttribute(cache_reserve_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           (3 * VERBO_CACHE_MAX_ROWS + kMaxChunks + 1) * 4);
+                           (5 * VERBO_CACHE_MAX_ROWS + kMaxChunks + 1) * 4);
   if (e != cudaSuccess) return e;
   e = launch_chained(cache_reserve_kernel, 1u, kReserveThreads, smem, 1, s, ReserveArgs{c, w, add, start, status});
   if (e != cudaSuccess) return e;
