@@ -26,6 +26,7 @@ class _State(ctypes.Structure):
 
 
 _ready = None
+_needs = {}  # workspace bytes by (requests, beams, take)
 
 
 def _beam():
@@ -88,9 +89,12 @@ def beam_select(logits, scores, beams, take, vocab=None, stream=None):
     requests = rows // beams
     sp = _list(scores, torch.float32, dev, "scores", rows)
     at = _stream_of(torch, dev, stream)
-    need = lib.verbo_beam_workspace(requests, beams, take)
-    if need < 0:
-        raise _err()
+    need = _needs.get((requests, beams, take))
+    if need is None:
+        need = lib.verbo_beam_workspace(requests, beams, take)
+        if need < 0:
+            raise _err()
+        _needs[requests, beams, take] = need
     out = _new(torch, logits, stream, requests, take, torch.float32)
     parents = _new(torch, logits, stream, requests, take, torch.int32)
     tokens = _new(torch, logits, stream, requests, take, torch.int32)
@@ -130,8 +134,11 @@ def beam_reorder(states, parents, beams, stream=None):
         if t.numel() == 0:
             continue
         inner = t.numel() // rows
-        if not t[0].is_contiguous():
-            raise VerboCudaError("a state's rows must be contiguous")
+        span = 1
+        for n, step in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+            if n > 1 and step != span:
+                raise VerboCudaError("a state's rows must be contiguous")
+            span *= n
         size = t.element_size()
         item.data, item.row_bytes = t.data_ptr(), inner * size
         item.stride_bytes = (t.stride(0) if rows > 1 else inner) * size

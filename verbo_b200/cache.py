@@ -12,7 +12,7 @@ import math
 
 from . import VerboCudaError, _err
 from .beam import _parents
-from .ops import _call, _INT_MAX, _list, _new, _ops, _stream_of
+from .ops import _call, _INT_MAX, _list, _ops, _stream_of
 
 __all__ = ["PagedCache"]
 
@@ -50,6 +50,16 @@ def _cache():
             fn.restype, fn.argtypes = res, args
         _ready = lib, torch, types
     return _ready
+
+
+def _new(torch, like, stream, shape, dtype):
+    """A new tensor that belongs to the call's stream."""
+    if stream is not None:
+        if not isinstance(stream, torch.cuda.Stream):
+            stream = torch.cuda.ExternalStream(stream, device=like.device)
+        with torch.cuda.stream(stream):
+            return torch.empty(shape, dtype=dtype, device=like.device)
+    return torch.empty(shape, dtype=dtype, device=like.device)
 
 
 class PagedCache:
@@ -145,10 +155,10 @@ class PagedCache:
         torch = self._torch
         at = _stream_of(torch, self.k.get_device(), stream)
         ap = self._ints(add, "add")
-        start = _new(torch, self.lens, stream, self.rows, None, torch.int32)
-        status = _new(torch, self.lens, stream, 1, None, torch.int32)
+        start = _new(torch, self.lens, stream, self.rows, torch.int32)
+        status = _new(torch, self.lens, stream, 1, torch.int32)
         # the workspace belongs to the call's stream: freed here, it is reused behind the call
-        ws = _new(torch, self.lens, stream, self._need, None, torch.uint8)
+        ws = _new(torch, self.lens, stream, self._need, torch.uint8)
         self._run(self._lib.verbo_cache_reserve, ap, start.data_ptr(), status.data_ptr(), ws.data_ptr(), self._need, at)
         return start, status
 
@@ -176,8 +186,8 @@ class PagedCache:
         (verbo_cache_compact).  Returns int32 [2]: live pages, pages that moved."""
         torch = self._torch
         at = _stream_of(torch, self.k.get_device(), stream)
-        info = _new(torch, self.lens, stream, 2, None, torch.int32)
-        ws = _new(torch, self.lens, stream, self._need, None, torch.uint8)
+        info = _new(torch, self.lens, stream, 2, torch.int32)
+        ws = _new(torch, self.lens, stream, self._need, torch.uint8)
         self._run(self._lib.verbo_cache_compact, info.data_ptr(), ws.data_ptr(), self._need, at)
         return info
 
@@ -244,12 +254,14 @@ class PagedCache:
             out_dtype = q.dtype if dtype is None else dtype
             if out_dtype not in self._types:
                 raise VerboCudaError("dtype must be float32, float16 or bfloat16")
-            out = _new(torch, q, stream, n, heads * self.dim, out_dtype).view(n, heads, self.dim)
-        elif dtype is not None and dtype != out.dtype:
-            raise VerboCudaError("out must be of dtype")
-        on, _, ldo, hdo, ocode = self._tokens(out, "out", heads)
-        if on != n:
-            raise VerboCudaError("out must have the tokens of q")
+            out = _new(torch, q, stream, (n, heads, self.dim), out_dtype)
+            ldo, hdo, ocode = heads * self.dim, self.dim, self._types[out_dtype]
+        else:
+            if dtype is not None and dtype != out.dtype:
+                raise VerboCudaError("out must be of dtype")
+            on, _, ldo, hdo, ocode = self._tokens(out, "out", heads)
+            if on != n:
+                raise VerboCudaError("out must have the tokens of q")
         at = _stream_of(torch, self.k.get_device(), stream)
         need = self._attend_need.get((heads, steps))
         if need is None:
@@ -258,7 +270,7 @@ class PagedCache:
             if need < 0:
                 raise _err()
             self._attend_need[heads, steps] = need
-        ws = _new(torch, q, stream, need, None, torch.uint8)
+        ws = _new(torch, q, stream, need, torch.uint8)
         self._run(self._lib.verbo_cache_attend, self._layer(layer), q.data_ptr(), code, ldq, hdq, heads, steps, scale,
                   out.data_ptr(), ocode, ldo, hdo, ws.data_ptr(), need, at)
         return out

@@ -557,10 +557,9 @@ cudaError_t run_select(const BeamSelectArgs& a, cudaStream_t s) {
   const long long grid = rows * C;
   if (grid > INT_MAX) return cudaErrorInvalidConfiguration;
   constexpr int smem = kSelStages * kSelWarps * (SHIFT ? kSelSlots : kSelWarpVecs) * 16;
-  const auto kernel = beam_rows_kernel<T, SHIFT>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = allow_smem<beam_rows_kernel<T, SHIFT>>(smem);
   if (e != cudaSuccess) return e;
-  e = launch_chained(kernel, static_cast<unsigned>(grid), kSelThreads, smem, C, s, a);
+  e = launch_chained(beam_rows_kernel<T, SHIFT>, static_cast<unsigned>(grid), kSelThreads, smem, C, s, a);
   if (e != cudaSuccess) return e;
   const size_t lists = static_cast<size_t>(a.beams) * ((a.take + 1) * 8 + a.take * 4);
   return launch_chained(beam_join_kernel, static_cast<unsigned>(a.requests), kJoinThreads, lists, 1, s, a);

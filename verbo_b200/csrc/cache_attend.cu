@@ -30,10 +30,8 @@ namespace {
 
 constexpr int kAttWarps = 8;
 constexpr int kAttThreads = kAttWarps * 32;
-constexpr int kAttRows = 8;    // query rows of a tile: heads that share a token, times steps
 constexpr int kAttPair = 2;    // blocks of a step
 constexpr int kAttFlush = 4;   // steps between two transfers of the sums
-constexpr int kAttStages = 3;  // steps whose copies are in flight
 constexpr int kAttHeads = 64;  // blocks that are known ahead, per warp
 // What the beginning and the end of a (row, head) cost a warp, in blocks: parts are
 // equal with it counted.  64 rows of up to 8192 tokens without it: KAPPA us.
@@ -55,7 +53,8 @@ struct AttendArgs {
   long long ld_out, hd_out;
   int group;  // query heads per head
   int steps;
-  int tiles;      // of kAttRows query rows
+  int tile_rows;  // query rows of a tile (heads that share a token, times steps): 8 or 16
+  int tiles;
   int teams;      // warps that share a part of the blocks, one tile each: grid warps / tiles
   int least;      // blocks that a warp takes at least
   int q_type, out_type;
@@ -64,7 +63,8 @@ struct AttendArgs {
   float* parts;      // [teams][tiles][2][part_floats]
   int* first;        // [rows + 1] blocks before each row
 };
-__host__ __device__ inline int part_floats(int dim) { return kAttRows * (dim + 2); }
+// A part: sums [tile_rows][dim], maxima [tile_rows], weights [tile_rows].
+__host__ __device__ inline int part_floats(int rows, int dim) { return rows * (dim + 2); }
 
 // The part of the blocks that a team takes.
 __device__ __forceinline__ long long blocks_each(const AttendArgs& a, long long all) {
@@ -200,30 +200,36 @@ struct __align__(16) BlockHead {
   int block;  // of the layer's pool
 };
 
-// DP: the head dimension filled up with zeros.  Shared memory per warp: kAttStages
-// steps of two blocks' keys and values, rows of DP bytes whose 16-byte chunks are
-// exchanged so that the fragment loads below meet no bank twice.
-template <int DP>
+// DP: the head dimension filled up with zeros.  RT: eights of query rows of a tile.
+// Shared memory per warp: a ring of steps of two blocks' keys and values, rows of DP
+// bytes whose 16-byte chunks are exchanged so that the fragment loads below meet no
+// bank twice; what is known of the blocks; the fragments of 16 queries.
+template <int DP, int RT>
 struct AttShape {
+  static constexpr int kStages = RT == 1 ? 3 : 2;          // steps whose copies are in flight
   static constexpr int kBlock = 16 * DP;                   // bytes of a block's keys, and of its values
   static constexpr int kStep = kAttPair * 2 * kBlock;      // of a step
-  static constexpr int kRing = kAttStages * kStep;
-  static constexpr int kWarp = kRing + kAttHeads * static_cast<int>(sizeof(BlockHead));
+  static constexpr int kRing = kStages * kStep;
+  static constexpr int kKnown = kAttHeads * static_cast<int>(sizeof(BlockHead));
+  static constexpr int kQuery = RT == 1 ? 0 : DP / 16 * 2 * 512;
+  static constexpr int kWarp = kRing + kKnown + kQuery;
 };
 
-template <int DP>
-__global__ void __launch_bounds__(kAttThreads, DP == 64 ? 2 : 1) cache_attend_kernel(const AttendArgs a) {
-  using S = AttShape<DP>;
+template <int DP, int RT>
+__global__ void __launch_bounds__(kAttThreads, DP == 64 && RT == 1 ? 2 : 1) cache_attend_kernel(const AttendArgs a) {
+  using S = AttShape<DP, RT>;
   constexpr int NJ = DP / 8;   // output tiles of 8 dims
   constexpr int KS = DP / 16;  // steps of 16 dims
   constexpr int CH = DP / 32;  // chunks that a lane copies of a block's keys
   constexpr int OWN = DP / 4;  // output dims of a lane
+  constexpr int ROWS = 8 * RT;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ int scan_ws[kAttWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
   unsigned char* ring = smem + warp * S::kWarp;
   BlockHead* known = reinterpret_cast<BlockHead*>(ring + S::kRing);
+  uint4* query = reinterpret_cast<uint4*>(ring + S::kRing + S::kKnown) + lane;  // [KS][rounded, rests][32]
   int* first = reinterpret_cast<int*>(smem + kAttWarps * S::kWarp);
   if (a.dim < DP)  // the filled-up dims stay zero
     for (int i = lane; i < S::kRing / 16; i += 32) reinterpret_cast<uint4*>(ring)[i] = make_uint4(0, 0, 0, 0);
@@ -308,7 +314,7 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 ? 2 : 1) cache_attend_ke
     const int* pages = a.table + static_cast<long long>(row) * a.width;
     const int steps = (n + 1) / 2;
 
-    // ---- copies, kAttStages - 1 steps ahead
+    // ---- copies, kStages - 1 steps ahead
     int slot_in = 0;
     int next_page = lane < n ? pages[(b0 + lane) * kCacheBlock / a.page] : -1;
     auto fetch = [&](int j) {
@@ -347,21 +353,24 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 ? 2 : 1) cache_attend_ke
             }
         }
       }
-      slot_in = slot_in == kAttStages - 1 ? 0 : slot_in + 1;
+      slot_in = slot_in == S::kStages - 1 ? 0 : slot_in + 1;
       cp_async_commit();
     };
 #pragma unroll
-    for (int j = 0; j < kAttStages - 1; ++j) fetch(j);
+    for (int j = 0; j < S::kStages - 1; ++j) fetch(j);
 
-    // ---- the queries of this lane's row: row g of the tile, its own dims
-    const int r = tile * kAttRows + g;  // step r / group, head r % group
-    const bool live = r < a.steps * a.group;
-    const int step = live ? r / a.group : 0;
-    const int q_head = head * a.group + (live ? r - step * a.group : 0);
-    const long long q_token = static_cast<long long>(row) * a.steps + step;
-    uint32_t qa[KS][4];
-    float c_hi, c_lo;  // the row's factors
-    {
+    // ---- the queries of this lane's rows, g (and g + 8) of the tile, its own dims
+    uint32_t qa[RT == 1 ? KS : 1][4];
+    float c_hi[RT], c_lo[RT];  // the rows' factors
+    int end[RT];               // places that a row sees
+#pragma unroll
+    for (int u = 0; u < RT; ++u) {
+      const int r = tile * ROWS + 8 * u + g;  // step r / group, head r % group
+      const bool live = r < a.steps * a.group;
+      const int step = live ? r / a.group : 0;
+      const long long q_at = (static_cast<long long>(row) * a.steps + step) * a.ld_q +
+                             static_cast<long long>(head * a.group + (live ? r - step * a.group : 0)) * a.hd_q;
+      end[u] = len - (a.steps - 1 - step);
       float x[OWN];
       float most = 0.0f;
 #pragma unroll
@@ -369,7 +378,7 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 ? 2 : 1) cache_attend_ke
         const int d = i * 64 + t * 16;
         float y[16];
         if (live && d < a.dim) {
-          load16(a.q, q_token * a.ld_q + q_head * a.hd_q + d, a.q_type, a.wide_q, y);
+          load16(a.q, q_at + d, a.q_type, a.wide_q, y);
         } else {
 #pragma unroll
           for (int k = 0; k < 16; ++k) y[k] = 0.0f;
@@ -388,124 +397,180 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 ? 2 : 1) cache_attend_ke
       e = min(e, 126);
       const float up = __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
       const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-      c_hi = a.c_hi * down;
-      c_lo = a.c_lo * down;
+      c_hi[u] = a.c_hi * down;
+      c_lo[u] = a.c_lo * down;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         const float* y = x + 4 * s;
-        qa[s][0] = two_halves(y[0] * up, y[1] * up);
-        qa[s][1] = two_rests(y[0] * up, y[1] * up, qa[s][0]);
-        qa[s][2] = two_halves(y[2] * up, y[3] * up);
-        qa[s][3] = two_rests(y[2] * up, y[3] * up, qa[s][2]);
+        const uint32_t h0 = two_halves(y[0] * up, y[1] * up), h1 = two_halves(y[2] * up, y[3] * up);
+        const uint32_t r0 = two_rests(y[0] * up, y[1] * up, h0), r1 = two_rests(y[2] * up, y[3] * up, h1);
+        if (RT == 1) {
+          qa[s][0] = h0, qa[s][1] = r0, qa[s][2] = h1, qa[s][3] = r1;
+        } else {
+          uint32_t* to = reinterpret_cast<uint32_t*>(query + s * 64) + u;
+          to[0] = h0, to[2] = h1, to[128] = r0, to[130] = r1;
+        }
       }
     }
-    const int end = len - (a.steps - 1 - step);  // places that the row sees
-    const int all_see = len - (a.steps - 1);     // places that every row sees
+    const int all_see = len - (a.steps - 1);  // places that every row sees
 
-    float acc[NJ][4], sum[NJ][2];
+    // RT == 1: rows of acc are the row's two parts, added in sum; else two rows
+    float acc[NJ][4], sum[NJ][2 * RT];
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
-      sum[j][0] = sum[j][1] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 2 * RT; ++i) sum[j][i] = 0.0f;
     }
-    float m = kNegInf, l = 0.0f, vref = 0.0f, vinv = 0.0f;
+    float m[RT], l[RT], vref = 0.0f, vinv = 0.0f;
+#pragma unroll
+    for (int u = 0; u < RT; ++u) {
+      m[u] = kNegInf;
+      l[u] = 0.0f;
+    }
     auto flush = [&]() {
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
-        sum[j][0] += acc[j][0] + acc[j][2];
-        sum[j][1] += acc[j][1] + acc[j][3];
+        if (RT == 1) {
+          sum[j][0] += acc[j][0] + acc[j][2];
+          sum[j][1] += acc[j][1] + acc[j][3];
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum[j][i % (2 * RT)] += acc[j][i];
+        }
         acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
       }
     };
 
     int slot = 0;
     for (int j = 0; j < steps; ++j) {
-      fetch(j + kAttStages - 1);
-      asm volatile("cp.async.wait_group %0;" ::"n"(kAttStages - 1) : "memory");
+      fetch(j + S::kStages - 1);
+      asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 1) : "memory");
       __syncwarp();
       const unsigned char* at = ring + slot * S::kStep;
-      slot = slot == kAttStages - 1 ? 0 : slot + 1;
+      slot = slot == S::kStages - 1 ? 0 : slot + 1;
       BlockHead h[kAttPair];
 #pragma unroll
       for (int u = 0; u < kAttPair; ++u) h[u] = known[(2 * j + u) & (kAttHeads - 1)];
 
       // scores: tokens 8 i + g are the columns, this lane has columns 2 t and 2 t + 1
-      float sc[2 * kAttPair][4];
+      float p[2 * kAttPair][2 * RT];
+      {
+        float sc[2 * kAttPair][4];
+        uint32_t w[2 * kAttPair][KS];
 #pragma unroll
-      for (int i = 0; i < 2 * kAttPair; ++i) {
-        sc[i][0] = sc[i][1] = sc[i][2] = sc[i][3] = 0.0f;
-        const unsigned char* kt = at + (i >> 1) * 2 * S::kBlock + (i & 1) * 8 * DP;
-        uint32_t w[KS];
-        const uint4 x = *reinterpret_cast<const uint4*>(kt + at_k0);
-        w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
-        if (DP == 128) {
-          const uint4 y = *reinterpret_cast<const uint4*>(kt + at_k1);
-          w[KS - 4] = y.x, w[KS - 3] = y.y, w[KS - 2] = y.z, w[KS - 1] = y.w;
+        for (int i = 0; i < 2 * kAttPair; ++i) {
+          sc[i][0] = sc[i][1] = sc[i][2] = sc[i][3] = 0.0f;
+          const unsigned char* kt = at + (i >> 1) * 2 * S::kBlock + (i & 1) * 8 * DP;
+          const uint4 x = *reinterpret_cast<const uint4*>(kt + at_k0);
+          w[i][0] = x.x, w[i][1] = x.y, w[i][2] = x.z, w[i][3] = x.w;
+          if (DP == 128) {
+            const uint4 y = *reinterpret_cast<const uint4*>(kt + at_k1);
+            w[i][KS - 4] = y.x, w[i][KS - 3] = y.y, w[i][KS - 2] = y.z, w[i][KS - 1] = y.w;
+          }
+          if (RT == 1) {
+#pragma unroll
+            for (int s = 0; s < KS; ++s) mma16816(sc[i], qa[s], codes_lo(w[i][s]), codes_hi(w[i][s]));
+          }
+        }
+        if (RT == 2) {
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+            const uint4 x = query[s * 64], y = query[s * 64 + 32];
+            const uint32_t hi[4] = {x.x, x.y, x.z, x.w}, lo[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int i = 0; i < 2 * kAttPair; ++i) {
+              const uint32_t k0 = codes_lo(w[i][s]), k1 = codes_hi(w[i][s]);
+              mma16816(sc[i], hi, k0, k1);
+              mma16816(sc[i], lo, k0, k1);
+            }
+          }
         }
 #pragma unroll
-        for (int s = 0; s < KS; ++s) mma16816(sc[i], qa[s], codes_lo(w[s]), codes_hi(w[s]));
-      }
-      float p[2 * kAttPair][2];
+        for (int i = 0; i < 2 * kAttPair; ++i)
 #pragma unroll
-      for (int u = 0; u < kAttPair; ++u) {
-        const float f_hi = c_hi * h[u].ks, f_lo = c_lo * h[u].ks;
+          for (int u = 0; u < RT; ++u) {
+            const float f_hi = c_hi[u] * h[i >> 1].ks, f_lo = c_lo[u] * h[i >> 1].ks;
 #pragma unroll
-        for (int i = 2 * u; i < 2 * u + 2; ++i)
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const float x = sc[i][k] + sc[i][k + 2];
-            p[i][k] = fmaf(x, f_hi, x * f_lo);
+            for (int k = 0; k < 2; ++k) {
+              const float x = RT == 1 ? sc[i][k] + sc[i][k + 2] : sc[i][2 * u + k];
+              p[i][2 * u + k] = fmaf(x, f_hi, x * f_lo);
+            }
           }
       }
       const int place = (b0 + 2 * j) * kCacheBlock;
       if (h[0].valid + h[1].valid < 2 * kCacheBlock || place + 2 * kCacheBlock > all_see) {
 #pragma unroll
-        for (int u = 0; u < kAttPair; ++u) {
-          const int lim = min(h[u].valid, end - place - u * kCacheBlock);
+        for (int i = 0; i < 2 * kAttPair; ++i)
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
+          for (int u = 0; u < RT; ++u) {
+            const int lim = min(h[i >> 1].valid, end[u] - place - (i >> 1) * kCacheBlock);
 #pragma unroll
             for (int k = 0; k < 2; ++k)
-              if (8 * i + 2 * t + k >= lim) p[2 * u + i][k] = kNegInf;
-        }
+              if (8 * (i & 1) + 2 * t + k >= lim) p[i][2 * u + k] = kNegInf;
+          }
       }
-      float mx = kNegInf;
+      float mx[RT];
+      bool grows = false;
 #pragma unroll
-      for (int i = 0; i < 2 * kAttPair; ++i) mx = fmaxf(mx, fmaxf(p[i][0], p[i][1]));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      for (int u = 0; u < RT; ++u) {
+        mx[u] = kNegInf;
+#pragma unroll
+        for (int i = 0; i < 2 * kAttPair; ++i) mx[u] = fmaxf(mx[u], fmaxf(p[i][2 * u], p[i][2 * u + 1]));
+        mx[u] = fmaxf(mx[u], __shfl_xor_sync(0xffffffffu, mx[u], 1));
+        mx[u] = fmaxf(mx[u], __shfl_xor_sync(0xffffffffu, mx[u], 2));
+        grows |= mx[u] > m[u];
+      }
       const float vmax = fmaxf(fabsf(h[0].vs), fabsf(h[1].vs));  // 0 where there is no page
-      if (__any_sync(0xffffffffu, mx > m || vmax > vref)) {
-        const float mn = fmaxf(m, mx), vn = fmaxf(vref, vmax);
-        const float alpha = m > kNegInf ? ex2(m - mn) : 0.0f;
-        const float both = vn > vref ? alpha * __fdiv_rn(vref, vn) : alpha;
+      if (__any_sync(0xffffffffu, grows || vmax > vref)) {
+        const float vn = fmaxf(vref, vmax);
+        const float less = vn > vref ? __fdiv_rn(vref, vn) : 1.0f;
+        float both[RT];
+#pragma unroll
+        for (int u = 0; u < RT; ++u) {
+          const float mn = fmaxf(m[u], mx[u]);
+          const float alpha = m[u] > kNegInf ? ex2(m[u] - mn) : 0.0f;
+          both[u] = alpha * less;
+          l[u] *= alpha;
+          m[u] = mn;
+        }
 #pragma unroll
         for (int i = 0; i < NJ; ++i) {
-          acc[i][0] *= both, acc[i][1] *= both, acc[i][2] *= both, acc[i][3] *= both;
-          sum[i][0] *= both, sum[i][1] *= both;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) acc[i][k] *= both[RT == 1 ? 0 : k >> 1];
+#pragma unroll
+          for (int k = 0; k < 2 * RT; ++k) sum[i][k] *= both[k >> 1];
         }
-        l *= alpha;
-        m = mn;
         if (vn > vref) vinv = __fdiv_rn(1.0f, vn);
         vref = vn;
       }
-      const float base = m > kNegInf ? m - kUp : 0.0f;
 #pragma unroll
-      for (int i = 0; i < 2 * kAttPair; ++i)
+      for (int u = 0; u < RT; ++u) {
+        const float base = m[u] > kNegInf ? m[u] - kUp : 0.0f;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) p[i][k] = ex2(p[i][k] - base);
-      l += ((p[0][0] + p[0][1]) + (p[1][0] + p[1][1])) + ((p[2][0] + p[2][1]) + (p[3][0] + p[3][1]));
+        for (int i = 0; i < 2 * kAttPair; ++i)
+#pragma unroll
+          for (int k = 2 * u; k < 2 * u + 2; ++k) p[i][k] = ex2(p[i][k] - base);
+        l[u] += ((p[0][2 * u] + p[0][2 * u + 1]) + (p[1][2 * u] + p[1][2 * u + 1])) +
+                ((p[2][2 * u] + p[2][2 * u + 1]) + (p[3][2 * u] + p[3][2 * u + 1]));
+      }
 
 #pragma unroll
       for (int u = 0; u < kAttPair; ++u) {
         const float ratio = h[u].vs * vinv;
-        uint32_t pa[4];
+        uint32_t pa[RT][4];  // RT == 1: rounded and rest in one; else the rounded, then the rests
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float x = p[2 * u + i][0] * ratio, y = p[2 * u + i][1] * ratio;
-          pa[2 * i] = two_halves(x, y);
-          pa[2 * i + 1] = two_rests(x, y, pa[2 * i]);
-        }
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int r = 0; r < RT; ++r) {
+            const float x = p[2 * u + i][2 * r] * ratio, y = p[2 * u + i][2 * r + 1] * ratio;
+            const uint32_t hi = two_halves(x, y), lo = two_rests(x, y, hi);
+            if (RT == 1) {
+              pa[0][2 * i] = hi, pa[0][2 * i + 1] = lo;
+            } else {
+              pa[0][2 * i + r] = hi, pa[RT - 1][2 * i + r] = lo;
+            }
+          }
         // values: this lane has tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9 at the dims g DP / 8 ...
         constexpr int W = DP / 32;  // words of a token
         uint32_t v[4][W];
@@ -523,11 +588,15 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 ? 2 : 1) cache_attend_ke
 #pragma unroll
         for (int w = 0; w < W; ++w) {
           const uint32_t a0 = __byte_perm(v[0][w], v[1][w], 0x5140), a1 = __byte_perm(v[0][w], v[1][w], 0x7362);
-          const uint32_t c0 = __byte_perm(v[2][w], v[3][w], 0x5140), c1 = __byte_perm(v[2][w], v[3][w], 0x7362);
-          mma16816(acc[4 * w], pa, codes_lo(a0), codes_lo(c0));
-          mma16816(acc[4 * w + 1], pa, codes_hi(a0), codes_hi(c0));
-          mma16816(acc[4 * w + 2], pa, codes_lo(a1), codes_lo(c1));
-          mma16816(acc[4 * w + 3], pa, codes_hi(a1), codes_hi(c1));
+          const uint32_t e0 = __byte_perm(v[2][w], v[3][w], 0x5140), e1 = __byte_perm(v[2][w], v[3][w], 0x7362);
+          const uint32_t b[4][2] = {{codes_lo(a0), codes_lo(e0)},
+                                    {codes_hi(a0), codes_hi(e0)},
+                                    {codes_lo(a1), codes_lo(e1)},
+                                    {codes_hi(a1), codes_hi(e1)}};
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int r = 0; r < RT; ++r) mma16816(acc[4 * w + i], pa[r], b[i][0], b[i][1]);
         }
       }
       if ((j & (kAttFlush - 1)) == kAttFlush - 1) flush();
@@ -535,30 +604,37 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 ? 2 : 1) cache_attend_ke
     }
     cp_async_wait_all();
     flush();
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
 
     // this lane's dims: OWN t + i, from the tiles i % NJ and the columns 2 t, 2 t + 1
     const bool whole = n == nb;
-    const float by = whole ? (l > 0.0f || l != l ? __fdiv_rn(vref, l) : 0.0f) : vref;
     float* to = whole ? nullptr
-                      : a.parts + ((static_cast<long long>(team) * a.tiles + tile) * 2 + part) * part_floats(a.dim);
+                      : a.parts + ((static_cast<long long>(team) * a.tiles + tile) * 2 + part) * part_floats(ROWS, a.dim);
 #pragma unroll
-    for (int i = 0; i < OWN / 16; ++i) {
-      const int d = OWN * t + 16 * i;
-      float y[16];
+    for (int u = 0; u < RT; ++u) {
+      l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
+      l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
+      const int r = tile * ROWS + 8 * u + g;
+      if (r >= a.steps * a.group) continue;
+      const int step = r / a.group;
+      const long long o = (static_cast<long long>(row) * a.steps + step) * a.ld_out +
+                          static_cast<long long>(head * a.group + r - step * a.group) * a.hd_out;
+      const float by = whole ? (l[u] > 0.0f || l[u] != l[u] ? __fdiv_rn(vref, l[u]) : 0.0f) : vref;
 #pragma unroll
-      for (int k = 0; k < 16; ++k) y[k] = sum[(16 * i + k) % NJ][(16 * i + k) / NJ] * by;
-      if (d >= a.dim) continue;
-      if (!live) continue;
-      if (!whole)
-        store16(to, g * a.dim + d, kOpsF32, true, y);
-      else
-        store16(a.out, q_token * a.ld_out + q_head * a.hd_out + d, a.out_type, a.wide_out, y);
-    }
-    if (!whole && t == 0) {
-      to[kAttRows * a.dim + g] = m;
-      to[kAttRows * a.dim + kAttRows + g] = l;
+      for (int i = 0; i < OWN / 16; ++i) {
+        const int d = OWN * t + 16 * i;
+        if (d >= a.dim) continue;
+        float y[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) y[k] = sum[(16 * i + k) % NJ][2 * u + (16 * i + k) / NJ] * by;
+        if (!whole)
+          store16(to, (8 * u + g) * a.dim + d, kOpsF32, true, y);
+        else
+          store16(a.out, o + d, a.out_type, a.wide_out, y);
+      }
+      if (!whole && t == 0) {
+        to[ROWS * a.dim + 8 * u + g] = m[u];
+        to[ROWS * a.dim + ROWS + 8 * u + g] = l[u];
+      }
     }
     part = 1;
   }
@@ -569,21 +645,22 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 ? 2 : 1) cache_attend_ke
 constexpr int kJoinFew = 4, kJoinMany = 16;
 constexpr int kJoinRows = 4;  // query rows of a CTA
 
-// One CTA per (row, head, half a tile): the parts of its blocks joined, in their
+// One CTA per (row, head, quarter or half of a tile): the parts of its blocks joined, in their
 // order; nothing to do where one warp had them all.  A warp takes every W-th part.
 template <int W>
 __global__ void __launch_bounds__(W * 32) cache_attend_join_kernel(const AttendArgs a) {
-  constexpr int R = kJoinRows, H = kAttRows / R, AHEAD = 2;
+  constexpr int R = kJoinRows, AHEAD = 2;
   extern __shared__ float4 os[];  // [W][R][dim / 4]
   __shared__ float ms[W][R], ls[W][R];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int H = a.tile_rows / R;
   const int half = blockIdx.x % H;
   const int tile = blockIdx.x / H % a.tiles;
   const int head = blockIdx.x / (H * a.tiles) % a.heads;
   const int row = blockIdx.x / (H * a.tiles) / a.heads;
   grid_wait();
   grid_release();
-  const int rows = min(R, a.steps * a.group - tile * kAttRows - half * R);  // of this CTA
+  const int rows = min(R, a.steps * a.group - tile * a.tile_rows - half * R);  // of this CTA
   if (rows <= 0) return;
   const int f0 = a.first[row], counted = a.first[row + 1] - f0, blocks = a.first[a.rows];
   const int quads = a.dim / 4;
@@ -618,10 +695,10 @@ __global__ void __launch_bounds__(W * 32) cache_attend_join_kernel(const AttendA
       for (int u = 0; u < AHEAD; ++u) {
         const int at = w + u * W;
         const int which = at * each < f;  // its second part, after the end of another
-        const float* from = a.parts + ((static_cast<long long>(at) * a.tiles + tile) * 2 + which) * part_floats(a.dim);
+        const float* from = a.parts + ((static_cast<long long>(at) * a.tiles + tile) * 2 + which) * part_floats(a.tile_rows, a.dim);
         ml[u] = lane < R ? kNegInf : 0.0f;
         if (at <= w1 && lane < 2 * R && lane % R < rows)
-          ml[u] = from[kAttRows * a.dim + lane / R * kAttRows + half * R + lane % R];
+          ml[u] = from[a.tile_rows * (a.dim + lane / R) + half * R + lane % R];
 #pragma unroll
         for (int i = 0; i < R; ++i)
           v[u][i] = at <= w1 && i < rows && lane < quads
@@ -669,7 +746,7 @@ __global__ void __launch_bounds__(W * 32) cache_attend_join_kernel(const AttendA
   }
   if (lane >= quads) return;
   const float inv = total > 0.0f || total != total ? __fdiv_rn(1.0f, total) : 0.0f;
-  const int qr = tile * kAttRows + half * R + warp, step = qr / a.group;
+  const int qr = tile * a.tile_rows + half * R + warp, step = qr / a.group;
   const long long o = (static_cast<long long>(row) * a.steps + step) * a.ld_out +
                       static_cast<long long>(head * a.group + qr - step * a.group) * a.hd_out + 4 * lane;
   store_any(a.out, o, a.out_type, y.x * inv);
@@ -681,33 +758,36 @@ __global__ void __launch_bounds__(W * 32) cache_attend_join_kernel(const AttendA
 constexpr int kAttMaxSmem = 227 * 1024;
 
 struct Plan {
-  int dp, grid, tiles, teams, least;
+  int dp, rt, grid, tiles, teams, least;
   size_t smem, parts_bytes;
 };
 Plan plan(const verbo_cache& c, int heads, int steps) {
   Plan p{};
+  const int rows = steps * (heads / c.heads);
   p.dp = c.dim <= 64 ? 64 : 128;
-  p.smem = static_cast<size_t>(kAttWarps) * (p.dp == 64 ? AttShape<64>::kWarp : AttShape<128>::kWarp) +
-           (static_cast<size_t>(c.rows) + 1) * 4;
+  // More than 8 query rows: 16 at a time, twice the products for one conversion and one
+  // copy of the keys and values.  KAPPA16
+  p.rt = rows > 8 ? 2 : 1;
+  const int warp = p.dp == 64 ? (p.rt == 1 ? AttShape<64, 1>::kWarp : AttShape<64, 2>::kWarp)
+                              : (p.rt == 1 ? AttShape<128, 1>::kWarp : AttShape<128, 2>::kWarp);
+  p.smem = static_cast<size_t>(kAttWarps) * warp + (static_cast<size_t>(c.rows) + 1) * 4;
   // small heads leave room for two CTAs an SM, unless there are very many rows
-  const int per_sm = p.dp == 64 && 2 * (p.smem + 1024) <= kAttMaxSmem + 1024 ? 2 : 1;
+  const int per_sm = p.dp == 64 && p.rt == 1 && 2 * (p.smem + 1024) <= kAttMaxSmem + 1024 ? 2 : 1;
   p.grid = sm_count() * per_sm;
-  p.tiles = (steps * (heads / c.heads) + kAttRows - 1) / kAttRows;
+  p.tiles = (rows + 8 * p.rt - 1) / (8 * p.rt);
   p.teams = std::max(1, p.grid * kAttWarps / p.tiles);
   p.least = 2;
-  p.parts_bytes = static_cast<size_t>(p.teams) * p.tiles * 2 * part_floats(c.dim) * 4;
+  p.parts_bytes = static_cast<size_t>(p.teams) * p.tiles * 2 * part_floats(8 * p.rt, c.dim) * 4;
   return p;
 }
 
-template <int DP>
+template <int DP, int RT>
 cudaError_t run_attend(const AttendArgs& a, const Plan& p, cudaStream_t s) {
-  static_assert(kAttWarps * AttShape<128>::kWarp + (VERBO_CACHE_MAX_ROWS + 1) * 4 + 64 <= kAttMaxSmem, "shared memory");
-  const auto kernel = cache_attend_kernel<DP>;
-  const cudaError_t e =
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           kAttWarps * AttShape<DP>::kWarp + (VERBO_CACHE_MAX_ROWS + 1) * 4);
+  constexpr int most = kAttWarps * AttShape<DP, RT>::kWarp + (VERBO_CACHE_MAX_ROWS + 1) * 4;
+  static_assert(most + 64 <= kAttMaxSmem, "shared memory");
+  const cudaError_t e = allow_smem<cache_attend_kernel<DP, RT>>(most);
   if (e != cudaSuccess) return e;
-  return launch_chained(kernel, static_cast<unsigned>(p.grid), kAttThreads, p.smem, 1, s, a);
+  return launch_chained(cache_attend_kernel<DP, RT>, static_cast<unsigned>(p.grid), kAttThreads, p.smem, 1, s, a);
 }
 
 }  // namespace
@@ -741,6 +821,7 @@ cudaError_t launch_cache_attend(const verbo_cache& c, int layer, const CacheQuer
   a.hd_out = x.hd_out;
   a.group = x.heads / c.heads;
   a.steps = x.steps;
+  a.tile_rows = 8 * p.rt;
   a.tiles = p.tiles;
   a.teams = p.teams;
   a.least = p.least;
@@ -757,9 +838,10 @@ cudaError_t launch_cache_attend(const verbo_cache& c, int layer, const CacheQuer
   };
   a.wide_q = wide(x.q, x.ld_q, x.hd_q, q_type);
   a.wide_out = wide(x.out, x.ld_out, x.hd_out, out_type);
-  const long long joins = static_cast<long long>(c.rows) * c.heads * p.tiles * (kAttRows / kJoinRows);
+  const long long joins = static_cast<long long>(c.rows) * c.heads * p.tiles * (8 * p.rt / kJoinRows);
   if (joins > INT_MAX) return cudaErrorInvalidConfiguration;
-  const cudaError_t e = p.dp == 64 ? run_attend<64>(a, p, s) : run_attend<128>(a, p, s);
+  const cudaError_t e = p.dp == 64 ? (p.rt == 1 ? run_attend<64, 1>(a, p, s) : run_attend<64, 2>(a, p, s))
+                                   : (p.rt == 1 ? run_attend<128, 1>(a, p, s) : run_attend<128, 2>(a, p, s));
   if (e != cudaSuccess) return e;
   const size_t smem = static_cast<size_t>(kJoinRows) * c.dim * 4;  // of a warp
   if (joins >= 2 * sm_count())

@@ -645,8 +645,7 @@ cudaError_t launch_cache_reserve(const verbo_cache& c, const int* add, int* star
                                  ScanArgs{c, w});
   if (e != cudaSuccess) return e;
   const size_t smem = (5 * ((static_cast<size_t>(c.rows) + 3) / 4 * 4) + chunks_of(c) + 1) * 4;
-  e = cudaFuncSetAttribute(cache_reserve_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           (5 * VERBO_CACHE_MAX_ROWS + kMaxChunks + 1) * 4);
+  e = allow_smem<cache_reserve_kernel>((5 * VERBO_CACHE_MAX_ROWS + kMaxChunks + 1) * 4);
   if (e != cudaSuccess) return e;
   e = launch_chained(cache_reserve_kernel, 1u, kReserveThreads, smem, 1, s, ReserveArgs{c, w, add, start, status});
   if (e != cudaSuccess) return e;

@@ -5,6 +5,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "device.cuh"
 
 namespace vb {
@@ -77,6 +79,21 @@ __device__ __forceinline__ uint4 all_neg_inf<__half>() {
 template <>
 __device__ __forceinline__ uint4 all_neg_inf<__nv_bfloat16>() {
   return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
+}
+
+// The shared memory that a kernel may have on the current device, set at its first
+// launch there (devices beyond the 64th: at every launch).
+template <auto Kernel>
+inline cudaError_t allow_smem(int bytes) {
+  static std::atomic<unsigned long long> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
 }
 
 // A kernel that may begin before the one before it in the stream has ended
