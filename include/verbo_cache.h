@@ -115,7 +115,7 @@ VERBO_CUDA_API int verbo_cache_attend(const verbo_cache* c, int layer, const voi
                                       long long hd_q, int heads, int steps, float scale, void* out, int out_type,
                                       long long ld_out, long long hd_out, void* workspace, long long workspace_bytes,
                                       void* stream);
-/* Bytes of that call on the current device, or -1. */
+/* Bytes of that call on the current device (0 for few rows and short tables), or -1. */
 VERBO_CUDA_API long long verbo_cache_attend_workspace(const verbo_cache* c, int heads, int steps);
 
 #ifdef __cplusplus

@@ -270,7 +270,7 @@ class PagedCache:
             if need < 0:
                 raise _err()
             self._attend_need[heads, steps] = need
-        ws = _new(torch, q, stream, need, torch.uint8)
+        ws = _new(torch, q, stream, need, torch.uint8) if need else None
         self._run(self._lib.verbo_cache_attend, self._layer(layer), q.data_ptr(), code, ldq, hdq, heads, steps, scale,
-                  out.data_ptr(), ocode, ldo, hdo, ws.data_ptr(), need, at)
+                  out.data_ptr(), ocode, ldo, hdo, ws.data_ptr() if need else None, need, at)
         return out

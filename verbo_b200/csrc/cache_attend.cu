@@ -60,6 +60,7 @@ struct AttendArgs {
   int q_type, out_type;
   bool wide_q, wide_out;  // 16 bytes at a time
   float c_hi, c_lo;  // scale * log2(e)
+  int members;       // CTAs of a cluster, where a cluster has a (row, head, tile)
   float* parts;      // [teams][tiles][2][part_floats]
   int* first;        // [rows + 1] blocks before each row
 };
@@ -215,7 +216,9 @@ struct AttShape {
   static constexpr int kWarp = kRing + kKnown + kQuery;
 };
 
-template <int DP, int RT>
+// CL: a cluster has one (row, head, tile), split evenly over its warps, and joins their
+// parts itself.
+template <int DP, int RT, bool CL>
 __global__ void __launch_bounds__(kAttThreads, DP == 64 && RT == 1 ? 2 : 1) cache_attend_kernel(const AttendArgs a) {
   using S = AttShape<DP, RT>;
   constexpr int NJ = DP / 8;   // output tiles of 8 dims
@@ -225,6 +228,8 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 && RT == 1 ? 2 : 1) cach
   constexpr int ROWS = 8 * RT;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ int scan_ws[kAttWarps];
+  __shared__ float4 joined[CL ? kAttWarps : 1][DP / 4];
+  __shared__ float2 joined_ml[CL ? kAttWarps : 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
   unsigned char* ring = smem + warp * S::kWarp;
@@ -235,18 +240,27 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 && RT == 1 ? 2 : 1) cach
     for (int i = lane; i < S::kRing / 16; i += 32) reinterpret_cast<uint4*>(ring)[i] = make_uint4(0, 0, 0, 0);
   grid_wait();
   grid_release();
-  scan_rows(a, first, scan_ws);
-  if (blockIdx.x == 0)
-    for (int r = tid; r <= a.rows; r += kAttThreads) a.first[r] = first[r];
-
-  const long long all = static_cast<long long>(first[a.rows]) * a.heads;
-  const long long each = blocks_each(a, all);
-  const int id = warp * gridDim.x + blockIdx.x;  // few blocks go to as many SMs as there are
-  const int team = id / a.tiles, tile = id - team * a.tiles;
-  if (team >= a.teams) return;
-  long long i0 = team * each;
-  const long long i1 = min(all, i0 + each);
-  if (i0 >= i1) return;
+  int team = 0, tile, row = 0, head = 0;
+  long long i0 = 0, i1 = 1, each = 0;
+  if (CL) {
+    const int unit = blockIdx.x / a.members;
+    tile = unit % a.tiles;
+    head = unit / a.tiles % a.heads;
+    row = unit / a.tiles / a.heads;
+  } else {
+    scan_rows(a, first, scan_ws);
+    if (blockIdx.x == 0)
+      for (int r = tid; r <= a.rows; r += kAttThreads) a.first[r] = first[r];
+    const long long all = static_cast<long long>(first[a.rows]) * a.heads;
+    each = blocks_each(a, all);
+    const int id = warp * gridDim.x + blockIdx.x;  // few blocks go to as many SMs as there are
+    team = id / a.tiles;
+    tile = id - team * a.tiles;
+    if (team >= a.teams) return;
+    i0 = team * each;
+    i1 = min(all, i0 + each);
+    if (i0 >= i1) return;
+  }
 
   // a lane's chunks of a block: where they go, which token they belong to
   const int per_token = a.dim / 16;
@@ -283,8 +297,7 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 && RT == 1 ? 2 : 1) cach
     at_v1 = S::kBlock + t * 128 + (((4 | (g >> 1)) ^ (t << 1)) << 4) + (g & 1) * 8;
   }
 
-  int row;
-  {
+  if (!CL) {
     const long long want = i0 / a.heads;  // a row's blocks come heads times in a row
     int lo = 0, hi = a.rows - 1;
     while (lo < hi) {  // the last row that begins at or before it (rows without blocks come first)
@@ -298,17 +311,29 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 && RT == 1 ? 2 : 1) cach
   }
   int part = 0;  // parts that this warp has written
   while (i0 < i1) {
-    while (static_cast<long long>(first[row + 1]) * a.heads <= i0) ++row;
-    const int counted = first[row + 1] - first[row], nb = counted - kAttStart;
-    const long long in_row = i0 - static_cast<long long>(first[row]) * a.heads;
-    const int head = static_cast<int>(in_row / counted);
-    const int c0 = static_cast<int>(in_row - static_cast<long long>(head) * counted);
-    const int c1 = static_cast<int>(min(static_cast<long long>(counted), c0 + (i1 - i0)));
-    i0 += c1 - c0;
-    const int b0 = max(0, c0 - kAttStart), n = max(0, c1 - kAttStart) - b0;
-    if (n == 0) {  // its start alone
-      part = 1;
-      continue;
+    int nb, b0, n;
+    if (CL) {
+      nb = (max(0, min(a.lens[row], a.width * a.page)) + kCacheBlock - 1) / kCacheBlock;
+      const int all = (nb + 1) / 2, warps = a.members * kAttWarps;
+      const int w = blockIdx.x % a.members * kAttWarps + warp;
+      b0 = 2 * (all * w / warps);
+      n = max(0, min(nb, 2 * (all * (w + 1) / warps)) - b0);
+      i0 = i1;
+    } else {
+      while (static_cast<long long>(first[row + 1]) * a.heads <= i0) ++row;
+      const int counted = first[row + 1] - first[row];
+      nb = counted - kAttStart;
+      const long long in_row = i0 - static_cast<long long>(first[row]) * a.heads;
+      head = static_cast<int>(in_row / counted);
+      const int c0 = static_cast<int>(in_row - static_cast<long long>(head) * counted);
+      const int c1 = static_cast<int>(min(static_cast<long long>(counted), c0 + (i1 - i0)));
+      i0 += c1 - c0;
+      b0 = max(0, c0 - kAttStart);
+      n = max(0, c1 - kAttStart) - b0;
+      if (n == 0) {  // its start alone
+        part = 1;
+        continue;
+      }
     }
     const int len = max(0, min(a.lens[row], a.width * a.page));
     const int* pages = a.table + static_cast<long long>(row) * a.width;
@@ -606,9 +631,14 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 && RT == 1 ? 2 : 1) cach
     flush();
 
     // this lane's dims: OWN t + i, from the tiles i % NJ and the columns 2 t, 2 t + 1
-    const bool whole = n == nb;
-    float* to = whole ? nullptr
-                      : a.parts + ((static_cast<long long>(team) * a.tiles + tile) * 2 + part) * part_floats(ROWS, a.dim);
+    const bool whole = !CL && n == nb;
+    float* to = nullptr;
+    if (CL) {
+      __syncwarp();
+      to = reinterpret_cast<float*>(ring);  // its copies are done
+    } else if (!whole) {
+      to = a.parts + ((static_cast<long long>(team) * a.tiles + tile) * 2 + part) * part_floats(ROWS, a.dim);
+    }
 #pragma unroll
     for (int u = 0; u < RT; ++u) {
       l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
@@ -637,6 +667,54 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 && RT == 1 ? 2 : 1) cach
       }
     }
     part = 1;
+  }
+
+  if constexpr (CL) {
+    cg::cluster_group cl = cg::this_cluster();
+    cluster_sync_all();  // every warp's part is there
+    const int rows = min(ROWS, a.steps * a.group - tile * ROWS), quads = a.dim / 4;
+    for (int r = cl.block_rank(); r < rows; r += a.members) {
+      // this warp takes the parts of its likes in all CTAs, then warp 0 the warps'
+      float pm = kNegInf, pl = 0.0f;
+      float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      auto add = [&](float qm, float ql, float4 v) {
+        const float mn = fmaxf(pm, qm);
+        const float s = pm > kNegInf ? ex2(pm - mn) : 1.0f;
+        const float u = qm > kNegInf ? ex2(qm - mn) : 1.0f;  // a part that sees nothing is zeros, or NaNs
+        pm = mn;
+        pl = pl * s + ql * u;
+        y.x = y.x * s + v.x * u, y.y = y.y * s + v.y * u, y.z = y.z * s + v.z * u, y.w = y.w * s + v.w * u;
+      };
+#pragma unroll 4
+      for (int c = 0; c < a.members; ++c) {
+        const float* from = cl.map_shared_rank(reinterpret_cast<float*>(ring), c);
+        add(from[ROWS * a.dim + r], from[ROWS * a.dim + ROWS + r],
+            lane < quads ? reinterpret_cast<const float4*>(from + r * a.dim)[lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f));
+      }
+      if (lane < quads) joined[warp][lane] = y;
+      if (lane == 0) joined_ml[warp] = make_float2(pm, pl);
+      __syncthreads();
+      if (warp == 0) {
+        pm = kNegInf;
+        pl = 0.0f;
+        y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < kAttWarps; ++w)
+          add(joined_ml[w].x, joined_ml[w].y, lane < quads ? joined[w][lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f));
+        if (lane < quads) {
+          const float inv = pl > 0.0f || pl != pl ? __fdiv_rn(1.0f, pl) : 0.0f;
+          const int qr = tile * ROWS + r, step = qr / a.group;
+          const long long o = (static_cast<long long>(row) * a.steps + step) * a.ld_out +
+                              static_cast<long long>(head * a.group + qr - step * a.group) * a.hd_out + 4 * lane;
+          store_any(a.out, o, a.out_type, y.x * inv);
+          store_any(a.out, o + 1, a.out_type, y.y * inv);
+          store_any(a.out, o + 2, a.out_type, y.z * inv);
+          store_any(a.out, o + 3, a.out_type, y.w * inv);
+        }
+      }
+      __syncthreads();
+    }
+    cluster_sync_all();  // nobody reads another's shared memory any more
   }
 }
 
@@ -757,24 +835,41 @@ __global__ void __launch_bounds__(W * 32) cache_attend_join_kernel(const AttendA
 
 constexpr int kAttMaxSmem = 227 * 1024;
 
+// A warp of a cluster takes at most this many steps, whatever the lengths are: longer
+// tables go to the parts, which are equal for any lengths.
+constexpr int kClusterSteps = 24;
+
 struct Plan {
-  int dp, rt, grid, tiles, teams, least;
+  int dp, rt, grid, tiles, teams, least, members;
   size_t smem, parts_bytes;
 };
 Plan plan(const verbo_cache& c, int heads, int steps) {
   Plan p{};
-  const int rows = steps * (heads / c.heads);
+  const int rows = steps * (heads / c.heads), sms = sm_count();
   p.dp = c.dim <= 64 ? 64 : 128;
   // More than 8 query rows: 16 at a time, twice the products for one conversion and one
   // copy of the keys and values.  KAPPA16
   p.rt = rows > 8 ? 2 : 1;
+  p.tiles = (rows + 8 * p.rt - 1) / (8 * p.rt);
   const int warp = p.dp == 64 ? (p.rt == 1 ? AttShape<64, 1>::kWarp : AttShape<64, 2>::kWarp)
                               : (p.rt == 1 ? AttShape<128, 1>::kWarp : AttShape<128, 2>::kWarp);
+  // Few (row, head, tile): a cluster for each, with as many CTAs as the SMs allow.
+  const long long units = static_cast<long long>(c.rows) * c.heads * p.tiles;
+  if (units <= sms) {
+    p.members = 1;
+    while (p.members < 8 && units * p.members * 2 <= sms) p.members *= 2;
+    const long long most = static_cast<long long>(c.width) * (c.page / kCacheBlock);  // blocks of a row
+    if (most <= 2ll * kClusterSteps * kAttWarps * p.members) {
+      p.grid = static_cast<int>(units) * p.members;
+      p.smem = static_cast<size_t>(kAttWarps) * warp;
+      return p;
+    }
+    p.members = 0;
+  }
   p.smem = static_cast<size_t>(kAttWarps) * warp + (static_cast<size_t>(c.rows) + 1) * 4;
   // small heads leave room for two CTAs an SM, unless there are very many rows
   const int per_sm = p.dp == 64 && p.rt == 1 && 2 * (p.smem + 1024) <= kAttMaxSmem + 1024 ? 2 : 1;
-  p.grid = sm_count() * per_sm;
-  p.tiles = (rows + 8 * p.rt - 1) / (8 * p.rt);
+  p.grid = sms * per_sm;
   p.teams = std::max(1, p.grid * kAttWarps / p.tiles);
   p.least = 2;
   p.parts_bytes = static_cast<size_t>(p.teams) * p.tiles * 2 * part_floats(8 * p.rt, c.dim) * 4;
@@ -783,17 +878,24 @@ Plan plan(const verbo_cache& c, int heads, int steps) {
 
 template <int DP, int RT>
 cudaError_t run_attend(const AttendArgs& a, const Plan& p, cudaStream_t s) {
+  if (p.members) {
+    const cudaError_t e = allow_smem<cache_attend_kernel<DP, RT, true>>(kAttWarps * AttShape<DP, RT>::kWarp);
+    if (e != cudaSuccess) return e;
+    return launch_chained(cache_attend_kernel<DP, RT, true>, static_cast<unsigned>(p.grid), kAttThreads, p.smem,
+                          p.members, s, a);
+  }
   constexpr int most = kAttWarps * AttShape<DP, RT>::kWarp + (VERBO_CACHE_MAX_ROWS + 1) * 4;
   static_assert(most + 64 <= kAttMaxSmem, "shared memory");
-  const cudaError_t e = allow_smem<cache_attend_kernel<DP, RT>>(most);
+  const cudaError_t e = allow_smem<cache_attend_kernel<DP, RT, false>>(most);
   if (e != cudaSuccess) return e;
-  return launch_chained(cache_attend_kernel<DP, RT>, static_cast<unsigned>(p.grid), kAttThreads, p.smem, 1, s, a);
+  return launch_chained(cache_attend_kernel<DP, RT, false>, static_cast<unsigned>(p.grid), kAttThreads, p.smem, 1, s, a);
 }
 
 }  // namespace
 
 size_t cache_attend_bytes(const verbo_cache& c, int heads, int steps) {
-  return (plan(c, heads, steps).parts_bytes + (static_cast<size_t>(c.rows) + 1) * 4 + 15) / 16 * 16;
+  const Plan p = plan(c, heads, steps);
+  return p.members || c.rows == 0 ? 0 : (p.parts_bytes + (static_cast<size_t>(c.rows) + 1) * 4 + 15) / 16 * 16;
 }
 
 cudaError_t launch_cache_attend(const verbo_cache& c, int layer, const CacheQuery& x, int q_type, int out_type,
@@ -825,6 +927,7 @@ cudaError_t launch_cache_attend(const verbo_cache& c, int layer, const CacheQuer
   a.tiles = p.tiles;
   a.teams = p.teams;
   a.least = p.least;
+  a.members = p.members;
   a.q_type = q_type;
   a.out_type = out_type;
   const double f = static_cast<double>(x.scale) * kLog2e;
@@ -842,7 +945,7 @@ cudaError_t launch_cache_attend(const verbo_cache& c, int layer, const CacheQuer
   if (joins > INT_MAX) return cudaErrorInvalidConfiguration;
   const cudaError_t e = p.dp == 64 ? (p.rt == 1 ? run_attend<64, 1>(a, p, s) : run_attend<64, 2>(a, p, s))
                                    : (p.rt == 1 ? run_attend<128, 1>(a, p, s) : run_attend<128, 2>(a, p, s));
-  if (e != cudaSuccess) return e;
+  if (e != cudaSuccess || p.members) return e;
   const size_t smem = static_cast<size_t>(kJoinRows) * c.dim * 4;  // of a warp
   if (joins >= 2 * sm_count())
     return launch_chained(cache_attend_join_kernel<kJoinFew>, static_cast<unsigned>(joins), kJoinFew * 32,

@@ -269,11 +269,12 @@ VERBO_CUDA_API int verbo_cache_attend(const verbo_cache* c, int layer, const voi
         const bool by_token = (heads - 1) * hd_out + c->dim <= ld_out || tokens == 1;
         const bool by_head = (tokens - 1) * ld_out + c->dim <= hd_out || heads == 1;
         if (!by_token && !by_head) fail("out: its tokens and heads overlap");
-        const Range ws = check_workspace(workspace, workspace_bytes, vb::cache_attend_bytes(*c, heads, steps),
-                                         "verbo_cache_attend_workspace");
-        check_output(ws, all);
-        check_apart(ws, rq);
-        check_apart(ws, ro);
+        if (const size_t need = vb::cache_attend_bytes(*c, heads, steps)) {
+          const Range ws = check_workspace(workspace, workspace_bytes, need, "verbo_cache_attend_workspace");
+          check_output(ws, all);
+          check_apart(ws, rq);
+          check_apart(ws, ro);
+        }
         const vb::CacheQuery x{q, ld_q, hd_q, out, ld_out, hd_out, heads, steps, scale, workspace};
         cuda_ok(vb::launch_cache_attend(*c, layer, x, q_type, out_type, static_cast<cudaStream_t>(stream)),
                 "kernel launch");
