@@ -26,14 +26,14 @@ namespace {
 // the threads' maxima, as in logprob_kernel); a cluster of CTAs shares a row where
 // the rows are few.  A second, small kernel joins the beams of a request: a lane
 // keeps the head of a beam's list, and the largest is taken `take` times.
-constexpr int kSelThreads = 512;
+constexpr int kSelThreads = 256;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kSelVecs = 4;                         // vectors per thread and batch
 constexpr int kSelStages = 2;                       // batches in flight
 constexpr int kSelWarpVecs = kSelVecs * 32;         // a warp's vectors lie side by side
 constexpr int kSelSlots = kSelWarpVecs + 1;         // one more for rows off the 16-byte grid
-constexpr int kSelGroups = 10;  // groups of batches whose maxima are kept
-constexpr int kSelCap = 1024;  // listed columns per CTA
+constexpr int kSelGroups = 8;  // groups of batches whose maxima are kept
+constexpr int kSelCap = 512;  // listed columns per CTA
 constexpr int kSelOffers = 32;  // maxima a warp offers at most
 constexpr int kSelMaxCluster = 8;
 constexpr float kSelLowest = -3.402823466e38f;
@@ -88,20 +88,22 @@ struct SelBatch {
   }
   // sum of e^(x - ref), NaNs left out
   __device__ __forceinline__ double sum(float ref) const {
-    float part[NV * N / 8];
-#pragma unroll
-    for (int c = 0; c < NV * N / 8; ++c) {
-      float t = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float d = x[(c * 8 + j) / N].get((c * 8 + j) % N) - ref;
-        t += ex2(fmaf(d, kLog2eHi, d * kLog2eLo));
-      }
-      part[c] = t;
-    }
+    constexpr int CHAINS = NV * N / 16;  // of two sums of eight terms
+    const Two away = two(-ref, -ref), c_hi = two(kLog2eHi, kLog2eHi), c_lo = two(kLog2eLo, kLog2eLo);
     double s = 0.0;
 #pragma unroll
-    for (int c = 0; c < NV * N / 8; c += 2) s += static_cast<double>(part[c]) + static_cast<double>(part[c + 1]);
+    for (int c = 0; c < CHAINS; ++c) {
+      Two t = two(0.0f, 0.0f);
+#pragma unroll
+      for (int j = 0; j < 16; j += 2) {
+        const int i = c * 16 + j;
+        const Two d = add2(two(x[i / N].get(i % N), x[i / N].get(i % N + 1)), away);
+        const float2 e = parts_of(fma2(d, c_hi, mul2(d, c_lo)));
+        t = add2(t, two(ex2(e.x), ex2(e.y)));
+      }
+      const float2 p = parts_of(t);
+      s += static_cast<double>(p.x) + static_cast<double>(p.y);
+    }
     if (s != s) {  // rare: a NaN was met
       s = 0.0;
 #pragma unroll
@@ -134,7 +136,7 @@ __device__ __forceinline__ double sel_scaled(double s, float from, float m) {
 // SHIFT: a row need not begin on the 16-byte grid; a thread joins its vector from
 // two that its warp copied.
 template <class T, bool SHIFT>
-__global__ void __launch_bounds__(kSelThreads, 2) beam_rows_kernel(const BeamSelectArgs a) {
+__global__ void __launch_bounds__(kSelThreads, 4) beam_rows_kernel(const BeamSelectArgs a) {
   constexpr int N = Vec<T>::N, NT = kSelThreads, NV = kSelVecs, SLOTS = SHIFT ? kSelSlots : kSelWarpVecs;
   extern __shared__ __align__(16) uint4 ring[];  // [kSelStages][kSelWarps][SLOTS]
   __shared__ SelPart parts[kSelWarps];
@@ -317,12 +319,23 @@ __global__ void __launch_bounds__(kSelThreads, 2) beam_rows_kernel(const BeamSel
   const int busy = nbatch > 1 ? kSelWarps : max(1, min(kSelWarps, (v1 - v0 + nv * 32 - 1) / max(1, nv * 32)));
   const int q = nbatch > 1 ? (2 * top + kSelWarps - 1) / kSelWarps : min(kSelOffers, (2 * top + busy - 1) / busy);
   uint32_t o = mine;
-  for (int i = 0; i < q; ++i) {
-    const uint32_t w = __reduce_max_sync(0xffffffffu, o);
-    const unsigned at = __ballot_sync(0xffffffffu, o == w);
-    if (lane == __ffs(at) - 1) {
-      offer[warp * q + i] = w;
-      o = 0;
+  if (q > 6) {  // the warp's maxima sorted, the largest first
+#pragma unroll
+    for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+      for (int j = k >> 1; j > 0; j >>= 1) {
+        const uint32_t w = __shfl_xor_sync(0xffffffffu, o, j);
+        o = ((lane & j) == 0) == ((lane & k) == 0) ? max(o, w) : min(o, w);
+      }
+    if (lane < q) offer[warp * q + lane] = o;
+  } else {
+    for (int i = 0; i < q; ++i) {
+      const uint32_t w = __reduce_max_sync(0xffffffffu, o);
+      const unsigned at = __ballot_sync(0xffffffffu, o == w);
+      if (lane == __ffs(at) - 1) {
+        offer[warp * q + i] = w;
+        o = 0;
+      }
     }
   }
   __syncthreads();
