@@ -42,7 +42,7 @@ typedef struct {
   int layers, pages;  /* pages of each layer: one table for all layers */
   int heads, dim;     /* of keys and values; dim a multiple of 16 up to 128 */
   int page;           /* tokens of a page, a multiple of 16 up to 256 */
-  int rows, width;    /* width * page < 2^31; rows * width * page and pages * heads * page < 2^35 */
+  int rows, width;    /* width * page <= 2^30; rows * width * page, pages * heads * page < 2^35 */
   unsigned char* k;   /* [layers][pages][heads][page][dim] codes, 16-byte aligned */
   unsigned char* v;
   float* k_scale;     /* [layers][pages][heads][page / 16] */

@@ -63,7 +63,8 @@ BAD_CACHES = [
     (dict(pages=4194305), "pages"), (dict(heads=0), "heads"), (dict(heads=257), "heads"), (dict(dim=0), "dim"),
     (dict(dim=72), "dim"), (dict(dim=144), "dim"), (dict(page=0), "page"), (dict(page=24), "page"),
     (dict(page=272), "page"), (dict(rows=-1), "rows"), (dict(rows=4097), "rows"), (dict(width=0), "width"),
-    (dict(width=1 << 27), "width"),
+    (dict(width=(1 << 26) + 1), "width"), (dict(rows=4096, width=1 << 20), "rows * width"),
+    (dict(pages=4194304, heads=256, page=256), "pages * heads"),
 ]
 BAD_ARRAYS = [
     (dict(k=None), "k must not be NULL"), (dict(v=None), "v must not be NULL"), (dict(k_scale=None), "NULL"),
@@ -192,6 +193,8 @@ def test_nothing(lib):
     assert append(lib, tokens=0, k=None, v=None, start=None) == 0
     assert attend(lib, cache=none, q=None, out=None, ws=None) == 0
     refused(lib, append(lib, cache=none, tokens=4), "multiple of rows")
+    empty = dict(rows=0, table=None, lens=None)
+    assert lib.verbo_cache_free(made(**empty), None, None) == 0
 
 
 def test_python_refusals():

@@ -167,6 +167,18 @@ def test_any_sequence(seed, rows, beams, pages, page, dim, heads):
         check(c, m)
 
 
+def test_no_rows():
+    c = new(rows=0, pages=5)
+    start, status = c.reserve(i32([]))
+    assert start.numel() == 0 and status.tolist() == [0]
+    c.fork(i32([]).view(0, 2), 2)
+    c.free(i32([]))
+    c.append(0, torch.empty(0, 2, 32, device="cuda"), torch.empty(0, 2, 32, device="cuda"), i32([]))
+    assert c.attend(0, torch.empty(0, 4, 32, device="cuda")).shape == (0, 4, 32)
+    assert c.compact().tolist() == [0, 0]
+    vb.check()
+
+
 def test_the_largest_tables():
     """4096 rows, pages of several chunks, one page shared by all."""
     c = new(layers=1, pages=20000, heads=1, dim=16, rows=4096, width=4)

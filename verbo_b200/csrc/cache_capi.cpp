@@ -47,7 +47,7 @@ void check_sizes(const verbo_cache* c) {
   check_number(c->page, VERBO_CACHE_BLOCK, VERBO_CACHE_MAX_PAGE, "page");
   if (c->page % VERBO_CACHE_BLOCK) fail("page must be a multiple of 16");
   check_number(c->rows, 0, VERBO_CACHE_MAX_ROWS, "rows");
-  check_number(c->width, 1, INT_MAX / c->page, "width");
+  check_number(c->width, 1, (1 << 30) / c->page, "width");
   // blocks are counted in 32 bits: those of a layer, and those of all tables
   const long long per = c->page / VERBO_CACHE_BLOCK;
   if (static_cast<long long>(c->pages) * c->heads * per > INT_MAX)
@@ -72,7 +72,7 @@ CacheRanges check_cache(const verbo_cache* c) {
   check_sizes(c);
   const CacheRanges all = ranges(c);
   for (int i = 0; i < 7; ++i) {
-    if (!all.r[i].p) fail(std::string(all.r[i].what) + " must not be NULL");
+    if (!all.r[i].p && all.r[i].bytes > 0) fail(std::string(all.r[i].what) + " must not be NULL");
     check_aligned(all.r[i].p, i < 2 ? 16 : 4, all.r[i].what);
     for (int j = 0; j < i; ++j) check_apart(all.r[i], all.r[j]);
   }

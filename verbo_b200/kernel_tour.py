@@ -33,6 +33,15 @@ the rows of every sampling step are larger than the 126 MB L2:
   q4       verbo_ops_q4_matvec, 151936 x 896 at 1 and 64 fp32 rows (q4_kernel;
            q4_image_kernel, q4_tile_kernel)
 
+  beams    verbo_beam_select, 64 x 8 beams of 151936 with 16 taken, and
+           verbo_beam_reorder of a state (beam_rows_kernel, beam_join_kernel,
+           beam_reorder_kernel)
+  cache    verbo_cache_reserve, _append and _attend of one token for 32 rows of
+           4096 and for one row, _fork, _free and _compact (cache_scan_kernel,
+           cache_reserve_kernel, cache_copy_kernel, cache_append_kernel,
+           cache_attend_kernel, cache_attend_join_kernel, cache_fork_kernel,
+           cache_free_kernel, cache_moves_kernel)
+
 Between steps a one-element torch fill marks the boundary in a launch list,
 and every input is made before the first step, so the only other kernels in
 a capture are those markers (and the fill that creates the marker).  Each
@@ -92,6 +101,18 @@ def main() -> None:
     ncols = c5[0].vocab // 8
     cv = torch.empty(8, 512, 64, dtype=torch.float32, device=dev)
     ci = torch.empty(8, 512, 64, dtype=torch.int32, device=dev)
+    bx = rows_of("c2", 512)[1]
+    bs = torch.zeros(512, device=dev)
+    bstate = torch.zeros(512, 65536, dtype=torch.uint8, device=dev)
+    bp = torch.randint(0, 8, (64, 8), device=dev).int()
+    cache = vb.PagedCache.new(1, 2200, 8, 128, 32, 66, page=64)
+    kv = torch.randn(32 * 4096, 8, 128, device=dev).bfloat16()
+    qs = torch.randn(32, 32, 128, device=dev).bfloat16()
+    start, _ = cache.reserve(torch.full((32,), 4096, dtype=torch.int32, device=dev))
+    cache.append(0, kv, kv, start)
+    one = torch.ones(32, dtype=torch.int32, device=dev)
+    keep = torch.full((32,), 4000, dtype=torch.int32, device=dev)
+    single = vb.PagedCache(cache.k, cache.v, cache.k_scale, cache.v_scale, cache.table[:1], cache.lens[:1], cache.refs)
     torch.cuda.synchronize()
 
     def step(name, fn):
@@ -153,6 +174,13 @@ def main() -> None:
     step("logprobs", lambda: vb.token_logprobs(c3[1], lids, top=20))
     step("q4 matvec x1", lambda: layer.matvec(hid[:1]))
     step("q4 matvec x64", lambda: layer.matvec(hid[:64]))
+    step("beams", lambda: vb.beam_reorder(bstate, vb.beam_select(bx, bs, 8, 16)[1], 8))
+    step("cache reserve, append", lambda: cache.append(0, kv[:32], kv[:32], cache.reserve(one)[0]))
+    step("cache attend", lambda: cache.attend(0, qs))
+    step("cache attend 1", lambda: single.attend(0, qs[:1]))
+    step("cache fork", lambda: cache.fork(bp[:4], 8))
+    step("cache reserve (copies)", lambda: cache.reserve(one))
+    step("cache free, compact", lambda: (cache.free(keep), cache.compact()))
     layer.close()
     for t in heads.values():
         t.close()

@@ -1,4 +1,5 @@
-"""Request batching for a server, over the library's verbo_cuda_server_*.
+"""Request batching for a server, over the library's verbo_cuda_server_*, and beam
+search over a batch of requests, over verbo_beam_* (``BeamSearch``, at the end).
 
 The reference's server (cli/serve.cpp:139-218) runs one request at a time
 behind a global mutex (:168), each through verbo::generate
@@ -82,6 +83,123 @@ class BatchServer:
         return True
 
     def run(self) -> Dict[int, Request]:
+        while self.step():
+            pass
+        return self.done
+
+
+@dataclass
+class Hypothesis:
+    tokens: List[int]
+    score: float  # the summed log-probability, the stop token's with it
+    value: float  # what hypotheses are ordered by: score / tokens ** length_penalty
+    stopped: bool  # ended on a stop id (else at the token limit)
+
+
+class BeamSearch:
+    """Beam search of ``requests`` requests with ``beams`` beams each on one GPU.
+
+    ``model(tokens, out)`` fills ``out`` (CUDA float32 [requests * beams, vocab], row
+    r * beams + b is beam b of request r) with each row's next logits.  ``tokens`` is
+    None in the first step, in which all rows of a request hold its prompt, and after
+    that int32 [requests * beams], the token that each row has got.
+
+    A step takes 2 * beams continuations of each request (``beam_select``): those that
+    end on a stop id among the first ``beams`` of them are finished hypotheses, the
+    first ``beams`` of the others live on.  What the rows carry follows them:
+    ``cache`` (a ``PagedCache`` with a row per beam) forks, ``states`` (tensors with a
+    row per beam) are reordered in place.  A request ends when it has ``beams``
+    finished hypotheses and no live one can be better than the worst of them, or after
+    ``max_tokens`` tokens.  Only continuations cross to the host."""
+
+    def __init__(self, model: Callable, requests: int, beams: int, vocab: int, max_tokens: int,
+                 stop_ids: Sequence[int] = (), length_penalty: float = 1.0, cache=None, states: Sequence = (),
+                 device: int = 0):
+        import torch
+
+        if requests < 1 or max_tokens < 1:
+            raise ValueError("requests and max_tokens must be at least 1")
+        if not 1 <= beams <= 32:
+            raise ValueError("beams must be in [1, 32]")
+        if cache is not None and cache.rows != requests * beams:
+            raise ValueError("the cache must have a row per beam")
+        self.torch, self.model = torch, model
+        self.requests, self.beams, self.vocab, self.max_tokens = requests, beams, vocab, max_tokens
+        self.stop_ids, self.length_penalty = frozenset(int(i) for i in stop_ids), float(length_penalty)
+        self.cache, self.states = cache, list(states)
+        self.device = torch.device("cuda", device)
+        self.logits = torch.zeros((requests * beams, vocab), dtype=torch.float32, device=self.device)
+        self.steps = 0
+        self.beam_tokens: List[List[List[int]]] = [[[] for _ in range(beams)] for _ in range(requests)]
+        self.done: List[List[Hypothesis]] = [[] for _ in range(requests)]
+        self.open = [True] * requests
+        first = [0.0] + [float("-inf")] * (beams - 1)
+        self.scores = torch.tensor([first] * requests, dtype=torch.float32, device=self.device)
+        self.tokens = None
+
+    def _value(self, score: float, tokens: int) -> float:
+        return score / max(1, tokens) ** self.length_penalty
+
+    def _advance(self, scores, parents, tokens):
+        """The host's part of a step, from its continuations ([requests][2 * beams] lists):
+        the live beams' (scores, parents, tokens)."""
+        beams, n = self.beams, self.steps + 1
+        out_s, out_p, out_t = [], [], []
+        for r in range(self.requests):
+            live_s, live_p, live_t, kept = [], [], [], []
+            if self.open[r]:
+                for i, (s, p, t) in enumerate(zip(scores[r], parents[r], tokens[r])):
+                    if p < 0 or len(live_s) == beams:
+                        break
+                    if t in self.stop_ids:
+                        if i < beams:
+                            self.done[r].append(Hypothesis(self.beam_tokens[r][p], s, self._value(s, n), True))
+                        continue
+                    live_s.append(s)
+                    live_p.append(p)
+                    live_t.append(t)
+                    kept.append(self.beam_tokens[r][p] + [t])
+                if n == self.max_tokens:
+                    self.done[r] += [Hypothesis(k, s, self._value(s, n), False) for k, s in zip(kept, live_s)]
+                self.done[r] = sorted(self.done[r], key=lambda h: -h.value)[:beams]
+                # what the best beam can still reach: its score only falls, its length may grow to the limit
+                best = live_s[0] if live_s else float("-inf")
+                reach = self._value(best, self.max_tokens if self.length_penalty > 0 else n)
+                full = len(self.done[r]) == beams and self.done[r][-1].value >= reach
+                if n == self.max_tokens or not live_s or full:
+                    self.open[r] = False
+            if not self.open[r]:
+                live_s, live_p, live_t, kept = [], [], [], []
+            # beams without a continuation stay where they are, with no score
+            spare = beams - len(live_s)
+            self.beam_tokens[r] = kept + [[]] * spare
+            out_s.append(live_s + [float("-inf")] * spare)
+            out_p.append(live_p + [-1] * spare)
+            out_t.append(live_t + [0] * spare)
+        self.steps = n
+        return out_s, out_p, out_t
+
+    def step(self) -> bool:
+        """One token for every open request; False when none is left."""
+        import verbo_b200 as vb
+
+        if not any(self.open):
+            return False
+        torch = self.torch
+        self.model(self.tokens, self.logits)
+        found = vb.beam_select(self.logits, self.scores, self.beams, 2 * self.beams)
+        live = self._advance(*(f.tolist() for f in found))
+        self.scores = torch.tensor(live[0], dtype=torch.float32, device=self.device)
+        parents = torch.tensor(live[1], dtype=torch.int32, device=self.device)
+        self.tokens = torch.tensor(live[2], dtype=torch.int32, device=self.device).view(-1)
+        if self.cache is not None:
+            self.cache.fork(parents, self.beams)
+        if self.states:
+            vb.beam_reorder(self.states, parents, self.beams)
+        return any(self.open)
+
+    def run(self) -> List[List[Hypothesis]]:
+        """The requests' finished hypotheses, the best first."""
         while self.step():
             pass
         return self.done
