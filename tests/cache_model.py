@@ -122,10 +122,12 @@ class Model:
         live = int((self.refs > 0).sum())
         holes = [p for p in range(live) if self.refs[p] == 0]
         moved = [p for p in range(self.refs.size - 1, live - 1, -1) if self.refs[p] > 0]
+        to = np.arange(self.refs.size)
         for s, d in zip(moved, holes):
             self.move(s, d)
             self.refs[d], self.refs[s] = self.refs[s], 0
-            self.table[self.table == s] = d
+            to[s] = d
+        self.table = np.where(self.table >= 0, to[self.table], self.table).astype(np.int32)
         return live, len(moved)
 
     def append(self, layer, k, v, start, off):

@@ -125,15 +125,18 @@ def test_fork_and_free_of_single_rows():
         check(c, m)
 
 
-@pytest.mark.parametrize("live", [0, 1, 20, 39, 40])
-def test_compact(live):
-    c = new(pages=40, rows=5, width=8)
-    order = np.random.default_rng(live).permutation(40)[:live]
-    t = np.full((5, 8), -1, dtype=np.int32)
+@pytest.mark.parametrize("pages,live", [(40, 0), (40, 1), (40, 20), (40, 39), (40, 40), (16384, 9000), (16385, 3),
+                                        (16385, 16385), (33000, 12345)])
+def test_compact(pages, live):
+    """Pools that one CTA looks through, and larger ones."""
+    width = -(-pages // 5)
+    c = new(pages=pages, rows=5, width=width, layers=2 if pages < 100 else 1, heads=1, dim=16)
+    order = np.random.default_rng(live).permutation(pages)[:live]
+    t = np.full((5, width), -1, dtype=np.int32)
     t.reshape(-1)[:live] = order
     c.table.copy_(i32(t))
     c.lens.copy_(i32((t >= 0).sum(1) * 16))
-    c.refs.copy_(i32(np.bincount(order, minlength=40)))
+    c.refs.copy_(i32(np.bincount(order, minlength=pages)))
     m = model(c)
     info = c.compact()
     want = m.compact()
@@ -145,6 +148,7 @@ def test_compact(live):
 
 @pytest.mark.parametrize("seed,rows,beams,pages,page,dim,heads", [
     (0, 8, 4, 300, 16, 16, 1), (1, 12, 3, 90, 32, 48, 2), (2, 5, 5, 60, 256, 128, 1), (3, 64, 32, 5000, 16, 16, 1),
+    (4, 12, 4, 17000, 16, 16, 1),
 ])
 def test_any_sequence(seed, rows, beams, pages, page, dim, heads):
     rng = np.random.default_rng(seed)

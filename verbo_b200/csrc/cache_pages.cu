@@ -111,6 +111,29 @@ __device__ __forceinline__ int free_page(const PageWs& w, int chunks, const int*
   return w.list[static_cast<size_t>(lo) * kChunk + (i - pre[lo])];
 }
 
+// Pools of up to 16384 pages: the CTA that needs the list makes it, 16 pages to a
+// thread, which costs it less than another launch would.  `mask`: this thread's free
+// pages, `before`: those before them.  Returns their number.
+constexpr int kSmallPool = 16384;
+constexpr int kSmallThreads = 1024;
+constexpr int kSmallPer = kSmallPool / kSmallThreads;
+__device__ __forceinline__ int scan_pool(const verbo_cache& c, const PageWs& w, int* ws, unsigned* mask, int* before) {
+  const int first = threadIdx.x * kSmallPer;
+  unsigned m = 0;
+#pragma unroll
+  for (int i = 0; i < kSmallPer; ++i)
+    if (first + i < c.pages) m |= static_cast<unsigned>(c.refs[first + i] == 0) << i;
+  int total;
+  int at = block_excl_scan<int, kSmallThreads>(__popc(m), ws, &total);
+  *mask = m;
+  *before = at;
+#pragma unroll
+  for (int i = 0; i < kSmallPer; ++i)
+    if (m >> i & 1u) w.list[at++] = first + i;
+  __syncthreads();
+  return total;
+}
+
 // --------------------------------------------------------------- reserve --
 struct ReserveArgs {
   verbo_cache c;
@@ -126,8 +149,10 @@ constexpr int kReserveThreads = 1024;
 // i such rows, the row copies the page if r - i > 1.  Then pages are dealt out
 // through the scan of the needs, one thread to a page.  Latency alone counts: the
 // chain is lengths, tables, references, and the list of free pages.
+template <bool SMALL>
 __global__ void __launch_bounds__(kReserveThreads) cache_reserve_kernel(const ReserveArgs a) {
   constexpr int NT = kReserveThreads;
+  static_assert(NT == kSmallThreads, "one thread layout");
   extern __shared__ __align__(16) int smem[];  // last, len, more, first, copied [rows + 3 each], then pre [chunks + 1]
   __shared__ int ws[NT / 32];
   __shared__ long long wide_ws[NT / 32];
@@ -167,8 +192,10 @@ __global__ void __launch_bounds__(kReserveThreads) cache_reserve_kernel(const Re
     more[r] = m;
     copied[r] = shared;
   }
-  const int total_free = scan_counts<NT>(a.w, chunks, pre, ws);
-  // a row needs up to 2^27 pages: sums in 64 bits, the copies' in the upper half
+  unsigned mask;
+  int before_mine;
+  const int total_free = SMALL ? scan_pool(c, a.w, ws, &mask, &before_mine) : scan_counts<NT>(a.w, chunks, pre, ws);
+  // a row needs up to 2^26 pages: sums in 64 bits, the copies' in the upper half
   long long sum = 0;
   for (int r0 = 0; r0 < rows; r0 += NT) {
     const int r = r0 + tid;
@@ -219,7 +246,7 @@ __global__ void __launch_bounds__(kReserveThreads) cache_reserve_kernel(const Re
       else
         hi = mid - 1;
     }
-    const int to = free_page(a.w, chunks, pre, i);
+    const int to = SMALL ? a.w.list[i] : free_page(a.w, chunks, pre, i);
     const int k = i - first[lo] - (copied[lo] > 0);
     int at = pages_for(len[lo], page) + k;
     if (k < 0) {  // a copy of the row's last page
@@ -308,42 +335,47 @@ struct MovesArgs {
 // Where each page goes.  live = the pages in use; those at or above it move, the
 // highest into the lowest free page: the i-th from the end of all live pages is
 // taken by the i-th free one.
-__global__ void __launch_bounds__(kScanThreads) cache_moves_kernel(const MovesArgs a) {
-  constexpr int PER = kChunk / kScanThreads;
-  __shared__ int pre[kMaxChunks + 1];
-  __shared__ int ws[kScanThreads / 32];
+template <bool SMALL>
+__global__ void __launch_bounds__(SMALL ? kSmallThreads : kScanThreads) cache_moves_kernel(const MovesArgs a) {
+  constexpr int PER = SMALL ? kSmallPer : kChunk / kScanThreads;
+  __shared__ int pre[SMALL ? 1 : kMaxChunks + 1];
+  __shared__ int ws[32];
   const verbo_cache& c = a.c;
   grid_wait();
   grid_release();
   const int chunks = chunks_of(c);
-  const int live = c.pages - scan_counts<kScanThreads>(a.w, chunks, pre, ws);
-  const int first = blockIdx.x * kChunk + threadIdx.x * PER;
-  int free_[PER], n = 0;
+  const int first = (SMALL ? 0 : blockIdx.x * kChunk) + threadIdx.x * PER;
+  unsigned mask = 0;  // this thread's free pages
+  int live, before;   // free pages before the thread's next one
+  if constexpr (SMALL) {
+    live = c.pages - scan_pool(c, a.w, ws, &mask, &before);
+  } else {
+    live = c.pages - scan_counts<kScanThreads>(a.w, chunks, pre, ws);
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    free_[i] = first + i < c.pages && c.refs[first + i] == 0;
-    n += free_[i];
+    for (int i = 0; i < PER; ++i)
+      if (first + i < c.pages) mask |= static_cast<unsigned>(c.refs[first + i] == 0) << i;
+    int total;
+    before = pre[blockIdx.x] + block_excl_scan<int, kScanThreads>(__popc(mask), ws, &total);
   }
-  int total;
-  int before = pre[blockIdx.x] + block_excl_scan<int, kScanThreads>(n, ws, &total);  // free pages before this one
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int p = first + i;
     if (p >= c.pages) break;
+    const bool is_free = mask >> i & 1u;
     int to = p;
     if (p == live) {
       a.info[0] = live;
       a.info[1] = a.w.head[0] = before;
       a.w.head[1] = live;
     }
-    if (p >= live && !free_[i]) {
+    if (p >= live && !is_free) {
       const int from_end = live - 1 - (p - before);
-      to = free_page(a.w, chunks, pre, from_end);
+      to = SMALL ? a.w.list[from_end] : free_page(a.w, chunks, pre, from_end);
       a.w.src[from_end] = p;
       a.w.dst[from_end] = to;
     }
     a.w.map[p] = to;
-    before += free_[i];
+    before += is_free;
   }
   if (live == c.pages && blockIdx.x == 0 && threadIdx.x == 0) {
     a.info[0] = live;
@@ -641,15 +673,20 @@ size_t cache_workspace_bytes(const verbo_cache& c) {
 cudaError_t launch_cache_reserve(const verbo_cache& c, const int* add, int* start, int* status, void* ws,
                                  cudaStream_t s) {
   const PageWs w = layout(c, ws);
-  cudaError_t e = launch_chained(cache_scan_kernel, static_cast<unsigned>(chunks_of(c)), kScanThreads, 0, 1, s,
-                                 ScanArgs{c, w});
-  if (e != cudaSuccess) return e;
-  const size_t smem = (5 * ((static_cast<size_t>(c.rows) + 3) / 4 * 4) + chunks_of(c) + 1) * 4;
-  e = allow_smem<cache_reserve_kernel>((5 * VERBO_CACHE_MAX_ROWS + kMaxChunks + 1) * 4);
-  if (e != cudaSuccess) return e;
-  e = launch_chained(cache_reserve_kernel, 1u, kReserveThreads, smem, 1, s, ReserveArgs{c, w, add, start, status});
-  if (e != cudaSuccess) return e;
-  return launch_copy(c, w, false, s);
+  const ReserveArgs a{c, w, add, start, status};
+  const size_t rows = 5 * ((static_cast<size_t>(c.rows) + 3) / 4 * 4) * 4;
+  constexpr int most = (5 * VERBO_CACHE_MAX_ROWS + kMaxChunks + 1) * 4;
+  cudaError_t e;
+  if (c.pages <= kSmallPool) {
+    e = allow_smem<cache_reserve_kernel<true>>(most);
+    if (e == cudaSuccess) e = launch_chained(cache_reserve_kernel<true>, 1u, kReserveThreads, rows, 1, s, a);
+  } else {
+    e = launch_chained(cache_scan_kernel, static_cast<unsigned>(chunks_of(c)), kScanThreads, 0, 1, s, ScanArgs{c, w});
+    if (e == cudaSuccess) e = allow_smem<cache_reserve_kernel<false>>(most);
+    if (e == cudaSuccess)
+      e = launch_chained(cache_reserve_kernel<false>, 1u, kReserveThreads, rows + (chunks_of(c) + 1) * 4, 1, s, a);
+  }
+  return e == cudaSuccess ? launch_copy(c, w, false, s) : e;
 }
 
 cudaError_t launch_cache_fork(const verbo_cache& c, const int* parents, long long ld_parents, int beams,
@@ -668,13 +705,16 @@ cudaError_t launch_cache_free(const verbo_cache& c, const int* keep, cudaStream_
 
 cudaError_t launch_cache_compact(const verbo_cache& c, int* info, void* ws, cudaStream_t s) {
   const PageWs w = layout(c, ws);
-  cudaError_t e = launch_chained(cache_scan_kernel, static_cast<unsigned>(chunks_of(c)), kScanThreads, 0, 1, s,
-                                 ScanArgs{c, w});
-  if (e != cudaSuccess) return e;
-  e = launch_chained(cache_moves_kernel, static_cast<unsigned>(chunks_of(c)), kScanThreads, 0, 1, s,
-                     MovesArgs{c, w, info});
-  if (e != cudaSuccess) return e;
-  return launch_copy(c, w, true, s);
+  const MovesArgs a{c, w, info};
+  cudaError_t e;
+  if (c.pages <= kSmallPool) {
+    e = launch_chained(cache_moves_kernel<true>, 1u, kSmallThreads, 0, 1, s, a);
+  } else {
+    e = launch_chained(cache_scan_kernel, static_cast<unsigned>(chunks_of(c)), kScanThreads, 0, 1, s, ScanArgs{c, w});
+    if (e == cudaSuccess)
+      e = launch_chained(cache_moves_kernel<false>, static_cast<unsigned>(chunks_of(c)), kScanThreads, 0, 1, s, a);
+  }
+  return e == cudaSuccess ? launch_copy(c, w, true, s) : e;
 }
 
 cudaError_t launch_cache_append(const verbo_cache& c, int layer, const CacheNew& x, int dtype, cudaStream_t s) {
