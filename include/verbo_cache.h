@@ -116,7 +116,7 @@ VERBO_CUDA_API int verbo_cache_attend(const verbo_cache* c, int layer, const voi
                                       long long ld_out, long long hd_out, void* workspace, long long workspace_bytes,
                                       void* stream);
 /* Bytes of that call on the current device (0 for few rows and short tables), or -1. */
-VERBO_CUDA_API long long verbo_cache_attend_workspace(const verbo_cache* c, int heads, int steps);
+VERBO_CUDA_API long long verbo_cache_attend_workspace(const verbo_cache* c, int heads, int steps, int q_type);
 
 #ifdef __cplusplus
 }

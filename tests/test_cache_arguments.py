@@ -79,7 +79,7 @@ BAD_ARRAYS = [
 @pytest.mark.parametrize("kw,msg", BAD_CACHES)
 def test_sizes(lib, kw, msg):
     refused(lib, lib.verbo_cache_workspace(made(**kw)), msg)
-    refused(lib, lib.verbo_cache_attend_workspace(made(**kw), 2, 1), msg)
+    refused(lib, lib.verbo_cache_attend_workspace(made(**kw), 2, 1, F16), msg)
     refused(lib, lib.verbo_cache_free(made(**kw), 30 * M, None), msg)
 
 

@@ -44,7 +44,7 @@ def _cache():
             ("verbo_cache_compact", _I, [c, _P, _P, _L, _P]),
             ("verbo_cache_append", _I, [c, _I, _P, _L, _L, _P, _L, _L, _I, _I, _P, _P, _P]),
             ("verbo_cache_attend", _I, [c, _I, _P, _I, _L, _L, _I, _I, ctypes.c_float, _P, _I, _L, _L, _P, _L, _P]),
-            ("verbo_cache_attend_workspace", _L, [c, _I, _I]),
+            ("verbo_cache_attend_workspace", _L, [c, _I, _I, _I]),
         ):
             fn = getattr(lib, name)
             fn.restype, fn.argtypes = res, args
@@ -109,7 +109,7 @@ class PagedCache:
         self._need = lib.verbo_cache_workspace(ctypes.byref(c))
         if self._need < 0:
             raise _err()
-        self._attend_need = {}  # workspace bytes by (heads, steps)
+        self._attend_need = {}  # workspace bytes by (heads, steps, type)
 
     @classmethod
     def new(cls, layers, pages, heads, dim, rows, width, page=64, device=None):
@@ -263,13 +263,13 @@ class PagedCache:
             if on != n:
                 raise VerboCudaError("out must have the tokens of q")
         at = _stream_of(torch, self.k.get_device(), stream)
-        need = self._attend_need.get((heads, steps))
+        need = self._attend_need.get((heads, steps, code))
         if need is None:
             with torch.cuda.device(self.device):
-                need = self._lib.verbo_cache_attend_workspace(ctypes.byref(self._c), heads, steps)
+                need = self._lib.verbo_cache_attend_workspace(ctypes.byref(self._c), heads, steps, code)
             if need < 0:
                 raise _err()
-            self._attend_need[heads, steps] = need
+            self._attend_need[heads, steps, code] = need
         ws = _new(torch, q, stream, need, torch.uint8) if need else None
         self._run(self._lib.verbo_cache_attend, self._layer(layer), q.data_ptr(), code, ldq, hdq, heads, steps, scale,
                   out.data_ptr(), ocode, ldo, hdo, ws.data_ptr() if need else None, need, at)

@@ -41,7 +41,7 @@ struct CacheQuery {
   float scale;
   void* workspace;
 };
-size_t cache_attend_bytes(const verbo_cache& c, int heads, int steps);
+size_t cache_attend_bytes(const verbo_cache& c, int heads, int steps, int q_type);
 cudaError_t launch_cache_attend(const verbo_cache& c, int layer, const CacheQuery& x, int q_type, int out_type,
                                 cudaStream_t s);
 

@@ -10,12 +10,12 @@
 // and nothing but its own shared memory is waited for.  Where a (row, head) is
 // split over warps a second kernel joins their parts.
 //
-// A warp copies its blocks (cp.async, several ahead) and multiplies them on
-// mma.m16n8k16 with fp16 operands: codes are exact in fp16.  Of the 16 rows of A, 8
-// hold the queries rounded to fp16 and 8 what the rounding left, so that products are
-// exact to 2^-22 whatever the query's type at no extra instruction (8 rows are
-// enough for the heads that share a token); the weights e^(s - m) are split the same
-// way.  Sums on the tensor cores are cut, not rounded, so they are taken over to
+// A warp copies its blocks (cp.async, a step or two ahead) and multiplies them on
+// mma.m16n8k16 with fp16 operands: codes are exact in fp16.  Tokens, then dims, are the
+// 16 rows of a product and the queries its 8 columns: scores K q^T, sums V^T p^T, the
+// weights turned in between (movmatrix).  fp32 queries, and all weights e^(s - m), come
+// in two parts, rounded to fp16 and what the rounding left, so that products are exact
+// to 2^-22.  Sums on the tensor cores are cut, not rounded, so they are taken over to
 // fp32 registers every few blocks.
 #include <algorithm>
 #include <climits>
@@ -28,8 +28,6 @@
 namespace vb {
 namespace {
 
-constexpr int kAttWarps = 8;
-constexpr int kAttThreads = kAttWarps * 32;
 constexpr int kAttPair = 2;    // blocks of a step
 constexpr int kAttFlush = 4;   // steps between two transfers of the sums
 constexpr int kAttHeads = 64;  // blocks that are known ahead, per warp
@@ -90,10 +88,14 @@ __device__ __forceinline__ uint32_t two_halves(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-// What the rounding of two values to fp16 left, in fp16.
-__device__ __forceinline__ uint32_t two_rests(float lo, float hi, uint32_t rounded) {
-  const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&rounded));
-  return two_halves(lo - r.x, hi - r.y);
+__device__ __forceinline__ float2 of_halves(uint32_t h) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+// An 8 x 8 matrix of 16-bit numbers, two of a row in a lane, turned.
+__device__ __forceinline__ uint32_t turned(uint32_t a) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
 }
 __device__ __forceinline__ uint32_t codes_lo(uint32_t w) {  // codes 0, 1 of a word as fp16
   uint32_t h;
@@ -105,10 +107,11 @@ __device__ __forceinline__ uint32_t codes_hi(uint32_t w) {  // codes 2, 3
   asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %1;\n cvt.rn.f16x2.e4m3x2 %0, h;\n}" : "=r"(r) : "r"(w));
   return r;
 }
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void cp_async16_if(uint32_t dst, const void* src, bool take) {  // zeros otherwise
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
@@ -118,66 +121,71 @@ __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 
-// 16 elements from `p` on, as floats.
-__device__ __forceinline__ void load16(const void* p, long long i, int type, bool wide, float (&x)[16]) {
+// N elements from `p` + i on, as floats, and back; `wide`: p is aligned to 16 bytes, i
+// to N elements.
+template <int N>
+__device__ __forceinline__ void load_n(const void* p, long long i, int type, bool wide, float* x) {
   if (!wide) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) x[j] = load_any(p, i + j, type);
+    for (int j = 0; j < N; ++j) x[j] = load_any(p, i + j, type);
   } else if (type == kOpsF32) {
     const float4* v = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < N / 4; ++j) {
       const float4 y = v[j];
       x[4 * j] = y.x, x[4 * j + 1] = y.y, x[4 * j + 2] = y.z, x[4 * j + 3] = y.w;
     }
   } else {
     const uint4* v = reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(p) + i);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < N / 8; ++j) {
       const uint4 y = v[j];
       const uint32_t w[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        float2 f;
-        if (type == kOpsF16)
-          f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
-        else
-          f = make_float2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
+        const float2 f = type == kOpsF16
+                             ? of_halves(w[k])
+                             : make_float2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
         x[8 * j + 2 * k] = f.x, x[8 * j + 2 * k + 1] = f.y;
       }
     }
   }
 }
-__device__ __forceinline__ void store16(void* p, long long i, int type, bool wide, const float (&x)[16]) {
+template <int N>
+__device__ __forceinline__ void store_n(void* p, long long i, int type, bool wide, const float* x) {
   if (!wide) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) store_any(p, i + j, type, x[j]);
+    for (int j = 0; j < N; ++j) store_any(p, i + j, type, x[j]);
   } else if (type == kOpsF32) {
     float4* v = reinterpret_cast<float4*>(static_cast<float*>(p) + i);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
+    for (int j = 0; j < N / 4; ++j) v[j] = make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
   } else {
-    uint4* v = reinterpret_cast<uint4*>(static_cast<unsigned short*>(p) + i);
-    uint32_t w[8];
+    uint2* v = reinterpret_cast<uint2*>(static_cast<unsigned short*>(p) + i);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (type == kOpsF16) {
-        w[j] = two_halves(x[2 * j], x[2 * j + 1]);
-      } else {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
-        w[j] = *reinterpret_cast<const uint32_t*>(&h);
+    for (int j = 0; j < N / 4; ++j) {
+      uint32_t w[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float lo = x[4 * j + 2 * k], hi = x[4 * j + 2 * k + 1];
+        if (type == kOpsF16) {
+          w[k] = two_halves(lo, hi);
+        } else {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+          w[k] = *reinterpret_cast<const uint32_t*>(&h);
+        }
       }
+      v[j] = make_uint2(w[0], w[1]);
     }
-    v[0] = make_uint4(w[0], w[1], w[2], w[3]);
-    v[1] = make_uint4(w[4], w[5], w[6], w[7]);
   }
 }
 
 // Blocks of 16 tokens before each row, kAttStart more for each row that has any, in
 // shared memory (rows + 1), by the CTA.
+template <int NT>
 __device__ __forceinline__ void scan_rows(const AttendArgs& a, int* first, int* ws) {
   int base = 0;
-  for (int r0 = 0; r0 < a.rows; r0 += kAttThreads) {
+  for (int r0 = 0; r0 < a.rows; r0 += NT) {
     const int r = r0 + threadIdx.x;
     int n = 0;
     if (r < a.rows) {
@@ -185,7 +193,7 @@ __device__ __forceinline__ void scan_rows(const AttendArgs& a, int* first, int* 
       n = len > 0 ? (len - 1) / kCacheBlock + 1 + kAttStart : 0;
     }
     int total;
-    const int at = block_excl_scan<int, kAttThreads>(n, ws, &total);
+    const int at = block_excl_scan<int, NT>(n, ws, &total);
     if (r < a.rows) first[r] = base + at;
     base += total;
     __syncthreads();
@@ -202,57 +210,64 @@ struct __align__(16) BlockHead {
 };
 
 // DP: the head dimension filled up with zeros.  RT: eights of query rows of a tile.
-// Shared memory per warp: a ring of steps of two blocks' keys and values, rows of DP
+// Shared memory per warp: a ring of steps of two blocks' keys and values, rows of kRow
 // bytes whose 16-byte chunks are exchanged so that the fragment loads below meet no
-// bank twice; what is known of the blocks; the fragments of 16 queries.
+// bank twice, and what is known of the blocks.
+// Warps: as many as the registers allow, up to 168 a lane for 12 of them; a step of a warp
+// is a chain of loads, products and exponentials, which only other warps fill.
 template <int DP, int RT>
 struct AttShape {
-  static constexpr int kStages = RT == 1 ? 3 : 2;          // steps whose copies are in flight
-  static constexpr int kBlock = 16 * DP;                   // bytes of a block's keys, and of its values
-  static constexpr int kStep = kAttPair * 2 * kBlock;      // of a step
+  static constexpr int kWarps = 8;
+  static constexpr int kCtas = DP == 64 && RT == 1 ? 2 : 1;  // per SM
+  static constexpr int kStages = RT == 1 ? 3 : 2;            // steps whose copies are in flight
+  static constexpr int kRow = DP == 64 ? 64 : 128;
+  static constexpr int kBlock = 16 * kRow;             // bytes of a block's keys, and of its values
+  static constexpr int kStep = kAttPair * 2 * kBlock;  // of a step
   static constexpr int kRing = kStages * kStep;
   static constexpr int kKnown = kAttHeads * static_cast<int>(sizeof(BlockHead));
-  static constexpr int kQuery = RT == 1 ? 0 : DP / 16 * 2 * 512;
+  static constexpr int kQuery = RT == 1 ? 0 : DP / 16 * 512;  // fragments of 16 queries
   static constexpr int kWarp = kRing + kKnown + kQuery;
 };
 
-// CL: a cluster has one (row, head, tile), split evenly over its warps, and joins their
-// parts itself.
-template <int DP, int RT, bool CL>
-__global__ void __launch_bounds__(kAttThreads, DP == 64 && RT == 1 ? 2 : 1) cache_attend_kernel(const AttendArgs a) {
+// LO: queries in two parts (fp32).  CL: a cluster has one (row, head, tile), split evenly
+// over its warps, and joins their parts itself.
+template <int DP, int RT, bool LO, bool CL>
+__global__ void __launch_bounds__(AttShape<DP, RT>::kWarps * 32, AttShape<DP, RT>::kCtas)
+    cache_attend_kernel(const AttendArgs a) {
   using S = AttShape<DP, RT>;
-  constexpr int NJ = DP / 8;   // output tiles of 8 dims
+  constexpr int NW = S::kWarps, NT = NW * 32;
+  constexpr int MT = DP / 16;  // products of 16 dims
   constexpr int KS = DP / 16;  // steps of 16 dims
   constexpr int CH = DP / 32;  // chunks that a lane copies of a block's keys
-  constexpr int OWN = DP / 4;  // output dims of a lane
+  constexpr int VW = DP / 32;  // words of a token's values in a lane
   constexpr int ROWS = 8 * RT;
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ int scan_ws[kAttWarps];
-  __shared__ float4 joined[CL ? kAttWarps : 1][DP / 4];
-  __shared__ float2 joined_ml[CL ? kAttWarps : 1];
+  __shared__ int scan_ws[NW];
+  __shared__ float4 joined[CL ? NW : 1][VERBO_CACHE_MAX_DIM / 4];
+  __shared__ float2 joined_ml[CL ? NW : 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
   unsigned char* ring = smem + warp * S::kWarp;
   BlockHead* known = reinterpret_cast<BlockHead*>(ring + S::kRing);
-  uint4* query = reinterpret_cast<uint4*>(ring + S::kRing + S::kKnown) + lane;  // [KS][rounded, rests][32]
-  int* first = reinterpret_cast<int*>(smem + kAttWarps * S::kWarp);
+  uint4* query = reinterpret_cast<uint4*>(ring + S::kRing + S::kKnown) + lane;  // [KS][32], a lane's own
+  int* first = reinterpret_cast<int*>(smem + NW * S::kWarp);
   if (a.dim < DP)  // the filled-up dims stay zero
     for (int i = lane; i < S::kRing / 16; i += 32) reinterpret_cast<uint4*>(ring)[i] = make_uint4(0, 0, 0, 0);
   grid_wait();
   grid_release();
   int team = 0, tile, row = 0, head = 0;
-  long long i0 = 0, i1 = 1, each = 0;
+  long long i0 = 0, i1 = 1;
   if (CL) {
     const int unit = blockIdx.x / a.members;
     tile = unit % a.tiles;
     head = unit / a.tiles % a.heads;
     row = unit / a.tiles / a.heads;
   } else {
-    scan_rows(a, first, scan_ws);
+    scan_rows<NT>(a, first, scan_ws);
     if (blockIdx.x == 0)
-      for (int r = tid; r <= a.rows; r += kAttThreads) a.first[r] = first[r];
+      for (int r = tid; r <= a.rows; r += NT) a.first[r] = first[r];
     const long long all = static_cast<long long>(first[a.rows]) * a.heads;
-    each = blocks_each(a, all);
+    const long long each = blocks_each(a, all);
     const int id = warp * gridDim.x + blockIdx.x;  // few blocks go to as many SMs as there are
     team = id / a.tiles;
     tile = id - team * a.tiles;
@@ -271,7 +286,7 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 && RT == 1 ? 2 : 1) cach
     const int c = lane + 32 * i;
     const int tok = c / per_token, col = c - tok * per_token;
     token_of[i] = c < a.dim ? tok : 64;
-    if (DP == 128) {
+    if (S::kRow == 128) {
       to_k[i] = tok * 128 + ((col ^ ((tok & 1) << 2)) << 4);
       to_v[i] = tok * 128 + ((col ^ (((tok >> 1) & 3) << 1)) << 4);
     } else {
@@ -283,18 +298,27 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 && RT == 1 ? 2 : 1) cach
   }
   const uint32_t ring_at = smem_u32(ring);
   const long long block_bytes = 16ll * a.dim;
-  // and where it reads fragments: keys of token g (and g + 8), values of tokens 2 t, 2 t + 1 (and + 8)
-  uint32_t at_k0, at_k1, at_v0, at_v1;
-  if (DP == 128) {
-    const int flip = (g & 1) << 2;
-    at_k0 = g * 128 + ((t ^ flip) << 4);
-    at_k1 = g * 128 + (((t + 4) ^ flip) << 4);
-    at_v0 = S::kBlock + 2 * t * 128 + ((g ^ (t << 1)) << 4);
-    at_v1 = at_v0 + 128;
-  } else {
-    at_k0 = at_k1 = g * 64 + (t << 4);
+  // and where it reads fragments: of the keys of token g (and g + 8) the dims 16 t ... and
+  // 64 + (DP - 64) / 4 t ...; of the values of tokens 2 t (v0) and 2 t + 1 (v1) (and + 8) the
+  // dims of `v_first` and `v_second` below
+  uint32_t at_k0, at_k1 = 0, at_v0, at_v1, at_v2 = 0, at_v3 = 0;
+  if (DP == 64) {
+    at_k0 = g * 64 + (t << 4);
     at_v0 = S::kBlock + t * 128 + (((g >> 1) ^ (t << 1)) << 4) + (g & 1) * 8;
     at_v1 = S::kBlock + t * 128 + (((4 | (g >> 1)) ^ (t << 1)) << 4) + (g & 1) * 8;
+  } else {
+    const int flip = (g & 1) << 2;
+    at_k0 = g * 128 + ((t ^ flip) << 4);
+    if (DP == 128) {
+      at_k1 = g * 128 + (((t + 4) ^ flip) << 4);
+      at_v0 = S::kBlock + 2 * t * 128 + ((g ^ (t << 1)) << 4);
+    } else {
+      at_k1 = g * 128 + (((4 + (t >> 1)) ^ flip) << 4) + (t & 1) * 8;
+      at_v0 = S::kBlock + 2 * t * 128 + (((g >> 1) ^ (t << 1)) << 4) + (g & 1) * 8;
+      at_v2 = S::kBlock + 2 * t * 128 + (((4 + (g >> 2)) ^ (t << 1)) << 4) + (g & 3) * 4;
+      at_v3 = at_v2 + 128;
+    }
+    at_v1 = at_v0 + 128;
   }
 
   if (!CL) {
@@ -314,8 +338,8 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 && RT == 1 ? 2 : 1) cach
     int nb, b0, n;
     if (CL) {
       nb = (max(0, min(a.lens[row], a.width * a.page)) + kCacheBlock - 1) / kCacheBlock;
-      const int all = (nb + 1) / 2, warps = a.members * kAttWarps;
-      const int w = blockIdx.x % a.members * kAttWarps + warp;
+      const int all = (nb + 1) / 2, warps = a.members * NW;
+      const int w = blockIdx.x % a.members * NW + warp;
       b0 = 2 * (all * w / warps);
       n = max(0, min(nb, 2 * (all * (w + 1) / warps)) - b0);
       i0 = i1;
@@ -384,10 +408,10 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 && RT == 1 ? 2 : 1) cach
 #pragma unroll
     for (int j = 0; j < S::kStages - 1; ++j) fetch(j);
 
-    // ---- the queries of this lane's rows, g (and g + 8) of the tile, its own dims
-    uint32_t qa[RT == 1 ? KS : 1][4];
-    float c_hi[RT], c_lo[RT];  // the rows' factors
-    int end[RT];               // places that a row sees
+    // ---- the queries: this lane has column g (of each eight), the dims of its keys
+    uint32_t qh[RT == 1 ? KS : 1][2], ql[LO ? KS : 1][2];
+    Two c_hi[RT], c_lo[RT];  // factors of the rows 2 t and 2 t + 1
+    int end[RT][2];          // places that they see
 #pragma unroll
     for (int u = 0; u < RT; ++u) {
       const int r = tile * ROWS + 8 * u + g;  // step r / group, head r % group
@@ -395,25 +419,17 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 && RT == 1 ? 2 : 1) cach
       const int step = live ? r / a.group : 0;
       const long long q_at = (static_cast<long long>(row) * a.steps + step) * a.ld_q +
                              static_cast<long long>(head * a.group + (live ? r - step * a.group : 0)) * a.hd_q;
-      end[u] = len - (a.steps - 1 - step);
-      float x[OWN];
+      float x[4 * KS];
+#pragma unroll
+      for (int i = 0; i < 4 * KS; ++i) x[i] = 0.0f;
+      if (live && 16 * t < a.dim) load_n<16>(a.q, q_at + 16 * t, a.q_type, a.wide_q, x);
+      if constexpr (DP > 64) {
+        constexpr int N = (DP - 64) / 4;
+        if (live && 64 + N * t < a.dim) load_n<N>(a.q, q_at + 64 + N * t, a.q_type, a.wide_q, x + 16);
+      }
       float most = 0.0f;
 #pragma unroll
-      for (int i = 0; i < OWN / 16; ++i) {
-        const int d = i * 64 + t * 16;
-        float y[16];
-        if (live && d < a.dim) {
-          load16(a.q, q_at + d, a.q_type, a.wide_q, y);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 16; ++k) y[k] = 0.0f;
-        }
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          x[16 * i + k] = y[k];
-          most = fmaxf(most, fabsf(y[k]));
-        }
-      }
+      for (int i = 0; i < 4 * KS; ++i) most = fmaxf(most, fabsf(x[i]));
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
       // the row times 2^e has its largest element in [2^14, 2^15)
@@ -422,49 +438,54 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 && RT == 1 ? 2 : 1) cach
       e = min(e, 126);
       const float up = __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
       const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-      c_hi[u] = a.c_hi * down;
-      c_lo[u] = a.c_lo * down;
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const float* y = x + 4 * s;
-        const uint32_t h0 = two_halves(y[0] * up, y[1] * up), h1 = two_halves(y[2] * up, y[3] * up);
-        const uint32_t r0 = two_rests(y[0] * up, y[1] * up, h0), r1 = two_rests(y[2] * up, y[3] * up, h1);
-        if (RT == 1) {
-          qa[s][0] = h0, qa[s][1] = r0, qa[s][2] = h1, qa[s][3] = r1;
-        } else {
-          uint32_t* to = reinterpret_cast<uint32_t*>(query + s * 64) + u;
-          to[0] = h0, to[2] = h1, to[128] = r0, to[130] = r1;
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float y = x[4 * s + 2 * k] * up, z = x[4 * s + 2 * k + 1] * up;
+          const uint32_t hi = two_halves(y, z);
+          if (RT == 1)
+            qh[RT == 1 ? s : 0][k] = hi;
+          else
+            reinterpret_cast<uint32_t*>(query + s * 32)[2 * u + k] = hi;
+          if (LO) {
+            const float2 back = of_halves(hi);
+            ql[LO ? s : 0][k] = two_halves(y - back.x, z - back.y);
+          }
         }
-      }
+      const int sees = len - (a.steps - 1 - step);
+      const float d0 = __shfl_sync(0xffffffffu, down, 8 * t), d1 = __shfl_sync(0xffffffffu, down, 8 * t + 4);
+      end[u][0] = __shfl_sync(0xffffffffu, sees, 8 * t);
+      end[u][1] = __shfl_sync(0xffffffffu, sees, 8 * t + 4);
+      c_hi[u] = two(a.c_hi * d0, a.c_hi * d1);
+      c_lo[u] = two(a.c_lo * d0, a.c_lo * d1);
     }
     const int all_see = len - (a.steps - 1);  // places that every row sees
 
-    // RT == 1: rows of acc are the row's two parts, added in sum; else two rows
-    float acc[NJ][4], sum[NJ][2 * RT];
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 2 * RT; ++i) sum[j][i] = 0.0f;
-    }
-    float m[RT], l[RT], vref = 0.0f, vinv = 0.0f;
+    // products: [even, odd dim] x [row 2 t, row 2 t + 1]
+    float acc[MT][RT][4];
+    Two sum[MT][RT][2];
+    float m[RT][2], vref = 0.0f, vinv = 0.0f;
+    Two l[RT];
 #pragma unroll
     for (int u = 0; u < RT; ++u) {
-      m[u] = kNegInf;
-      l[u] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        acc[i][u][0] = acc[i][u][1] = acc[i][u][2] = acc[i][u][3] = 0.0f;
+        sum[i][u][0] = sum[i][u][1] = two(0.0f, 0.0f);
+      }
+      m[u][0] = m[u][1] = kNegInf;
+      l[u] = two(0.0f, 0.0f);
     }
     auto flush = [&]() {
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        if (RT == 1) {
-          sum[j][0] += acc[j][0] + acc[j][2];
-          sum[j][1] += acc[j][1] + acc[j][3];
-        } else {
+      for (int i = 0; i < MT; ++i)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sum[j][i % (2 * RT)] += acc[j][i];
+        for (int u = 0; u < RT; ++u) {
+          sum[i][u][0] = add2(sum[i][u][0], two(acc[i][u][0], acc[i][u][1]));
+          sum[i][u][1] = add2(sum[i][u][1], two(acc[i][u][2], acc[i][u][3]));
+          acc[i][u][0] = acc[i][u][1] = acc[i][u][2] = acc[i][u][3] = 0.0f;
         }
-        acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
-      }
     };
 
     int slot = 0;
@@ -476,152 +497,169 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 && RT == 1 ? 2 : 1) cach
       slot = slot == S::kStages - 1 ? 0 : slot + 1;
       BlockHead h[kAttPair];
 #pragma unroll
-      for (int u = 0; u < kAttPair; ++u) h[u] = known[(2 * j + u) & (kAttHeads - 1)];
+      for (int b = 0; b < kAttPair; ++b) h[b] = known[(2 * j + b) & (kAttHeads - 1)];
 
-      // scores: tokens 8 i + g are the columns, this lane has columns 2 t and 2 t + 1
-      float p[2 * kAttPair][2 * RT];
-      {
-        float sc[2 * kAttPair][4];
-        uint32_t w[2 * kAttPair][KS];
+      // scores of the tokens g (0) and g + 8 (1) of each block for the rows 2 t and 2 t + 1
+      Two p[kAttPair][RT][2];
 #pragma unroll
-        for (int i = 0; i < 2 * kAttPair; ++i) {
-          sc[i][0] = sc[i][1] = sc[i][2] = sc[i][3] = 0.0f;
-          const unsigned char* kt = at + (i >> 1) * 2 * S::kBlock + (i & 1) * 8 * DP;
+      for (int b = 0; b < kAttPair; ++b) {
+        uint32_t w[2][KS];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const unsigned char* kt = at + b * 2 * S::kBlock + i * 8 * S::kRow;
           const uint4 x = *reinterpret_cast<const uint4*>(kt + at_k0);
           w[i][0] = x.x, w[i][1] = x.y, w[i][2] = x.z, w[i][3] = x.w;
-          if (DP == 128) {
+          if constexpr (DP == 128) {
             const uint4 y = *reinterpret_cast<const uint4*>(kt + at_k1);
-            w[i][KS - 4] = y.x, w[i][KS - 3] = y.y, w[i][KS - 2] = y.z, w[i][KS - 1] = y.w;
-          }
-          if (RT == 1) {
-#pragma unroll
-            for (int s = 0; s < KS; ++s) mma16816(sc[i], qa[s], codes_lo(w[i][s]), codes_hi(w[i][s]));
-          }
-        }
-        if (RT == 2) {
-#pragma unroll
-          for (int s = 0; s < KS; ++s) {
-            const uint4 x = query[s * 64], y = query[s * 64 + 32];
-            const uint32_t hi[4] = {x.x, x.y, x.z, x.w}, lo[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-            for (int i = 0; i < 2 * kAttPair; ++i) {
-              const uint32_t k0 = codes_lo(w[i][s]), k1 = codes_hi(w[i][s]);
-              mma16816(sc[i], hi, k0, k1);
-              mma16816(sc[i], lo, k0, k1);
-            }
+            w[i][4] = y.x, w[i][5] = y.y, w[i][6] = y.z, w[i][7] = y.w;
+          } else if constexpr (DP == 96) {
+            const uint2 y = *reinterpret_cast<const uint2*>(kt + at_k1);
+            w[i][4] = y.x, w[i][5] = y.y;
           }
         }
+        float sc[RT][2][4];  // two chains each
 #pragma unroll
-        for (int i = 0; i < 2 * kAttPair; ++i)
+        for (int u = 0; u < RT; ++u)
 #pragma unroll
-          for (int u = 0; u < RT; ++u) {
-            const float f_hi = c_hi[u] * h[i >> 1].ks, f_lo = c_lo[u] * h[i >> 1].ks;
+          for (int k = 0; k < 2; ++k) sc[u][k][0] = sc[u][k][1] = sc[u][k][2] = sc[u][k][3] = 0.0f;
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const float x = RT == 1 ? sc[i][k] + sc[i][k + 2] : sc[i][2 * u + k];
-              p[i][2 * u + k] = fmaf(x, f_hi, x * f_lo);
-            }
+        for (int s = 0; s < KS; ++s) {
+          const uint32_t a0 = codes_lo(w[0][s]), a1 = codes_lo(w[1][s]), a2 = codes_hi(w[0][s]), a3 = codes_hi(w[1][s]);
+          if constexpr (RT == 1) {
+            mma16816(sc[0][s & 1], a0, a1, a2, a3, qh[s][0], qh[s][1]);
+            if (LO) mma16816(sc[0][s & 1], a0, a1, a2, a3, ql[LO ? s : 0][0], ql[LO ? s : 0][1]);
+          } else {
+            const uint4 q = query[s * 32];
+            mma16816(sc[0][s & 1], a0, a1, a2, a3, q.x, q.y);
+            mma16816(sc[RT - 1][s & 1], a0, a1, a2, a3, q.z, q.w);
           }
+        }
+        const Two ks = two(h[b].ks, h[b].ks);
+#pragma unroll
+        for (int u = 0; u < RT; ++u) {
+          const Two f_hi = mul2(c_hi[u], ks), f_lo = mul2(c_lo[u], ks);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const Two x = add2(two(sc[u][0][2 * i], sc[u][0][2 * i + 1]), two(sc[u][1][2 * i], sc[u][1][2 * i + 1]));
+            p[b][u][i] = fma2(x, f_hi, mul2(x, f_lo));
+          }
+        }
       }
       const int place = (b0 + 2 * j) * kCacheBlock;
       if (h[0].valid + h[1].valid < 2 * kCacheBlock || place + 2 * kCacheBlock > all_see) {
 #pragma unroll
-        for (int i = 0; i < 2 * kAttPair; ++i)
+        for (int b = 0; b < kAttPair; ++b)
 #pragma unroll
           for (int u = 0; u < RT; ++u) {
-            const int lim = min(h[i >> 1].valid, end[u] - place - (i >> 1) * kCacheBlock);
+            const int at0 = g + place + b * kCacheBlock, valid = h[b].valid - g;
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
-              if (8 * (i & 1) + 2 * t + k >= lim) p[i][2 * u + k] = kNegInf;
+            for (int i = 0; i < 2; ++i) {
+              const float2 x = parts_of(p[b][u][i]);
+              const bool there = 8 * i < valid;
+              p[b][u][i] = two(there && at0 + 8 * i < end[u][0] ? x.x : kNegInf,
+                               there && at0 + 8 * i < end[u][1] ? x.y : kNegInf);
+            }
           }
       }
-      float mx[RT];
+      float mx[RT][2];
       bool grows = false;
 #pragma unroll
       for (int u = 0; u < RT; ++u) {
-        mx[u] = kNegInf;
+        const float2 x = parts_of(p[0][u][0]), y = parts_of(p[0][u][1]);
+        const float2 z = parts_of(p[1][u][0]), w = parts_of(p[1][u][1]);
+        mx[u][0] = fmaxf(fmaxf(x.x, y.x), fmaxf(z.x, w.x));
+        mx[u][1] = fmaxf(fmaxf(x.y, y.y), fmaxf(z.y, w.y));
 #pragma unroll
-        for (int i = 0; i < 2 * kAttPair; ++i) mx[u] = fmaxf(mx[u], fmaxf(p[i][2 * u], p[i][2 * u + 1]));
-        mx[u] = fmaxf(mx[u], __shfl_xor_sync(0xffffffffu, mx[u], 1));
-        mx[u] = fmaxf(mx[u], __shfl_xor_sync(0xffffffffu, mx[u], 2));
-        grows |= mx[u] > m[u];
+        for (int o = 4; o < 32; o <<= 1) {
+          mx[u][0] = fmaxf(mx[u][0], __shfl_xor_sync(0xffffffffu, mx[u][0], o));
+          mx[u][1] = fmaxf(mx[u][1], __shfl_xor_sync(0xffffffffu, mx[u][1], o));
+        }
+        grows |= mx[u][0] > m[u][0] || mx[u][1] > m[u][1];
       }
       const float vmax = fmaxf(fabsf(h[0].vs), fabsf(h[1].vs));  // 0 where there is no page
       if (__any_sync(0xffffffffu, grows || vmax > vref)) {
         const float vn = fmaxf(vref, vmax);
         const float less = vn > vref ? __fdiv_rn(vref, vn) : 1.0f;
-        float both[RT];
 #pragma unroll
         for (int u = 0; u < RT; ++u) {
-          const float mn = fmaxf(m[u], mx[u]);
-          const float alpha = m[u] > kNegInf ? ex2(m[u] - mn) : 0.0f;
-          both[u] = alpha * less;
-          l[u] *= alpha;
-          m[u] = mn;
-        }
+          float alpha[2];
 #pragma unroll
-        for (int i = 0; i < NJ; ++i) {
+          for (int k = 0; k < 2; ++k) {
+            const float mn = fmaxf(m[u][k], mx[u][k]);
+            alpha[k] = m[u][k] > kNegInf ? ex2(m[u][k] - mn) : 0.0f;
+            m[u][k] = mn;
+          }
+          l[u] = mul2(l[u], two(alpha[0], alpha[1]));
+          const float f0 = alpha[0] * less, f1 = alpha[1] * less;
+          const Two both = two(f0, f1);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) acc[i][k] *= both[RT == 1 ? 0 : k >> 1];
-#pragma unroll
-          for (int k = 0; k < 2 * RT; ++k) sum[i][k] *= both[k >> 1];
+          for (int i = 0; i < MT; ++i) {
+            acc[i][u][0] *= f0, acc[i][u][1] *= f1, acc[i][u][2] *= f0, acc[i][u][3] *= f1;
+            sum[i][u][0] = mul2(sum[i][u][0], both);
+            sum[i][u][1] = mul2(sum[i][u][1], both);
+          }
         }
         if (vn > vref) vinv = __fdiv_rn(1.0f, vn);
         vref = vn;
       }
 #pragma unroll
       for (int u = 0; u < RT; ++u) {
-        const float base = m[u] > kNegInf ? m[u] - kUp : 0.0f;
+        const Two base = two(m[u][0] > kNegInf ? kUp - m[u][0] : 0.0f, m[u][1] > kNegInf ? kUp - m[u][1] : 0.0f);
 #pragma unroll
-        for (int i = 0; i < 2 * kAttPair; ++i)
+        for (int b = 0; b < kAttPair; ++b)
 #pragma unroll
-          for (int k = 2 * u; k < 2 * u + 2; ++k) p[i][k] = ex2(p[i][k] - base);
-        l[u] += ((p[0][2 * u] + p[0][2 * u + 1]) + (p[1][2 * u] + p[1][2 * u + 1])) +
-                ((p[2][2 * u] + p[2][2 * u + 1]) + (p[3][2 * u] + p[3][2 * u + 1]));
+          for (int i = 0; i < 2; ++i) {
+            const float2 x = parts_of(add2(p[b][u][i], base));
+            p[b][u][i] = two(ex2(x.x), ex2(x.y));
+          }
+        l[u] = add2(l[u], add2(add2(p[0][u][0], p[0][u][1]), add2(p[1][u][0], p[1][u][1])));
       }
 
 #pragma unroll
-      for (int u = 0; u < kAttPair; ++u) {
-        const float ratio = h[u].vs * vinv;
-        uint32_t pa[RT][4];  // RT == 1: rounded and rest in one; else the rounded, then the rests
+      for (int b = 0; b < kAttPair; ++b) {
+        const float share = h[b].vs * vinv;
+        const Two ratio = two(share, share), minus = two(-1.0f, -1.0f);
+        uint32_t ph[RT][2], pl[RT][2];  // rounded, and what that left: of row g, tokens 2 t, 2 t + 1 (and + 8)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int u = 0; u < RT; ++u)
 #pragma unroll
-          for (int r = 0; r < RT; ++r) {
-            const float x = p[2 * u + i][2 * r] * ratio, y = p[2 * u + i][2 * r + 1] * ratio;
-            const uint32_t hi = two_halves(x, y), lo = two_rests(x, y, hi);
-            if (RT == 1) {
-              pa[0][2 * i] = hi, pa[0][2 * i + 1] = lo;
-            } else {
-              pa[0][2 * i + r] = hi, pa[RT - 1][2 * i + r] = lo;
-            }
+          for (int i = 0; i < 2; ++i) {
+            const Two x = mul2(p[b][u][i], ratio);
+            const float2 y = parts_of(x);
+            const uint32_t hi = two_halves(y.x, y.y);
+            const float2 back = of_halves(hi);
+            const float2 rest = parts_of(fma2(two(back.x, back.y), minus, x));
+            ph[u][i] = turned(hi);
+            pl[u][i] = turned(two_halves(rest.x, rest.y));
           }
-        // values: this lane has tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9 at the dims g DP / 8 ...
-        constexpr int W = DP / 32;  // words of a token
-        uint32_t v[4][W];
+        // values: this lane has tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+        uint32_t v[4][VW];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const unsigned char* vt = at + u * 2 * S::kBlock + (i >> 1) * 8 * DP + (i & 1 ? at_v1 : at_v0);
-          if (DP == 128) {
-            const uint4 x = *reinterpret_cast<const uint4*>(vt);
-            v[i][0] = x.x, v[i][1] = x.y, v[i][W - 2] = x.z, v[i][W - 1] = x.w;
+          const unsigned char* vt = at + b * 2 * S::kBlock + (i >> 1) * 8 * S::kRow;
+          if constexpr (DP == 128) {
+            const uint4 x = *reinterpret_cast<const uint4*>(vt + (i & 1 ? at_v1 : at_v0));
+            v[i][0] = x.x, v[i][1] = x.y, v[i][2] = x.z, v[i][3] = x.w;
           } else {
-            const uint2 x = *reinterpret_cast<const uint2*>(vt);
+            const uint2 x = *reinterpret_cast<const uint2*>(vt + (i & 1 ? at_v1 : at_v0));
             v[i][0] = x.x, v[i][1] = x.y;
+            if constexpr (DP == 96) v[i][2] = *reinterpret_cast<const uint32_t*>(vt + (i & 1 ? at_v3 : at_v2));
           }
         }
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
+        for (int w = 0; w < VW; ++w) {
           const uint32_t a0 = __byte_perm(v[0][w], v[1][w], 0x5140), a1 = __byte_perm(v[0][w], v[1][w], 0x7362);
           const uint32_t e0 = __byte_perm(v[2][w], v[3][w], 0x5140), e1 = __byte_perm(v[2][w], v[3][w], 0x7362);
-          const uint32_t b[4][2] = {{codes_lo(a0), codes_lo(e0)},
-                                    {codes_hi(a0), codes_hi(e0)},
-                                    {codes_lo(a1), codes_lo(e1)},
-                                    {codes_hi(a1), codes_hi(e1)}};
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t x = i ? a1 : a0, y = i ? e1 : e0;
+            const uint32_t c0 = codes_lo(x), c1 = codes_hi(x), c2 = codes_lo(y), c3 = codes_hi(y);
 #pragma unroll
-            for (int r = 0; r < RT; ++r) mma16816(acc[4 * w + i], pa[r], b[i][0], b[i][1]);
+            for (int u = 0; u < RT; ++u) {
+              mma16816(acc[2 * w + i][u], c0, c1, c2, c3, ph[u][0], ph[u][1]);
+              mma16816(acc[2 * w + i][u], c0, c1, c2, c3, pl[u][0], pl[u][1]);
+            }
+          }
         }
       }
       if ((j & (kAttFlush - 1)) == kAttFlush - 1) flush();
@@ -630,7 +668,9 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 && RT == 1 ? 2 : 1) cach
     cp_async_wait_all();
     flush();
 
-    // this lane's dims: OWN t + i, from the tiles i % NJ and the columns 2 t, 2 t + 1
+    // this lane's dims of the rows 2 t and 2 t + 1: 4 w + i of word w
+    constexpr int N1 = DP == 128 ? 16 : 8, N2 = DP == 96 ? 4 : 0;
+    const int d1 = N1 * g, d2 = 64 + 4 * g;
     const bool whole = !CL && n == nb;
     float* to = nullptr;
     if (CL) {
@@ -641,29 +681,43 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 && RT == 1 ? 2 : 1) cach
     }
 #pragma unroll
     for (int u = 0; u < RT; ++u) {
-      l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
-      l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
-      const int r = tile * ROWS + 8 * u + g;
-      if (r >= a.steps * a.group) continue;
-      const int step = r / a.group;
-      const long long o = (static_cast<long long>(row) * a.steps + step) * a.ld_out +
-                          static_cast<long long>(head * a.group + r - step * a.group) * a.hd_out;
-      const float by = whole ? (l[u] > 0.0f || l[u] != l[u] ? __fdiv_rn(vref, l[u]) : 0.0f) : vref;
+      const float2 l2 = parts_of(l[u]);
+      float ls[2] = {l2.x, l2.y};
 #pragma unroll
-      for (int i = 0; i < OWN / 16; ++i) {
-        const int d = OWN * t + 16 * i;
-        if (d >= a.dim) continue;
-        float y[16];
-#pragma unroll
-        for (int k = 0; k < 16; ++k) y[k] = sum[(16 * i + k) % NJ][2 * u + (16 * i + k) / NJ] * by;
-        if (!whole)
-          store16(to, (8 * u + g) * a.dim + d, kOpsF32, true, y);
-        else
-          store16(a.out, o + d, a.out_type, a.wide_out, y);
+      for (int o = 4; o < 32; o <<= 1) {
+        ls[0] += __shfl_xor_sync(0xffffffffu, ls[0], o);
+        ls[1] += __shfl_xor_sync(0xffffffffu, ls[1], o);
       }
-      if (!whole && t == 0) {
-        to[ROWS * a.dim + 8 * u + g] = m[u];
-        to[ROWS * a.dim + ROWS + 8 * u + g] = l[u];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int local = 8 * u + 2 * t + k, r = tile * ROWS + local;
+        if (r >= a.steps * a.group) continue;
+        const float by = whole ? (ls[k] > 0.0f || ls[k] != ls[k] ? __fdiv_rn(vref, ls[k]) : 0.0f) : vref;
+        float y[4 * VW];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const float2 even = parts_of(sum[i][u][0]), odd = parts_of(sum[i][u][1]);
+          y[2 * i] = (k ? even.y : even.x) * by;
+          y[2 * i + 1] = (k ? odd.y : odd.x) * by;
+        }
+        if (!whole) {
+          if (d1 < a.dim) store_n<N1>(to, local * a.dim + d1, kOpsF32, true, y);
+          if constexpr (N2 > 0) {
+            if (d2 < a.dim) store_n<N2>(to, local * a.dim + d2, kOpsF32, true, y + N1);
+          }
+          if (g == 0) {
+            to[ROWS * a.dim + local] = m[u][k];
+            to[ROWS * a.dim + ROWS + local] = ls[k];
+          }
+        } else {
+          const int step = r / a.group;
+          const long long o = (static_cast<long long>(row) * a.steps + step) * a.ld_out +
+                              static_cast<long long>(head * a.group + r - step * a.group) * a.hd_out;
+          if (d1 < a.dim) store_n<N1>(a.out, o + d1, a.out_type, a.wide_out, y);
+          if constexpr (N2 > 0) {
+            if (d2 < a.dim) store_n<N2>(a.out, o + d2, a.out_type, a.wide_out, y + N1);
+          }
+        }
       }
     }
     part = 1;
@@ -699,7 +753,7 @@ __global__ void __launch_bounds__(kAttThreads, DP == 64 && RT == 1 ? 2 : 1) cach
         pl = 0.0f;
         y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (int w = 0; w < kAttWarps; ++w)
+        for (int w = 0; w < NW; ++w)
           add(joined_ml[w].x, joined_ml[w].y, lane < quads ? joined[w][lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f));
         if (lane < quads) {
           const float inv = pl > 0.0f || pl != pl ? __fdiv_rn(1.0f, pl) : 0.0f;
@@ -840,67 +894,84 @@ constexpr int kAttMaxSmem = 227 * 1024;
 constexpr int kClusterSteps = 24;
 
 struct Plan {
-  int dp, rt, grid, tiles, teams, least, members;
+  int dp, rt, warps, grid, tiles, teams, least, members;
   size_t smem, parts_bytes;
 };
-Plan plan(const verbo_cache& c, int heads, int steps) {
+template <int DP, int RT>
+void shape(Plan* p, int* warp_bytes, int* ctas) {
+  p->warps = AttShape<DP, RT>::kWarps;
+  *warp_bytes = AttShape<DP, RT>::kWarp;
+  *ctas = AttShape<DP, RT>::kCtas;
+}
+Plan plan(const verbo_cache& c, int heads, int steps, int q_type) {
   Plan p{};
   const int rows = steps * (heads / c.heads), sms = sm_count();
-  p.dp = c.dim <= 64 ? 64 : 128;
+  p.dp = c.dim <= 64 ? 64 : c.dim <= 96 ? 96 : 128;
   // More than 8 query rows: 16 at a time, twice the products for one conversion and one
-  // copy of the keys and values.  KAPPA16
-  p.rt = rows > 8 ? 2 : 1;
+  // copy of the keys and values.  KAPPA16  fp32 queries, in two parts, leave no registers.
+  p.rt = rows > 8 && q_type != kOpsF32 ? 2 : 1;
   p.tiles = (rows + 8 * p.rt - 1) / (8 * p.rt);
-  const int warp = p.dp == 64 ? (p.rt == 1 ? AttShape<64, 1>::kWarp : AttShape<64, 2>::kWarp)
-                              : (p.rt == 1 ? AttShape<128, 1>::kWarp : AttShape<128, 2>::kWarp);
+  int warp = 0, ctas = 1;
+  if (p.dp == 64)
+    p.rt == 1 ? shape<64, 1>(&p, &warp, &ctas) : shape<64, 2>(&p, &warp, &ctas);
+  else if (p.dp == 96)
+    p.rt == 1 ? shape<96, 1>(&p, &warp, &ctas) : shape<96, 2>(&p, &warp, &ctas);
+  else
+    p.rt == 1 ? shape<128, 1>(&p, &warp, &ctas) : shape<128, 2>(&p, &warp, &ctas);
   // Few (row, head, tile): a cluster for each, with as many CTAs as the SMs allow.
   const long long units = static_cast<long long>(c.rows) * c.heads * p.tiles;
   if (units <= sms) {
     p.members = 1;
     while (p.members < 8 && units * p.members * 2 <= sms) p.members *= 2;
     const long long most = static_cast<long long>(c.width) * (c.page / kCacheBlock);  // blocks of a row
-    if (most <= 2ll * kClusterSteps * kAttWarps * p.members) {
+    if (most <= 2ll * kClusterSteps * p.warps * p.members) {
       p.grid = static_cast<int>(units) * p.members;
-      p.smem = static_cast<size_t>(kAttWarps) * warp;
+      p.smem = static_cast<size_t>(p.warps) * warp;
       return p;
     }
     p.members = 0;
   }
-  p.smem = static_cast<size_t>(kAttWarps) * warp + (static_cast<size_t>(c.rows) + 1) * 4;
-  // small heads leave room for two CTAs an SM, unless there are very many rows
-  const int per_sm = p.dp == 64 && p.rt == 1 && 2 * (p.smem + 1024) <= kAttMaxSmem + 1024 ? 2 : 1;
-  p.grid = sms * per_sm;
-  p.teams = std::max(1, p.grid * kAttWarps / p.tiles);
+  p.smem = static_cast<size_t>(p.warps) * warp + (static_cast<size_t>(c.rows) + 1) * 4;
+  // very many rows leave room for one CTA an SM
+  if (ctas * (p.smem + 1024) > kAttMaxSmem + 1024) ctas = 1;
+  p.grid = sms * ctas;
+  p.teams = std::max(1, p.grid * p.warps / p.tiles);
   p.least = 2;
   p.parts_bytes = static_cast<size_t>(p.teams) * p.tiles * 2 * part_floats(8 * p.rt, c.dim) * 4;
   return p;
 }
 
-template <int DP, int RT>
+template <int DP, int RT, bool LO>
 cudaError_t run_attend(const AttendArgs& a, const Plan& p, cudaStream_t s) {
+  constexpr int threads = AttShape<DP, RT>::kWarps * 32, warps = AttShape<DP, RT>::kWarps * AttShape<DP, RT>::kWarp;
   if (p.members) {
-    const cudaError_t e = allow_smem<cache_attend_kernel<DP, RT, true>>(kAttWarps * AttShape<DP, RT>::kWarp);
+    const cudaError_t e = allow_smem<cache_attend_kernel<DP, RT, LO, true>>(warps);
     if (e != cudaSuccess) return e;
-    return launch_chained(cache_attend_kernel<DP, RT, true>, static_cast<unsigned>(p.grid), kAttThreads, p.smem,
+    return launch_chained(cache_attend_kernel<DP, RT, LO, true>, static_cast<unsigned>(p.grid), threads, p.smem,
                           p.members, s, a);
   }
-  constexpr int most = kAttWarps * AttShape<DP, RT>::kWarp + (VERBO_CACHE_MAX_ROWS + 1) * 4;
+  constexpr int most = warps + (VERBO_CACHE_MAX_ROWS + 1) * 4;
   static_assert(most + 64 <= kAttMaxSmem, "shared memory");
-  const cudaError_t e = allow_smem<cache_attend_kernel<DP, RT, false>>(most);
+  const cudaError_t e = allow_smem<cache_attend_kernel<DP, RT, LO, false>>(most);
   if (e != cudaSuccess) return e;
-  return launch_chained(cache_attend_kernel<DP, RT, false>, static_cast<unsigned>(p.grid), kAttThreads, p.smem, 1, s, a);
+  return launch_chained(cache_attend_kernel<DP, RT, LO, false>, static_cast<unsigned>(p.grid), threads, p.smem, 1, s, a);
+}
+template <int DP>
+cudaError_t run_attend(const AttendArgs& a, const Plan& p, cudaStream_t s) {
+  if (p.rt == 2) return run_attend<DP, 2, false>(a, p, s);
+  return a.q_type == kOpsF32 ? run_attend<DP, 1, true>(a, p, s) : run_attend<DP, 1, false>(a, p, s);
 }
 
 }  // namespace
 
-size_t cache_attend_bytes(const verbo_cache& c, int heads, int steps) {
-  const Plan p = plan(c, heads, steps);
+size_t cache_attend_bytes(const verbo_cache& c, int heads, int steps, int q_type) {
+  const Plan p = plan(c, heads, steps, q_type);
   return p.members || c.rows == 0 ? 0 : (p.parts_bytes + (static_cast<size_t>(c.rows) + 1) * 4 + 15) / 16 * 16;
 }
 
 cudaError_t launch_cache_attend(const verbo_cache& c, int layer, const CacheQuery& x, int q_type, int out_type,
                                 cudaStream_t s) {
-  const Plan p = plan(c, x.heads, x.steps);
+  const Plan p = plan(c, x.heads, x.steps, q_type);
   AttendArgs a{};
   const size_t per = static_cast<size_t>(c.pages) * c.heads * c.page;
   a.k = c.k + layer * per * c.dim;
@@ -943,8 +1014,9 @@ cudaError_t launch_cache_attend(const verbo_cache& c, int layer, const CacheQuer
   a.wide_out = wide(x.out, x.ld_out, x.hd_out, out_type);
   const long long joins = static_cast<long long>(c.rows) * c.heads * p.tiles * (8 * p.rt / kJoinRows);
   if (joins > INT_MAX) return cudaErrorInvalidConfiguration;
-  const cudaError_t e = p.dp == 64 ? (p.rt == 1 ? run_attend<64, 1>(a, p, s) : run_attend<64, 2>(a, p, s))
-                                   : (p.rt == 1 ? run_attend<128, 1>(a, p, s) : run_attend<128, 2>(a, p, s));
+  const cudaError_t e = p.dp == 64   ? run_attend<64>(a, p, s)
+                        : p.dp == 96 ? run_attend<96>(a, p, s)
+                                     : run_attend<128>(a, p, s);
   if (e != cudaSuccess || p.members) return e;
   const size_t smem = static_cast<size_t>(kJoinRows) * c.dim * 4;  // of a warp
   if (joins >= 2 * sm_count())

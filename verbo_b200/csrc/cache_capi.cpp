@@ -237,12 +237,13 @@ void check_attend(const verbo_cache* c, int heads, int steps) {
 }
 }  // namespace
 
-VERBO_CUDA_API long long verbo_cache_attend_workspace(const verbo_cache* c, int heads, int steps) {
+VERBO_CUDA_API long long verbo_cache_attend_workspace(const verbo_cache* c, int heads, int steps, int q_type) {
   return guard(
       [&]() -> long long {
         check_sizes(c);
         check_attend(c, heads, steps);
-        return static_cast<long long>(vb::cache_attend_bytes(*c, heads, steps));
+        check_type(q_type, "q_type");
+        return static_cast<long long>(vb::cache_attend_bytes(*c, heads, steps, q_type));
       },
       -1);
 }
@@ -269,7 +270,7 @@ VERBO_CUDA_API int verbo_cache_attend(const verbo_cache* c, int layer, const voi
         const bool by_token = (heads - 1) * hd_out + c->dim <= ld_out || tokens == 1;
         const bool by_head = (tokens - 1) * ld_out + c->dim <= hd_out || heads == 1;
         if (!by_token && !by_head) fail("out: its tokens and heads overlap");
-        if (const size_t need = vb::cache_attend_bytes(*c, heads, steps)) {
+        if (const size_t need = vb::cache_attend_bytes(*c, heads, steps, q_type)) {
           const Range ws = check_workspace(workspace, workspace_bytes, need, "verbo_cache_attend_workspace");
           check_output(ws, all);
           check_apart(ws, rq);
