@@ -213,13 +213,16 @@ struct __align__(16) BlockHead {
 // Shared memory per warp: a ring of steps of two blocks' keys and values, rows of kRow
 // bytes whose 16-byte chunks are exchanged so that the fragment loads below meet no
 // bank twice, and what is known of the blocks.
-// Warps: as many as the registers allow, up to 168 a lane for 12 of them; a step of a warp
-// is a chain of loads, products and exponentials, which only other warps fill.
+// A warp's step is a chain of loads, products and exponentials, and two steps ahead
+// cover the memory's latency: 8 warps with three steps of shared memory at 230 registers.
+// With 96 dims 168 registers do, and 12 warps with two steps each take 148 us where 8
+// with three take 157 (64 rows of 8192 tokens of 80 dims); with 128 dims those spill,
+// and 64 rows of 4096 tokens take 124 us against 102.
 template <int DP, int RT>
 struct AttShape {
-  static constexpr int kWarps = 8;
+  static constexpr int kWarps = DP == 96 && RT == 1 ? 12 : 8;
   static constexpr int kCtas = DP == 64 && RT == 1 ? 2 : 1;  // per SM
-  static constexpr int kStages = RT == 1 ? 3 : 2;            // steps whose copies are in flight
+  static constexpr int kStages = RT == 1 && DP != 96 ? 3 : 2;  // steps whose copies are in flight
   static constexpr int kRow = DP == 64 ? 64 : 128;
   static constexpr int kBlock = 16 * kRow;             // bytes of a block's keys, and of its values
   static constexpr int kStep = kAttPair * 2 * kBlock;  // of a step
