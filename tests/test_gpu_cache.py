@@ -362,6 +362,13 @@ def check_attend(c, q, layer=0, scale=None, dtype=None, out=None):
     return got
 
 
+def widened(c, tokens=80000):
+    """The same cache with room for longer rows: its attention is split over the card, not over a cluster."""
+    table = torch.full((c.rows, -(-tokens // c.page)), -1, dtype=torch.int32, device="cuda")
+    table[:, :c.width] = c.table
+    return vb.PagedCache(c.k, c.v, c.k_scale, c.v_scale, table, c.lens, c.refs)
+
+
 def queries(n, heads, dim, dtype, seed=1, size=2.0):
     g = torch.Generator(device="cuda")
     g.manual_seed(seed)
@@ -373,16 +380,20 @@ def queries(n, heads, dim, dtype, seed=1, size=2.0):
 @pytest.mark.parametrize("heads,group", [(1, 1), (2, 7), (3, 8), (1, 12)])
 def test_attend_shapes(dtype, dim, heads, group):
     c = filled([0, 1, 15, 16, 17, 100, 1, 333], heads, dim, 16)
-    check_attend(c, queries(8, heads * group, dim, dtype))
+    q = queries(8, heads * group, dim, dtype)
+    check_attend(c, q)
+    check_attend(widened(c), q)
 
 
 @pytest.mark.parametrize("page", [16, 48, 256])
 @pytest.mark.parametrize("steps", [1, 2, 5, 32])
-@pytest.mark.parametrize("dim,group", [(64, 4), (128, 3)])
-def test_attend_steps(page, steps, dim, group):
+@pytest.mark.parametrize("dim,group,dtype", [(64, 4, BF16), (128, 3, BF16), (80, 5, F16), (128, 2, F32)])
+def test_attend_steps(page, steps, dim, group, dtype):
     """Several last tokens, each sees up to its own; rows shorter than them."""
     c = filled([40, 0, 1, 5, 31, 32, 33, 700], 2, dim, page, layers=2)
-    check_attend(c, queries(8 * steps, 2 * group, dim, BF16), layer=1, dtype=F32)
+    q = queries(8 * steps, 2 * group, dim, dtype)
+    check_attend(c, q, layer=1, dtype=F32)
+    check_attend(widened(c), q, layer=1, dtype=F32)
 
 
 @pytest.mark.parametrize("dim,heads,group,lens", [
@@ -563,6 +574,56 @@ def test_streams():
     for i in range(4):
         want = caches[i].attend(0, qs[i])
         assert all(torch.equal(g, want) for g in got[i])
+
+
+def test_free_and_compact_captured():
+    c = filled([40, 33, 16, 1], 2, 64, 16, spare=20, width=4)
+    keep = i32([-1, 10, 0, 1])
+    c.free(i32([-1] * 4))
+    c.compact()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.free(keep)
+        info = c.compact()
+    for kept in ([-1, 10, 0, 1], [20, 20, 20, 0], [0, 3, 1, 1]):
+        keep.copy_(i32(kept))
+        m = model(c)
+        graph.replay()
+        m.free(np.asarray(kept))
+        want = m.compact()
+        assert info.tolist() == list(want)
+        check(c, m)
+
+
+def test_threads():
+    """Host threads, each with its own cache and stream, one step after the other."""
+    import threading
+
+    def work(i, out):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            c = filled([50 + i, 7, 333], 2, 64, 16, seed=i, spare=20, width=30)
+            add = i32([1, 0, 2])
+            for n in range(20):
+                start, status = c.reserve(add)
+                c.append(0, tokens(6, 2, 64, F16, n), tokens(6, 2, 64, F16, n + 1), start,
+                         off=torch.tensor([0, 1, 1, 3], device="cuda"))
+                y = c.attend(0, queries(3, 4, 64, BF16, seed=n))
+                s = vb.beam_select(y.view(3, -1), torch.zeros(3, device="cuda"), 3, 5)
+            torch.cuda.current_stream().synchronize()
+            out[i] = (y, *s, c.table, c.lens, status)
+
+    alone, together = {}, {}
+    for i in range(4):
+        work(i, alone)
+    threads = [threading.Thread(target=work, args=(i, together)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    vb.check()
+    for i in range(4):
+        assert all(torch.equal(a, b) for a, b in zip(alone[i], together[i]))
 
 
 def test_python_refusals():

@@ -70,12 +70,14 @@ class PagedCache:
     [rows, width], the rows' pages, -1 behind the last; lens: int32 [rows], their
     tokens; refs: int32 [pages], how many entries of the table hold a page (0: free).
     All contiguous CUDA tensors on one device, the caller's own: the object keeps
-    them and nothing else.  ``new`` makes an empty cache.
+    them, and a workspace of about 12 bytes a page.  ``new`` makes an empty cache.
 
     A decode step: ``reserve`` makes room for the rows' new tokens, then per layer
     ``append`` writes their keys and values and ``attend`` reads them.  A step of
     beam search ends with ``fork``.  Nothing waits for the device; what a call has to
-    say (``status``, ``info``) it writes into a tensor."""
+    say (``status``, ``info``) it writes into a tensor.  Calls on one cache have to follow
+    one another (one stream, or streams that wait for one another), but for ``append`` and
+    ``attend`` of different layers."""
 
     def __init__(self, k, v, k_scale, v_scale, table, lens, refs):
         self._lib, self._torch, self._types = lib, torch, _ = _cache()
@@ -109,6 +111,8 @@ class PagedCache:
         self._need = lib.verbo_cache_workspace(ctypes.byref(c))
         if self._need < 0:
             raise _err()
+        # reserve's and compact's: no two of them may run on one cache at the same time
+        self._ws = torch.empty(self._need, dtype=torch.uint8, device=k.device)
         self._attend_need = {}  # workspace bytes by (heads, steps, type)
 
     @classmethod
@@ -157,9 +161,8 @@ class PagedCache:
         ap = self._ints(add, "add")
         start = _new(torch, self.lens, stream, self.rows, torch.int32)
         status = _new(torch, self.lens, stream, 1, torch.int32)
-        # the workspace belongs to the call's stream: freed here, it is reused behind the call
-        ws = _new(torch, self.lens, stream, self._need, torch.uint8)
-        self._run(self._lib.verbo_cache_reserve, ap, start.data_ptr(), status.data_ptr(), ws.data_ptr(), self._need, at)
+        self._run(self._lib.verbo_cache_reserve, ap, start.data_ptr(), status.data_ptr(), self._ws.data_ptr(), self._need,
+                  at)
         return start, status
 
     def fork(self, parents, beams, stream=None):
@@ -187,8 +190,7 @@ class PagedCache:
         torch = self._torch
         at = _stream_of(torch, self.k.get_device(), stream)
         info = _new(torch, self.lens, stream, 2, torch.int32)
-        ws = _new(torch, self.lens, stream, self._need, torch.uint8)
-        self._run(self._lib.verbo_cache_compact, info.data_ptr(), ws.data_ptr(), self._need, at)
+        self._run(self._lib.verbo_cache_compact, info.data_ptr(), self._ws.data_ptr(), self._need, at)
         return info
 
     def _tokens(self, t, what, heads=None):
@@ -270,6 +272,7 @@ class PagedCache:
             if need < 0:
                 raise _err()
             self._attend_need[heads, steps, code] = need
+        # this workspace belongs to the call's stream: freed here, it is reused behind the call
         ws = _new(torch, q, stream, need, torch.uint8) if need else None
         self._run(self._lib.verbo_cache_attend, self._layer(layer), q.data_ptr(), code, ldq, hdq, heads, steps, scale,
                   out.data_ptr(), ocode, ldo, hdo, ws.data_ptr() if need else None, need, at)
