@@ -18,7 +18,7 @@ namespace {
 // to well below the distance of two candidates: fp32's 1e-7 would swap a pair
 // now and then.  The terms are fp32 but without a common error (the factor log2(e)
 // is taken in two parts, so a term is off by its own roundings alone, which cancel
-// in the sum), eight of them are added in fp32 and the rest in 64 bits.  A sum goes by
+// in the sum), up to sixteen of them are added in fp32 and the rest in 64 bits.  A sum goes by
 // the columns alone, not by where a row lies in memory: equal rows have equal sums
 // to the last bit, and equal candidates are ordered by their beams.
 //
@@ -88,22 +88,16 @@ struct SelBatch {
   }
   // sum of e^(x - ref), NaNs left out
   __device__ __forceinline__ double sum(float ref) const {
-    constexpr int CHAINS = NV * N / 16;  // of two sums of eight terms
     const Two away = two(-ref, -ref), c_hi = two(kLog2eHi, kLog2eHi), c_lo = two(kLog2eLo, kLog2eLo);
-    double s = 0.0;
+    Two t[2] = {two(0.0f, 0.0f), two(0.0f, 0.0f)};
 #pragma unroll
-    for (int c = 0; c < CHAINS; ++c) {
-      Two t = two(0.0f, 0.0f);
-#pragma unroll
-      for (int j = 0; j < 16; j += 2) {
-        const int i = c * 16 + j;
-        const Two d = add2(two(x[i / N].get(i % N), x[i / N].get(i % N + 1)), away);
-        const float2 e = parts_of(fma2(d, c_hi, mul2(d, c_lo)));
-        t = add2(t, two(ex2(e.x), ex2(e.y)));
-      }
-      const float2 p = parts_of(t);
-      s += static_cast<double>(p.x) + static_cast<double>(p.y);
+    for (int i = 0; i < NV * N; i += 2) {
+      const Two d = add2(two(x[i / N].get(i % N), x[i / N].get(i % N + 1)), away);
+      const float2 e = parts_of(fma2(d, c_hi, mul2(d, c_lo)));
+      t[i / 2 % 2] = add2(t[i / 2 % 2], two(ex2(e.x), ex2(e.y)));
     }
+    const float2 p = parts_of(add2(t[0], t[1]));
+    double s = static_cast<double>(p.x) + static_cast<double>(p.y);
     if (s != s) {  // rare: a NaN was met
       s = 0.0;
 #pragma unroll
