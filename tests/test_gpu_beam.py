@@ -184,6 +184,23 @@ def test_more_batches_than_maxima_are_kept_of(dtype):
     check(x, s, 1, 40)
 
 
+def test_many_requests():
+    """More rows than CTAs fit, of a few columns each; and one beam each."""
+    x, s = make(24000, 37, F16, 12)
+    v, p, t = vb.beam_select(x, s, 3, 4)
+    pick = [0, 1, 4000, 7999]
+    rows = [3 * r + b for r in pick for b in range(3)]
+    w = check(x[rows].contiguous(), s[rows].contiguous(), 3, 4)
+    for a, b in zip((v, p, t), w):
+        assert torch.equal(a[pick], b)
+    x, s = make(70000, 5, F32, 13)
+    v, p, t = vb.beam_select(x, s, 1, 2)
+    assert torch.equal(t.long(), x.topk(2, 1).indices) and bool((p == 0).all())
+    state = torch.arange(70000, device="cuda").view(-1, 1).repeat(1, 3)
+    vb.beam_reorder(state, torch.zeros(35000, 2, dtype=torch.int32, device="cuda"), 2)
+    assert torch.equal(state[1::2], state[::2]) and torch.equal(state[::2, 0], torch.arange(0, 70000, 2, device="cuda"))
+
+
 def test_scores_in_place():
     """out_scores may be the scores where as many are taken."""
     x, s = make(4, 700, F32, 11)
