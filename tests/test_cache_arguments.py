@@ -2,7 +2,9 @@
 the exported symbols and the refusals, which come before the GPU is touched."""
 from __future__ import annotations
 
+import copy
 import ctypes
+import pickle
 import re
 import subprocess
 from pathlib import Path
@@ -195,6 +197,18 @@ def test_nothing(lib):
     refused(lib, append(lib, cache=none, tokens=4), "multiple of rows")
     empty = dict(rows=0, table=None, lens=None)
     assert lib.verbo_cache_free(made(**empty), None, None) == 0
+
+
+@pytest.mark.parametrize("how", [copy.copy, copy.deepcopy, pickle.dumps], ids=["copy", "deepcopy", "pickle"])
+def test_a_cache_is_not_copied(how):
+    """Nor can its tensors be exchanged: the library has their addresses."""
+    c = object.__new__(vb.PagedCache)
+    c._held = {"lens": torch.zeros(2)}
+    with pytest.raises(TypeError, match="PagedCache"):
+        how(c)
+    with pytest.raises(AttributeError):
+        c.lens = torch.zeros(3)
+    assert c.lens.numel() == 2
 
 
 def test_python_refusals():

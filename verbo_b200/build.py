@@ -31,7 +31,7 @@ NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC,-fvisibility=hidden,-O2",
-    "-shared", "-cudart", "static",
+    "-shared", "-cudart", "static", "--threads", "0",
 ]
 
 

@@ -97,6 +97,7 @@ class PagedCache:
         codes, f32, i32 = torch.float8_e4m3fn, torch.float32, torch.int32
         blocks = (layers, pages, heads, page // BLOCK)
         c = self._c = _Cache(layers, pages, heads, dim, page, rows, width)
+        self._held = {}  # the library has their addresses: other tensors are another cache
         for name, t, dtype, shape in (("k", k, codes, k.shape), ("v", v, codes, k.shape),
                                       ("k_scale", k_scale, f32, blocks), ("v_scale", v_scale, f32, blocks),
                                       ("table", table, i32, table.shape), ("lens", lens, i32, (rows,)),
@@ -104,7 +105,7 @@ class PagedCache:
             if tuple(t.shape) != tuple(shape):
                 raise VerboCudaError(f"{name} must be {list(shape)}")
             setattr(c, name, _list(t, dtype, dev, name))
-            setattr(self, name, t)
+            self._held[name] = t
         self.layers, self.pages, self.heads, self.page, self.dim = layers, pages, heads, page, dim
         self.rows, self.width = rows, width
         self.device = k.device
@@ -139,6 +140,17 @@ class PagedCache:
         i32 = torch.int32
         return cls(pool(), pool(), scales(), scales(), make((rows, width), i32, -1), make((rows,), i32, 0),
                    make((pages,), i32, 0))
+
+    def __reduce_ex__(self, protocol):
+        raise TypeError("a PagedCache cannot be copied or pickled")
+
+    k = property(lambda self: self._held["k"])
+    v = property(lambda self: self._held["v"])
+    k_scale = property(lambda self: self._held["k_scale"])
+    v_scale = property(lambda self: self._held["v_scale"])
+    table = property(lambda self: self._held["table"])
+    lens = property(lambda self: self._held["lens"])
+    refs = property(lambda self: self._held["refs"])
 
     def _run(self, fn, *args):
         _call(fn, self._torch, self.k.get_device(), ctypes.byref(self._c), *args)
