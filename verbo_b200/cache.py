@@ -62,6 +62,19 @@ def _new(torch, like, stream, shape, dtype):
     return torch.empty(shape, dtype=dtype, device=like.device)
 
 
+def _tensor(name):
+    """A tensor of the cache: changed in place (``cache.lens += 1`` too), not exchanged."""
+
+    def get(self):
+        return self._held[name]
+
+    def put(self, t):
+        if t is not self._held[name]:
+            raise AttributeError(f"the cache's {name} cannot be another tensor")
+
+    return property(get, put)
+
+
 class PagedCache:
     """Keys and values of ``rows`` rows in pages that they may share.
 
@@ -144,13 +157,8 @@ class PagedCache:
     def __reduce_ex__(self, protocol):
         raise TypeError("a PagedCache cannot be copied or pickled")
 
-    k = property(lambda self: self._held["k"])
-    v = property(lambda self: self._held["v"])
-    k_scale = property(lambda self: self._held["k_scale"])
-    v_scale = property(lambda self: self._held["v_scale"])
-    table = property(lambda self: self._held["table"])
-    lens = property(lambda self: self._held["lens"])
-    refs = property(lambda self: self._held["refs"])
+    k, v, k_scale, v_scale = _tensor("k"), _tensor("v"), _tensor("k_scale"), _tensor("v_scale")
+    table, lens, refs = _tensor("table"), _tensor("lens"), _tensor("refs")
 
     def _run(self, fn, *args):
         _call(fn, self._torch, self.k.get_device(), ctypes.byref(self._c), *args)
