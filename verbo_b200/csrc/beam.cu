@@ -148,6 +148,7 @@ __global__ void __launch_bounds__(kSelThreads, 4) beam_rows_kernel(const BeamSel
   __shared__ float group_max[kSelGroups * NT];
   __shared__ unsigned short hits[kSelGroups * NT];  // group * NT + thread
   __shared__ __align__(16) uint32_t offer[kSelWarps * kSelOffers];
+  __shared__ uint32_t first_max[kSelWarps];
   __shared__ int count, nhits;
   __shared__ uint32_t bound;
   __shared__ uint64_t bound_key;
@@ -276,9 +277,9 @@ __global__ void __launch_bounds__(kSelThreads, 4) beam_rows_kernel(const BeamSel
     mx = fmaxf(mx, bm);
     if (b == 0) {
       const uint32_t w = __reduce_max_sync(0xffffffffu, ord32(bm + 0.0f));
-      if (lane == 0) offer[warp] = w;
+      if (lane == 0) first_max[warp] = w;
       __syncthreads();
-      ref = unord32(__reduce_max_sync(0xffffffffu, lane < kSelWarps ? offer[lane] : 0u));
+      ref = unord32(__reduce_max_sync(0xffffffffu, lane < kSelWarps ? first_max[lane] : 0u));
       if (ref == -kNegInf) ref = kNegInf;
     }
     if (bm == -kNegInf) {
@@ -302,6 +303,8 @@ __global__ void __launch_bounds__(kSelThreads, 4) beam_rows_kernel(const BeamSel
       ++group;
     }
   }
+
+  cp_async_wait_all();  // a row without candidates has copies under way
 
   // the CTA's part of the row: sums of one reference are added as they are
   SelPart p;

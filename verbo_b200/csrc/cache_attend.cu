@@ -308,8 +308,8 @@ __global__ void __launch_bounds__(AttShape<DP, RT>::kWarps * 32, AttShape<DP, RT
   const uint32_t ring_at = smem_u32(ring);
   const long long block_bytes = 16ll * a.dim;
   // and where it reads fragments: of the keys of token g (and g + 8) the dims 16 t ... and
-  // 64 + (DP - 64) / 4 t ...; of the values of tokens 2 t (v0) and 2 t + 1 (v1) (and + 8) the
-  // dims of `v_first` and `v_second` below
+  // 64 + (DP - 64) / 4 t ...; of the values of tokens 2 t (v0, v2) and 2 t + 1 (v1, v3) (and
+  // + 8) the dims N1 g ... and, of 96, 64 + 4 g ...
   uint32_t at_k0, at_k1 = 0, at_v0, at_v1, at_v2 = 0, at_v3 = 0;
   if (DP == 64) {
     at_k0 = g * 64 + (t << 4);
