@@ -362,7 +362,7 @@ def check_attend(c, q, layer=0, scale=None, dtype=None, out=None):
     return got
 
 
-def widened(c, tokens=80000):
+def widened(c, tokens=100000):
     """The same cache with room for longer rows: its attention is split over the card, not over a cluster."""
     table = torch.full((c.rows, -(-tokens // c.page)), -1, dtype=torch.int32, device="cuda")
     table[:, :c.width] = c.table

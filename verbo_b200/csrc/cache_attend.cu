@@ -781,8 +781,9 @@ __global__ void __launch_bounds__(AttShape<DP, RT>::kWarps * 32, AttShape<DP, RT
   }
 }
 
-// Warps of a join's CTA: few where there are many (row, head) of few parts each; many
-// where a few of them are split over most of the card's warps.
+// Warps of a join's CTA: few where there are many (row, head) of few parts each (64 rows of
+// 4096 tokens 102 us, 113 with many); many where a few are split over most of the card's
+// warps.
 constexpr int kJoinFew = 4, kJoinMany = 16;
 constexpr int kJoinRows = 4;  // query rows of a CTA
 
@@ -900,17 +901,24 @@ constexpr int kAttMaxSmem = 227 * 1024;
 
 // A warp of a cluster takes at most this many steps, whatever the lengths are: longer
 // tables go to the parts, which are equal for any lengths.
-constexpr int kClusterSteps = 24;
+constexpr int kClusterSteps = 32;
 
 struct Plan {
   int dp, rt, warps, grid, tiles, teams, least, members;
   size_t smem, parts_bytes;
 };
+// Warps, their shared memory, and the largest cluster of which `units` run at once (0:
+// they do not as single CTAs either).
 template <int DP, int RT>
-void shape(Plan* p, int* warp_bytes, int* ctas) {
-  p->warps = AttShape<DP, RT>::kWarps;
-  *warp_bytes = AttShape<DP, RT>::kWarp;
-  *ctas = AttShape<DP, RT>::kCtas;
+void shape(Plan* p, int* warp_bytes, int* ctas, long long units) {
+  using S = AttShape<DP, RT>;
+  p->warps = S::kWarps;
+  *warp_bytes = S::kWarp;
+  *ctas = S::kCtas;
+  p->members = 8;
+  while (p->members &&
+         units > clusters_at_once<cache_attend_kernel<DP, RT, false, true>>(p->members, S::kWarps * 32, S::kWarps * S::kWarp))
+    p->members /= 2;
 }
 Plan plan(const verbo_cache& c, int heads, int steps, int q_type) {
   Plan p{};
@@ -921,27 +929,27 @@ Plan plan(const verbo_cache& c, int heads, int steps, int q_type) {
   // 108 us, 130 in two tiles of 8.  fp32 queries, in two parts, leave no registers for it.
   p.rt = rows > 8 && q_type != kOpsF32 ? 2 : 1;
   p.tiles = (rows + 8 * p.rt - 1) / (8 * p.rt);
+  const long long units = static_cast<long long>(c.rows) * c.heads * p.tiles;
   int warp = 0, ctas = 1;
   if (p.dp == 64)
-    p.rt == 1 ? shape<64, 1>(&p, &warp, &ctas) : shape<64, 2>(&p, &warp, &ctas);
+    p.rt == 1 ? shape<64, 1>(&p, &warp, &ctas, units) : shape<64, 2>(&p, &warp, &ctas, units);
   else if (p.dp == 96)
-    p.rt == 1 ? shape<96, 1>(&p, &warp, &ctas) : shape<96, 2>(&p, &warp, &ctas);
+    p.rt == 1 ? shape<96, 1>(&p, &warp, &ctas, units) : shape<96, 2>(&p, &warp, &ctas, units);
   else
-    p.rt == 1 ? shape<128, 1>(&p, &warp, &ctas) : shape<128, 2>(&p, &warp, &ctas);
-  // Few (row, head, tile): a cluster for each, with as many CTAs as the SMs allow: no
-  // second kernel and no search.  One row of 1500 tokens 6.8 us, 11.3 split over the card.
-  const long long units = static_cast<long long>(c.rows) * c.heads * p.tiles;
-  if (units <= sms) {
-    p.members = 1;
-    while (p.members < 8 && units * p.members * 2 <= sms) p.members *= 2;
-    const long long most = static_cast<long long>(c.width) * (c.page / kCacheBlock);  // blocks of a row
-    if (most <= 2ll * kClusterSteps * p.warps * p.members) {
-      p.grid = static_cast<int>(units) * p.members;
-      p.smem = static_cast<size_t>(p.warps) * warp;
-      return p;
-    }
-    p.members = 0;
+    p.rt == 1 ? shape<128, 1>(&p, &warp, &ctas, units) : shape<128, 2>(&p, &warp, &ctas, units);
+  // Few (row, head, tile): a cluster for each, as large as all of them fit at once: no
+  // second kernel and no search.  One row of 1500 tokens 6.8 us, 11.3 split over the card;
+  // 18 rows of 8000 tokens, a CTA to a (row, head), 56 and 65.  Lengths are not known
+  // before the launch: long or uneven rows lose by it, but not more than kClusterSteps
+  // take.  One row of 49152 tokens 38 us, 34 split; with three of 100 beside it, on half
+  // the CTAs, 66 and 36 (not taken: 49152 tokens are 48 steps then).
+  const long long most = static_cast<long long>(c.width) * (c.page / kCacheBlock);  // blocks of a row
+  if (p.members && most <= 2ll * kClusterSteps * p.warps * p.members) {
+    p.grid = static_cast<int>(units) * p.members;
+    p.smem = static_cast<size_t>(p.warps) * warp;
+    return p;
   }
+  p.members = 0;
   p.smem = static_cast<size_t>(p.warps) * warp + (static_cast<size_t>(c.rows) + 1) * 4;
   // very many rows leave room for one CTA an SM
   if (ctas * (p.smem + 1024) > kAttMaxSmem + 1024) ctas = 1;

@@ -112,7 +112,8 @@ __device__ __forceinline__ int free_page(const PageWs& w, int chunks, const int*
 }
 
 // Pools of up to 16384 pages: the CTA that needs the list makes it, 16 pages to a
-// thread, which costs it less than another launch would.  `mask`: this thread's free
+// thread: as long on the device as another kernel (5000 pages, 28 us for a fork and a
+// reserve either way), and 3 us less of the calling thread's time.  `mask`: this thread's free
 // pages, `before`: those before them.  Returns their number.
 constexpr int kSmallPool = 16384;
 constexpr int kSmallThreads = 1024;
@@ -692,7 +693,8 @@ cudaError_t launch_cache_reserve(const verbo_cache& c, const int* add, int* star
 cudaError_t launch_cache_fork(const verbo_cache& c, const int* parents, long long ld_parents, int beams,
                               cudaStream_t s) {
   const int groups = c.rows / beams;
-  // CTAs per group: as many as the columns give work to, while SMs are left
+  // CTAs per group: as many as the columns give work to, while SMs are left (8 rows of 1024
+  // pages 4.0 us, 8.7 with one; of 8192 pages 10 and 58)
   int C = 1;
   while (C < 8 && C * kForkThreads < c.width && groups * C * 2 <= sm_count()) C <<= 1;
   return launch_chained(cache_fork_kernel, static_cast<unsigned>(groups * C), kForkThreads,

@@ -127,6 +127,38 @@ inline cudaError_t allow_smem(int bytes) {
   return e;
 }
 
+// How many clusters of 1, 2, 4 or 8 CTAs of a kernel the current device holds at a time
+// (0: it could not be asked); asked once per device.
+template <auto Kernel>
+inline int clusters_at_once(int cluster, int threads, int smem) {
+  static std::atomic<int> known[64][4];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  const int i = cluster == 8 ? 3 : cluster == 4 ? 2 : cluster == 2 ? 1 : 0;
+  if (dev < 64) {
+    const int n = known[dev][i].load(std::memory_order_relaxed);
+    if (n) return n - 1;
+  }
+  int n = 0;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(cluster);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cluster;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  if (allow_smem<Kernel>(smem) != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, Kernel, &cfg) != cudaSuccess) {
+    (void)cudaGetLastError();  // the launch that follows says what is wrong
+    return 0;
+  }
+  if (dev < 64) known[dev][i].store(n + 1, std::memory_order_relaxed);
+  return n;
+}
+
 // A kernel that may begin before the one before it in the stream has ended
 // (grid_wait), with `cluster` CTAs a cluster.
 template <class K, class A>
