@@ -198,6 +198,30 @@ def test_the_largest_tables():
     check(c, m)
 
 
+def test_the_largest_pool():
+    """4194304 pages: the lowest free ones first, and the highest live ones moved first."""
+    pages = 4194304
+    c = vb.PagedCache.new(1, pages, 1, 16, 2, 8, 16)
+    far = [4194303, 3, 2048, 4192256]
+    c.table[0, :4] = i32(far)
+    c.refs[torch.tensor(far, device="cuda")] = 1
+    c.lens[0] = 60
+    for n, p in enumerate(far):
+        c.k.view(torch.uint8)[0, p] = n + 1
+        c.v_scale[0, p] = n + 1
+    start, status = c.reserve(i32([5, 33]))
+    assert status.tolist() == [0] and start.tolist() == [60, 0]
+    assert c.table.tolist() == [far + [0, -1, -1, -1], [1, 2, 4, -1, -1, -1, -1, -1]]
+    c.free(i32([-1, 17]))
+    assert c.table[1].tolist() == [1, 2] + [-1] * 6
+    assert c.compact().tolist() == [7, 3]  # live: 0, 1, 2, 3, 2048, 4192256, 4194303
+    assert c.table.tolist() == [[4, 3, 6, 5, 0, -1, -1, -1], [1, 2, -1, -1, -1, -1, -1, -1]]
+    assert c.refs[:8].tolist() == [1] * 7 + [0] and int(c.refs.sum()) == 7
+    assert [int(c.k.view(torch.uint8)[0, p].max()) for p in (4, 3, 6, 5)] == [1, 2, 3, 4]
+    assert [float(c.v_scale[0, p].max()) for p in (4, 3, 6, 5)] == [1, 2, 3, 4]
+    vb.check()
+
+
 # ----------------------------------------------------------------- append --
 def tokens(n, heads, dim, dtype, seed, spread=3.0):
     g = torch.Generator(device="cuda")
