@@ -122,6 +122,7 @@ class PagedCache:
         self.layers, self.pages, self.heads, self.page, self.dim = layers, pages, heads, page, dim
         self.rows, self.width = rows, width
         self.device = k.device
+        self._dev, self._ref = dev, ctypes.byref(c)
         self._need = lib.verbo_cache_workspace(ctypes.byref(c))
         if self._need < 0:
             raise _err()
@@ -161,11 +162,11 @@ class PagedCache:
     table, lens, refs = _tensor("table"), _tensor("lens"), _tensor("refs")
 
     def _run(self, fn, *args):
-        _call(fn, self._torch, self.k.get_device(), ctypes.byref(self._c), *args)
+        _call(fn, self._torch, self._dev, self._ref, *args)
 
     def _ints(self, t, what):
         """Address of int32 [rows] on the cache's device; a number stands for every row."""
-        return _list(t, self._torch.int32, self.k.get_device(), what, self.rows)
+        return _list(t, self._torch.int32, self._dev, what, self.rows)
 
     def reserve(self, add, stream=None):
         """Room for ``add`` more tokens of each row (int32 [rows]; 0: none): pages, the
@@ -177,7 +178,7 @@ class PagedCache:
         row r that the table is too narrow for.  Unless status is 0 nothing was changed
         and every start is -1, for which ``append`` writes nothing."""
         torch = self._torch
-        at = _stream_of(torch, self.k.get_device(), stream)
+        at = _stream_of(torch, self._dev, stream)
         ap = self._ints(add, "add")
         start = _new(torch, self.lens, stream, self.rows, torch.int32)
         status = _new(torch, self.lens, stream, 1, torch.int32)
@@ -194,21 +195,20 @@ class PagedCache:
         beams = int(beams)
         if not 1 <= beams <= 32 or self.rows % beams:
             raise VerboCudaError("beams must be in [1, 32] and divide the rows")
-        dev = self.k.get_device()
-        pp, ld = _parents(parents, torch, self.rows // beams, beams, dev)
-        self._run(self._lib.verbo_cache_fork, pp, ld, beams, _stream_of(torch, dev, stream))
+        pp, ld = _parents(parents, torch, self.rows // beams, beams, self._dev)
+        self._run(self._lib.verbo_cache_fork, pp, ld, beams, _stream_of(torch, self._dev, stream))
 
     def free(self, keep, stream=None):
         """Row r keeps its first keep[r] tokens (int32 [rows]; negative: all), and gives
         the pages behind them back (verbo_cache_free)."""
         self._run(self._lib.verbo_cache_free, self._ints(keep, "keep"),
-                  _stream_of(self._torch, self.k.get_device(), stream))
+                  _stream_of(self._torch, self._dev, stream))
 
     def compact(self, stream=None):
         """Moves the live pages to the front of the pool, in all layers
         (verbo_cache_compact).  Returns int32 [2]: live pages, pages that moved."""
         torch = self._torch
-        at = _stream_of(torch, self.k.get_device(), stream)
+        at = _stream_of(torch, self._dev, stream)
         info = _new(torch, self.lens, stream, 2, torch.int32)
         self._run(self._lib.verbo_cache_compact, info.data_ptr(), self._ws.data_ptr(), self._need, at)
         return info
@@ -219,7 +219,7 @@ class PagedCache:
             raise VerboCudaError(f"{what} must be [tokens, {heads or 'heads'}, {self.dim}]")
         if t.shape[0] > _INT_MAX or t.shape[1] > _INT_MAX:
             raise VerboCudaError(f"{what} must have at most {_INT_MAX} tokens and heads")
-        if t.get_device() != self.k.get_device():
+        if t.get_device() != self._dev:
             raise VerboCudaError(f"{what} must be a CUDA tensor on the device of the cache")
         code = self._types.get(t.dtype)
         if code is None:
@@ -242,7 +242,7 @@ class PagedCache:
         nv, _, ldv, hdv, vcode = self._tokens(v, "v", self.heads)
         if nv != n or vcode != code:
             raise VerboCudaError("k and v must have the same tokens and type")
-        dev = self.k.get_device()
+        dev = self._dev
         sp = self._ints(start, "start")
         op = _list(off, torch.int64, dev, "off", self.rows + 1)
         self._run(self._lib.verbo_cache_append, self._layer(layer), k.data_ptr(), ldk, hdk, v.data_ptr(), ldv, hdv,
@@ -284,11 +284,11 @@ class PagedCache:
             on, _, ldo, hdo, ocode = self._tokens(out, "out", heads)
             if on != n:
                 raise VerboCudaError("out must have the tokens of q")
-        at = _stream_of(torch, self.k.get_device(), stream)
+        at = _stream_of(torch, self._dev, stream)
         need = self._attend_need.get((heads, steps, code))
         if need is None:
             with torch.cuda.device(self.device):
-                need = self._lib.verbo_cache_attend_workspace(ctypes.byref(self._c), heads, steps, code)
+                need = self._lib.verbo_cache_attend_workspace(self._ref, heads, steps, code)
             if need < 0:
                 raise _err()
             self._attend_need[heads, steps, code] = need
