@@ -150,9 +150,10 @@ def test_nothing_and_infinities(dtype):
     assert (p == -1).all() and (t == -1).all() and (v == -INF).all()
 
 
-@pytest.mark.parametrize("low", [-1e10, -3.4e38])
-def test_large_finite_masks(low):
-    x, s = make(6, 5000, F32, 9)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("low", [-1e10, -3.38e38])
+def test_large_finite_masks(low, dtype):
+    x, s = make(6, 5000, dtype, 9)
     x[0] = low
     x[1, 7:] = low
     x[2, :4999] = low

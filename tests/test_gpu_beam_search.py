@@ -4,7 +4,9 @@ cache, its attention, selection, forks) against the same decoder whose beams own
 their pages and are copied."""
 from __future__ import annotations
 
-import math
+import subprocess
+import sys
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -15,6 +17,9 @@ torch = pytest.importorskip("torch")
 
 import verbo_b200 as vb  # noqa: E402
 from verbo_b200.serving import BeamSearch  # noqa: E402
+
+
+ROOT = Path(__file__).resolve().parent.parent
 
 
 @pytest.fixture(autouse=True)
@@ -33,6 +38,12 @@ def reference(table, first, beams, steps, stop):
         live = [c for c in cand if c[2] != stop][:beams]
     done += [(s, t, len(t)) for s, t, _ in live]
     return sorted(done, key=lambda d: -d[0] / d[2])[:beams]
+
+
+def test_first_calls_are_captured(cuda_lib):
+    r = subprocess.run([sys.executable, str(ROOT / "tests" / "beam_capture_calls.py")], capture_output=True, text=True,
+                       timeout=300, cwd=ROOT)
+    assert r.returncode == 0 and r.stdout.strip().endswith("same"), r.stderr[-2000:]
 
 
 @pytest.mark.parametrize("beams", [1, 2, 5])
