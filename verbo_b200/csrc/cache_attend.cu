@@ -781,28 +781,34 @@ __global__ void __launch_bounds__(AttShape<DP, RT>::kWarps * 32, AttShape<DP, RT
   }
 }
 
-// Warps of a join's CTA: few where there are many (row, head) of few parts each (64 rows of
-// 4096 tokens 102 us, 113 with many); many where a few are split over most of the card's
-// warps.
-constexpr int kJoinFew = 4, kJoinMany = 16;
-constexpr int kJoinRows = 4;  // query rows of a CTA
+// Of a join's CTA. Few warps where there are many (row, head) of few parts each (64 rows of
+// 4096 tokens 102 us, 113 with many); many, with fewer query rows and more parts on their
+// way, where a few are split over most of the card's warps (one row of 131072 tokens 58 us,
+// 61 with as many rows and parts as the others).
+template <bool MANY>
+struct JoinShape {
+  static constexpr int kWarps = MANY ? 16 : 4;
+  static constexpr int kRows = MANY ? 2 : 4;   // query rows
+  static constexpr int kAhead = MANY ? 6 : 2;  // a warp's parts on their way
+};
 
-// One CTA per (row, head, quarter or half of a tile): the parts of its blocks joined, in their
+// One CTA per (row, head, some rows of a tile): the parts of its blocks joined, in their
 // order; nothing to do where one warp had them all.  A warp takes every W-th part.
-template <int W>
-__global__ void __launch_bounds__(W * 32) cache_attend_join_kernel(const AttendArgs a) {
-  constexpr int R = kJoinRows, AHEAD = 2;
+template <bool MANY>
+__global__ void __launch_bounds__(JoinShape<MANY>::kWarps * 32) cache_attend_join_kernel(const AttendArgs a) {
+  using S = JoinShape<MANY>;
+  constexpr int W = S::kWarps, R = S::kRows, AHEAD = S::kAhead;
   extern __shared__ float4 os[];  // [W][R][dim / 4]
   __shared__ float ms[W][R], ls[W][R];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int H = a.tile_rows / R;
-  const int half = blockIdx.x % H;
-  const int tile = blockIdx.x / H % a.tiles;
-  const int head = blockIdx.x / (H * a.tiles) % a.heads;
-  const int row = blockIdx.x / (H * a.tiles) / a.heads;
+  const int slices = a.tile_rows / R;
+  const int slice = blockIdx.x % slices;
+  const int tile = blockIdx.x / slices % a.tiles;
+  const int head = blockIdx.x / (slices * a.tiles) % a.heads;
+  const int row = blockIdx.x / (slices * a.tiles) / a.heads;
   grid_wait();
   grid_release();
-  const int rows = min(R, a.steps * a.group - tile * a.tile_rows - half * R);  // of this CTA
+  const int rows = min(R, a.steps * a.group - tile * a.tile_rows - slice * R);  // of this CTA
   if (rows <= 0) return;
   const int f0 = a.first[row], counted = a.first[row + 1] - f0, blocks = a.first[a.rows];
   const int quads = a.dim / 4;
@@ -840,11 +846,11 @@ __global__ void __launch_bounds__(W * 32) cache_attend_join_kernel(const AttendA
         const float* from = a.parts + ((static_cast<long long>(at) * a.tiles + tile) * 2 + which) * part_floats(a.tile_rows, a.dim);
         ml[u] = lane < R ? kNegInf : 0.0f;
         if (at <= w1 && lane < 2 * R && lane % R < rows)
-          ml[u] = from[a.tile_rows * (a.dim + lane / R) + half * R + lane % R];
+          ml[u] = from[a.tile_rows * (a.dim + lane / R) + slice * R + lane % R];
 #pragma unroll
         for (int i = 0; i < R; ++i)
           v[u][i] = at <= w1 && i < rows && lane < quads
-                        ? reinterpret_cast<const float4*>(from)[(half * R + i) * quads + lane]
+                        ? reinterpret_cast<const float4*>(from)[(slice * R + i) * quads + lane]
                         : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       }
 #pragma unroll
@@ -888,7 +894,7 @@ __global__ void __launch_bounds__(W * 32) cache_attend_join_kernel(const AttendA
   }
   if (lane >= quads) return;
   const float inv = total > 0.0f || total != total ? __fdiv_rn(1.0f, total) : 0.0f;
-  const int qr = tile * a.tile_rows + half * R + warp, step = qr / a.group;
+  const int qr = tile * a.tile_rows + slice * R + warp, step = qr / a.group;
   const long long o = (static_cast<long long>(row) * a.steps + step) * a.ld_out +
                       static_cast<long long>(head * a.group + qr - step * a.group) * a.hd_out + 4 * lane;
   store_any(a.out, o, a.out_type, y.x * inv);
@@ -926,7 +932,7 @@ Plan plan(const verbo_cache& c, int heads, int steps, int q_type) {
   p.dp = c.dim <= 64 ? 64 : c.dim <= 96 ? 96 : 128;
   // More than 8 query rows: 16 at a time, twice the products for one conversion and one
   // copy of the keys and values: rows of 100003 and 131072 tokens with 16 query rows take
-  // 108 us, 130 in two tiles of 8.  fp32 queries, in two parts, leave no registers for it.
+  // 106 us, 130 in two tiles of 8.  fp32 queries, in two parts, leave no registers for it.
   p.rt = rows > 8 && q_type != kOpsF32 ? 2 : 1;
   p.tiles = (rows + 8 * p.rt - 1) / (8 * p.rt);
   const long long units = static_cast<long long>(c.rows) * c.heads * p.tiles;
@@ -981,6 +987,13 @@ cudaError_t run_attend(const AttendArgs& a, const Plan& p, cudaStream_t s) {
   return a.q_type == kOpsF32 ? run_attend<DP, 1, true>(a, p, s) : run_attend<DP, 1, false>(a, p, s);
 }
 
+template <bool MANY>
+cudaError_t run_join(const AttendArgs& a, long long ctas, cudaStream_t s) {
+  using S = JoinShape<MANY>;
+  return launch_chained(cache_attend_join_kernel<MANY>, static_cast<unsigned>(ctas), S::kWarps * 32,
+                        static_cast<size_t>(S::kWarps) * S::kRows * a.dim * 4, 1, s, a);
+}
+
 }  // namespace
 
 size_t cache_attend_bytes(const verbo_cache& c, int heads, int steps, int q_type) {
@@ -1031,18 +1044,15 @@ cudaError_t launch_cache_attend(const verbo_cache& c, int layer, const CacheQuer
   };
   a.wide_q = wide(x.q, x.ld_q, x.hd_q, q_type);
   a.wide_out = wide(x.out, x.ld_out, x.hd_out, out_type);
-  const long long joins = static_cast<long long>(c.rows) * c.heads * p.tiles * (8 * p.rt / kJoinRows);
+  const long long tiles = static_cast<long long>(c.rows) * c.heads * p.tiles;
+  const bool many = tiles * (a.tile_rows / JoinShape<false>::kRows) < 2 * sm_count();
+  const long long joins = tiles * (a.tile_rows / (many ? JoinShape<true>::kRows : JoinShape<false>::kRows));
   if (joins > INT_MAX) return cudaErrorInvalidConfiguration;
   const cudaError_t e = p.dp == 64   ? run_attend<64>(a, p, s)
                         : p.dp == 96 ? run_attend<96>(a, p, s)
                                      : run_attend<128>(a, p, s);
   if (e != cudaSuccess || p.members) return e;
-  const size_t smem = static_cast<size_t>(kJoinRows) * c.dim * 4;  // of a warp
-  if (joins >= 2 * sm_count())
-    return launch_chained(cache_attend_join_kernel<kJoinFew>, static_cast<unsigned>(joins), kJoinFew * 32,
-                          kJoinFew * smem, 1, s, a);
-  return launch_chained(cache_attend_join_kernel<kJoinMany>, static_cast<unsigned>(joins), kJoinMany * 32,
-                        kJoinMany * smem, 1, s, a);
+  return many ? run_join<true>(a, joins, s) : run_join<false>(a, joins, s);
 }
 
 }  // namespace vb
