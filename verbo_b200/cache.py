@@ -83,7 +83,8 @@ class PagedCache:
     [rows, width], the rows' pages, -1 behind the last; lens: int32 [rows], their
     tokens; refs: int32 [pages], how many entries of the table hold a page (0: free).
     All contiguous CUDA tensors on one device, the caller's own: the object keeps
-    them, and a workspace of about 12 bytes a page.  ``new`` makes an empty cache.
+    them, and, where it is made on the default stream, a workspace of about 12 bytes a page for
+    the calls there.  ``new`` makes an empty cache.
 
     A decode step: ``reserve`` makes room for the rows' new tokens, then per layer
     ``append`` writes their keys and values and ``attend`` reads them.  A step of
@@ -126,8 +127,11 @@ class PagedCache:
         self._need = lib.verbo_cache_workspace(ctypes.byref(c))
         if self._need < 0:
             raise _err()
-        # reserve's and compact's: no two of them may run on one cache at the same time
-        self._ws = torch.empty(self._need, dtype=torch.uint8, device=k.device)
+        # reserve's and compact's on the default stream (0): what is made there and used there alone may be
+        # dropped at any time, and no graph holds its address, for that stream cannot be captured
+        self._ws = None
+        if torch._C._cuda_getCurrentRawStream(dev) == 0:
+            self._ws = torch.empty(self._need, dtype=torch.uint8, device=k.device)
         self._attend_need = {}  # workspace bytes by (heads, steps, type)
 
     @classmethod
@@ -164,8 +168,15 @@ class PagedCache:
     def _run(self, fn, *args):
         _call(fn, self._torch, self._dev, self._ref, *args)
 
+    def _workspace(self, stream, at):
+        """Memory for a reserve or a compact on a stream: the kept one, or one that belongs to the call's stream
+        (freed behind the call, it is reused behind the call's work)."""
+        if at == 0 and self._ws is not None:
+            return self._ws
+        return _new(self._torch, self.lens, stream, self._need, self._torch.uint8)
+
     def _ints(self, t, what):
-        """Address of int32 [rows] on the cache's device; a number stands for every row."""
+        """Address of int32 [rows] on the cache's device."""
         return _list(t, self._torch.int32, self._dev, what, self.rows)
 
     def reserve(self, add, stream=None):
@@ -182,8 +193,8 @@ class PagedCache:
         ap = self._ints(add, "add")
         start = _new(torch, self.lens, stream, self.rows, torch.int32)
         status = _new(torch, self.lens, stream, 1, torch.int32)
-        self._run(self._lib.verbo_cache_reserve, ap, start.data_ptr(), status.data_ptr(), self._ws.data_ptr(), self._need,
-                  at)
+        ws = self._workspace(stream, at)
+        self._run(self._lib.verbo_cache_reserve, ap, start.data_ptr(), status.data_ptr(), ws.data_ptr(), self._need, at)
         return start, status
 
     def fork(self, parents, beams, stream=None):
@@ -210,7 +221,8 @@ class PagedCache:
         torch = self._torch
         at = _stream_of(torch, self._dev, stream)
         info = _new(torch, self.lens, stream, 2, torch.int32)
-        self._run(self._lib.verbo_cache_compact, info.data_ptr(), self._ws.data_ptr(), self._need, at)
+        ws = self._workspace(stream, at)
+        self._run(self._lib.verbo_cache_compact, info.data_ptr(), ws.data_ptr(), self._need, at)
         return info
 
     def _tokens(self, t, what, heads=None):
