@@ -42,6 +42,7 @@ constexpr int kAttHeads = 64;  // blocks that are known ahead, per warp
 constexpr int kAttStart = 4;
 constexpr float kUp = 14.0f;   // weights are held times 2^14: fp16's subnormals begin at 2^-28 of the largest
 constexpr double kLog2e = 1.4426950408889634;
+constexpr uint32_t kCodeBits = 0x7f7f7f7fu;  // of four codes, without their signs: all set in a NaN's
 
 struct AttendArgs {
   const unsigned char* k;
@@ -502,11 +503,64 @@ __global__ void __launch_bounds__(AttShape<DP, RT>::kWarps * 32, AttShape<DP, RT
       fetch(j + S::kStages - 1);
       asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 1) : "memory");
       __syncwarp();
-      const unsigned char* at = ring + slot * S::kStep;
+      unsigned char* at = ring + slot * S::kStep;
       slot = slot == S::kStages - 1 ? 0 : slot + 1;
       BlockHead h[kAttPair];
 #pragma unroll
       for (int b = 0; b < kAttPair; ++b) h[b] = known[(2 * j + b) & (kAttHeads - 1)];
+
+      const int place = (b0 + 2 * j) * kCacheBlock;
+      // Several steps, and not every query row sees all of these tokens: a row's weight for
+      // one that it does not see is 0, and 0 times a NaN is not.  So NaN codes (or all of a
+      // block whose scale is none) become zeros here, and the sums that see one NaNs, in the
+      // few registers that are left (64 rows of 4096 tokens with 16 query rows: of 128 dims 126
+      // us with and without it, of 80 dims 116 and 113).
+      if (a.steps > 1 && place + kAttPair * kCacheBlock > all_see) {
+        bool any = false;
+#pragma unroll
+        for (int b = 0; b < kAttPair; ++b) {
+          const bool no_scale = !(fabsf(h[b].vs) <= 3.402823466e38f);
+          unsigned char* vt = at + b * 2 * S::kBlock + S::kBlock;
+          any |= no_scale;
+#pragma unroll 1
+          for (int i = lane * 16; i < S::kBlock; i += 512) {
+            const uint4 x = *reinterpret_cast<const uint4*>(vt + i);
+            any |= (__vcmpeq4(x.x & kCodeBits, kCodeBits) | __vcmpeq4(x.y & kCodeBits, kCodeBits) |
+                    __vcmpeq4(x.z & kCodeBits, kCodeBits) | __vcmpeq4(x.w & kCodeBits, kCodeBits)) != 0;
+          }
+        }
+        if (__any_sync(0xffffffffu, any)) {
+#pragma unroll 1
+          for (int i = 0; i < kAttPair * kCacheBlock; ++i) {
+            const int tok = i % kCacheBlock, line = DP == 64 ? tok >> 1 : tok;
+            const bool second = i >= kCacheBlock;
+            const bool no_scale = !(fabsf(second ? h[1].vs : h[0].vs) <= 3.402823466e38f);
+            unsigned char* vt = at + (second ? 3 : 1) * S::kBlock + line * 128;
+            const int flip = DP == 64 ? (line & 3) << 1 : ((tok >> 1) & 3) << 1, first_of = DP == 64 ? (tok & 1) << 2 : 0;
+#pragma unroll
+            for (int w = 0; w < VW; ++w) {  // this lane's words of the token
+              const int d = DP == 128 ? 16 * g + 4 * w : w < 2 ? 8 * g + 4 * w : 64 + 4 * g;
+              uint32_t* word = reinterpret_cast<uint32_t*>(vt + (((first_of | (d >> 4)) ^ flip) << 4) + (d & 15));
+              const uint32_t nan = no_scale ? 0xffffffffu : __vcmpeq4(*word & kCodeBits, kCodeBits);
+              __syncwarp();  // four lanes have read the same word
+              if (nan == 0) continue;
+              *word &= ~nan;
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int u = 0; u < RT; ++u)
+#pragma unroll
+                  for (int k = 0; k < 2; ++k)
+                    if ((nan >> 8 * c & 1u) && place + i < end[u][k])
+                      acc[2 * w + c / 2][u][2 * (c & 1) + k] = __int_as_float(0x7fc00000);
+            }
+          }
+          __syncwarp();
+#pragma unroll
+          for (int b = 0; b < kAttPair; ++b)
+            if (!(fabsf(h[b].vs) <= 3.402823466e38f)) h[b].vs = 0.0f;
+        }
+      }
 
       // scores of the tokens g (0) and g + 8 (1) of each block for the rows 2 t and 2 t + 1
       Two p[kAttPair][RT][2];
@@ -554,7 +608,6 @@ __global__ void __launch_bounds__(AttShape<DP, RT>::kWarps * 32, AttShape<DP, RT
           }
         }
       }
-      const int place = (b0 + 2 * j) * kCacheBlock;
       if (h[0].valid + h[1].valid < 2 * kCacheBlock || place + 2 * kCacheBlock > all_see) {
 #pragma unroll
         for (int b = 0; b < kAttPair; ++b)
