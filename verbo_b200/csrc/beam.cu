@@ -15,10 +15,14 @@ namespace {
 // value(b, i) = score[b] + (x[b][i] - lse[b]),  lse[b] = m + log sum_j e^(x[b][j] - m)
 //
 // Two beams' candidates are ordered by their values, so the sums have to be exact
-// to well below the distance of two candidates: fp32's 1e-7 would swap a pair
-// now and then.  The terms are fp32 but without a common error (the factor log2(e)
-// is taken in two parts, so a term is off by its own roundings alone, which cancel
-// in the sum), up to sixteen of them are added in fp32 and the rest in 64 bits.  A sum goes by
+// to below the distance of two candidates.  What makes up a row is its largest column: it
+// is a 1 that is added in 64 bits, and the others' terms are seen from it.  Those are fp32
+// (the factor log2(e) is taken in two parts, so a term is off by the roundings of x - m and of
+// its product, 2^-23 |x - m| of itself, and by the exponential's 2^-22), eight to sixteen of them are
+// added in fp32 and the rest in 64 bits.  Measured, lse is off by up to 6e-8: 4.5e-8 where
+// thousands of columns share the row (the exponential is low by as much in the mean), 1e-8
+// with deviations of 6, below 1e-9 where one column stands out by 10.  With a term of the first
+// batch's maximum in the place of the 1, and fp32 sums, it was up to 3e-6.  A sum goes by
 // the columns alone, not by where a row lies in memory: equal rows have equal sums
 // to the last bit, and equal candidates are ordered by their beams.
 //
@@ -27,7 +31,7 @@ namespace {
 // the rows are few.  A second, small kernel joins the beams of a request: a lane
 // keeps the head of a beam's list, and the largest is taken `take` times.
 //
-// Measured on B200: 512 bf16 rows of 151936 with 16 taken 41 us, 3.8 TB/s: the exponential
+// Measured on B200: 512 bf16 rows of 151936 with 16 taken 42 us, 3.7 TB/s: the exponential
 // unit (16 lanes) is busy 60% of the time, issue slots 56%; fp32 65 us, 4.8 TB/s: 512 rows
 // on 592 places leave SMs three or four.  CTAs of 512 threads, two to an SM, took 48 and 62;
 // two CTAs to a row of a large batch 45 and 65.  One row of 49152 13 us, most of it
@@ -115,6 +119,26 @@ struct SelBatch {
         }
     }
     return s;
+  }
+  // How many columns are at v; they are at -inf after it.
+  __device__ __forceinline__ int take_out(float v) {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      uint32_t w[4] = {x[i].raw.x, x[i].raw.y, x[i].raw.z, x[i].raw.w};
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (x[i].get(j) == v) {
+          ++n;
+          if constexpr (N == 4)
+            w[j] = 0xff800000u;
+          else
+            w[j / 2] = j % 2 ? (w[j / 2] & 0xffffu) | (all_neg_inf<T>().x & 0xffff0000u)
+                             : (w[j / 2] & 0xffff0000u) | (all_neg_inf<T>().x & 0xffffu);
+        }
+      x[i].raw = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    return n;
   }
   __device__ __forceinline__ int count_inf() const {
     int n = 0;
@@ -285,13 +309,14 @@ __global__ void __launch_bounds__(kSelThreads, 4) beam_rows_kernel(const BeamSel
     if (bm == -kNegInf) {
       ninf += x.count_inf();
     } else if (bm > kNegInf) {
-      // The first batch's maximum is kept, the CTA's: terms may be above 1, but not by
-      // more than 2^64.
-      if (ref == kNegInf) {
-        ref = bm;
-      } else if (bm - ref > 44.0f) {
+      // The sum is seen from the largest column so far or one that is less than 1 below it: the
+      // CTA's of the first batch, then the thread's own.  That column is a 1 added in 64 bits:
+      // where it makes up the row, no fp32 rounding is left in the sum.
+      const float up = bm - ref;
+      if (up > 1.0f || (b == 0 && up == 0.0f)) {
         sum = sel_scaled(sum, ref, bm);
         ref = bm;
+        sum += x.take_out(bm);
       }
       sum += x.sum(ref);
     }
