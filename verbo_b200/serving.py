@@ -104,9 +104,11 @@ class BeamSearch:
     None in the first step, in which all rows of a request hold its prompt, and after
     that int32 [requests * beams], the token that each row has got.
 
-    A step takes 2 * beams continuations of each request (``beam_select``): those that
+    A step takes the best continuations of each request (``beam_select``): those that
     end on a stop id among the first ``beams`` of them are finished hypotheses, the
-    first ``beams`` of the others live on.  What the rows carry follows them:
+    first ``beams`` of the others live on.  With n stop ids (1 + n) * beams are taken,
+    enough for both, or 64: where those do not hold ``beams`` that live on, every beam's own
+    first 64 are.  What the rows carry follows them:
     ``cache`` (a ``PagedCache`` with a row per beam) forks, ``states`` (tensors with a
     row per beam) are reordered in place.  A request ends when it has ``beams``
     finished hypotheses and no live one can be better than the worst of them, or after
@@ -179,6 +181,37 @@ class BeamSearch:
         self.steps = n
         return out_s, out_p, out_t
 
+    def _short(self, parents, tokens) -> bool:
+        """Whether an open request's continuations are fewer that live on than beams, and not all there are."""
+        return any(is_open and p[-1] >= 0 and sum(i not in self.stop_ids for i in t) < self.beams
+                   for is_open, p, t in zip(self.open, parents, tokens))
+
+    def _find(self):
+        """The step's continuations of each request: (scores, parents, tokens) as lists."""
+        import verbo_b200 as vb
+
+        most, beams = 64, self.beams  # beam_select's limit
+        ends = sum(0 <= i < self.vocab for i in self.stop_ids)
+        take = min(most, max(2, 1 + ends) * beams)
+        found = [f.tolist() for f in vb.beam_select(self.logits, self.scores, beams, take)]
+        if take == max(2, 1 + ends) * beams or not self._short(*found[1:]):
+            return found
+        # a beam at a time: no more than `beams` of one live on.  These scores are rounded to fp32, equal ones
+        # go by the beam.
+        scores, parents, tokens = (f.tolist() for f in vb.beam_select(self.logits, self.scores, 1, most))
+        found = [], [], []
+        for r in range(self.requests):
+            rows = range(r * beams, (r + 1) * beams)
+            best = sorted(((s, b, t) for b, i in enumerate(rows) for s, p, t in zip(scores[i], parents[i], tokens[i])
+                           if p >= 0), key=lambda c: -c[0])
+            live = [s for s, _, t in best if t not in self.stop_ids]
+            worst = live[beams - 1] if len(live) >= beams else float("-inf")
+            if any(parents[i][-1] >= 0 and scores[i][-1] > worst for i in rows):
+                raise vb.VerboCudaError(f"too many stop ids among the first {most} continuations of a beam")
+            for out, column in zip(found, ([c[k] for c in best] for k in range(3))):
+                out.append(column)
+        return found
+
     def step(self) -> bool:
         """One token for every open request; False when none is left."""
         import verbo_b200 as vb
@@ -187,8 +220,7 @@ class BeamSearch:
             return False
         torch = self.torch
         self.model(self.tokens, self.logits)
-        found = vb.beam_select(self.logits, self.scores, self.beams, 2 * self.beams)
-        live = self._advance(*(f.tolist() for f in found))
+        live = self._advance(*self._find())
         self.scores = torch.tensor(live[0], dtype=torch.float32, device=self.device)
         parents = torch.tensor(live[1], dtype=torch.int32, device=self.device)
         self.tokens = torch.tensor(live[2], dtype=torch.int32, device=self.device).view(-1)
