@@ -7,6 +7,7 @@ are checked here and in the C ABI; both raise ``VerboCudaError``.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 
@@ -162,6 +163,18 @@ class PagedCache:
     def __reduce_ex__(self, protocol):
         raise TypeError("a PagedCache cannot be copied or pickled")
 
+    _said = None  # what `statuses` collects
+
+    @contextlib.contextmanager
+    def statuses(self):
+        """A list of the statuses (device tensors) of the reserves that are called inside, but for captured ones, which
+        a replay writes.  Of two collections, one inside the other, the inner one has what is called in it."""
+        before, self._said = self._said, []
+        try:
+            yield self._said
+        finally:
+            self._said = before
+
     k, v, k_scale, v_scale = _tensor("k"), _tensor("v"), _tensor("k_scale"), _tensor("v_scale")
     table, lens, refs = _tensor("table"), _tensor("lens"), _tensor("refs")
 
@@ -195,6 +208,8 @@ class PagedCache:
         status = _new(torch, self.lens, stream, 1, torch.int32)
         ws = self._workspace(stream, at)
         self._run(self._lib.verbo_cache_reserve, ap, start.data_ptr(), status.data_ptr(), ws.data_ptr(), self._need, at)
+        if self._said is not None and not torch.cuda.is_current_stream_capturing():
+            self._said.append(status)
         return start, status
 
     def fork(self, parents, beams, stream=None):

@@ -16,6 +16,7 @@ the same object (verbo_cuda_server_prepare / _step / _result).
 """
 from __future__ import annotations
 
+import contextlib
 from dataclasses import dataclass, field
 from typing import Callable, Dict, List, Optional, Sequence
 
@@ -112,7 +113,10 @@ class BeamSearch:
     ``cache`` (a ``PagedCache`` with a row per beam) forks, ``states`` (tensors with a
     row per beam) are reordered in place.  A request ends when it has ``beams``
     finished hypotheses and no live one can be better than the worst of them, or after
-    ``max_tokens`` tokens.  Only continuations cross to the host."""
+    ``max_tokens`` tokens.  Only continuations cross to the host, and the statuses of the
+    ``cache.reserve`` calls of the model (not of a graph that it replays): one that was
+    refused raises ``VerboCudaError``, unless the model collects it itself
+    (``cache.statuses``)."""
 
     def __init__(self, model: Callable, requests: int, beams: int, vocab: int, max_tokens: int,
                  stop_ids: Sequence[int] = (), length_penalty: float = 1.0, cache=None, states: Sequence = (),
@@ -219,8 +223,14 @@ class BeamSearch:
         if not any(self.open):
             return False
         torch = self.torch
-        self.model(self.tokens, self.logits)
-        live = self._advance(*self._find())
+        with getattr(self.cache, "statuses", contextlib.nullcontext)() as said:
+            self.model(self.tokens, self.logits)
+        found = self._find()
+        for status in torch.cat(said).tolist() if said else ():
+            if status:
+                raise vb.VerboCudaError("the cache does not hold the step's tokens: " + (
+                    f"{status} pages are missing" if status > 0 else f"row {-status - 1} would be longer than its table"))
+        live = self._advance(*found)
         self.scores = torch.tensor(live[0], dtype=torch.float32, device=self.device)
         parents = torch.tensor(live[1], dtype=torch.int32, device=self.device)
         self.tokens = torch.tensor(live[2], dtype=torch.int32, device=self.device).view(-1)
