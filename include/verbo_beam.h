@@ -44,7 +44,7 @@ extern "C" {
    workspace     verbo_beam_workspace() bytes, 16-byte aligned, its own until the
                  call's work is done.
    lse is off by at most the sum of the columns' shares of the row times 2^-23
-   (|x - m| + 6.5), where a column that stands out by more than 1 counts nothing: by
+   (|x - m| + 7.5), where a column that stands out by more than 1 counts nothing: by
    some 1e-8 in a model's rows, and by less than 1e-7 in all that were measured.
    Candidates of two beams that lie nearer to each other may change places.  Equal rows
    have equal sums wherever they lie. */

@@ -76,7 +76,8 @@ VERBO_CUDA_API int verbo_cache_fork(const verbo_cache* c, const int* parents, lo
 
 /* Row r keeps its first keep[r] tokens (all if keep[r] < 0 or above its length); the
    pages behind them are given back.  0 frees a row, its length less the rejected
-   tokens undoes a speculation. */
+   tokens undoes a speculation, but for its rounding: where a rejected token raised the
+   scale of the block that it shares with kept ones, those stay rounded to that scale. */
 VERBO_CUDA_API int verbo_cache_free(const verbo_cache* c, const int* keep, void* stream);
 
 /* Moves the live pages to the front of the pools, all layers, and sets the tables
@@ -109,8 +110,12 @@ VERBO_CUDA_API int verbo_cache_append(const verbo_cache* c, int layer, const voi
                  gets zeros.  Tokens in a page outside [0, pages) are left out.
    workspace     verbo_cache_attend_workspace() bytes, 16-byte aligned, its own
                  until the call's work is done.
-   Products are exact to 2^-22 of a row's largest element, sums fp32, whatever the
-   types.  The same call gives the same bits. */
+   Scores' products are exact to 2^-22 of a row's largest element, sums fp32, whatever
+   the types.  A weight e^(s - m) is off by at most 2^-22 of itself or, if that is more,
+   2^-39 times the quotient of the largest scale among the values of the row's head, be
+   their weights 0, and its own block's: 2e-9 where scales are within a factor of
+   1000, 2e-6 where one block has values a million times as large as the others.  The same
+   call gives the same bits. */
 VERBO_CUDA_API int verbo_cache_attend(const verbo_cache* c, int layer, const void* q, int q_type, long long ld_q,
                                       long long hd_q, int heads, int steps, float scale, void* out, int out_type,
                                       long long ld_out, long long hd_out, void* workspace, long long workspace_bytes,

@@ -226,7 +226,8 @@ class PagedCache:
 
     def free(self, keep, stream=None):
         """Row r keeps its first keep[r] tokens (int32 [rows]; negative: all), and gives
-        the pages behind them back (verbo_cache_free)."""
+        the pages behind them back (verbo_cache_free).  Kept tokens stay rounded to the scale
+        of their block, also where a token that is not kept has raised it."""
         self._run(self._lib.verbo_cache_free, self._ints(keep, "keep"),
                   _stream_of(self._torch, self._dev, stream))
 

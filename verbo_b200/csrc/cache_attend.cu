@@ -15,7 +15,8 @@
 // 16 rows of a product and the queries its 8 columns: scores K q^T, sums V^T p^T, the
 // weights turned in between (movmatrix).  fp32 queries, and all weights e^(s - m), come
 // in two parts, rounded to fp16 and what the rounding left, so that products are exact
-// to 2^-22.  Sums on the tensor cores are cut, not rounded, so they are taken over to
+// to 2^-22; weights have their block's scale in them, as a part of the largest that the warp has
+// met, and the second part ends at 2^-39 of a weight of 1 there.  Sums on the tensor cores are cut, not rounded, so they are taken over to
 // fp32 registers every few blocks (8 rows of 65536 tokens: off by 6e-7 with it, by 8e-6
 // without).
 //
