@@ -32,7 +32,7 @@ namespace {
 // keeps the head of a beam's list, and the largest is taken `take` times.
 //
 // Measured on B200: 512 bf16 rows of 151936 with 16 taken 42 us, 3.7 TB/s: the exponential
-// unit (16 lanes) is busy 60% of the time, issue slots 56%; fp32 65 us, 4.8 TB/s: 512 rows
+// unit (16 lanes) is busy 57% of the time, issue slots 56%; fp32 65 us, 4.8 TB/s: 512 rows
 // on 592 places leave SMs three or four.  CTAs of 512 threads, two to an SM, took 48 and 62;
 // two CTAs to a row of a large batch 45 and 65.  One row of 49152 13 us, most of it
 // round trips and barriers.

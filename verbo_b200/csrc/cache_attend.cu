@@ -222,7 +222,7 @@ struct __align__(16) BlockHead {
 // bytes whose 16-byte chunks are exchanged so that the fragment loads below meet no
 // bank twice, and what is known of the blocks.
 // A warp's step is a chain of loads, products and exponentials, and two steps ahead
-// cover the memory's latency: 8 warps with three steps of shared memory at 230 registers.
+// cover the memory's latency: 8 warps with three steps of shared memory at 226 registers.
 // With 96 dims 168 registers do, and 12 warps with two steps each take 148 us where 8
 // with three take 157 (64 rows of 8192 tokens of 80 dims); with 128 dims those spill,
 // and 64 rows of 4096 tokens take 124 us against 102.
@@ -986,7 +986,7 @@ Plan plan(const verbo_cache& c, int heads, int steps, int q_type) {
   p.dp = c.dim <= 64 ? 64 : c.dim <= 96 ? 96 : 128;
   // More than 8 query rows: 16 at a time, twice the products for one conversion and one
   // copy of the keys and values: rows of 100003 and 131072 tokens with 16 query rows take
-  // 106 us, 130 in two tiles of 8.  fp32 queries, in two parts, leave no registers for it.
+  // 107 us, 130 in two tiles of 8.  fp32 queries, in two parts, leave no registers for it.
   p.rt = rows > 8 && q_type != kOpsF32 ? 2 : 1;
   p.tiles = (rows + 8 * p.rt - 1) / (8 * p.rt);
   const long long units = static_cast<long long>(c.rows) * c.heads * p.tiles;
